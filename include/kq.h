@@ -325,6 +325,72 @@ KQ_API int kq_quantize_rows(kq_ctx* ctx, uint64_t x_f32_dptr, uint32_t rows, uin
 KQ_API int kq_linear_a8(kq_ctx* ctx, kq_weight w, uint64_t xq_i8_dptr, uint64_t xs_f32_dptr, uint64_t bias_dptr,
                         uint64_t out_dptr, uint32_t m);
 
+/* ---- the attention half of a decoder layer ------------------------------------------------
+ * What stands between the linears of a layer, so that a host can run whole layers beside
+ * kq_linear_fused: q | k | v -> append -> attention -> o.  (The reference keeps f32 states and
+ * has no packed cache.)
+ *
+ * Rotation table: f32 [positions, rotary / 2, 2], (cos, sin) of every position and pair, as the host
+ * computes them (scalings for long contexts included).  The pairs of a head are its values (i, i + rotary / 2),
+ * or (2 i, 2 i + 1) with KQ_ROPE_INTERLEAVED; (x0, x1) becomes (x0 c - x1 s, x1 c + x0 s), every
+ * product and sum rounded to f32; values from `rotary` on stay.  A position outside the table gives NaN
+ * in what it would have rotated, as kq_embedding does for its indices.
+ *
+ * kq_rope: x is [tokens, heads, head_dim] of x_dtype, consecutive tokens x_stride elements apart;
+ * positions is i32 [tokens]; out has x's type and may be x. */
+enum kq_rope_flags { KQ_ROPE_INTERLEAVED = 1 };
+KQ_API int kq_rope(kq_ctx* ctx, uint64_t x_dptr, int x_dtype, uint32_t tokens, uint32_t heads, uint32_t head_dim,
+                   uint64_t x_stride, uint64_t positions_dptr, uint64_t table_dptr, uint32_t table_positions,
+                   uint32_t rotary, uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride);
+
+/* Keys and values in 4 bits, in pages of page_tokens (16, 32, 64, 128 or 256) tokens.  The pool is the
+ * caller's device memory (16-byte aligned, kq_cache_bytes() bytes): [pages][kv_heads][block], a block of
+ *   K codes [page_tokens][head_dim / 2] | V codes, likewise | K (scale, offset) [page_tokens][2] binary16 | V, likewise
+ * (element 2 i in the low nibble of byte i), (head_dim + 8) bytes a token and head.  A row x of head_dim
+ * (64, 128 or 256) values, a key after its rotation, is held as
+ *   offset = f16(min x), scale = max(f16((max x - offset) * f32(1 / 15)), 0)
+ *   code = clamp(round_ties_even((x - offset) * (1 / scale)), 0, 15), 0 where scale is 0
+ * (f32 operations, each rounded) and stands for fround(code * scale + offset).  A row with a NaN or infinity,
+ * or beyond binary16's range, is held as NaN.  The handle keeps the pool's address and shape, nothing else:
+ * freeing it leaves the pool. */
+typedef uint64_t kq_cache; /* opaque handle, 0 is never valid */
+KQ_API uint64_t kq_cache_bytes(uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim);
+KQ_API int kq_cache_create(kq_ctx* ctx, uint64_t pool_dptr, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads,
+                           uint32_t head_dim, kq_cache* out);
+KQ_API int kq_cache_free(kq_ctx* ctx, kq_cache cache);
+
+/* The sequences of a call are device arrays of i32: `page_table` [sequences, table_width] with the pages
+ * of each sequence in order, `lengths` [sequences], and `starts` [sequences + 1]: sequence b's new tokens are
+ * rows starts[b] .. starts[b + 1] of the call's tensors and its last tokens, lengths[b] counting them.
+ * starts == 0: every sequence has one new token, row b.  `most` bounds the new tokens of any sequence (0: not
+ * known); it chooses kernels, results do not depend on it.  All of this is read on the device at launch, so
+ * that a recorded step can be replayed with other lengths and pages.  A page number outside the pool, or a
+ * token beyond table_width pages, is not written and reads as NaN; a sequence may be idle (length 0).
+ *
+ * kq_cache_append: k and v are [tokens, kv_heads, head_dim] of `dtype`, k_stride / v_stride elements apart
+ * (columns of a fused projection); keys are rotated on the way (table_dptr == 0: not).  Two rows that name the
+ * same page and slot race.
+ * kq_cache_read: what the cache holds for the new tokens (starts = running sums of lengths: for all), f32
+ * [tokens, kv_heads, head_dim]; NaN where there is no such token.
+ * kq_cache_attention: for query i of a sequence with n new tokens, at position p = length - n + i,
+ *   out = sum_j softmax_j(scale * q . k_j) v_j   over the keys j in [window ? max(0, p - window + 1) : 0, p],
+ * zeros where there is none.  q is [tokens, heads, head_dim] of q_dtype (heads a multiple of kv_heads; query
+ * head h reads kv head h / (heads / kv_heads)), rotated on the way (table_dptr == 0: not); out has q's type.
+ * Scores, softmax and sums are f32; f32 queries keep 22 bits or more through the tensor cores, 16-bit
+ * ones are multiplied in binary16. */
+KQ_API int kq_cache_append(kq_ctx* ctx, kq_cache cache, uint64_t k_dptr, uint64_t k_stride, uint64_t v_dptr,
+                           uint64_t v_stride, int dtype, uint32_t sequences, uint64_t page_table_dptr,
+                           uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,
+                           uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags);
+KQ_API int kq_cache_read(kq_ctx* ctx, kq_cache cache, uint32_t sequences, uint64_t page_table_dptr,
+                         uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,
+                         uint64_t k_f32_dptr, uint64_t v_f32_dptr);
+KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads,
+                              uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width,
+                              uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens, uint32_t most, float scale,
+                              uint32_t window, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary,
+                              uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride);
+
 /* ---- replayable plans -----------------------------------------------------------
  * Records every kq_* launch between begin and end into a CUDA graph that
  * kq_graph_launch replays.  Replaces the reference's baked plan replay

@@ -6,8 +6,9 @@ it is not built.
 """
 from ._lib import (KQ_BF16, KQ_F16, KQ_F32, KQ_SHARD_COLUMN, KQ_SHARD_NONE, KQ_SHARD_ROW,
                    KQ_STORAGE_I4, KQ_STORAGE_I8, LIB_PATH, lib)
-from .runtime import Gpu, KqError, Weight, acquire_gpu
+from .rotary import rope_frequencies, rope_table
+from .runtime import CacheBatch, Gpu, KqError, KvCache, Rope, Weight, acquire_gpu
 
-__all__ = ["Gpu", "KqError", "Weight", "acquire_gpu", "lib", "LIB_PATH",
+__all__ = ["Gpu", "KqError", "Weight", "Rope", "CacheBatch", "KvCache", "rope_frequencies", "rope_table", "acquire_gpu", "lib", "LIB_PATH",
            "KQ_F32", "KQ_F16", "KQ_BF16", "KQ_STORAGE_I4", "KQ_STORAGE_I8",
            "KQ_SHARD_NONE", "KQ_SHARD_COLUMN", "KQ_SHARD_ROW"]

@@ -66,6 +66,14 @@ SYMBOLS = {
     "kq_silu_mul": (_i32, [_vp, _u64, _u64, _u64, _u64]),
     "kq_add": (_i32, [_vp, _u64, _u64, _u64, _u64]),
     "kq_linear_fused": (_i32, [_vp, _u32, _pu64, _u64, _i32, _u64, ctypes.c_float, _pu64, _u64, _pu64, _u32, _u32]),
+    "kq_rope": (_i32, [_vp, _u64, _i32, _u32, _u32, _u32, _u64, _u64, _u64, _u32, _u32, _u32, _u64, _u64]),
+    "kq_cache_bytes": (_u64, [_u32, _u32, _u32, _u32]),
+    "kq_cache_create": (_i32, [_vp, _u64, _u32, _u32, _u32, _u32, _pu64]),
+    "kq_cache_free": (_i32, [_vp, _u64]),
+    "kq_cache_append": (_i32, [_vp, _u64, _u64, _u64, _u64, _u64, _i32, _u32, _u64, _u32, _u64, _u64, _u32, _u64, _u32, _u32, _u32]),
+    "kq_cache_read": (_i32, [_vp, _u64, _u32, _u64, _u32, _u64, _u64, _u32, _u64, _u64]),
+    "kq_cache_attention": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, ctypes.c_float, _u32,
+                                  _u64, _u32, _u32, _u32, _u64, _u64]),
     "kq_graph_begin": (_i32, [_vp]),
     "kq_graph_end": (_i32, [_vp, _pu64]),
     "kq_graph_launch": (_i32, [_vp, _u64]),

@@ -22,6 +22,7 @@ struct kq_ctx {
   bool capturing = false;
   std::string error;
   std::unordered_map<uint64_t, Weight*> weights;
+  std::unordered_map<uint64_t, kq::Cache> caches;
   std::unordered_map<uint64_t, cudaGraphExec_t> graphs;
   std::unordered_map<uint64_t, uint64_t> graph_kernels;  // kernel nodes per recorded graph
   std::unordered_map<uint64_t, kq::Plan*> plans;
@@ -418,6 +419,51 @@ int run_linear(kq_ctx* ctx, uint32_t count, const kq_weight* handles, uint64_t x
   return KQ_OK;
 }
 
+const kq::Cache* find_cache(kq_ctx* ctx, kq_cache h) {
+  auto it = ctx->caches.find(h);
+  return it == ctx->caches.end() ? nullptr : &it->second;
+}
+
+bool cache_shape_ok(uint32_t page_tokens, uint32_t head_dim) {
+  return is_pow2(page_tokens) && page_tokens >= 16 && page_tokens <= 256 && (head_dim == 64 || head_dim == 128 || head_dim == 256);
+}
+
+// Rows of [heads, head_dim] `stride` elements apart, read and written 16 bytes at a time.
+int check_rows(kq_ctx* ctx, const char* who, const char* name, uint64_t ptr, uint64_t stride, int dtype, uint64_t heads, uint32_t head_dim) {
+  if (dtype != KQ_F32 && dtype != KQ_F16 && dtype != KQ_BF16)
+    return fail(ctx, KQ_ERR_BAD_ARG, "%s: dtype %d: expected KQ_F32, KQ_F16 or KQ_BF16", who, dtype);
+  if (!ptr || (ptr & 15u) || (stride * dtype_bytes(dtype)) % 16 != 0)
+    return fail(ctx, KQ_ERR_BAD_ARG, "%s: %s must be a device pointer, rows 16-byte aligned", who, name);
+  if (stride < heads * head_dim || stride > (1ull << 40))
+    return fail(ctx, KQ_ERR_SHAPE, "%s: rows of %s %llu elements apart do not hold [%llu, %u]", who, name, (unsigned long long)stride,
+                (unsigned long long)heads, head_dim);
+  return KQ_OK;
+}
+
+int check_rope(kq_ctx* ctx, const char* who, uint64_t table, uint32_t positions, uint32_t rotary, uint32_t flags, uint32_t head_dim,
+               kq::RopeTable* out) {
+  *out = kq::RopeTable{reinterpret_cast<const float2*>(table), positions, rotary, (flags & KQ_ROPE_INTERLEAVED) != 0};
+  if (flags & ~static_cast<uint32_t>(KQ_ROPE_INTERLEAVED)) return fail(ctx, KQ_ERR_BAD_ARG, "%s: unknown rope_flags %u", who, flags);
+  if (!table) return KQ_OK;
+  if (table & 7u) return fail(ctx, KQ_ERR_BAD_ARG, "%s: the rotation table must be 8-byte aligned", who);
+  if (rotary < 2 || rotary % 2 != 0 || rotary > head_dim)
+    return fail(ctx, KQ_ERR_SHAPE, "%s: rotary %u is not an even part of head_dim %u", who, rotary, head_dim);
+  return KQ_OK;
+}
+
+int check_batch(kq_ctx* ctx, const char* who, uint32_t sequences, uint64_t pages, uint32_t width, uint64_t lengths, uint64_t starts,
+                uint32_t tokens, uint32_t most, kq::CacheBatch* out) {
+  *out = kq::CacheBatch{reinterpret_cast<const int*>(pages), reinterpret_cast<const int*>(lengths), reinterpret_cast<const int*>(starts),
+                        sequences, width, tokens, starts ? (most && most < tokens ? most : tokens) : 1u};
+  if (!sequences || !width || !pages || !lengths || ((pages | lengths | starts) & 3u))
+    return fail(ctx, KQ_ERR_BAD_ARG, "%s: page_table [sequences, table_width], lengths [sequences] and starts are i32 device arrays", who);
+  if (!starts && tokens != sequences)
+    return fail(ctx, KQ_ERR_SHAPE, "%s: %u rows for %u sequences: without starts each has one", who, tokens, sequences);
+  if (tokens > (1u << 30) || sequences > (1u << 24) || width > (1u << 27))
+    return fail(ctx, KQ_ERR_SHAPE, "%s: %u rows, %u sequences, %u pages each: beyond 2^30, 2^24, 2^27", who, tokens, sequences, width);
+  return KQ_OK;
+}
+
 }  // namespace
 
 namespace kq {
@@ -748,6 +794,137 @@ int kq_linear_host(kq_ctx* ctx, kq_weight h, const void* x_host, int x_dtype, ui
   if (rc != KQ_OK) return rc;
   KQ_CUDA(ctx, cudaMemcpyAsync(out_host, ctx->host_dev_out, obytes, cudaMemcpyDeviceToHost, ctx->stream));
   return kq_sync(ctx);
+}
+
+int kq_rope(kq_ctx* ctx, uint64_t x_dptr, int x_dtype, uint32_t tokens, uint32_t heads, uint32_t head_dim, uint64_t x_stride,
+            uint64_t positions_dptr, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags, uint64_t out_dptr,
+            uint64_t out_stride) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_rope cannot be recorded into a fused plan");
+  kq::RopeTable rope;
+  int rc = check_rope(ctx, "kq_rope", table_dptr, table_positions, rotary, rope_flags, head_dim, &rope);
+  if (rc != KQ_OK) return rc;
+  if (x_dtype != KQ_F32 && x_dtype != KQ_F16 && x_dtype != KQ_BF16)
+    return fail(ctx, KQ_ERR_BAD_ARG, "kq_rope: x_dtype %d: expected KQ_F32, KQ_F16 or KQ_BF16", x_dtype);
+  if (tokens == 0 || heads == 0) return KQ_OK;
+  const uint64_t row = static_cast<uint64_t>(heads) * head_dim, mask = dtype_bytes(x_dtype) - 1;
+  if (!x_dptr || !out_dptr || !positions_dptr || !table_dptr || ((x_dptr | out_dptr) & mask) || (positions_dptr & 3u))
+    return fail(ctx, KQ_ERR_BAD_ARG, "kq_rope: x, out, positions and the table must be aligned device pointers");
+  if (row > 0xffffffffull || x_stride < row || out_stride < row || x_stride > (1ull << 40) || out_stride > (1ull << 40) || tokens > (1u << 30) ||
+      static_cast<uint64_t>(tokens) * row > (1ull << 38))
+    return fail(ctx, KQ_ERR_SHAPE, "kq_rope: rows of [%u, %u] do not fit strides %llu and %llu, or are too many", heads, head_dim,
+                (unsigned long long)x_stride, (unsigned long long)out_stride);
+  if (x_dptr == out_dptr && x_stride != out_stride) return fail(ctx, KQ_ERR_BAD_ARG, "kq_rope: in place, both strides must be the same");
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_rope(env_of(ctx), reinterpret_cast<const void*>(x_dptr), x_dtype, tokens, heads, head_dim, x_stride,
+                                  reinterpret_cast<const int*>(positions_dptr), rope, reinterpret_cast<void*>(out_dptr), out_stride);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "rope launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+uint64_t kq_cache_bytes(uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim) {
+  return cache_shape_ok(page_tokens, head_dim) ? static_cast<uint64_t>(pages) * kv_heads * page_tokens * (head_dim + 8u) : 0;
+}
+
+int kq_cache_create(kq_ctx* ctx, uint64_t pool_dptr, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, kq_cache* out) {
+  if (!ctx || !out) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_create: null argument");
+  *out = 0;
+  if (!cache_shape_ok(page_tokens, head_dim))
+    return fail(ctx, KQ_ERR_SHAPE, "kq_cache_create: pages of %u tokens, heads of %u values: pages are 16, 32, 64, 128 or 256 tokens, heads 64, 128 or 256 values",
+                page_tokens, head_dim);
+  if (!pages || pages > (1u << 30) || !kv_heads || kv_heads > 1024)
+    return fail(ctx, KQ_ERR_SHAPE, "kq_cache_create: %u pages, %u kv heads: 1..2^30 and 1..1024", pages, kv_heads);
+  if (!pool_dptr || (pool_dptr & 15u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_create: the pool must be a 16-byte aligned device pointer");
+  const uint64_t handle = ctx->next_handle++;
+  ctx->caches[handle] = kq::Cache{reinterpret_cast<uint8_t*>(pool_dptr), pages, page_tokens, kv_heads, head_dim};
+  *out = handle;
+  return KQ_OK;
+}
+
+int kq_cache_free(kq_ctx* ctx, kq_cache h) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  if (!ctx->caches.erase(h)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_free: unknown cache handle");
+  return KQ_OK;
+}
+
+int kq_cache_append(kq_ctx* ctx, kq_cache h, uint64_t k_dptr, uint64_t k_stride, uint64_t v_dptr, uint64_t v_stride, int dtype,
+                    uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr,
+                    uint32_t tokens, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_cache_append cannot be recorded into a fused plan (record a graph)");
+  const kq::Cache* c = find_cache(ctx, h);
+  if (!c) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_append: unknown cache handle");
+  if (tokens == 0) return KQ_OK;
+  kq::CacheBatch batch;
+  kq::RopeTable rope;
+  int rc = check_batch(ctx, "kq_cache_append", sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr, tokens, 0, &batch);
+  if (rc == KQ_OK) rc = check_rope(ctx, "kq_cache_append", table_dptr, table_positions, rotary, rope_flags, c->head_dim, &rope);
+  if (rc == KQ_OK) rc = check_rows(ctx, "kq_cache_append", "k", k_dptr, k_stride, dtype, c->kv_heads, c->head_dim);
+  if (rc == KQ_OK) rc = check_rows(ctx, "kq_cache_append", "v", v_dptr, v_stride, dtype, c->kv_heads, c->head_dim);
+  if (rc != KQ_OK) return rc;
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_cache_append(env_of(ctx), *c, batch, reinterpret_cast<const void*>(k_dptr), k_stride,
+                                          reinterpret_cast<const void*>(v_dptr), v_stride, dtype, rope);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_append launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+int kq_cache_read(kq_ctx* ctx, kq_cache h, uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr,
+                  uint64_t starts_dptr, uint32_t tokens, uint64_t k_f32_dptr, uint64_t v_f32_dptr) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_cache_read cannot be recorded into a fused plan (record a graph)");
+  const kq::Cache* c = find_cache(ctx, h);
+  if (!c) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_read: unknown cache handle");
+  if (tokens == 0) return KQ_OK;
+  kq::CacheBatch batch;
+  const int rc = check_batch(ctx, "kq_cache_read", sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr, tokens, 0, &batch);
+  if (rc != KQ_OK) return rc;
+  if (!k_f32_dptr || !v_f32_dptr || ((k_f32_dptr | v_f32_dptr) & 15u))
+    return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_read: k and v must be 16-byte aligned device pointers");
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_cache_read(env_of(ctx), *c, batch, reinterpret_cast<float*>(k_f32_dptr), reinterpret_cast<float*>(v_f32_dptr));
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_read launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+int kq_cache_attention(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads, uint32_t sequences,
+                       uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,
+                       uint32_t most, float scale, uint32_t window, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary,
+                       uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_cache_attention cannot be recorded into a fused plan (record a graph)");
+  const kq::Cache* c = find_cache(ctx, h);
+  if (!c) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_attention: unknown cache handle");
+  if (!heads || heads % c->kv_heads != 0 || heads > 65536)
+    return fail(ctx, KQ_ERR_SHAPE, "kq_cache_attention: %u query heads do not share %u kv heads evenly", heads, c->kv_heads);
+  if (!(scale > 0.0f) || !(scale < __builtin_inff())) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_attention: scale must be finite and positive");
+  if (tokens == 0) return KQ_OK;
+  kq::AttendArgs a;
+  a.cache = *c;
+  int rc = check_batch(ctx, "kq_cache_attention", sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr, tokens, most, &a.batch);
+  if (rc == KQ_OK) rc = check_rope(ctx, "kq_cache_attention", table_dptr, table_positions, rotary, rope_flags, c->head_dim, &a.rope);
+  if (rc == KQ_OK) rc = check_rows(ctx, "kq_cache_attention", "q", q_dptr, q_stride, q_dtype, heads, c->head_dim);
+  if (rc == KQ_OK) rc = check_rows(ctx, "kq_cache_attention", "out", out_dptr, out_stride, q_dtype, heads, c->head_dim);
+  if (rc != KQ_OK) return rc;
+  if (static_cast<uint64_t>(tokens) * heads > (1ull << 30))
+    return fail(ctx, KQ_ERR_SHAPE, "kq_cache_attention: %u rows of %u heads: beyond 2^30", tokens, heads);
+  a.q = reinterpret_cast<const void*>(q_dptr);
+  a.out = reinterpret_cast<void*>(out_dptr);
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.dtype = q_dtype;
+  a.heads = heads;
+  a.window = window;
+  a.scale = scale;
+  DeviceGuard guard(ctx->device);
+  int launched = 0;
+  cudaError_t e = kq::launch_attend(env_of(ctx), a, &launched);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_attention launch");
+  ctx->launches += launched;
+  return KQ_OK;
 }
 
 int kq_graph_begin(kq_ctx* ctx) {

@@ -1,0 +1,285 @@
+// Rotary positions, and rows into and out of the paged 4-bit cache (layout in kq_cache.cuh).
+//
+//   rope    (x0, x1) -> (x0 c - x1 s, x1 c + x0 s) for the pairs of a head
+//   append  key rows rotated, then each row of D values as codes 0..15 with a binary16 scale and offset
+//   read    the f32 values that rows stand for
+//
+// All three are bound by memory: a value is read once and written once.
+#include <algorithm>
+
+#include "kq_cache.cuh"
+
+namespace kq {
+namespace {
+
+constexpr int kThreads = 256;
+
+// ---- rope -----------------------------------------------------------------------------------
+// A thread owns one run of V values of a head (half layout: and the run it is paired with) and loops over heads with the
+// angles in registers.
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Run {
+  T v[V];
+};
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+struct RopeParams {
+  const void* x;
+  void* out;
+  uint64_t x_stride, out_stride;
+  const int* positions;
+  RopeTable rope;
+  uint32_t tokens, heads, dim;
+  uint32_t units;        // runs (or pairs of runs) a head
+  uint32_t head_groups;  // threads that share a token's heads for one unit
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
+  using R = Run<T, V>;
+  const uint64_t id = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const uint32_t unit = id % p.units;
+  const uint32_t group = id / p.units % p.head_groups;
+  const uint64_t token = id / (static_cast<uint64_t>(p.units) * p.head_groups);
+  if (token >= p.tokens) return;
+  const uint32_t half = p.rope.rotary / 2, turning = p.rope.interleaved && V > 1 ? p.rope.rotary / V : half / V;
+  const T* x = static_cast<const T*>(p.x) + token * p.x_stride;
+  T* out = static_cast<T*>(p.out) + token * p.out_stride;
+  if (unit >= turning) {  // behind the rotated part
+    const uint32_t at = p.rope.rotary + (unit - turning) * V;
+    if (x != out)
+      for (uint32_t h = group; h < p.heads; h += p.head_groups)
+        *reinterpret_cast<R*>(out + h * p.dim + at) = *reinterpret_cast<const R*>(x + h * p.dim + at);
+    return;
+  }
+  const int position = p.positions[token];
+  const bool inside = position >= 0 && static_cast<uint32_t>(position) < p.rope.positions;
+  const float2* row = p.rope.table + static_cast<size_t>(inside ? position : 0) * half;
+  float2 cs[V];
+  if constexpr (V > 1) {
+    if (p.rope.interleaved) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) cs[i] = inside ? row[unit * (V / 2) + i] : make_float2(quiet_nan(), quiet_nan());
+      for (uint32_t h = group; h < p.heads; h += p.head_groups) {
+        const uint32_t at = h * p.dim + unit * V;
+        R r = *reinterpret_cast<const R*>(x + at);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          const float2 y = rotate_pair(to_f32(r.v[i]), to_f32(r.v[i + 1]), cs[i / 2]);
+          r.v[i] = from_f32<T>(y.x);
+          r.v[i + 1] = from_f32<T>(y.y);
+        }
+        *reinterpret_cast<R*>(out + at) = r;
+      }
+      return;
+    }
+  }
+  // runs of V values and what they are paired with: rotary / 2 further on, or (interleaved, one value at a time) the next one
+  const uint32_t step = p.rope.interleaved ? 2 : V, pair = p.rope.interleaved ? 1 : half;
+#pragma unroll
+  for (int i = 0; i < V; ++i) cs[i] = inside ? row[unit * V + i] : make_float2(quiet_nan(), quiet_nan());
+  for (uint32_t h = group; h < p.heads; h += p.head_groups) {
+    const uint32_t at = h * p.dim + unit * step;
+    R a = *reinterpret_cast<const R*>(x + at), b = *reinterpret_cast<const R*>(x + at + pair);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 y = rotate_pair(to_f32(a.v[i]), to_f32(b.v[i]), cs[i]);
+      a.v[i] = from_f32<T>(y.x);
+      b.v[i] = from_f32<T>(y.y);
+    }
+    *reinterpret_cast<R*>(out + at) = a;
+    *reinterpret_cast<R*>(out + at + pair) = b;
+  }
+}
+
+template <typename T, int V>
+cudaError_t rope_as(const LaunchEnv& env, RopeParams& p) {
+  const uint32_t half = p.rope.rotary / 2;
+  p.units = (p.rope.interleaved && V > 1 ? p.rope.rotary / V : half / V) + (p.dim - p.rope.rotary) / V;
+  p.head_groups = p.heads;
+  const uint64_t threads = static_cast<uint64_t>(p.tokens) * p.units * p.head_groups;
+  rope_kernel<T, V><<<static_cast<unsigned>((threads + kThreads - 1) / kThreads), kThreads, 0, env.stream>>>(p);
+  return cudaGetLastError();
+}
+
+// The longest run, up to 16 bytes, that divides the rotated part, the rest of a head and every address.
+template <typename T>
+cudaError_t rope_of(const LaunchEnv& env, RopeParams& p) {
+  const uint64_t part = p.rope.interleaved ? p.rope.rotary : p.rope.rotary / 2;
+  const uint64_t all = part | p.dim | p.x_stride | p.out_stride | (reinterpret_cast<uint64_t>(p.x) | reinterpret_cast<uint64_t>(p.out)) / sizeof(T);
+  if constexpr (sizeof(T) == 2)
+    if (all % 8 == 0) return rope_as<T, 8>(env, p);
+  if (all % 4 == 0) return rope_as<T, 4>(env, p);
+  if (all % 2 == 0) return rope_as<T, 2>(env, p);
+  return rope_as<T, 1>(env, p);
+}
+
+// ---- append and read ------------------------------------------------------------------------
+// D / 8 neighbouring lanes hold a row, eight values each.
+struct AppendParams {
+  Cache cache;
+  CacheBatch batch;
+  RopeTable rope;
+  const void *k, *v;
+  uint64_t k_stride, v_stride;
+};
+
+// The row number of the calling lanes: token-major, then K rows, then V rows of the heads.
+struct RowOf {
+  uint32_t token, head;
+  bool value;
+};
+__device__ __forceinline__ RowOf row_of(uint64_t row, uint32_t heads) {
+  RowOf r;
+  r.token = static_cast<uint32_t>(row / (2 * heads));
+  const uint32_t in = static_cast<uint32_t>(row % (2 * heads));
+  r.value = in >= heads;
+  r.head = r.value ? in - heads : in;
+  return r;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendParams p) {
+  constexpr int kLanes = D / 8;
+  const uint32_t lane = threadIdx.x % kLanes;
+  const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
+  const bool there = row < static_cast<uint64_t>(p.batch.tokens) * 2 * p.cache.kv_heads;
+  const RowOf r = row_of(there ? row : 0, p.cache.kv_heads);
+  const uint32_t seq = sequence_of(p.batch, r.token);
+  const Span span = span_of(p.batch, seq);
+  const int position = span.length - span.count + static_cast<int>(r.token) - span.first;
+  const bool mine = there && static_cast<int>(r.token) >= span.first && static_cast<int>(r.token) < span.first + span.count && position >= 0;
+  float x[8];
+  const T* from = r.value ? static_cast<const T*>(p.v) + r.token * p.v_stride : static_cast<const T*>(p.k) + r.token * p.k_stride;
+  from += r.head * D;
+  if (r.value) load8(from + lane * 8, x);
+  else load8_rotated(from, lane * 8, p.rope, position, x);
+  float low = x[0], high = x[0];
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    low = fminf(low, x[i]);
+    high = fmaxf(high, x[i]);
+    nan |= x[i] != x[i];
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o /= 2) {
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    nan |= __shfl_xor_sync(0xffffffffu, static_cast<int>(nan), o) != 0;
+  }
+  __half offset = __float2half_rn(low);
+  const float off = __half2float(offset);
+  __half scale = __float2half_rn(__fmul_rn(__fsub_rn(high, off), 1.0f / 15.0f));
+  float step = __half2float(scale);
+  const bool lost = nan || isinf(off) || isinf(step) || step != step;
+  if (lost) scale = offset = __ushort_as_half(0x7E00);
+  else if (!(step > 0.0f)) scale = __ushort_as_half(0);
+  uint32_t word = 0;
+  if (!lost && step > 0.0f) {
+    const float inv = __fdiv_rn(1.0f, step);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float u = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], off), inv)), 0.0f), 15.0f);
+      word |= static_cast<uint32_t>(u) << (4 * i);
+    }
+  }
+  if (!mine) return;
+  const uint32_t P = p.cache.page_tokens, slot = static_cast<uint32_t>(position) % P;
+  uint8_t* block = cache_block(p.cache, p.batch, seq, static_cast<uint32_t>(position) / P, r.head);
+  if (!block) return;
+  *reinterpret_cast<uint32_t*>(block + ((r.value ? P : 0u) + slot) * (D / 2) + lane * 4) = word;
+  if (lane == 0) *reinterpret_cast<__half2*>(block + static_cast<size_t>(P) * D + ((r.value ? P : 0u) + slot) * 4) = __halves2half2(scale, offset);
+}
+
+struct ReadParams {
+  Cache cache;
+  CacheBatch batch;
+  float *k, *v;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadParams p) {
+  constexpr int kLanes = D / 8;
+  const uint32_t lane = threadIdx.x % kLanes;
+  const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
+  if (row >= static_cast<uint64_t>(p.batch.tokens) * 2 * p.cache.kv_heads) return;
+  const RowOf r = row_of(row, p.cache.kv_heads);
+  const uint32_t seq = sequence_of(p.batch, r.token);
+  const Span span = span_of(p.batch, seq);
+  const int position = span.length - span.count + static_cast<int>(r.token) - span.first;
+  const bool mine = static_cast<int>(r.token) >= span.first && static_cast<int>(r.token) < span.first + span.count && position >= 0;
+  const uint32_t P = p.cache.page_tokens, slot = static_cast<uint32_t>(position) % P;
+  const uint8_t* block = mine ? cache_block(p.cache, p.batch, seq, static_cast<uint32_t>(position) / P, r.head) : nullptr;
+  float scale = quiet_nan(), off = quiet_nan();
+  uint32_t word = 0;
+  if (block) {
+    word = *reinterpret_cast<const uint32_t*>(block + ((r.value ? P : 0u) + slot) * (D / 2) + lane * 4);
+    const __half2 so = *reinterpret_cast<const __half2*>(block + static_cast<size_t>(P) * D + ((r.value ? P : 0u) + slot) * 4);
+    scale = __low2float(so);
+    off = __high2float(so);
+  }
+  float4 o[2];
+  float* f = reinterpret_cast<float*>(o);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = fmaf(static_cast<float>((word >> (4 * i)) & 15u), scale, off);
+  float4* to = reinterpret_cast<float4*>((r.value ? p.v : p.k) + (static_cast<size_t>(r.token) * p.cache.kv_heads + r.head) * D + lane * 8);
+  to[0] = o[0];
+  to[1] = o[1];
+}
+
+unsigned blocks_for(const Cache& cache, const CacheBatch& batch) {
+  const uint64_t threads = static_cast<uint64_t>(batch.tokens) * 2 * cache.kv_heads * (cache.head_dim / 8);
+  return static_cast<unsigned>((threads + kThreads - 1) / kThreads);
+}
+
+template <typename T>
+cudaError_t append_as(const LaunchEnv& env, const AppendParams& p) {
+  const unsigned grid = blocks_for(p.cache, p.batch);
+  switch (p.cache.head_dim) {
+    case 64: cache_append_kernel<T, 64><<<grid, kThreads, 0, env.stream>>>(p); break;
+    case 128: cache_append_kernel<T, 128><<<grid, kThreads, 0, env.stream>>>(p); break;
+    case 256: cache_append_kernel<T, 256><<<grid, kThreads, 0, env.stream>>>(p); break;
+    default: return cudaErrorInvalidValue;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_rope(const LaunchEnv& env, const void* x, int dtype, uint32_t tokens, uint32_t heads, uint32_t dim, uint64_t x_stride,
+                        const int* positions, const RopeTable& rope, void* out, uint64_t out_stride) {
+  RopeParams p = {x, out, x_stride, out_stride, positions, rope, tokens, heads, dim, 0, 0};
+  if (dtype == KQ_F32) return rope_of<float>(env, p);
+  if (dtype == KQ_F16) return rope_of<__half>(env, p);
+  return rope_of<__nv_bfloat16>(env, p);
+}
+
+cudaError_t launch_cache_append(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, const void* k, uint64_t k_stride,
+                                const void* v, uint64_t v_stride, int dtype, const RopeTable& rope) {
+  const AppendParams p = {cache, batch, rope, k, v, k_stride, v_stride};
+  if (dtype == KQ_F32) return append_as<float>(env, p);
+  if (dtype == KQ_F16) return append_as<__half>(env, p);
+  return append_as<__nv_bfloat16>(env, p);
+}
+
+cudaError_t launch_cache_read(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, float* k, float* v) {
+  const ReadParams p = {cache, batch, k, v};
+  const unsigned grid = blocks_for(cache, batch);
+  switch (cache.head_dim) {
+    case 64: cache_read_kernel<64><<<grid, kThreads, 0, env.stream>>>(p); break;
+    case 128: cache_read_kernel<128><<<grid, kThreads, 0, env.stream>>>(p); break;
+    case 256: cache_read_kernel<256><<<grid, kThreads, 0, env.stream>>>(p); break;
+    default: return cudaErrorInvalidValue;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace kq

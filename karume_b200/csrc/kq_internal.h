@@ -202,3 +202,40 @@ cudaError_t launch_linear_idot(cudaStream_t stream, const Weight& w, const int8_
                                const int* row_sum, const int* group_sum, const float* bias, float* out,
                                uint32_t m, int* launches);
 }  // namespace kq
+
+// ---- rotary positions, the paged 4-bit cache and attention over it (kq_cache.cu, kq_attend.cu) ----
+namespace kq {
+struct Cache {
+  uint8_t* pool = nullptr;  // [pages][kv_heads][block], a block as described in kq_cache.cuh
+  uint32_t pages = 0, page_tokens = 0, kv_heads = 0, head_dim = 0;
+};
+// The sequences of one call, all pointers on the device.
+struct CacheBatch {
+  const int* pages;    // [sequences, width] page numbers, in token order
+  const int* lengths;  // [sequences] tokens of each sequence, the new ones included
+  const int* starts;   // [sequences + 1] first row of each sequence's new tokens, or null: row b is sequence b's one new token
+  uint32_t sequences, width, tokens, most;  // most: no sequence has more new tokens
+};
+struct RopeTable {
+  const float2* table;  // [positions, rotary / 2] (cos, sin), or null: no rotation
+  uint32_t positions, rotary;
+  bool interleaved;
+};
+struct AttendArgs {
+  Cache cache;
+  CacheBatch batch;
+  RopeTable rope;
+  const void* q;   // [tokens] rows of [heads, head_dim], q_stride elements apart
+  void* out;       // the same with out_stride, of q's type
+  uint64_t q_stride, out_stride;
+  int dtype;
+  uint32_t heads, window;
+  float scale;
+};
+cudaError_t launch_rope(const LaunchEnv& env, const void* x, int dtype, uint32_t tokens, uint32_t heads, uint32_t dim, uint64_t x_stride,
+                        const int* positions, const RopeTable& rope, void* out, uint64_t out_stride);
+cudaError_t launch_cache_append(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, const void* k, uint64_t k_stride,
+                                const void* v, uint64_t v_stride, int dtype, const RopeTable& rope);
+cudaError_t launch_cache_read(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, float* k, float* v);
+cudaError_t launch_attend(const LaunchEnv& env, const AttendArgs& args, int* launches);
+}  // namespace kq

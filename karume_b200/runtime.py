@@ -95,6 +95,71 @@ class Weight:
             self.handle = 0
 
 
+@dataclass
+class Rope:
+    """Rotation angles: table f32 CUDA [positions, rotary / 2, 2] of (cos, sin) (rope_table makes one); pairs are
+    (i, i + rotary / 2) of a head, or (2 i, 2 i + 1) with interleaved."""
+    table: object
+    interleaved: bool = False
+
+    def __post_init__(self):
+        t = self.table
+        if t.dtype != _torch().float32 or not t.is_cuda or t.dim() != 3 or t.shape[2] != 2 or not t.is_contiguous():
+            raise KqError(2, "the rotation table is a contiguous CUDA f32 tensor [positions, rotary / 2, 2]")
+        self.positions, self.rotary = int(t.shape[0]), 2 * int(t.shape[1])
+        self.args = (t.data_ptr(), self.positions, self.rotary, 1 if self.interleaved else 0)
+
+
+class CacheBatch:
+    """The sequences of a call: pages i32 CUDA [sequences, width] (page numbers in token order), lengths i32
+    [sequences] (the new tokens included) and starts i32 [sequences + 1] (rows of each sequence's new tokens; None: one
+    each).  tokens is the number of rows, most a bound of any sequence's new tokens; both are host numbers, the
+    tensors are read on the device at each launch and may change between replays of a recorded step."""
+
+    def __init__(self, pages, lengths, starts=None, tokens: int = 0, most: int = 0):
+        torch = _torch()
+        for name, t, dims in (("pages", pages, 2), ("lengths", lengths, 1), ("starts", starts, 1)):
+            if t is not None and (t.dtype != torch.int32 or not t.is_cuda or t.dim() != dims or not t.is_contiguous()):
+                raise KqError(2, f"{name} must be a contiguous CUDA int32 tensor of {dims} dimension(s)")
+        self.sequences, self.width = (int(n) for n in pages.shape)
+        if lengths.numel() != self.sequences or (starts is not None and starts.numel() != self.sequences + 1):
+            raise KqError(2, f"{self.sequences} sequences need as many lengths and one more starts")
+        if starts is not None and tokens <= 0:
+            raise KqError(2, "with starts, tokens says how many rows there are")
+        self.pages, self.lengths, self.starts = pages, lengths, starts
+        self.tokens = int(tokens) if starts is not None else self.sequences
+        self.most = int(most) if starts is not None else 1
+        self.args = (self.sequences, pages.data_ptr(), self.width, lengths.data_ptr(), starts.data_ptr() if starts is not None else 0,
+                     self.tokens)
+
+
+@dataclass
+class KvCache:
+    """Pages of keys and values in 4 bits: pool uint8 CUDA [pages, kv_heads, page_tokens * (head_dim + 8)] and its handle."""
+    gpu: "Gpu"
+    handle: int
+    pool: object
+    pages: int
+    page_tokens: int
+    kv_heads: int
+    head_dim: int
+
+    def free(self) -> None:
+        if self.handle:
+            self.gpu._check(L.kq_cache_free(self.gpu._ctx, self.handle))
+            self.handle = 0
+
+
+_NO_ROPE = (0, 0, 0, 0)
+
+
+def _rows(t, heads: int, dim: int, name: str):
+    """(address, elements between tokens) of a CUDA tensor [tokens, heads, dim] whose tokens may be strided."""
+    if not t.is_cuda or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+        raise KqError(2, f"{name} must be a CUDA tensor [tokens, {heads}, {dim}] with heads and values dense")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
 class Gpu:
     """One CUDA device = one libkq context (the reference's GpuContext)."""
 
@@ -347,6 +412,69 @@ class Gpu:
         out = np.empty(x.shape[:-1] + (weight.n,), np.float32)
         self._check(L.kq_linear_host(self._ctx, weight.handle, x.ctypes.data, _NP_DTYPES[x.dtype],
                                      bias.data_ptr(), out.ctypes.data, m))
+        return out
+
+    # -- the attention half of a decoder layer --------------------------------------------------
+    def rope(self, x, positions, rope: Rope, out=None):
+        """x [tokens, heads, head_dim] (f32 / f16 / bf16, tokens may be strided) rotated to positions (CUDA int32 [tokens])."""
+        torch = _torch()
+        tokens, heads, dim = x.shape
+        px, stride = _rows(x, heads, dim, "x")
+        if positions.dtype != torch.int32 or not positions.is_cuda or positions.numel() != tokens or not positions.is_contiguous():
+            raise KqError(2, f"positions must be a contiguous CUDA int32 tensor [{tokens}]")
+        if out is None:
+            out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+        elif out.dtype != x.dtype or out.shape != x.shape:
+            raise KqError(2, "out must have x's type and shape")
+        po, out_stride = _rows(out, heads, dim, "out")
+        self._check(L.kq_rope(self._ctx, px, _tensor_dtype_code(x), tokens, heads, dim, stride, positions.data_ptr(), *rope.args, po, out_stride))
+        return out
+
+    def kv_cache(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, pool=None) -> KvCache:
+        """Pages for keys and values in 4 bits; pool: the caller's uint8 CUDA memory of kq_cache_bytes() bytes (None: allocated)."""
+        torch = _torch()
+        need = int(L.kq_cache_bytes(pages, page_tokens, kv_heads, head_dim))
+        if pool is None:
+            pool = torch.zeros((pages, kv_heads, need // max(1, pages * kv_heads)), dtype=torch.uint8, device=self.device)
+        if pool.dtype != torch.uint8 or not pool.is_cuda or not pool.is_contiguous() or pool.numel() < need:
+            raise KqError(2, f"the pool must be {need} bytes of contiguous CUDA uint8 memory")
+        handle = ctypes.c_uint64(0)
+        self._check(L.kq_cache_create(self._ctx, pool.data_ptr(), pages, page_tokens, kv_heads, head_dim, ctypes.byref(handle)))
+        return KvCache(self, handle.value, pool, pages, page_tokens, kv_heads, head_dim)
+
+    def cache_append(self, cache: KvCache, k, v, batch: CacheBatch, rope: "Rope | None" = None) -> None:
+        """Stores the new tokens' keys (rotated on the way) and values [tokens, kv_heads, head_dim] in the cache's pages."""
+        if k.shape[0] != batch.tokens or v.shape[0] != batch.tokens or k.dtype != v.dtype:
+            raise KqError(2, f"k and v must be [{batch.tokens}, {cache.kv_heads}, {cache.head_dim}] of one type")
+        pk, k_stride = _rows(k, cache.kv_heads, cache.head_dim, "k")
+        pv, v_stride = _rows(v, cache.kv_heads, cache.head_dim, "v")
+        self._check(L.kq_cache_append(self._ctx, cache.handle, pk, k_stride, pv, v_stride, _tensor_dtype_code(k), *batch.args,
+                                      *(rope.args if rope is not None else _NO_ROPE)))
+
+    def cache_read(self, cache: KvCache, batch: CacheBatch):
+        """(k, v) f32 [tokens, kv_heads, head_dim]: what the cache holds for the new tokens of `batch`."""
+        torch = _torch()
+        k, v = (torch.empty((batch.tokens, cache.kv_heads, cache.head_dim), dtype=torch.float32, device=self.device) for _ in range(2))
+        self._check(L.kq_cache_read(self._ctx, cache.handle, *batch.args, k.data_ptr(), v.data_ptr()))
+        return k, v
+
+    def cache_attention(self, cache: KvCache, q, batch: CacheBatch, scale: "float | None" = None, window: int = 0,
+                        rope: "Rope | None" = None, out=None):
+        """Causal attention of q [tokens, heads, head_dim] (f32 / f16 / bf16, rotated on the way) over each sequence's keys
+        in the cache, the last `window` of them if given; scale defaults to head_dim^-0.5.  Returns q's type."""
+        torch = _torch()
+        heads, dim = int(q.shape[1]), cache.head_dim
+        if q.shape[0] != batch.tokens:
+            raise KqError(2, f"q must have {batch.tokens} rows")
+        pq, q_stride = _rows(q, heads, dim, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.dtype != q.dtype or out.shape != q.shape:
+            raise KqError(2, "out must have q's type and shape")
+        po, out_stride = _rows(out, heads, dim, "out")
+        self._check(L.kq_cache_attention(self._ctx, cache.handle, pq, q_stride, _tensor_dtype_code(q), heads, *batch.args, batch.most,
+                                         float(scale if scale is not None else dim ** -0.5), int(window),
+                                         *(rope.args if rope is not None else _NO_ROPE), po, out_stride))
         return out
 
     # -- replayable plans -------------------------------------------------------
