@@ -1,7 +1,32 @@
-// Attention over the paged 4-bit cache (layout in kq_cache.cuh):
-//   out = sum_j softmax_j(scale q . k_j) v_j,  k_j = u_j s_j + o_j,  v_j likewise
-// A block takes one query row (token and head): a thread per key for the scores, a running maximum and sum, a thread per
-// value for the output.
+// Attention over the paged 4-bit cache (layout in kq_cache.cuh) for few query rows a sequence: single tokens, drafts.
+//
+//   out = sum_j softmax_j(scale q . k_j) v_j,   k_j = u_j s_j + o_j, v_j likewise, codes u in 0..15
+//
+// The cache is read once, so the floor is its bytes; what the kernel is built around is that a code must cost few
+// instructions on its way into the tensor cores.  (w & 0x000F000F) of a word of eight codes IS a pair of binary16 numbers,
+// the subnormals u 2^-24, and (w & 0x00F000F0) the pair u 2^-20: no conversion, the powers of two are taken out of q and of
+// the output.  Scores and outputs are built transposed, keys and values as the M side of mma.m16n8k16:
+//
+//   S^T [16 tokens, 8 columns] += K [16, 16 dims] q^T      a thread's words of a token are its A fragments
+//   O^T [16 dims, 8 columns]   += V^T [16, 16 tokens] P^T  the words of two tokens, joined by two PRMTs
+//
+// A column is one query row (query and head of the kv head's group) for 16-bit queries; f32 queries are two binary16
+// parts in neighbouring columns, and so are their weights, whose products are added in f32 (22 bits or more).  The weights
+// get from S^T's fragment to the B fragment of P^T by one movmatrix a 8 x 8 block, nothing passes through shared memory.
+//
+//   score    s_j = scale log2(e) (s_j (q . u_j) + o_j sum q)            (base 2, f32)
+//   weight   p_j = 2^(s_j - M + 6), and P = p_j s'_j (s' the value's scale) is what enters the tensor core.  M follows the
+//            largest s_j + log2 of s'_j's binade, and moves only when a weight would grow past 2^8 of it: P fits binary16
+//            with its full precision wherever it matters, whatever the size of the values.
+//   output   sum_j P_j (u'_j - 7.5) + sum_j p_j (o'_j + 7.5 s'_j): codes around zero, because sums of many uncentred
+//            ones cancel (70001 keys: 1e-3 of the result was lost); f32 queries add each 32 tokens' sums in registers,
+//            the tensor core's own chain would truncate.
+//
+// Work: every (sequence, kv head, block of query rows) is a run of tiles of 32 tokens.  All runs of the call, laid end to
+// end, are cut into equal ranges, one for each CTA (one CTA an SM), by what the lengths say on the device: ragged batches
+// and one long sequence fill the machine alike, and a recorded launch follows the lengths.  The warps of a CTA take the
+// tiles in turn, each with a ring of its own that bulk copies fill (page by page: K codes, V codes, scales).  A run that
+// several CTAs share leaves partial sums in the scratch; the last CTA to finish joins them in order.
 #include <algorithm>
 
 #include "kq_cache.cuh"
@@ -9,129 +34,745 @@
 namespace kq {
 namespace {
 
-constexpr int kAttendThreads = 128;
+constexpr int kTile = 32;            // tokens a warp takes at a time
+constexpr uint32_t kFewWaitLimit = 1u << 22;
+constexpr int kFewTimeout = 40;      // status word: a copy of the cache did not arrive
 
 template <typename T>
-__device__ __forceinline__ void store_as(T* p, float v);
+struct Parts {
+  static constexpr int n = 1;  // 16-bit queries enter the tensor core as they are
+};
 template <>
-__device__ __forceinline__ void store_as<float>(float* p, float v) { *p = v; }
-template <>
-__device__ __forceinline__ void store_as<__half>(__half* p, float v) { *p = __float2half_rn(v); }
-template <>
-__device__ __forceinline__ void store_as<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+struct Parts<float> {
+  static constexpr int n = 2;
+};
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttendThreads) attend_row_kernel(const AttendArgs a) {
-  constexpr int kPer = (D + kAttendThreads - 1) / kAttendThreads;
-  __shared__ float q_s[D];
-  __shared__ float p_s[kAttendThreads], pv_s[kAttendThreads];  // weight, and weight * scale of the value
-  __shared__ const uint8_t* v_s[kAttendThreads];
-  __shared__ float part[kAttendThreads / 32];
-  const uint32_t tid = threadIdx.x, token = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  const uint32_t kv_head = head / (a.heads / a.cache.kv_heads);
-  const uint32_t seq = sequence_of(a.batch, token);
-  const Span span = span_of(a.batch, seq);
-  const int position = span.length - span.count + static_cast<int>(token) - span.first;
-  const bool mine = static_cast<int>(token) >= span.first && static_cast<int>(token) < span.first + span.count;
-  T* out = static_cast<T*>(a.out) + token * a.out_stride + head * D;
-  if (!mine || position < 0) {
-    for (uint32_t d = tid; d < D; d += kAttendThreads) store_as(out + d, 0.0f);
-    return;
+// ---- shapes of one instance -------------------------------------------------------------------
+template <typename T, int D, int NT>
+struct Few {
+  static constexpr int kParts = Parts<T>::n;
+  static constexpr int kRows = 8 * NT / kParts;      // query rows of a block
+  static constexpr int kWarps = NT == 1 && D <= 128 ? 16 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kStages = 2;
+  static constexpr int kSteps = D / 16;              // k-steps of S^T
+  static constexpr int kWords = D / 32;              // words of a token in a thread (keys)
+  static constexpr int kVWords = D / 64;             // ... (values)
+  static constexpr int kTileBytes = kTile * (D + 8);
+  static constexpr int kMergeWarps = 4;              // warps whose sums are added in one round
+  static constexpr bool kQInRegisters = NT * kSteps <= 16;
+  static constexpr int kPartFloats = kRows * (D + 2);  // a partial result in the scratch: sums, M, l
+
+  static constexpr int kRing = 0;
+  static constexpr int kMerge = kRing + kWarps * kStages * kTileBytes;
+  static constexpr int kQFrag = kMerge + kMergeWarps * kRows * D * 4;  // [NT][kSteps][32] x 8 B
+  static constexpr int kRowConst = kQFrag + NT * kSteps * 32 * 8;      // factor, offset, last key, first key of each row
+  static constexpr int kWarpStat = kRowConst + kRows * 16;             // [kWarps][kRows] x (M, l, centre sum)
+  static constexpr int kScan = kWarpStat + kWarps * kRows * 12 + 8;    // [kThreads] x 8 B, and what the scan found
+  static constexpr int kBars = kScan + kThreads * 8 + 32;
+  static constexpr int kMisc = kBars + kWarps * kStages * 8;
+  static constexpr int kSmem = kMisc + 16;
+};
+
+struct FewParams {
+  AttendArgs a;
+  uint32_t group;        // query heads of a kv head
+  float* parts;          // [2 * grid][kPartFloats]
+  unsigned int* counters;  // [grid], zero between launches
+  int* status;
+  uint32_t least;        // tiles a CTA should have at least
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(__half lo, __half hi) {
+  return static_cast<uint32_t>(__half_as_ushort(lo)) | (static_cast<uint32_t>(__half_as_ushort(hi)) << 16);
+}
+__device__ __forceinline__ uint32_t hfma2_u(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hadd2_u(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4]);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+template <>
+__device__ __forceinline__ void store4<__half>(__half* p, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_half2(__float2half_rn(v[0]), __float2half_rn(v[1])), pack_half2(__float2half_rn(v[2]), __float2half_rn(v[3])));
+}
+template <>
+__device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const float (&v)[4]) {
+  __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+}
+
+// ---- the work list --------------------------------------------------------------------------
+// A sequence's runs: `units` = kv heads x blocks of rows, each of `tiles` tiles from tile_lo on.
+struct Runs {
+  Span span;
+  int tile_lo, tiles;
+  uint32_t blocks, units;
+};
+__device__ __forceinline__ Runs runs_of(const FewParams& p, uint32_t b, int rows) {
+  Runs r;
+  r.span = span_of(p.a.batch, b);
+  const int first = r.span.length - r.span.count;  // position of the first query
+  const int window = static_cast<int>(min(p.a.window, 0x7fffffffu));
+  const int from = window && first + 1 > window ? first + 1 - window : 0;
+  r.tile_lo = from / kTile;
+  r.tiles = r.span.length > 0 ? (r.span.length - 1) / kTile + 1 - r.tile_lo : 1;  // an idle sequence's rows are written too
+  r.blocks = (static_cast<uint32_t>(r.span.count) * p.group + rows - 1) / rows;
+  r.units = r.blocks * p.a.cache.kv_heads;
+  return r;
+}
+
+// A place in the list: tile `off` of unit `unit` of sequence b.
+struct Walk {
+  uint32_t b, unit;
+  unsigned long long off;
+  Runs runs;
+};
+__device__ __forceinline__ void settle(Walk& w, const FewParams& p, int rows) {  // carry off into units and sequences
+  while (w.b < p.a.batch.sequences) {
+    if (w.unit < w.runs.units) {
+      if (w.off < static_cast<unsigned>(w.runs.tiles)) return;
+      const unsigned long long skip = min(w.off / static_cast<unsigned>(w.runs.tiles), static_cast<unsigned long long>(w.runs.units - w.unit));
+      w.unit += static_cast<uint32_t>(skip);
+      w.off -= skip * static_cast<unsigned>(w.runs.tiles);
+      if (w.unit < w.runs.units) continue;
+    }
+    w.unit = 0;
+    if (++w.b < p.a.batch.sequences) w.runs = runs_of(p, w.b, rows);
   }
-  if (tid < D / 8) {
-    float v[8];
-    load8_rotated(static_cast<const T*>(a.q) + token * a.q_stride + head * D, tid * 8, a.rope, position, v);
-    for (int i = 0; i < 8; ++i) q_s[tid * 8 + i] = v[i] * (a.scale * 1.4426950408889634f);
+}
+
+// Keys that the rows of a block see: from the first row's first to the last row's last.
+struct Keys {
+  int first, last;       // of any row
+  int first_all, last_all;  // of all rows
+};
+__device__ __forceinline__ Keys keys_of(const FewParams& p, const Runs& r, uint32_t block, int rows) {
+  const int q0 = static_cast<int>(block * rows / p.group);
+  const int q1 = min(static_cast<int>(((block + 1) * rows - 1) / p.group), r.span.count - 1);
+  const int base = r.span.length - r.span.count, window = static_cast<int>(min(p.a.window, 0x7fffffffu));
+  Keys k;
+  k.last = base + q1;
+  k.last_all = base + q0;
+  k.first = window && base + q0 + 1 > window ? base + q0 + 1 - window : 0;
+  k.first_all = window && base + q1 + 1 > window ? base + q1 + 1 - window : 0;
+  return k;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(const __grid_constant__ FewParams p) {
+  using F = Few<T, D, NT>;
+  constexpr int kRows = F::kRows, kParts = F::kParts, kWarps = F::kWarps, kStages = F::kStages;
+  constexpr int kPer = kParts == 1 ? 2 : 1;  // query rows of a thread in one n-tile
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  float* merge = reinterpret_cast<float*>(smem + F::kMerge);
+  uint2* q_frag = reinterpret_cast<uint2*>(smem + F::kQFrag);
+  float4* row_const = reinterpret_cast<float4*>(smem + F::kRowConst);
+  float* warp_stat = reinterpret_cast<float*>(smem + F::kWarpStat);
+  unsigned long long* scan = reinterpret_cast<unsigned long long*>(smem + F::kScan);
+  unsigned long long* found = scan + F::kThreads;  // sequence, tiles in front of it
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F::kMisc);
+  volatile unsigned int* arrived = reinterpret_cast<volatile unsigned int*>(smem + F::kMisc + 4);
+  const uint32_t bars = smem_u32(smem + F::kBars) + warp * kStages * 8;
+  if (lane < kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + lane * 8) : "memory");
+  if (tid == 0) *abort_flag = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+
+  // ---- this CTA's range of the list --------------------------------------------------------------
+  const uint32_t sequences = p.a.batch.sequences, each = (sequences + F::kThreads - 1) / F::kThreads;
+  unsigned long long mine = 0;
+  for (uint32_t b = tid * each; b < min((tid + 1) * each, sequences); ++b) {
+    const Runs r = runs_of(p, b, kRows);
+    mine += static_cast<unsigned long long>(r.tiles) * r.units;
+  }
+  unsigned long long upto = mine;  // inclusive sum over the threads
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= static_cast<uint32_t>(o)) upto += v;
+  }
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  unsigned long long total = 0;
+  for (int i = 0; i < kWarps; ++i) {
+    if (static_cast<uint32_t>(i) < warp) upto += scan[i];
+    total += scan[i];
+  }
+  // rows that belong to no sequence are zero
+  if (p.a.batch.starts) {
+    const int head_rows = min(max(p.a.batch.starts[0], 0), static_cast<int>(p.a.batch.tokens));
+    const int tail = min(max(p.a.batch.starts[sequences], 0), static_cast<int>(p.a.batch.tokens));
+    const int extra = head_rows + static_cast<int>(p.a.batch.tokens) - max(tail, head_rows);
+    for (int i = blockIdx.x; i < extra; i += gridDim.x) {
+      const int row = i < head_rows ? i : max(tail, head_rows) + i - head_rows;
+      T* out = static_cast<T*>(p.a.out) + row * p.a.out_stride;
+      const float zero[4] = {};
+      for (uint32_t d = tid * 4; d < p.a.heads * D; d += F::kThreads * 4) store4(out + d, zero);
+    }
+  }
+  const unsigned long long ranges = min(static_cast<unsigned long long>(gridDim.x), max(total / p.least, 1ull));
+  const unsigned long long per = max((total + ranges - 1) / ranges, 1ull);
+  const unsigned long long begin = min(blockIdx.x * per, total), end = min(begin + per, total);
+  if (begin >= end) return;
+  if (upto - mine <= begin && begin < upto) {
+    found[0] = tid * each;
+    found[1] = upto - mine;
   }
   __syncthreads();
-  const int from = a.window && position + 1 > static_cast<int>(a.window) ? position + 1 - static_cast<int>(a.window) : 0;
-  const uint32_t P = a.cache.page_tokens;
-  float top = -INFINITY, total = 0.0f, o[kPer] = {}, off_sum = 0.0f;
-  for (int at = from; at <= position; at += kAttendThreads) {
-    const int key = at + static_cast<int>(tid);
-    float s = -INFINITY, v_scale = 0.0f, v_off = 0.0f;
-    const uint8_t* v_row = nullptr;
-    if (key <= position) {
-      const uint8_t* block = cache_block(a.cache, a.batch, seq, static_cast<uint32_t>(key) / P, kv_head);
-      if (block) {
-        const uint32_t slot = static_cast<uint32_t>(key) % P;
-        const uint32_t* row = reinterpret_cast<const uint32_t*>(block + static_cast<size_t>(slot) * (D / 2));
-        float dot = 0.0f, sum = 0.0f;
-        for (int w = 0; w < D / 8; ++w) {
-          const uint32_t word = row[w];
-          for (int i = 0; i < 8; ++i) {
-            dot = fmaf(q_s[w * 8 + i], static_cast<float>((word >> (4 * i)) & 15u), dot);
-            sum += q_s[w * 8 + i];
+  Walk at;
+  at.b = static_cast<uint32_t>(found[0]);
+  at.unit = 0;
+  at.off = begin - found[1];
+  at.runs = runs_of(p, at.b, kRows);
+  settle(at, p, kRows);
+
+  // ---- copies: the warp's tiles, a ring's length ahead --------------------------------------------
+  const uint32_t ring = smem_u32(smem + F::kRing) + warp * kStages * F::kTileBytes;
+  uint8_t* const ring_ptr = smem + F::kRing + warp * kStages * F::kTileBytes;
+  Walk ahead = at;
+  ahead.off += warp;
+  unsigned long long ahead_at = begin + warp;
+  if (ahead_at < end) settle(ahead, p, kRows);
+  uint32_t issued = 0, used = 0;
+  auto issue_next = [&]() {
+    for (; ahead_at < end;) {
+      const Keys keys = keys_of(p, ahead.runs, ahead.unit % ahead.runs.blocks, kRows);
+      const int first = (ahead.runs.tile_lo + static_cast<int>(ahead.off)) * kTile;
+      const bool needed = first <= keys.last && first + kTile > keys.first;
+      if (needed) {
+        const uint32_t stage = issued % kStages, bar = bars + stage * 8, to = ring + stage * F::kTileBytes;
+        const uint32_t P = p.a.cache.page_tokens, run = min(P, static_cast<uint32_t>(kTile));  // tokens of a piece
+        const uint32_t pieces = kTile / run;
+        const bool piece = lane < pieces && first + static_cast<int>(lane * run) <= keys.last;
+        const uint32_t key = static_cast<uint32_t>(first) + lane * run, slot = key % P;
+        const uint8_t* block = piece ? cache_block(p.a.cache, p.a.batch, ahead.b, key / P, ahead.unit / ahead.runs.blocks) : nullptr;
+        const uint32_t have = __ballot_sync(0xffffffffu, block != nullptr), lost = __ballot_sync(0xffffffffu, piece && !block);
+        if (lost) {  // no such page: what it would hold is NaN
+          uint32_t* params = reinterpret_cast<uint32_t*>(ring_ptr + stage * F::kTileBytes + kTile * D);
+          for (uint32_t i = lane; i < kTile; i += 32)
+            if (lost >> (i / run) & 1) params[i] = params[kTile + i] = 0x7E007E00u;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(have) * run * (D + 8)) : "memory");
+        __syncwarp();
+        if (block) {
+          const uint32_t sizes[2] = {run * (D / 2), run * 4};
+          const uint8_t* from[4] = {block + slot * (D / 2), block + (P + slot) * (D / 2), block + P * D + slot * 4, block + P * D + (P + slot) * 4};
+          const uint32_t dst[4] = {to + lane * run * (D / 2), to + (kTile + lane * run) * (D / 2), to + kTile * D + lane * run * 4,
+                                   to + kTile * D + (kTile + lane * run) * 4};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(dst[i]), "l"(from[i]), "r"(sizes[i / 2]), "r"(bar) : "memory");
+        }
+        ++issued;
+      }
+      ahead_at += kWarps;
+      ahead.off += kWarps;
+      if (ahead_at < end) settle(ahead, p, kRows);
+      if (needed) return;
+    }
+  };
+  __syncwarp();
+  for (int i = 0; i < kStages; ++i) issue_next();
+
+  const uint32_t odd = t & 1;  // the order of a thread's tokens in a pair of rows: neighbouring rows fall into different banks
+  const uint32_t token_g = g ^ ((g >> 1) & 1);
+  const uint32_t token_t0 = 2 * t + odd, token_t1 = 2 * t + 1 - odd;
+  constexpr uint32_t kCentre0 = 0x800F800Fu;  // -15 2^-24, twice: 2 u - 15
+  constexpr uint32_t kCentre1 = 0x80788078u;  // -7.5 2^-20, twice
+
+  // ---- run by run --------------------------------------------------------------------------------
+  for (unsigned long long pos = begin; pos < end;) {
+    const unsigned long long left = static_cast<unsigned long long>(at.runs.tiles) - at.off;
+    const unsigned long long stop = min(end, pos + left);
+    const uint32_t kv_head = at.unit / at.runs.blocks, block = at.unit % at.runs.blocks;
+    const int q_rows = at.runs.span.count * static_cast<int>(p.group);
+    const int base = at.runs.span.length - at.runs.span.count;
+    const Keys keys = keys_of(p, at.runs, block, kRows);
+
+    // queries: rotated, scaled to binary16's range by a power of two, in the order of the B fragments
+    for (int r = static_cast<int>(warp); r < kRows; r += kWarps) {
+      const int row = static_cast<int>(block) * kRows + r, query = row / static_cast<int>(p.group);
+      const int head = static_cast<int>(kv_head * p.group) + row % static_cast<int>(p.group);
+      const bool there = row < q_rows;
+      float v[8] = {};
+      if (there && lane < D / 8)
+        load8_rotated(static_cast<const T*>(p.a.q) + static_cast<size_t>(at.runs.span.first + query) * p.a.q_stride + static_cast<size_t>(head) * D,
+                      lane * 8, p.a.rope, base + query, v);
+      float big = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        big = fmaxf(big, fabsf(v[i]));
+        sum += v[i];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      sum = warp_sum(sum);
+      // 2^(13 - exponent of the largest): parts below 2^14, and their sixteenth is still a normal number where it counts
+      const int e = static_cast<int>(__float_as_uint(big) >> 23);
+      const int up = big > 0.0f && e < 255 ? min(max(140 - e, -100), 120) : 0;
+      const float lift = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+      if (lane < D / 8) {
+        // word W = lane of a key lies with thread tt as its word ww
+        const uint32_t tt = D == 64 ? lane / 2 : lane % 16 / 4, ww = D == 64 ? lane % 2 : lane / 16 * 4 + lane % 4;
+        __half hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = v[i] * ((i & 1) ? lift * 0.0625f : lift);
+          hi[i] = __float2half_rn(x);
+          lo[i] = __float2half_rn(x - __half2float(hi[i]));
+        }
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          const uint32_t col = r * kParts + part, n = col / 8, c = col % 8;
+          const __half* h = part ? lo : hi;
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            q_frag[(n * F::kSteps + 2 * ww + half) * 32 + c * 4 + tt] =
+                make_uint2(pack_half2(h[2 * half], h[2 * half + 4]), pack_half2(h[2 * half + 1], h[2 * half + 5]));
+        }
+      }
+      if (lane == 0) {
+        const float factor = p.a.scale * 1.4426950408889634f;
+        const int last = there ? base + query : -1, window = static_cast<int>(min(p.a.window, 0x7fffffffu));
+        const int from = window && last + 1 > window ? last + 1 - window : 0;
+        // the accumulators hold 2^(up - 24) q . u
+        row_const[r] = make_float4(factor * exp2f(static_cast<float>(24 - up)), factor * sum, __int_as_float(last), __int_as_float(from));
+      }
+    }
+    __syncthreads();
+    uint2 bq[F::kQInRegisters ? NT : 1][F::kQInRegisters ? F::kSteps : 1];
+    if constexpr (F::kQInRegisters) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int s = 0; s < F::kSteps; ++s) bq[n][s] = q_frag[(n * F::kSteps + s) * 32 + lane];
+    }
+    // a thread's query rows in n-tile n: n * 8 / parts + t * kPer + i
+    float factor[NT][kPer], offset[NT][kPer];
+    int last[NT][kPer], from[NT][kPer];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float4 c = row_const[n * (8 / kParts) + t * kPer + i];
+        factor[n][i] = c.x;
+        offset[n][i] = c.y;
+        last[n][i] = __float_as_int(c.z);
+        from[n][i] = __float_as_int(c.w);
+      }
+    float M[NT][kPer], l[NT][kPer] = {}, centre[NT][kPer] = {};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) M[n][i] = -INFINITY;
+    // f32 queries: sums of a thread's dims for its one row; 16-bit ones: the accumulators (two rows)
+    float O[NT][F::kVWords * 4][2 * kPer] = {};
+
+    for (unsigned long long f = pos + (warp + kWarps - static_cast<uint32_t>((pos - begin) % kWarps)) % kWarps; f < stop; f += kWarps) {
+      const int first = (at.runs.tile_lo + static_cast<int>(at.off + (f - pos))) * kTile;
+      if (first > keys.last || first + kTile <= keys.first) continue;
+      const uint32_t stage = used % kStages, parity = used / kStages & 1;
+      {
+        const uint32_t bar = bars + stage * 8;
+        uint32_t done = 0;
+        for (uint32_t spin = 0; spin < kFewWaitLimit && !done; ++spin) {
+          asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                       : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+          if (!done && (spin & 1023u) == 1023u && *abort_flag) break;
+        }
+        if (!done) {
+          *abort_flag = 1;
+          *reinterpret_cast<volatile int*>(p.status) = kFewTimeout;
+        }
+      }
+      __syncwarp();
+      const uint8_t* tile = ring_ptr + stage * F::kTileBytes;
+      const bool whole = first >= keys.first_all && first + kTile - 1 <= keys.last_all;
+      float s[2][NT][kPer][2];  // [subtile][..][row][token half]
+      uint32_t vp[2][2];        // the values' (scale, offset) of the thread's tokens
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        float acc[NT][4] = {};
+        const uint8_t* row0 = tile + (sub * 16 + token_g) * (D / 2);
+        const uint8_t* row1 = row0 + 8 * (D / 2);
+        uint32_t x0[F::kWords], x1[F::kWords];
+        if constexpr (D == 64) {
+          *reinterpret_cast<uint2*>(x0) = *reinterpret_cast<const uint2*>(row0 + t * 8);
+          *reinterpret_cast<uint2*>(x1) = *reinterpret_cast<const uint2*>(row1 + t * 8);
+        } else {
+#pragma unroll
+          for (int i = 0; i < F::kWords / 4; ++i) {
+            *reinterpret_cast<uint4*>(x0 + 4 * i) = *reinterpret_cast<const uint4*>(row0 + i * 64 + t * 16);
+            *reinterpret_cast<uint4*>(x1 + 4 * i) = *reinterpret_cast<const uint4*>(row1 + i * 64 + t * 16);
           }
         }
-        const __half2* par = reinterpret_cast<const __half2*>(block + static_cast<size_t>(P) * D);
-        const __half2 ks = par[slot], vs = par[P + slot];
-        s = fmaf(dot, __low2float(ks), sum * __high2float(ks));
-        v_scale = __low2float(vs);
-        v_off = fmaf(7.5f, v_scale, __high2float(vs));  // of codes around zero: sums of many values that cancel keep their bits
-        v_row = block + static_cast<size_t>(P + slot) * (D / 2);
+#pragma unroll
+        for (int w = 0; w < F::kWords; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t a = half ? x0[w] >> 8 : x0[w], b = half ? x1[w] >> 8 : x1[w];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint2 bb = F::kQInRegisters ? bq[F::kQInRegisters ? n : 0][F::kQInRegisters ? 2 * w + half : 0]
+                                                : q_frag[(n * F::kSteps + 2 * w + half) * 32 + lane];
+              mma16816(acc[n], a & 0x000F000Fu, b & 0x000F000Fu, a & 0x00F000F0u, b & 0x00F000F0u, bb.x, bb.y);
+            }
+          }
+        const uint32_t* params = reinterpret_cast<const uint32_t*>(tile + kTile * D) + sub * 16 + token_g;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t kp = params[half * 8];
+          vp[sub][half] = params[kTile + half * 8];
+          const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&kp));
+          const int key = first + sub * 16 + half * 8 + static_cast<int>(token_g);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const float dot = kParts == 2 ? acc[n][2 * half] + acc[n][2 * half + 1] : acc[n][2 * half + i];
+              float v = fmaf(dot, so.x * factor[n][i], so.y * offset[n][i]);
+              if (!whole && (key > last[n][i] || key < from[n][i])) v = -INFINITY;
+              s[sub][n][i][half] = v;
+            }
+        }
+      }
+      // M: the largest score plus its value's binade (never less than log2 of the scale)
+      float binade[2][2];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) binade[sub][half] = static_cast<float>(max(static_cast<int>(vp[sub][half] >> 10 & 31u), 1) - 14);
+      bool more = false;
+      float top[NT][kPer];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          top[n][i] = fmaxf(fmaxf(s[0][n][i][0] + binade[0][0], s[0][n][i][1] + binade[0][1]),
+                            fmaxf(s[1][n][i][0] + binade[1][0], s[1][n][i][1] + binade[1][1]));
+          more |= top[n][i] > M[n][i] + 8.0f;
+        }
+      if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            float m = top[n][i];
+#pragma unroll
+            for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            m = fmaxf(m, M[n][i]);
+            const float keep = m == -INFINITY ? 1.0f : exp2_fast(M[n][i] - m);
+            M[n][i] = m;
+            l[n][i] *= keep;
+            centre[n][i] *= keep;
+#pragma unroll
+            for (int d = 0; d < F::kVWords * 4; ++d) {
+              O[n][d][i] *= keep;
+              O[n][d][kPer + i] *= keep;
+            }
+          }
+      }
+      float tile_acc[kParts == 2 ? NT : 1][kParts == 2 ? F::kVWords * 4 : 1][4] = {};
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        uint32_t bp[NT][2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&vp[sub][half]));
+          const float mid = fmaf(7.5f, so.x, so.y);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float P[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const float sc = s[sub][n][i][half];
+              const float w = exp2_fast(sc - ((M[n][i] == -INFINITY ? 0.0f : M[n][i]) - 6.0f));
+              l[n][i] += w;
+              const bool seen = whole || sc != -INFINITY;  // what is not seen may hold anything
+              centre[n][i] = fmaf(w, seen ? mid : 0.0f, centre[n][i]);
+              P[i] = w * (seen ? so.x : 0.0f);
+            }
+            if constexpr (kParts == 2) {
+              const __half hi = __float2half_rn(P[0]);
+              bp[n][half] = pack_half2(hi, __float2half_rn(P[0] - __half2float(hi)));
+            } else {
+              bp[n][half] = pack_half2(__float2half_rn(P[0]), __float2half_rn(P[kPer - 1]));
+            }
+            bp[n][half] = transposed(bp[n][half]);
+          }
+        }
+        const uint8_t* v0 = tile + kTile * (D / 2) + sub * 16 * (D / 2) + g * (D / 16);
+        uint32_t xa[F::kVWords], xb[F::kVWords], xc[F::kVWords], xd[F::kVWords];
+        auto load_v = [&](uint32_t (&x)[F::kVWords], uint32_t token) {
+          const uint8_t* from_v = v0 + token * (D / 2);
+          if constexpr (D == 64) x[0] = *reinterpret_cast<const uint32_t*>(from_v);
+          else if constexpr (D == 128) *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(from_v);
+          else *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(from_v);
+        };
+        load_v(xa, token_t0);
+        load_v(xb, token_t1);
+        load_v(xc, token_t0 + 8);
+        load_v(xd, token_t1 + 8);
+#pragma unroll
+        for (int w = 0; w < F::kVWords; ++w) {
+          const uint32_t lo01 = __byte_perm(xa[w], xb[w], 0x5410), hi01 = __byte_perm(xa[w], xb[w], 0x7632);
+          const uint32_t lo23 = __byte_perm(xc[w], xd[w], 0x5410), hi23 = __byte_perm(xc[w], xd[w], 0x7632);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // dims i (rows g) and i + 4 (rows g + 8) of the word
+            uint32_t a[4] = {lo01, hi01, lo23, hi23};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t x = i >= 2 ? a[j] >> 8 : a[j];
+              a[j] = (i & 1) ? hadd2_u(x & 0x00F000F0u, kCentre1) : hfma2_u(x & 0x000F000Fu, 0x40004000u, kCentre0);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              if constexpr (kParts == 2) mma16816(tile_acc[n][w * 4 + i], a[0], a[1], a[2], a[3], bp[n][0], bp[n][1]);
+              else mma16816(O[n][w * 4 + i], a[0], a[1], a[2], a[3], bp[n][0], bp[n][1]);
+            }
+          }
+        }
+      }
+      if constexpr (kParts == 2) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int d = 0; d < F::kVWords * 4; ++d) {
+            O[n][d][0] += tile_acc[n][d][0] + tile_acc[n][d][1];
+            O[n][d][1] += tile_acc[n][d][2] + tile_acc[n][d][3];
+          }
+      }
+      ++used;
+      __syncwarp();
+      issue_next();
+    }
+
+    // ---- the warps' sums, joined ---------------------------------------------------------------
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) {
+          l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], o);
+          centre[n][i] += __shfl_xor_sync(0xffffffffu, centre[n][i], o);
+        }
+    if (g == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          float* st = warp_stat + (warp * kRows + n * (8 / kParts) + t * kPer + i) * 3;
+          st[0] = M[n][i];
+          st[1] = l[n][i];
+          st[2] = centre[n][i];
+        }
+    }
+    __syncthreads();
+    // a thread's own rows: what all warps agree on, then its sums in that scale
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        float m = -INFINITY;
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[(w * kRows + n * (8 / kParts) + t * kPer + i) * 3]);
+        const float keep = M[n][i] == -INFINITY ? 0.0f : exp2_fast(M[n][i] - m);
+        // codes' powers of two: even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
+#pragma unroll
+        for (int d = 0; d < F::kVWords * 4; ++d) {
+          const float back = keep * ((d & 1) ? 1048576.0f : 8388608.0f);
+          O[n][d][i] *= back;
+          O[n][d][kPer + i] *= back;
+        }
+      }
+    constexpr int kQuads = kRows * D / 4;                       // outputs of the block, by four
+    constexpr int kLoops = (kQuads + F::kThreads - 1) / F::kThreads;
+    float sum[kLoops][4] = {};
+    for (int round = 0; round < kWarps / F::kMergeWarps; ++round) {
+      if (static_cast<int>(warp) / F::kMergeWarps == round) {
+        float* to = merge + (warp % F::kMergeWarps) * kRows * D;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int w = 0; w < F::kVWords; ++w)
+#pragma unroll
+              for (int half = 0; half < 2; ++half)  // dims 0..3, then 4..7 of the thread's word
+                *reinterpret_cast<float4*>(to + (n * (8 / kParts) + t * kPer + i) * D + g * (D / 8) + w * 8 + half * 4) =
+                    make_float4(O[n][w * 4][half * kPer + i], O[n][w * 4 + 1][half * kPer + i], O[n][w * 4 + 2][half * kPer + i],
+                                O[n][w * 4 + 3][half * kPer + i]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kLoops; ++k) {
+        const int quad = static_cast<int>(tid) + k * F::kThreads;
+        if (quad < kQuads)
+          for (int w = 0; w < F::kMergeWarps; ++w) {
+            const float4 v = reinterpret_cast<const float4*>(merge + w * kRows * D)[quad];
+            sum[k][0] += v.x;
+            sum[k][1] += v.y;
+            sum[k][2] += v.z;
+            sum[k][3] += v.w;
+          }
+      }
+      __syncthreads();
+    }
+    const bool complete = at.off == 0 && left <= end - pos;
+    const unsigned long long run_begin = pos - at.off, run_end = pos + left;
+    const uint32_t c0 = static_cast<uint32_t>(run_begin / per), c1 = static_cast<uint32_t>((run_end - 1) / per);
+    float* part = p.parts + static_cast<size_t>(blockIdx.x == c0 ? 2 * c0 + 1 : 2 * blockIdx.x) * F::kPartFloats;
+    auto store_row = [&](int quad, const float (&v)[4], float total_l) {
+      const int row = static_cast<int>(block) * kRows + quad / (D / 4), query = row / static_cast<int>(p.group);
+      if (row >= q_rows) return;
+      const int head = static_cast<int>(kv_head * p.group) + row % static_cast<int>(p.group);
+      const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
+      const float o[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+      store4(static_cast<T*>(p.a.out) + static_cast<size_t>(at.runs.span.first + query) * p.a.out_stride + static_cast<size_t>(head) * D + quad % (D / 4) * 4, o);
+    };
+#pragma unroll
+    for (int k = 0; k < kLoops; ++k) {
+      const int quad = static_cast<int>(tid) + k * F::kThreads;
+      if (quad >= kQuads) break;
+      const int row = quad / (D / 4);
+      float m = -INFINITY, total_l = 0.0f, mid = 0.0f;
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[(w * kRows + row) * 3]);
+      for (int w = 0; w < kWarps; ++w) {
+        const float* st = warp_stat + (w * kRows + row) * 3;
+        const float keep = st[0] == -INFINITY ? 0.0f : exp2_fast(st[0] - m);
+        total_l = fmaf(keep, st[1], total_l);
+        mid = fmaf(keep, st[2], mid);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[k][i] += mid;
+      if (complete) {
+        store_row(quad, sum[k], total_l);
       } else {
-        s = quiet_nan();
+        reinterpret_cast<float4*>(part)[quad] = make_float4(sum[k][0], sum[k][1], sum[k][2], sum[k][3]);
+        if (quad % (D / 4) == 0) {
+          part[kRows * D + row * 2] = m;
+          part[kRows * D + row * 2 + 1] = total_l;
+        }
       }
     }
-    const bool nan = __syncthreads_or(s != s);
-    float m = s;
-    for (int x = 16; x > 0; x /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    if (tid % 32 == 0) part[tid / 32] = m;
-    __syncthreads();
-    float now = top;
-    for (int w = 0; w < kAttendThreads / 32; ++w) now = fmaxf(now, part[w]);
-    if (nan) now = quiet_nan();
-    const float keep = top == -INFINITY ? 0.0f : exp2f(top - now);
-    const float p = key <= position ? exp2f(s - now) : 0.0f;
-    top = now;
-    total = total * keep + p;
-    off_sum = off_sum * keep + (key <= position ? p * v_off : 0.0f);
-    p_s[tid] = p;
-    pv_s[tid] = key <= position ? p * v_scale : 0.0f;
-    v_s[tid] = v_row;
-    for (int i = 0; i < kPer; ++i) o[i] *= keep;
-    __syncthreads();
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t d = tid + i * kAttendThreads;
-      if (d >= D) break;
-      float sum = 0.0f;
-      for (int j = 0; j < kAttendThreads && at + j <= position; ++j) {
-        const uint32_t byte = v_s[j] ? v_s[j][d / 2] : 0u;
-        sum = fmaf(pv_s[j], static_cast<float>((byte >> (4 * (d & 1))) & 15u) - 7.5f, sum);
+    if (!complete) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned int before = atomicAdd(p.counters + c0, 1u);
+        if (before == c1 - c0) p.counters[c0] = 0;
+        *arrived = before;
       }
-      o[i] += sum;
+      __syncthreads();
+      if (*arrived == c1 - c0) {  // the last one: all parts of the run in order
+        __threadfence();
+        const int n_parts = static_cast<int>(c1 - c0) + 1;
+        auto part_of = [&](int k) { return p.parts + static_cast<size_t>(k == 0 ? 2 * c0 + 1 : 2 * (c0 + k)) * F::kPartFloats; };
+#pragma unroll
+        for (int k = 0; k < kLoops; ++k) {
+          const int quad = static_cast<int>(tid) + k * F::kThreads;
+          if (quad >= kQuads) break;
+          const int row = quad / (D / 4);
+          float m = -INFINITY, total_l = 0.0f, v[4] = {};
+          for (int j = 0; j < n_parts; ++j) m = fmaxf(m, __ldcg(part_of(j) + kRows * D + row * 2));
+          for (int j = 0; j < n_parts; ++j) {
+            const float* from_part = part_of(j);
+            const float pm = __ldcg(from_part + kRows * D + row * 2);
+            const float keep = pm == -INFINITY ? 0.0f : exp2_fast(pm - m);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(from_part) + quad);
+            total_l = fmaf(keep, __ldcg(from_part + kRows * D + row * 2 + 1), total_l);
+            v[0] = fmaf(keep, x.x, v[0]);
+            v[1] = fmaf(keep, x.y, v[1]);
+            v[2] = fmaf(keep, x.z, v[2]);
+            v[3] = fmaf(keep, x.w, v[3]);
+          }
+          store_row(quad, v, total_l);
+        }
+      }
     }
-    __syncthreads();
+    __syncthreads();  // q_frag, row_const and warp_stat belong to the next run
+    at.off += stop - pos;
+    pos = stop;
+    if (pos < end) settle(at, p, kRows);
   }
-  total = warp_sum(total);
-  off_sum = warp_sum(off_sum);
-  if (tid % 32 == 0) {
-    p_s[tid / 32] = total;
-    pv_s[tid / 32] = off_sum;
-  }
-  __syncthreads();
-  total = off_sum = 0.0f;
-  for (int w = 0; w < kAttendThreads / 32; ++w) {
-    total += p_s[w];
-    off_sum += pv_s[w];
-  }
-  for (int i = 0; i < kPer; ++i) {
-    const uint32_t d = tid + i * kAttendThreads;
-    if (d < D) store_as(out + d, (o[i] + off_sum) / total);
-  }
+}
+
+template <typename T, int D, int NT>
+cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
+  using F = Few<T, D, NT>;
+  static_assert(F::kSmem <= 227 * 1024, "shared memory");
+  static OncePerDevice once;
+  cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_few_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem); });
+  if (e != cudaSuccess) return e;
+  FewParams p;
+  p.a = a;
+  p.group = a.heads / a.cache.kv_heads;
+  p.parts = static_cast<float*>(env.workspace);
+  p.counters = env.counters;
+  p.status = env.status;
+  p.least = 8;
+  // a CTA's two parts must fit the scratch; one CTA alone shares no run
+  const uint64_t fit = env.workspace ? env.workspace_bytes / (2ull * F::kPartFloats * sizeof(float)) : 0;
+  const unsigned grid = static_cast<unsigned>(std::max<uint64_t>(1, std::min<uint64_t>({static_cast<uint64_t>(env.sm_count), fit, env.counter_count})));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(F::kThreads);
+  cfg.dynamicSmemBytes = F::kSmem;
+  cfg.stream = env.stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = env.overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, attend_few_kernel<T, D, NT>, p);
+}
+
+template <typename T, int D>
+cudaError_t few_of(const LaunchEnv& env, const AttendArgs& a) {
+  const uint64_t columns = static_cast<uint64_t>(a.batch.most) * (a.heads / a.cache.kv_heads) * Parts<T>::n;
+  if (columns <= 8) return few_as<T, D, 1>(env, a);
+  if (columns <= 16 || D > 128) return few_as<T, D, 2>(env, a);
+  if constexpr (D <= 128) return few_as<T, D, 4>(env, a);
+  return cudaErrorInvalidValue;
 }
 
 template <typename T>
 cudaError_t attend_as(const LaunchEnv& env, const AttendArgs& a) {
-  const unsigned grid = a.batch.tokens * a.heads;
   switch (a.cache.head_dim) {
-    case 64: attend_row_kernel<T, 64><<<grid, kAttendThreads, 0, env.stream>>>(a); break;
-    case 128: attend_row_kernel<T, 128><<<grid, kAttendThreads, 0, env.stream>>>(a); break;
-    case 256: attend_row_kernel<T, 256><<<grid, kAttendThreads, 0, env.stream>>>(a); break;
+    case 64: return few_of<T, 64>(env, a);
+    case 128: return few_of<T, 128>(env, a);
+    case 256: return few_of<T, 256>(env, a);
     default: return cudaErrorInvalidValue;
   }
-  return cudaGetLastError();
 }
 
 }  // namespace
