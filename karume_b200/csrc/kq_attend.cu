@@ -52,35 +52,40 @@ template <typename T, int D, int NT>
 struct Few {
   static constexpr int kParts = Parts<T>::n;
   static constexpr int kRows = 8 * NT / kParts;      // query rows of a block
-  static constexpr int kWarps = NT == 1 && D <= 128 ? 16 : 8;
+  static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kStages = 2;
   static constexpr int kSteps = D / 16;              // k-steps of S^T
   static constexpr int kWords = D / 32;              // words of a token in a thread (keys)
   static constexpr int kVWords = D / 64;             // ... (values)
   static constexpr int kTileBytes = kTile * (D + 8);
-  static constexpr int kMergeWarps = 4;              // warps whose sums are added in one round
   static constexpr bool kQInRegisters = NT * kSteps <= 16;
   static constexpr int kPartFloats = kRows * (D + 2);  // a partial result in the scratch: sums, M, l
+  static constexpr int kSpans = 128;                   // sequences whose lengths are kept in shared memory
 
   static constexpr int kRing = 0;
   static constexpr int kMerge = kRing + kWarps * kStages * kTileBytes;
-  static constexpr int kQFrag = kMerge + kMergeWarps * kRows * D * 4;  // [NT][kSteps][32] x 8 B
+  static constexpr int kQFrag = kMerge + kWarps * kRows * D * 4;       // [NT][kSteps][32] x 8 B
   static constexpr int kRowConst = kQFrag + NT * kSteps * 32 * 8;      // factor, offset, last key, first key of each row
   static constexpr int kWarpStat = kRowConst + kRows * 16;             // [kWarps][kRows] x (M, l, centre sum)
-  static constexpr int kScan = kWarpStat + kWarps * kRows * 12 + 8;    // [kThreads] x 8 B, and what the scan found
-  static constexpr int kBars = kScan + kThreads * 8 + 32;
+  static constexpr int kScan = kWarpStat + (kWarps * kRows * 12 + 15) / 16 * 16;  // sums of the warps, what the scan found
+  static constexpr int kSpan = kScan + kWarps * 8 + 16;
+  static constexpr int kBars = kSpan + kSpans * 16;
   static constexpr int kMisc = kBars + kWarps * kStages * 8;
   static constexpr int kSmem = kMisc + 16;
+  // CTAs of an SM: what waits in one is hidden by the others; as many as registers and shared memory allow
+  static constexpr int kFit = 228 * 1024 / (kSmem + 1024);
+  static constexpr int kCtas = NT == 1 && D <= 128 ? (kFit < 4 ? kFit : 4) : (kFit < 2 ? kFit : 2);
 };
 
 struct FewParams {
   AttendArgs a;
-  uint32_t group;        // query heads of a kv head
-  float* parts;          // [2 * grid][kPartFloats]
-  unsigned int* counters;  // [grid], zero between launches
+  uint32_t group;          // query heads of a kv head
+  uint32_t page_shift;     // log2 of a page's tokens
+  float* parts;            // [4 * grid][kPartFloats]: two of a CTA, and two of the groups that begin with it
+  unsigned int* counters;  // [3 * grid], zero between launches
   int* status;
-  uint32_t least;        // tiles a CTA should have at least
+  uint32_t least;          // tiles a CTA should have at least
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -131,42 +136,22 @@ struct Runs {
   int tile_lo, tiles;
   uint32_t blocks, units;
 };
-__device__ __forceinline__ Runs runs_of(const FewParams& p, uint32_t b, int rows) {
+__device__ __forceinline__ Runs runs_of(const FewParams& p, const Span& span, int rows) {
   Runs r;
-  r.span = span_of(p.a.batch, b);
-  const int first = r.span.length - r.span.count;  // position of the first query
+  r.span = span;
+  const int first = span.length - span.count;  // position of the first query
   const int window = static_cast<int>(min(p.a.window, 0x7fffffffu));
   const int from = window && first + 1 > window ? first + 1 - window : 0;
   r.tile_lo = from / kTile;
-  r.tiles = r.span.length > 0 ? (r.span.length - 1) / kTile + 1 - r.tile_lo : 1;  // an idle sequence's rows are written too
-  r.blocks = (static_cast<uint32_t>(r.span.count) * p.group + rows - 1) / rows;
+  r.tiles = (span.length - 1) / kTile + 1 - r.tile_lo;
+  r.blocks = span.length > 0 ? (static_cast<uint32_t>(span.count) * p.group + rows - 1) / rows : 0;  // idle: no work
   r.units = r.blocks * p.a.cache.kv_heads;
   return r;
 }
 
-// A place in the list: tile `off` of unit `unit` of sequence b.
-struct Walk {
-  uint32_t b, unit;
-  unsigned long long off;
-  Runs runs;
-};
-__device__ __forceinline__ void settle(Walk& w, const FewParams& p, int rows) {  // carry off into units and sequences
-  while (w.b < p.a.batch.sequences) {
-    if (w.unit < w.runs.units) {
-      if (w.off < static_cast<unsigned>(w.runs.tiles)) return;
-      const unsigned long long skip = min(w.off / static_cast<unsigned>(w.runs.tiles), static_cast<unsigned long long>(w.runs.units - w.unit));
-      w.unit += static_cast<uint32_t>(skip);
-      w.off -= skip * static_cast<unsigned>(w.runs.tiles);
-      if (w.unit < w.runs.units) continue;
-    }
-    w.unit = 0;
-    if (++w.b < p.a.batch.sequences) w.runs = runs_of(p, w.b, rows);
-  }
-}
-
 // Keys that the rows of a block see: from the first row's first to the last row's last.
 struct Keys {
-  int first, last;       // of any row
+  int first, last;          // of any row
   int first_all, last_all;  // of all rows
 };
 __device__ __forceinline__ Keys keys_of(const FewParams& p, const Runs& r, uint32_t block, int rows) {
@@ -181,8 +166,34 @@ __device__ __forceinline__ Keys keys_of(const FewParams& p, const Runs& r, uint3
   return k;
 }
 
+// A place in the list: tile `tile` (counted from the sequence's first) of a run.
+struct Walk {
+  uint32_t b, head, block;
+  int tile;
+  Runs runs;
+  Keys keys;
+};
+// Carries a tile number beyond the run's end into the following runs; false behind the last one.
+template <typename SpanAt>
+__device__ __forceinline__ bool settle(Walk& w, const FewParams& p, int rows, SpanAt span_at) {
+  while (w.tile >= w.runs.tile_lo + w.runs.tiles || w.runs.units == 0) {
+    if (w.runs.units != 0) w.tile -= w.runs.tiles;
+    if (w.runs.units == 0 || (++w.block == w.runs.blocks && ++w.head == p.a.cache.kv_heads)) {
+      if (++w.b >= p.a.batch.sequences) return false;
+      w.tile -= w.runs.units != 0 ? w.runs.tile_lo : 0;
+      w.runs = runs_of(p, span_at(w.b), rows);
+      w.tile += w.runs.units != 0 ? w.runs.tile_lo : 0;
+      w.head = w.block = 0;
+    } else if (w.block == w.runs.blocks) {
+      w.block = 0;
+    }
+    if (w.runs.units != 0) w.keys = keys_of(p, w.runs, w.block, rows);
+  }
+  return true;
+}
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas) attend_few_kernel(const __grid_constant__ FewParams p) {
   using F = Few<T, D, NT>;
   constexpr int kRows = F::kRows, kParts = F::kParts, kWarps = F::kWarps, kStages = F::kStages;
   constexpr int kPer = kParts == 1 ? 2 : 1;  // query rows of a thread in one n-tile
@@ -193,7 +204,8 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
   float4* row_const = reinterpret_cast<float4*>(smem + F::kRowConst);
   float* warp_stat = reinterpret_cast<float*>(smem + F::kWarpStat);
   unsigned long long* scan = reinterpret_cast<unsigned long long*>(smem + F::kScan);
-  unsigned long long* found = scan + F::kThreads;  // sequence, tiles in front of it
+  unsigned long long* found = scan + kWarps;  // sequence, tiles in front of it
+  int4* spans = reinterpret_cast<int4*>(smem + F::kSpan);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F::kMisc);
   volatile unsigned int* arrived = reinterpret_cast<volatile unsigned int*>(smem + F::kMisc + 4);
   const uint32_t bars = smem_u32(smem + F::kBars) + warp * kStages * 8;
@@ -205,10 +217,19 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
 
   // ---- this CTA's range of the list --------------------------------------------------------------
   const uint32_t sequences = p.a.batch.sequences, each = (sequences + F::kThreads - 1) / F::kThreads;
+  const bool kept = sequences <= F::kSpans;
   unsigned long long mine = 0;
   for (uint32_t b = tid * each; b < min((tid + 1) * each, sequences); ++b) {
-    const Runs r = runs_of(p, b, kRows);
-    mine += static_cast<unsigned long long>(r.tiles) * r.units;
+    const Span span = span_of(p.a.batch, b);
+    if (kept) spans[b] = make_int4(span.first, span.count, span.length, 0);
+    const Runs r = runs_of(p, span, kRows);
+    mine += static_cast<unsigned long long>(r.units) * static_cast<unsigned>(r.tiles);
+    if (span.length == 0 && blockIdx.x == b % gridDim.x)  // an idle sequence's rows are zero
+      for (int i = 0; i < span.count; ++i)
+        for (uint32_t d = 0; d < p.a.heads * D; d += 4) {
+          const float zero[4] = {};
+          store4(static_cast<T*>(p.a.out) + static_cast<size_t>(span.first + i) * p.a.out_stride + d, zero);
+        }
   }
   unsigned long long upto = mine;  // inclusive sum over the threads
 #pragma unroll
@@ -225,12 +246,10 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
   }
   // rows that belong to no sequence are zero
   if (p.a.batch.starts) {
-    const int head_rows = min(max(p.a.batch.starts[0], 0), static_cast<int>(p.a.batch.tokens));
-    const int tail = min(max(p.a.batch.starts[sequences], 0), static_cast<int>(p.a.batch.tokens));
-    const int extra = head_rows + static_cast<int>(p.a.batch.tokens) - max(tail, head_rows);
-    for (int i = blockIdx.x; i < extra; i += gridDim.x) {
-      const int row = i < head_rows ? i : max(tail, head_rows) + i - head_rows;
-      T* out = static_cast<T*>(p.a.out) + row * p.a.out_stride;
+    const int tokens = static_cast<int>(p.a.batch.tokens);
+    const int head_rows = min(max(p.a.batch.starts[0], 0), tokens), tail = max(min(p.a.batch.starts[sequences], tokens), head_rows);
+    for (int i = blockIdx.x; i < head_rows + tokens - tail; i += gridDim.x) {
+      T* out = static_cast<T*>(p.a.out) + static_cast<size_t>(i < head_rows ? i : tail + i - head_rows) * p.a.out_stride;
       const float zero[4] = {};
       for (uint32_t d = tid * 4; d < p.a.heads * D; d += F::kThreads * 4) store4(out + d, zero);
     }
@@ -244,60 +263,64 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
     found[1] = upto - mine;
   }
   __syncthreads();
+  auto span_at = [&](uint32_t b) {
+    if (!kept) return span_of(p.a.batch, b);
+    const int4 v = spans[b];
+    return Span{v.x, v.y, v.z};
+  };
   Walk at;
   at.b = static_cast<uint32_t>(found[0]);
-  at.unit = 0;
-  at.off = begin - found[1];
-  at.runs = runs_of(p, at.b, kRows);
-  settle(at, p, kRows);
+  at.runs = runs_of(p, span_at(at.b), kRows);
+  unsigned long long skip = begin - found[1];
+  while (skip >= static_cast<unsigned long long>(at.runs.units) * static_cast<unsigned>(at.runs.tiles)) {  // sequences of one thread's share
+    skip -= static_cast<unsigned long long>(at.runs.units) * static_cast<unsigned>(at.runs.tiles);
+    at.runs = runs_of(p, span_at(++at.b), kRows);
+  }
+  const uint32_t unit = static_cast<uint32_t>(skip / static_cast<unsigned>(at.runs.tiles));
+  at.head = unit / at.runs.blocks;
+  at.block = unit % at.runs.blocks;
+  at.tile = at.runs.tile_lo + static_cast<int>(skip % static_cast<unsigned>(at.runs.tiles));
+  at.keys = keys_of(p, at.runs, at.block, kRows);
 
   // ---- copies: the warp's tiles, a ring's length ahead --------------------------------------------
   const uint32_t ring = smem_u32(smem + F::kRing) + warp * kStages * F::kTileBytes;
   uint8_t* const ring_ptr = smem + F::kRing + warp * kStages * F::kTileBytes;
+  const uint32_t P = p.a.cache.page_tokens, run = min(P, static_cast<uint32_t>(kTile));  // tokens of a piece
   Walk ahead = at;
-  ahead.off += warp;
-  unsigned long long ahead_at = begin + warp;
-  if (ahead_at < end) settle(ahead, p, kRows);
+  ahead.tile += static_cast<int>(warp);
+  int to_issue = end - begin > warp ? static_cast<int>((end - begin - warp + kWarps - 1) / kWarps) : 0;  // tiles of this warp not passed yet
   uint32_t issued = 0, used = 0;
   auto issue_next = [&]() {
-    for (; ahead_at < end;) {
-      const Keys keys = keys_of(p, ahead.runs, ahead.unit % ahead.runs.blocks, kRows);
-      const int first = (ahead.runs.tile_lo + static_cast<int>(ahead.off)) * kTile;
-      const bool needed = first <= keys.last && first + kTile > keys.first;
-      if (needed) {
-        const uint32_t stage = issued % kStages, bar = bars + stage * 8, to = ring + stage * F::kTileBytes;
-        const uint32_t P = p.a.cache.page_tokens, run = min(P, static_cast<uint32_t>(kTile));  // tokens of a piece
-        const uint32_t pieces = kTile / run;
-        const bool piece = lane < pieces && first + static_cast<int>(lane * run) <= keys.last;
-        const uint32_t key = static_cast<uint32_t>(first) + lane * run, slot = key % P;
-        const uint8_t* block = piece ? cache_block(p.a.cache, p.a.batch, ahead.b, key / P, ahead.unit / ahead.runs.blocks) : nullptr;
-        const uint32_t have = __ballot_sync(0xffffffffu, block != nullptr), lost = __ballot_sync(0xffffffffu, piece && !block);
-        if (lost) {  // no such page: what it would hold is NaN
-          uint32_t* params = reinterpret_cast<uint32_t*>(ring_ptr + stage * F::kTileBytes + kTile * D);
-          for (uint32_t i = lane; i < kTile; i += 32)
-            if (lost >> (i / run) & 1) params[i] = params[kTile + i] = 0x7E007E00u;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(have) * run * (D + 8)) : "memory");
+    for (bool more = true; more && to_issue > 0; ahead.tile += kWarps, --to_issue) {
+      settle(ahead, p, kRows, span_at);
+      const int first = ahead.tile * kTile;
+      if (first > ahead.keys.last || first + kTile <= ahead.keys.first) continue;
+      const uint32_t stage = issued % kStages, bar = bars + stage * 8, to = ring + stage * F::kTileBytes;
+      const uint32_t key = static_cast<uint32_t>(first) + lane * run, slot = key & (P - 1);
+      const bool piece = lane * run < kTile && static_cast<int>(key) <= ahead.keys.last;
+      const uint8_t* block = piece ? cache_block(p.a.cache, p.a.batch, ahead.b, key >> p.page_shift, ahead.head) : nullptr;
+      const uint32_t have = __ballot_sync(0xffffffffu, block != nullptr), lost = __ballot_sync(0xffffffffu, piece && !block);
+      if (lost) {  // no such page: what it would hold is NaN
+        uint32_t* params = reinterpret_cast<uint32_t*>(ring_ptr + stage * F::kTileBytes + kTile * D);
+        if (lost >> (lane / run) & 1) params[lane] = params[kTile + lane] = 0x7E007E00u;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (block) {
-          const uint32_t sizes[2] = {run * (D / 2), run * 4};
-          const uint8_t* from[4] = {block + slot * (D / 2), block + (P + slot) * (D / 2), block + P * D + slot * 4, block + P * D + (P + slot) * 4};
-          const uint32_t dst[4] = {to + lane * run * (D / 2), to + (kTile + lane * run) * (D / 2), to + kTile * D + lane * run * 4,
-                                   to + kTile * D + (kTile + lane * run) * 4};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                         ::"r"(dst[i]), "l"(from[i]), "r"(sizes[i / 2]), "r"(bar) : "memory");
-        }
-        ++issued;
       }
-      ahead_at += kWarps;
-      ahead.off += kWarps;
-      if (ahead_at < end) settle(ahead, p, kRows);
-      if (needed) return;
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(have) * run * (D + 8)) : "memory");
+      __syncwarp();
+      if (block) {
+        const uint32_t sizes[2] = {run * (D / 2), run * 4};
+        const uint8_t* from[4] = {block + slot * (D / 2), block + (P + slot) * (D / 2), block + P * D + slot * 4, block + P * D + (P + slot) * 4};
+        const uint32_t dst[4] = {to + lane * run * (D / 2), to + (kTile + lane * run) * (D / 2), to + kTile * D + lane * run * 4,
+                                 to + kTile * D + (kTile + lane * run) * 4};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(dst[i]), "l"(from[i]), "r"(sizes[i / 2]), "r"(bar) : "memory");
+      }
+      ++issued;
+      more = false;
     }
   };
   __syncwarp();
@@ -311,17 +334,16 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
 
   // ---- run by run --------------------------------------------------------------------------------
   for (unsigned long long pos = begin; pos < end;) {
-    const unsigned long long left = static_cast<unsigned long long>(at.runs.tiles) - at.off;
-    const unsigned long long stop = min(end, pos + left);
-    const uint32_t kv_head = at.unit / at.runs.blocks, block = at.unit % at.runs.blocks;
+    const int run_end = at.runs.tile_lo + at.runs.tiles;
+    const int stop = static_cast<int>(min(static_cast<unsigned long long>(run_end), at.tile + (end - pos)));
     const int q_rows = at.runs.span.count * static_cast<int>(p.group);
     const int base = at.runs.span.length - at.runs.span.count;
-    const Keys keys = keys_of(p, at.runs, block, kRows);
+    const Keys keys = at.keys;
 
     // queries: rotated, scaled to binary16's range by a power of two, in the order of the B fragments
     for (int r = static_cast<int>(warp); r < kRows; r += kWarps) {
-      const int row = static_cast<int>(block) * kRows + r, query = row / static_cast<int>(p.group);
-      const int head = static_cast<int>(kv_head * p.group) + row % static_cast<int>(p.group);
+      const int row = static_cast<int>(at.block) * kRows + r, query = row / static_cast<int>(p.group);
+      const int head = static_cast<int>(at.head * p.group) + row - query * static_cast<int>(p.group);
       const bool there = row < q_rows;
       float v[8] = {};
       if (there && lane < D / 8)
@@ -378,7 +400,6 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
     }
     // a thread's query rows in n-tile n: n * 8 / parts + t * kPer + i
     float factor[NT][kPer], offset[NT][kPer];
-    int last[NT][kPer], from[NT][kPer];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -386,8 +407,6 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
         const float4 c = row_const[n * (8 / kParts) + t * kPer + i];
         factor[n][i] = c.x;
         offset[n][i] = c.y;
-        last[n][i] = __float_as_int(c.z);
-        from[n][i] = __float_as_int(c.w);
       }
     float M[NT][kPer], l[NT][kPer] = {}, centre[NT][kPer] = {};
 #pragma unroll
@@ -397,8 +416,9 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
     // f32 queries: sums of a thread's dims for its one row; 16-bit ones: the accumulators (two rows)
     float O[NT][F::kVWords * 4][2 * kPer] = {};
 
-    for (unsigned long long f = pos + (warp + kWarps - static_cast<uint32_t>((pos - begin) % kWarps)) % kWarps; f < stop; f += kWarps) {
-      const int first = (at.runs.tile_lo + static_cast<int>(at.off + (f - pos))) * kTile;
+    const int ahead_of = static_cast<int>((pos - begin) % kWarps);
+    for (int tile_at = at.tile + (static_cast<int>(warp) + kWarps - ahead_of) % kWarps; tile_at < stop; tile_at += kWarps) {
+      const int first = tile_at * kTile;
       if (first > keys.last || first + kTile <= keys.first) continue;
       const uint32_t stage = used % kStages, parity = used / kStages & 1;
       {
@@ -421,7 +441,9 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
       uint32_t vp[2][2];        // the values' (scale, offset) of the thread's tokens
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        float acc[NT][4] = {};
+        // f32 queries: chains of two MMAs, added in f32 (the tensor core truncates)
+        constexpr int kChains = kParts == 2 ? F::kSteps / 2 : 1;
+        float acc[NT][kChains][4] = {};
         const uint8_t* row0 = tile + (sub * 16 + token_g) * (D / 2);
         const uint8_t* row1 = row0 + 8 * (D / 2);
         uint32_t x0[F::kWords], x1[F::kWords];
@@ -444,7 +466,7 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
             for (int n = 0; n < NT; ++n) {
               const uint2 bb = F::kQInRegisters ? bq[F::kQInRegisters ? n : 0][F::kQInRegisters ? 2 * w + half : 0]
                                                 : q_frag[(n * F::kSteps + 2 * w + half) * 32 + lane];
-              mma16816(acc[n], a & 0x000F000Fu, b & 0x000F000Fu, a & 0x00F000F0u, b & 0x00F000F0u, bb.x, bb.y);
+              mma16816(acc[n][w % kChains], a & 0x000F000Fu, b & 0x000F000Fu, a & 0x00F000F0u, b & 0x00F000F0u, bb.x, bb.y);
             }
           }
         const uint32_t* params = reinterpret_cast<const uint32_t*>(tile + kTile * D) + sub * 16 + token_g;
@@ -453,32 +475,46 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
           const uint32_t kp = params[half * 8];
           vp[sub][half] = params[kTile + half * 8];
           const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&kp));
-          const int key = first + sub * 16 + half * 8 + static_cast<int>(token_g);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-              const float dot = kParts == 2 ? acc[n][2 * half] + acc[n][2 * half + 1] : acc[n][2 * half + i];
-              float v = fmaf(dot, so.x * factor[n][i], so.y * offset[n][i]);
-              if (!whole && (key > last[n][i] || key < from[n][i])) v = -INFINITY;
-              s[sub][n][i][half] = v;
+              float dot = kParts == 2 ? acc[n][0][2 * half] + acc[n][0][2 * half + 1] : acc[n][0][2 * half + i];
+#pragma unroll
+              for (int c = 1; c < kChains; ++c) dot += acc[n][c][2 * half] + acc[n][c][2 * half + 1];
+              s[sub][n][i][half] = fmaf(dot, so.x * factor[n][i], so.y * offset[n][i]);
             }
         }
       }
-      // M: the largest score plus its value's binade (never less than log2 of the scale)
-      float binade[2][2];
+      uint32_t scale_bits[4] = {vp[0][0], vp[0][1], vp[1][0], vp[1][1]};
+      if (!whole) {
+        uint32_t seen = 0;
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) binade[sub][half] = static_cast<float>(max(static_cast<int>(vp[sub][half] >> 10 & 31u), 1) - 14);
+          for (int i = 0; i < kPer; ++i) {
+            const float4 c = row_const[n * (8 / kParts) + t * kPer + i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int key = first + j * 8 + static_cast<int>(token_g);
+              if (key > __float_as_int(c.z) || key < __float_as_int(c.w)) s[j / 2][n][i][j % 2] = -INFINITY;
+              else seen |= 1u << j;
+            }
+          }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!(seen >> j & 1)) scale_bits[j] = 0;  // what is not seen may hold anything
+      }
+      // M: the largest score and the largest binade of the values' scales (at least log2 of a scale)
+      const uint32_t big_scale = max(max(scale_bits[0] & 0x7C00u, scale_bits[1] & 0x7C00u), max(scale_bits[2] & 0x7C00u, scale_bits[3] & 0x7C00u));
+      const float binade = static_cast<float>(max(static_cast<int>(big_scale >> 10), 1) - 14);
       bool more = false;
       float top[NT][kPer];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          top[n][i] = fmaxf(fmaxf(s[0][n][i][0] + binade[0][0], s[0][n][i][1] + binade[0][1]),
-                            fmaxf(s[1][n][i][0] + binade[1][0], s[1][n][i][1] + binade[1][1]));
+          top[n][i] = fmaxf(fmaxf(s[0][n][i][0], s[0][n][i][1]), fmaxf(s[1][n][i][0], s[1][n][i][1])) + binade;
           more |= top[n][i] > M[n][i] + 8.0f;
         }
       if (__any_sync(0xffffffffu, more)) {
@@ -501,6 +537,11 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
             }
           }
       }
+      float shift[NT][kPer];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) shift[n][i] = M[n][i] == -INFINITY ? 6.0f : 6.0f - M[n][i];
       float tile_acc[kParts == 2 ? NT : 1][kParts == 2 ? F::kVWords * 4 : 1][4] = {};
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
@@ -511,21 +552,22 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
           const float mid = fmaf(7.5f, so.x, so.y);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float P[kPer];
+            float pv[kPer];
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-              const float sc = s[sub][n][i][half];
-              const float w = exp2_fast(sc - ((M[n][i] == -INFINITY ? 0.0f : M[n][i]) - 6.0f));
+              const float w = exp2_fast(s[sub][n][i][half] + shift[n][i]);
               l[n][i] += w;
-              const bool seen = whole || sc != -INFINITY;  // what is not seen may hold anything
-              centre[n][i] = fmaf(w, seen ? mid : 0.0f, centre[n][i]);
-              P[i] = w * (seen ? so.x : 0.0f);
+              pv[i] = w * so.x;
+              float mid_w = w * mid;
+              if (!whole && s[sub][n][i][half] == -INFINITY) pv[i] = mid_w = 0.0f;
+              centre[n][i] += mid_w;
             }
             if constexpr (kParts == 2) {
-              const __half hi = __float2half_rn(P[0]);
-              bp[n][half] = pack_half2(hi, __float2half_rn(P[0] - __half2float(hi)));
+              const __half hi = __float2half_rn(pv[0]);
+              bp[n][half] = pack_half2(hi, __float2half_rn(pv[0] - __half2float(hi)));
             } else {
-              bp[n][half] = pack_half2(__float2half_rn(P[0]), __float2half_rn(P[kPer - 1]));
+              const __half2 both = __floats2half2_rn(pv[0], pv[kPer - 1]);
+              bp[n][half] = *reinterpret_cast<const uint32_t*>(&both);
             }
             bp[n][half] = transposed(bp[n][half]);
           }
@@ -597,64 +639,30 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
           st[2] = centre[n][i];
         }
     }
-    __syncthreads();
-    // a thread's own rows: what all warps agree on, then its sums in that scale
+    // the codes' powers of two: even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        float m = -INFINITY;
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[(w * kRows + n * (8 / kParts) + t * kPer + i) * 3]);
-        const float keep = M[n][i] == -INFINITY ? 0.0f : exp2_fast(M[n][i] - m);
-        // codes' powers of two: even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
+      for (int i = 0; i < kPer; ++i)
 #pragma unroll
-        for (int d = 0; d < F::kVWords * 4; ++d) {
-          const float back = keep * ((d & 1) ? 1048576.0f : 8388608.0f);
-          O[n][d][i] *= back;
-          O[n][d][kPer + i] *= back;
-        }
-      }
-    constexpr int kQuads = kRows * D / 4;                       // outputs of the block, by four
+        for (int w = 0; w < F::kVWords; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)  // dims 0..3, then 4..7 of the thread's word
+            *reinterpret_cast<float4*>(merge + (warp * kRows + n * (8 / kParts) + t * kPer + i) * D + g * (D / 8) + w * 8 + half * 4) =
+                make_float4(O[n][w * 4][half * kPer + i] * 8388608.0f, O[n][w * 4 + 1][half * kPer + i] * 1048576.0f,
+                            O[n][w * 4 + 2][half * kPer + i] * 8388608.0f, O[n][w * 4 + 3][half * kPer + i] * 1048576.0f);
+    __syncthreads();
+    constexpr int kQuads = kRows * D / 4;  // outputs of the block, by four
     constexpr int kLoops = (kQuads + F::kThreads - 1) / F::kThreads;
-    float sum[kLoops][4] = {};
-    for (int round = 0; round < kWarps / F::kMergeWarps; ++round) {
-      if (static_cast<int>(warp) / F::kMergeWarps == round) {
-        float* to = merge + (warp % F::kMergeWarps) * kRows * D;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < kPer; ++i)
-#pragma unroll
-            for (int w = 0; w < F::kVWords; ++w)
-#pragma unroll
-              for (int half = 0; half < 2; ++half)  // dims 0..3, then 4..7 of the thread's word
-                *reinterpret_cast<float4*>(to + (n * (8 / kParts) + t * kPer + i) * D + g * (D / 8) + w * 8 + half * 4) =
-                    make_float4(O[n][w * 4][half * kPer + i], O[n][w * 4 + 1][half * kPer + i], O[n][w * 4 + 2][half * kPer + i],
-                                O[n][w * 4 + 3][half * kPer + i]);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kLoops; ++k) {
-        const int quad = static_cast<int>(tid) + k * F::kThreads;
-        if (quad < kQuads)
-          for (int w = 0; w < F::kMergeWarps; ++w) {
-            const float4 v = reinterpret_cast<const float4*>(merge + w * kRows * D)[quad];
-            sum[k][0] += v.x;
-            sum[k][1] += v.y;
-            sum[k][2] += v.z;
-            sum[k][3] += v.w;
-          }
-      }
-      __syncthreads();
-    }
-    const bool complete = at.off == 0 && left <= end - pos;
-    const unsigned long long run_begin = pos - at.off, run_end = pos + left;
-    const uint32_t c0 = static_cast<uint32_t>(run_begin / per), c1 = static_cast<uint32_t>((run_end - 1) / per);
-    float* part = p.parts + static_cast<size_t>(blockIdx.x == c0 ? 2 * c0 + 1 : 2 * blockIdx.x) * F::kPartFloats;
+    const bool complete = at.tile == at.runs.tile_lo && stop == run_end;
+    const unsigned long long run_begin = pos - static_cast<unsigned>(at.tile - at.runs.tile_lo);
+    const uint32_t c0 = static_cast<uint32_t>(run_begin / per), c1 = static_cast<uint32_t>((run_begin + static_cast<unsigned>(at.runs.tiles) - 1) / per);
+    auto slot_of = [&](uint32_t c) { return c == c0 ? 2 * c0 + 1 : 2 * c; };  // a CTA's last run goes on, or its first came from before
+    float* part = p.parts + static_cast<size_t>(slot_of(blockIdx.x)) * F::kPartFloats;
     auto store_row = [&](int quad, const float (&v)[4], float total_l) {
-      const int row = static_cast<int>(block) * kRows + quad / (D / 4), query = row / static_cast<int>(p.group);
+      const int row = static_cast<int>(at.block) * kRows + quad / (D / 4), query = row / static_cast<int>(p.group);
       if (row >= q_rows) return;
-      const int head = static_cast<int>(kv_head * p.group) + row % static_cast<int>(p.group);
+      const int head = static_cast<int>(at.head * p.group) + row - query * static_cast<int>(p.group);
       const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
       const float o[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
       store4(static_cast<T*>(p.a.out) + static_cast<size_t>(at.runs.span.first + query) * p.a.out_stride + static_cast<size_t>(head) * D + quad % (D / 4) * 4, o);
@@ -664,85 +672,116 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, 1) attend_few_kernel(
       const int quad = static_cast<int>(tid) + k * F::kThreads;
       if (quad >= kQuads) break;
       const int row = quad / (D / 4);
-      float m = -INFINITY, total_l = 0.0f, mid = 0.0f;
+      float m = -INFINITY, total_l = 0.0f, mid = 0.0f, sum[4] = {};
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[(w * kRows + row) * 3]);
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float* st = warp_stat + (w * kRows + row) * 3;
         const float keep = st[0] == -INFINITY ? 0.0f : exp2_fast(st[0] - m);
+        const float4 v = reinterpret_cast<const float4*>(merge + w * kRows * D)[quad];
         total_l = fmaf(keep, st[1], total_l);
         mid = fmaf(keep, st[2], mid);
+        sum[0] = fmaf(keep, v.x, sum[0]);
+        sum[1] = fmaf(keep, v.y, sum[1]);
+        sum[2] = fmaf(keep, v.z, sum[2]);
+        sum[3] = fmaf(keep, v.w, sum[3]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[k][i] += mid;
+      for (int i = 0; i < 4; ++i) sum[i] += mid;
       if (complete) {
-        store_row(quad, sum[k], total_l);
+        store_row(quad, sum, total_l);
       } else {
-        reinterpret_cast<float4*>(part)[quad] = make_float4(sum[k][0], sum[k][1], sum[k][2], sum[k][3]);
-        if (quad % (D / 4) == 0) {
-          part[kRows * D + row * 2] = m;
-          part[kRows * D + row * 2 + 1] = total_l;
-        }
+        __stcg(reinterpret_cast<float4*>(part) + quad, make_float4(sum[0], sum[1], sum[2], sum[3]));
+        if (quad % (D / 4) == 0) __stcg(reinterpret_cast<float2*>(part + kRows * D) + row, make_float2(m, total_l));
       }
     }
     if (!complete) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const unsigned int before = atomicAdd(p.counters + c0, 1u);
-        if (before == c1 - c0) p.counters[c0] = 0;
-        *arrived = before;
-      }
-      __syncthreads();
-      if (*arrived == c1 - c0) {  // the last one: all parts of the run in order
+      // the last CTA of sixteen neighbours joins their parts, the last of these groups the groups'
+      constexpr uint32_t kGroup = 16;
+      const uint32_t group0 = max(c0, blockIdx.x / kGroup * kGroup), group1 = min(c1, blockIdx.x / kGroup * kGroup + kGroup - 1);
+      const uint32_t groups = c1 / kGroup - c0 / kGroup + 1;
+      auto last_of = [&](unsigned int* counter, uint32_t count) {
         __threadfence();
-        const int n_parts = static_cast<int>(c1 - c0) + 1;
-        auto part_of = [&](int k) { return p.parts + static_cast<size_t>(k == 0 ? 2 * c0 + 1 : 2 * (c0 + k)) * F::kPartFloats; };
+        __syncthreads();
+        if (tid == 0) {
+          const unsigned int before = atomicAdd(counter, 1u);
+          if (before == count - 1) *counter = 0;
+          *arrived = before;
+        }
+        __syncthreads();
+        const bool is_last = *arrived == count - 1;
+        __threadfence();
+        return is_last;
+      };
+      // joins the parts in slots slot(0 .. count), in order; into `to`, or (null) the output
+      auto join = [&](auto slot, uint32_t count, float* to) {
 #pragma unroll
         for (int k = 0; k < kLoops; ++k) {
           const int quad = static_cast<int>(tid) + k * F::kThreads;
           if (quad >= kQuads) break;
           const int row = quad / (D / 4);
           float m = -INFINITY, total_l = 0.0f, v[4] = {};
-          for (int j = 0; j < n_parts; ++j) m = fmaxf(m, __ldcg(part_of(j) + kRows * D + row * 2));
-          for (int j = 0; j < n_parts; ++j) {
-            const float* from_part = part_of(j);
-            const float pm = __ldcg(from_part + kRows * D + row * 2);
-            const float keep = pm == -INFINITY ? 0.0f : exp2_fast(pm - m);
+          for (uint32_t j = 0; j < count; ++j) m = fmaxf(m, __ldcg(p.parts + static_cast<size_t>(slot(j)) * F::kPartFloats + kRows * D + row * 2));
+#pragma unroll 4
+          for (uint32_t j = 0; j < count; ++j) {
+            const float* from_part = p.parts + static_cast<size_t>(slot(j)) * F::kPartFloats;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(from_part + kRows * D) + row);
             const float4 x = __ldcg(reinterpret_cast<const float4*>(from_part) + quad);
-            total_l = fmaf(keep, __ldcg(from_part + kRows * D + row * 2 + 1), total_l);
+            const float keep = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - m);
+            total_l = fmaf(keep, ml.y, total_l);
             v[0] = fmaf(keep, x.x, v[0]);
             v[1] = fmaf(keep, x.y, v[1]);
             v[2] = fmaf(keep, x.z, v[2]);
             v[3] = fmaf(keep, x.w, v[3]);
           }
-          store_row(quad, v, total_l);
+          if (!to) {
+            store_row(quad, v, total_l);
+          } else {
+            __stcg(reinterpret_cast<float4*>(to) + quad, make_float4(v[0], v[1], v[2], v[3]));
+            if (quad % (D / 4) == 0) __stcg(reinterpret_cast<float2*>(to + kRows * D) + row, make_float2(m, total_l));
+          }
+        }
+      };
+      if (last_of(p.counters + slot_of(group0), group1 - group0 + 1)) {
+        if (groups == 1) {
+          join([&](uint32_t j) { return slot_of(group0 + j); }, group1 - group0 + 1, nullptr);
+        } else {
+          join([&](uint32_t j) { return slot_of(group0 + j); }, group1 - group0 + 1, p.parts + static_cast<size_t>(2 * gridDim.x + slot_of(group0)) * F::kPartFloats);
+          if (last_of(p.counters + 2 * gridDim.x + c0, groups))
+            join([&](uint32_t j) { return 2 * gridDim.x + slot_of(j == 0 ? c0 : (c0 / kGroup + j) * kGroup); }, groups, nullptr);
         }
       }
     }
-    __syncthreads();  // q_frag, row_const and warp_stat belong to the next run
-    at.off += stop - pos;
-    pos = stop;
-    if (pos < end) settle(at, p, kRows);
+    __syncthreads();  // q_frag, row_const, merge and warp_stat belong to the next run
+    pos += static_cast<unsigned>(stop - at.tile);
+    at.tile = stop;
+    if (pos < end) settle(at, p, kRows, span_at);
   }
 }
 
 template <typename T, int D, int NT>
 cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
   using F = Few<T, D, NT>;
-  static_assert(F::kSmem <= 227 * 1024, "shared memory");
+  static_assert(F::kCtas >= 1, "shared memory");
+  static_assert(F::kMerge % 16 == 0 && F::kQFrag % 16 == 0 && F::kRowConst % 16 == 0 && F::kScan % 16 == 0 && F::kSpan % 16 == 0 && F::kBars % 8 == 0 &&
+                    F::kPartFloats % 4 == 0, "alignment of the shared arrays and of the parts");
   static OncePerDevice once;
   cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_few_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem); });
   if (e != cudaSuccess) return e;
   FewParams p;
   p.a = a;
   p.group = a.heads / a.cache.kv_heads;
+  p.page_shift = 0;
+  while ((1u << p.page_shift) < a.cache.page_tokens) ++p.page_shift;
   p.parts = static_cast<float*>(env.workspace);
   p.counters = env.counters;
   p.status = env.status;
   p.least = 8;
-  // a CTA's two parts must fit the scratch; one CTA alone shares no run
-  const uint64_t fit = env.workspace ? env.workspace_bytes / (2ull * F::kPartFloats * sizeof(float)) : 0;
-  const unsigned grid = static_cast<unsigned>(std::max<uint64_t>(1, std::min<uint64_t>({static_cast<uint64_t>(env.sm_count), fit, env.counter_count})));
+  // a CTA's two parts and those of its groups must fit the scratch; one CTA alone shares no run
+  const uint64_t fit = env.workspace ? env.workspace_bytes / (4ull * F::kPartFloats * sizeof(float)) : 0;
+  const unsigned grid = static_cast<unsigned>(
+      std::max<uint64_t>(1, std::min<uint64_t>({static_cast<uint64_t>(env.sm_count) * F::kCtas, fit, env.counter_count / 3})));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(F::kThreads);
