@@ -11,16 +11,16 @@
 //   O^T [16 dims, 8 columns]   += V^T [16, 16 tokens] P^T  the words of two tokens, joined by two PRMTs
 //
 // A column is one query row (query and head of the kv head's group) for 16-bit queries; f32 queries are two binary16
-// parts in neighbouring columns, and so are their weights, whose products are added in f32 (22 bits or more).  The weights
+// parts in neighbouring columns (fixed-point, exact sums), and so are their weights; the parts' sums are added in f32.  The weights
 // get from S^T's fragment to the B fragment of P^T by one movmatrix a 8 x 8 block, nothing passes through shared memory.
 //
 //   score    s_j = scale log2(e) (s_j (q . u_j) + o_j sum q)            (base 2, f32)
-//   weight   p_j = 2^(s_j - M + 6), and P = p_j s'_j (s' the value's scale) is what enters the tensor core.  M follows the
+//   weight   p_j = 2^(s_j - M), and P = p_j s'_j (s' the value's scale) is what enters the tensor core.  M follows the
 //            largest s_j + log2 of s'_j's binade, and moves only when a weight would grow past 2^8 of it: P fits binary16
 //            with its full precision wherever it matters, whatever the size of the values.
 //   output   sum_j P_j (u'_j - 7.5) + sum_j p_j (o'_j + 7.5 s'_j): codes around zero, because sums of many uncentred
 //            ones cancel (70001 keys: 1e-3 of the result was lost); f32 queries add each 32 tokens' sums in registers,
-//            the tensor core's own chain would truncate.
+//            where the tensor core's own chain would truncate.
 //
 // Work: every (sequence, kv head, block of query rows) is a run of tiles of 32 tokens.  All runs of the call, laid end to
 // end, are cut into equal ranges, one for each CTA (one CTA an SM), by what the lengths say on the device: ragged batches
@@ -28,6 +28,7 @@
 // tiles in turn, each with a ring of its own that bulk copies fill (page by page: K codes, V codes, scales).  A run that
 // several CTAs share leaves partial sums in the scratch; the last CTA to finish joins them in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "kq_cache.cuh"
 
@@ -38,20 +39,15 @@ constexpr int kTile = 32;            // tokens a warp takes at a time
 constexpr uint32_t kFewWaitLimit = 1u << 22;
 constexpr int kFewTimeout = 40;      // status word: a copy of the cache did not arrive
 
-template <typename T>
-struct Parts {
-  static constexpr int n = 1;  // 16-bit queries enter the tensor core as they are
-};
-template <>
-struct Parts<float> {
-  static constexpr int n = 2;
-};
-
 // ---- shapes of one instance -------------------------------------------------------------------
-template <typename T, int D, int NT>
+// kPair: a query row has two neighbouring columns of an n-tile, so that a thread works on one row: the parts of f32 queries,
+// or one 16-bit query and nothing (four rows or fewer: half the softmax work of two rows a thread).  Otherwise a column each.
+template <typename T, int D, int NT, bool kPair>
 struct Few {
-  static constexpr int kParts = Parts<T>::n;
-  static constexpr int kRows = 8 * NT / kParts;      // query rows of a block
+  static constexpr bool kSplit = sizeof(T) == 4;
+  static_assert(kPair || !kSplit, "f32 queries are pairs of parts");
+  static constexpr int kOf = kPair ? 4 : 8;          // query rows of an n-tile
+  static constexpr int kRows = kOf * NT;             // ... and of a block
   static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kStages = 2;
@@ -192,11 +188,12 @@ __device__ __forceinline__ bool settle(Walk& w, const FewParams& p, int rows, Sp
   return true;
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas) attend_few_kernel(const __grid_constant__ FewParams p) {
-  using F = Few<T, D, NT>;
-  constexpr int kRows = F::kRows, kParts = F::kParts, kWarps = F::kWarps, kStages = F::kStages;
-  constexpr int kPer = kParts == 1 ? 2 : 1;  // query rows of a thread in one n-tile
+template <typename T, int D, int NT, bool kPair>
+__global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, kPair>::kCtas) attend_few_kernel(const __grid_constant__ FewParams p) {
+  using F = Few<T, D, NT, kPair>;
+  constexpr int kRows = F::kRows, kOf = F::kOf, kWarps = F::kWarps, kStages = F::kStages;
+  constexpr bool kSplit = F::kSplit;
+  constexpr int kPer = kPair ? 1 : 2;  // query rows of a thread in one n-tile
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   float* merge = reinterpret_cast<float*>(smem + F::kMerge);
@@ -285,42 +282,47 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
   // ---- copies: the warp's tiles, a ring's length ahead --------------------------------------------
   const uint32_t ring = smem_u32(smem + F::kRing) + warp * kStages * F::kTileBytes;
   uint8_t* const ring_ptr = smem + F::kRing + warp * kStages * F::kTileBytes;
-  const uint32_t P = p.a.cache.page_tokens, run = min(P, static_cast<uint32_t>(kTile));  // tokens of a piece
+  // lane 4 i + j copies array j (K codes, V codes, K scales, V scales) of the tile's i-th piece, a run of tokens in one page
+  const uint32_t P = p.a.cache.page_tokens, run = min(P, static_cast<uint32_t>(kTile));
+  const uint32_t piece = lane / 4, array = lane % 4, token_bytes = array < 2 ? D / 2 : 4;
+  const bool copies = piece * run < kTile;
+  const uint32_t from_block = (array >= 2 ? P * D : 0u) + (array & 1 ? P * token_bytes : 0u);
+  const uint32_t to_stage = (array >= 2 ? kTile * D : 0) + ((array & 1 ? kTile : 0) + piece * run) * token_bytes;
+  const uint64_t block_bytes = cache_block_bytes(P, D);
   Walk ahead = at;
   ahead.tile += static_cast<int>(warp);
   int to_issue = end - begin > warp ? static_cast<int>((end - begin - warp + kWarps - 1) / kWarps) : 0;  // tiles of this warp not passed yet
   uint32_t issued = 0, used = 0;
   auto issue_next = [&]() {
-    for (bool more = true; more && to_issue > 0; ahead.tile += kWarps, --to_issue) {
+    for (; to_issue > 0; ahead.tile += kWarps, --to_issue) {
       settle(ahead, p, kRows, span_at);
       const int first = ahead.tile * kTile;
       if (first > ahead.keys.last || first + kTile <= ahead.keys.first) continue;
-      const uint32_t stage = issued % kStages, bar = bars + stage * 8, to = ring + stage * F::kTileBytes;
-      const uint32_t key = static_cast<uint32_t>(first) + lane * run, slot = key & (P - 1);
-      const bool piece = lane * run < kTile && static_cast<int>(key) <= ahead.keys.last;
-      const uint8_t* block = piece ? cache_block(p.a.cache, p.a.batch, ahead.b, key >> p.page_shift, ahead.head) : nullptr;
-      const uint32_t have = __ballot_sync(0xffffffffu, block != nullptr), lost = __ballot_sync(0xffffffffu, piece && !block);
+      const uint32_t stage = issued % kStages, bar = bars + stage * 8;
+      const uint32_t key = static_cast<uint32_t>(first) + piece * run, index = key >> p.page_shift;
+      const bool wanted = copies && static_cast<int>(key) <= ahead.keys.last;
+      uint32_t page = 0xFFFFFFFFu;
+      if (wanted && index < p.a.batch.width) page = static_cast<uint32_t>(p.a.batch.pages[static_cast<size_t>(ahead.b) * p.a.batch.width + index]);
+      const bool have = page < p.a.cache.pages;  // a negative number is not
+      const uint32_t all = __ballot_sync(0xffffffffu, have), lost = __ballot_sync(0xffffffffu, wanted && !have);
       if (lost) {  // no such page: what it would hold is NaN
         uint32_t* params = reinterpret_cast<uint32_t*>(ring_ptr + stage * F::kTileBytes + kTile * D);
-        if (lost >> (lane / run) & 1) params[lane] = params[kTile + lane] = 0x7E007E00u;
+        if (lost >> (lane / run * 4) & 1) params[lane] = params[kTile + lane] = 0x7E007E00u;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
       if (lane == 0)
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(have) * run * (D + 8)) : "memory");
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(all) / 4 * run * (D + 8)) : "memory");
       __syncwarp();
-      if (block) {
-        const uint32_t sizes[2] = {run * (D / 2), run * 4};
-        const uint8_t* from[4] = {block + slot * (D / 2), block + (P + slot) * (D / 2), block + P * D + slot * 4, block + P * D + (P + slot) * 4};
-        const uint32_t dst[4] = {to + lane * run * (D / 2), to + (kTile + lane * run) * (D / 2), to + kTile * D + lane * run * 4,
-                                 to + kTile * D + (kTile + lane * run) * 4};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                       ::"r"(dst[i]), "l"(from[i]), "r"(sizes[i / 2]), "r"(bar) : "memory");
+      if (have) {
+        const uint8_t* from = p.a.cache.pool + (static_cast<uint64_t>(page) * p.a.cache.kv_heads + ahead.head) * block_bytes + from_block + (key & (P - 1)) * token_bytes;
+        asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(ring + stage * F::kTileBytes + to_stage), "l"(from), "r"(run * token_bytes), "r"(bar) : "memory");
       }
       ++issued;
-      more = false;
+      ahead.tile += kWarps;
+      --to_issue;
+      return;
     }
   };
   __syncwarp();
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
 #pragma unroll
       for (int o = 16; o > 0; o /= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
       sum = warp_sum(sum);
-      // 2^(13 - exponent of the largest): parts below 2^14, and their sixteenth is still a normal number where it counts
+      // 2^(13 - exponent of the largest): all below 2^14
       const int e = static_cast<int>(__float_as_uint(big) >> 23);
       const int up = big > 0.0f && e < 255 ? min(max(140 - e, -100), 120) : 0;
       const float lift = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
@@ -368,13 +370,16 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
         __half hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float x = v[i] * ((i & 1) ? lift * 0.0625f : lift);
-          hi[i] = __float2half_rn(x);
-          lo[i] = __float2half_rn(x - __half2float(hi[i]));
+          const float x = v[i] * lift, down = (i & 1) ? 0.0625f : 1.0f;
+          // f32: fixed-point parts, multiples of 8 and of 2^-8.  Their products with codes are whole multiples too, 22 bits in
+          // all of a row, so that the tensor core (which cuts each product at a place set by the largest) adds them exactly
+          const float top = kSplit ? rintf(x * 0.125f) * 8.0f : x;
+          hi[i] = __float2half_rn(top * down);
+          lo[i] = kSplit ? __float2half_rn(rintf((x - top) * 256.0f) * (0.00390625f * down)) : __ushort_as_half(0);
         }
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-          const uint32_t col = r * kParts + part, n = col / 8, c = col % 8;
+        for (int part = 0; part < (kPair ? 2 : 1); ++part) {
+          const uint32_t col = r * (kPair ? 2 : 1) + part, n = col / 8, c = col % 8;
           const __half* h = part ? lo : hi;
 #pragma unroll
           for (int half = 0; half < 2; ++half)
@@ -398,13 +403,13 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
 #pragma unroll
         for (int s = 0; s < F::kSteps; ++s) bq[n][s] = q_frag[(n * F::kSteps + s) * 32 + lane];
     }
-    // a thread's query rows in n-tile n: n * 8 / parts + t * kPer + i
+    // a thread's query rows in n-tile n: n * kOf + t * kPer + i
     float factor[NT][kPer], offset[NT][kPer];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const float4 c = row_const[n * (8 / kParts) + t * kPer + i];
+        const float4 c = row_const[n * kOf + t * kPer + i];
         factor[n][i] = c.x;
         offset[n][i] = c.y;
       }
@@ -413,8 +418,9 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < kPer; ++i) M[n][i] = -INFINITY;
-    // f32 queries: sums of a thread's dims for its one row; 16-bit ones: the accumulators (two rows)
-    float O[NT][F::kVWords * 4][2 * kPer] = {};
+    // f32 queries: sums of a thread's two dims an MMA for its one row; 16-bit ones: the accumulators of two columns
+    constexpr int kHold = kSplit ? 2 : 4, kSide = kSplit ? 1 : 2;  // row i's dims are [i] and [kSide + i]
+    float O[NT][F::kVWords * 4][kHold] = {};
 
     const int ahead_of = static_cast<int>((pos - begin) % kWarps);
     for (int tile_at = at.tile + (static_cast<int>(warp) + kWarps - ahead_of) % kWarps; tile_at < stop; tile_at += kWarps) {
@@ -441,9 +447,7 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
       uint32_t vp[2][2];        // the values' (scale, offset) of the thread's tokens
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        // f32 queries: chains of two MMAs, added in f32 (the tensor core truncates)
-        constexpr int kChains = kParts == 2 ? F::kSteps / 2 : 1;
-        float acc[NT][kChains][4] = {};
+        float acc[NT][4] = {};
         const uint8_t* row0 = tile + (sub * 16 + token_g) * (D / 2);
         const uint8_t* row1 = row0 + 8 * (D / 2);
         uint32_t x0[F::kWords], x1[F::kWords];
@@ -466,7 +470,7 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
             for (int n = 0; n < NT; ++n) {
               const uint2 bb = F::kQInRegisters ? bq[F::kQInRegisters ? n : 0][F::kQInRegisters ? 2 * w + half : 0]
                                                 : q_frag[(n * F::kSteps + 2 * w + half) * 32 + lane];
-              mma16816(acc[n][w % kChains], a & 0x000F000Fu, b & 0x000F000Fu, a & 0x00F000F0u, b & 0x00F000F0u, bb.x, bb.y);
+              mma16816(acc[n], a & 0x000F000Fu, b & 0x000F000Fu, a & 0x00F000F0u, b & 0x00F000F0u, bb.x, bb.y);
             }
           }
         const uint32_t* params = reinterpret_cast<const uint32_t*>(tile + kTile * D) + sub * 16 + token_g;
@@ -479,42 +483,49 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-              float dot = kParts == 2 ? acc[n][0][2 * half] + acc[n][0][2 * half + 1] : acc[n][0][2 * half + i];
-#pragma unroll
-              for (int c = 1; c < kChains; ++c) dot += acc[n][c][2 * half] + acc[n][c][2 * half + 1];
+              const float dot = kSplit ? acc[n][2 * half] + acc[n][2 * half + 1] : acc[n][2 * half + i];
               s[sub][n][i][half] = fmaf(dot, so.x * factor[n][i], so.y * offset[n][i]);
             }
         }
       }
-      uint32_t scale_bits[4] = {vp[0][0], vp[0][1], vp[1][0], vp[1][1]};
-      if (!whole) {
-        uint32_t seen = 0;
+      // the largest binade of the values' scales that a row sees (at least log2 of a scale)
+      auto binade_of = [](uint32_t bits) { return static_cast<float>(max(static_cast<int>(bits >> 10), 1) - 14); };
+      const uint32_t scale_bits[4] = {vp[0][0] & 0x7C00u, vp[0][1] & 0x7C00u, vp[1][0] & 0x7C00u, vp[1][1] & 0x7C00u};
+      float binade[NT][kPer];
+      if (whole) {
+        const float common = binade_of(max(max(scale_bits[0], scale_bits[1]), max(scale_bits[2], scale_bits[3])));
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) binade[n][i] = common;
+      } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            const float4 c = row_const[n * (8 / kParts) + t * kPer + i];
+            const float4 c = row_const[n * kOf + t * kPer + i];
+            uint32_t big = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int key = first + j * 8 + static_cast<int>(token_g);
               if (key > __float_as_int(c.z) || key < __float_as_int(c.w)) s[j / 2][n][i][j % 2] = -INFINITY;
-              else seen |= 1u << j;
+              else big = max(big, scale_bits[j]);
             }
+            binade[n][i] = binade_of(big);
           }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (!(seen >> j & 1)) scale_bits[j] = 0;  // what is not seen may hold anything
       }
-      // M: the largest score and the largest binade of the values' scales (at least log2 of a scale)
-      const uint32_t big_scale = max(max(scale_bits[0] & 0x7C00u, scale_bits[1] & 0x7C00u), max(scale_bits[2] & 0x7C00u, scale_bits[3] & 0x7C00u));
-      const float binade = static_cast<float>(max(static_cast<int>(big_scale >> 10), 1) - 14);
+      // M: the largest score with its binade
       bool more = false;
       float top[NT][kPer];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          top[n][i] = fmaxf(fmaxf(s[0][n][i][0], s[0][n][i][1]), fmaxf(s[1][n][i][0], s[1][n][i][1])) + binade;
+          top[n][i] = fmaxf(fmaxf(s[0][n][i][0], s[0][n][i][1]), fmaxf(s[1][n][i][0], s[1][n][i][1])) + binade[n][i];
+          if constexpr (kSplit) {  // the tile's largest
+#pragma unroll
+            for (int o = 4; o < 32; o *= 2) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], o));
+          }
           more |= top[n][i] > M[n][i] + 8.0f;
         }
       if (__any_sync(0xffffffffu, more)) {
@@ -523,8 +534,10 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
             float m = top[n][i];
+            if constexpr (!kSplit) {
 #pragma unroll
-            for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+              for (int o = 4; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            }
             m = fmaxf(m, M[n][i]);
             const float keep = m == -INFINITY ? 1.0f : exp2_fast(M[n][i] - m);
             M[n][i] = m;
@@ -533,45 +546,59 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
 #pragma unroll
             for (int d = 0; d < F::kVWords * 4; ++d) {
               O[n][d][i] *= keep;
-              O[n][d][kPer + i] *= keep;
+              O[n][d][kSide + i] *= keep;
             }
           }
       }
-      float shift[NT][kPer];
+      float shift[NT][kPer], lift[NT], drop[NT];  // f32: P is lifted to just below 2^14 in each tile, and back when its sums are added
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) shift[n][i] = M[n][i] == -INFINITY ? 6.0f : 6.0f - M[n][i];
-      float tile_acc[kParts == 2 ? NT : 1][kParts == 2 ? F::kVWords * 4 : 1][4] = {};
+        for (int i = 0; i < kPer; ++i) shift[n][i] = M[n][i] == -INFINITY ? 0.0f : -M[n][i];
+        const int up = kSplit ? min(max(14 - static_cast<int>(ceilf(top[n][0] + shift[n][0])), 0), 120) : 6;
+        lift[n] = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+        drop[n] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+      }
+      uint32_t bp[2][NT][2];
+      auto weigh = [&](auto all_seen) {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&vp[sub][half]));
+            const float mid = fmaf(7.5f, so.x, so.y);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float pv[kPer];
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) {
+                const float sc = s[sub][n][i][half], w = exp2_fast(sc + shift[n][i]);
+                l[n][i] += w;
+                if (decltype(all_seen)::value || sc != -INFINITY) {
+                  centre[n][i] = fmaf(w, mid, centre[n][i]);
+                  pv[i] = w * so.x;
+                } else {
+                  pv[i] = 0.0f;  // what is not seen may hold anything
+                }
+                pv[i] *= lift[n];
+              }
+              uint32_t both;
+              if constexpr (kSplit) {  // fixed-point parts, as the queries'
+                const float hi = rintf(pv[0] * 0.125f) * 8.0f;
+                both = pack_half2(__float2half_rn(hi), __float2half_rn(rintf((pv[0] - hi) * 256.0f) * 0.00390625f));
+              } else {
+                const __half2 h = __floats2half2_rn(pv[0], kPair ? 0.0f : pv[kPer - 1]);
+                both = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              bp[sub][n][half] = transposed(both);
+            }
+          }
+      };
+      if (whole) weigh(std::true_type());
+      else weigh(std::false_type());
+      float tile_acc[kSplit ? NT : 1][kSplit ? F::kVWords * 4 : 1][4] = {};
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        uint32_t bp[NT][2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&vp[sub][half]));
-          const float mid = fmaf(7.5f, so.x, so.y);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float pv[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const float w = exp2_fast(s[sub][n][i][half] + shift[n][i]);
-              l[n][i] += w;
-              pv[i] = w * so.x;
-              float mid_w = w * mid;
-              if (!whole && s[sub][n][i][half] == -INFINITY) pv[i] = mid_w = 0.0f;
-              centre[n][i] += mid_w;
-            }
-            if constexpr (kParts == 2) {
-              const __half hi = __float2half_rn(pv[0]);
-              bp[n][half] = pack_half2(hi, __float2half_rn(pv[0] - __half2float(hi)));
-            } else {
-              const __half2 both = __floats2half2_rn(pv[0], pv[kPer - 1]);
-              bp[n][half] = *reinterpret_cast<const uint32_t*>(&both);
-            }
-            bp[n][half] = transposed(bp[n][half]);
-          }
-        }
         const uint8_t* v0 = tile + kTile * (D / 2) + sub * 16 * (D / 2) + g * (D / 16);
         uint32_t xa[F::kVWords], xb[F::kVWords], xc[F::kVWords], xd[F::kVWords];
         auto load_v = [&](uint32_t (&x)[F::kVWords], uint32_t token) {
@@ -598,19 +625,19 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              if constexpr (kParts == 2) mma16816(tile_acc[n][w * 4 + i], a[0], a[1], a[2], a[3], bp[n][0], bp[n][1]);
-              else mma16816(O[n][w * 4 + i], a[0], a[1], a[2], a[3], bp[n][0], bp[n][1]);
+              if constexpr (kSplit) mma16816(tile_acc[n][w * 4 + i], a[0], a[1], a[2], a[3], bp[sub][n][0], bp[sub][n][1]);
+              else mma16816(O[n][w * 4 + i], a[0], a[1], a[2], a[3], bp[sub][n][0], bp[sub][n][1]);
             }
           }
         }
       }
-      if constexpr (kParts == 2) {
+      if constexpr (kSplit) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int d = 0; d < F::kVWords * 4; ++d) {
-            O[n][d][0] += tile_acc[n][d][0] + tile_acc[n][d][1];
-            O[n][d][1] += tile_acc[n][d][2] + tile_acc[n][d][3];
+            O[n][d][0] = fmaf(tile_acc[n][d][0] + tile_acc[n][d][1], drop[n], O[n][d][0]);
+            O[n][d][1] = fmaf(tile_acc[n][d][2] + tile_acc[n][d][3], drop[n], O[n][d][1]);
           }
       }
       ++used;
@@ -633,13 +660,14 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          float* st = warp_stat + (warp * kRows + n * (8 / kParts) + t * kPer + i) * 3;
+          float* st = warp_stat + (warp * kRows + n * kOf + t * kPer + i) * 3;
           st[0] = M[n][i];
           st[1] = l[n][i];
           st[2] = centre[n][i];
         }
     }
-    // the codes' powers of two: even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
+    // the codes' powers of two, even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20, and the 16-bit weights' 2^6
+    constexpr float kEven = kSplit ? 8388608.0f : 131072.0f, kOdd = kSplit ? 1048576.0f : 16384.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -647,10 +675,11 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
 #pragma unroll
         for (int w = 0; w < F::kVWords; ++w)
 #pragma unroll
-          for (int half = 0; half < 2; ++half)  // dims 0..3, then 4..7 of the thread's word
-            *reinterpret_cast<float4*>(merge + (warp * kRows + n * (8 / kParts) + t * kPer + i) * D + g * (D / 8) + w * 8 + half * 4) =
-                make_float4(O[n][w * 4][half * kPer + i] * 8388608.0f, O[n][w * 4 + 1][half * kPer + i] * 1048576.0f,
-                            O[n][w * 4 + 2][half * kPer + i] * 8388608.0f, O[n][w * 4 + 3][half * kPer + i] * 1048576.0f);
+          for (int half = 0; half < 2; ++half) {  // dims 0..3, then 4..7 of the thread's word
+            const int e = half * kSide + i;
+            *reinterpret_cast<float4*>(merge + (warp * kRows + n * kOf + t * kPer + i) * D + g * (D / 8) + w * 8 + half * 4) =
+                make_float4(O[n][w * 4][e] * kEven, O[n][w * 4 + 1][e] * kOdd, O[n][w * 4 + 2][e] * kEven, O[n][w * 4 + 3][e] * kOdd);
+          }
     __syncthreads();
     constexpr int kQuads = kRows * D / 4;  // outputs of the block, by four
     constexpr int kLoops = (kQuads + F::kThreads - 1) / F::kThreads;
@@ -760,14 +789,14 @@ __global__ void __launch_bounds__(Few<T, D, NT>::kThreads, Few<T, D, NT>::kCtas)
   }
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kPair>
 cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
-  using F = Few<T, D, NT>;
+  using F = Few<T, D, NT, kPair>;
   static_assert(F::kCtas >= 1, "shared memory");
   static_assert(F::kMerge % 16 == 0 && F::kQFrag % 16 == 0 && F::kRowConst % 16 == 0 && F::kScan % 16 == 0 && F::kSpan % 16 == 0 && F::kBars % 8 == 0 &&
                     F::kPartFloats % 4 == 0, "alignment of the shared arrays and of the parts");
   static OncePerDevice once;
-  cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_few_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem); });
+  cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_few_kernel<T, D, NT, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem); });
   if (e != cudaSuccess) return e;
   FewParams p;
   p.a = a;
@@ -792,15 +821,22 @@ cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = env.overlap ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, attend_few_kernel<T, D, NT>, p);
+  return cudaLaunchKernelEx(&cfg, attend_few_kernel<T, D, NT, kPair>, p);
 }
 
+// By the rows that a sequence's new tokens make with one kv head; beyond the widest block, blocks of it.
 template <typename T, int D>
 cudaError_t few_of(const LaunchEnv& env, const AttendArgs& a) {
-  const uint64_t columns = static_cast<uint64_t>(a.batch.most) * (a.heads / a.cache.kv_heads) * Parts<T>::n;
-  if (columns <= 8) return few_as<T, D, 1>(env, a);
-  if (columns <= 16 || D > 128) return few_as<T, D, 2>(env, a);
-  if constexpr (D <= 128) return few_as<T, D, 4>(env, a);
+  const uint64_t rows = static_cast<uint64_t>(a.batch.most) * (a.heads / a.cache.kv_heads);
+  if (rows <= 4) return few_as<T, D, 1, true>(env, a);
+  if constexpr (sizeof(T) == 4) {
+    if (rows <= 8 || D > 128) return few_as<T, D, 2, true>(env, a);
+    if constexpr (D <= 128) return few_as<T, D, 4, true>(env, a);
+  } else {
+    if (rows <= 8) return few_as<T, D, 1, false>(env, a);
+    if (rows <= 16 || D > 128) return few_as<T, D, 2, false>(env, a);
+    if constexpr (D <= 128) return few_as<T, D, 4, false>(env, a);
+  }
   return cudaErrorInvalidValue;
 }
 
