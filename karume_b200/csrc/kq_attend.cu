@@ -57,6 +57,7 @@ struct Few {
   static constexpr int kTileBytes = kTile * (D + 8);
   static constexpr bool kQInRegisters = NT * kSteps <= 16;
   static constexpr int kPartFloats = kRows * (D + 2);  // a partial result in the scratch: sums, M, l
+  static constexpr int kShort = 16;                    // tiles of a run that is not shared by CTAs
   static constexpr int kSpans = 128;                   // sequences whose lengths are kept in shared memory
 
   static constexpr int kRing = 0;
@@ -65,7 +66,7 @@ struct Few {
   static constexpr int kRowConst = kQFrag + NT * kSteps * 32 * 8;      // factor, offset, last key, first key of each row
   static constexpr int kWarpStat = kRowConst + kRows * 16;             // [kWarps][kRows] x (M, l, centre sum)
   static constexpr int kScan = kWarpStat + (kWarps * kRows * 12 + 15) / 16 * 16;  // sums of the warps, what the scan found
-  static constexpr int kSpan = kScan + kWarps * 8 + 16;
+  static constexpr int kSpan = kScan + kWarps * 8 + 32 + kWarps * 8;
   static constexpr int kBars = kSpan + kSpans * 16;
   static constexpr int kMisc = kBars + kWarps * kStages * 8;
   static constexpr int kSmem = kMisc + 16;
@@ -81,7 +82,6 @@ struct FewParams {
   float* parts;            // [4 * grid][kPartFloats]: two of a CTA, and two of the groups that begin with it
   unsigned int* counters;  // [3 * grid], zero between launches
   int* status;
-  uint32_t least;          // tiles a CTA should have at least
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
   float4* row_const = reinterpret_cast<float4*>(smem + F::kRowConst);
   float* warp_stat = reinterpret_cast<float*>(smem + F::kWarpStat);
   unsigned long long* scan = reinterpret_cast<unsigned long long*>(smem + F::kScan);
-  unsigned long long* found = scan + kWarps;  // sequence, tiles in front of it
+  unsigned long long* found = scan + kWarps;  // sequence and tiles in front of it, of both cuts; runs of each warp's sequences
   int4* spans = reinterpret_cast<int4*>(smem + F::kSpan);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F::kMisc);
   volatile unsigned int* arrived = reinterpret_cast<volatile unsigned int*>(smem + F::kMisc + 4);
@@ -216,11 +216,13 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
   const uint32_t sequences = p.a.batch.sequences, each = (sequences + F::kThreads - 1) / F::kThreads;
   const bool kept = sequences <= F::kSpans;
   unsigned long long mine = 0;
+  uint32_t mine_runs = 0;
   for (uint32_t b = tid * each; b < min((tid + 1) * each, sequences); ++b) {
     const Span span = span_of(p.a.batch, b);
     if (kept) spans[b] = make_int4(span.first, span.count, span.length, 0);
     const Runs r = runs_of(p, span, kRows);
     mine += static_cast<unsigned long long>(r.units) * static_cast<unsigned>(r.tiles);
+    mine_runs += r.units;
     if (span.length == 0 && blockIdx.x == b % gridDim.x)  // an idle sequence's rows are zero
       for (int i = 0; i < span.count; ++i)
         for (uint32_t d = 0; d < p.a.heads * D; d += 4) {
@@ -234,12 +236,15 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
     const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= static_cast<uint32_t>(o)) upto += v;
   }
+  const uint32_t warp_runs = __reduce_add_sync(0xffffffffu, mine_runs);
   if (lane == 31) scan[warp] = upto;
+  if (lane == 30) found[4 + warp] = warp_runs;
   __syncthreads();
-  unsigned long long total = 0;
+  unsigned long long total = 0, runs = 0;
   for (int i = 0; i < kWarps; ++i) {
     if (static_cast<uint32_t>(i) < warp) upto += scan[i];
     total += scan[i];
+    runs += found[4 + i];
   }
   // rows that belong to no sequence are zero
   if (p.a.batch.starts) {
@@ -251,33 +256,49 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       for (uint32_t d = tid * 4; d < p.a.heads * D; d += F::kThreads * 4) store4(out + d, zero);
     }
   }
-  const unsigned long long ranges = min(static_cast<unsigned long long>(gridDim.x), max(total / p.least, 1ull));
-  const unsigned long long per = max((total + ranges - 1) / ranges, 1ull);
-  const unsigned long long begin = min(blockIdx.x * per, total), end = min(begin + per, total);
-  if (begin >= end) return;
-  if (upto - mine <= begin && begin < upto) {
-    found[0] = tid * each;
-    found[1] = upto - mine;
-  }
+  if (total == 0) return;
+  // equal ranges, of eight tiles at least, or of a run's where those are shorter: then as many CTAs as runs share the work
+  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, min(8ull, (total + runs - 1) / runs));
+  const unsigned long long cut[2] = {blockIdx.x * per, min(blockIdx.x * per + per, total)};
+  if (cut[0] >= total) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (upto - mine <= cut[i] && cut[i] < upto) {
+      found[2 * i] = tid * each;
+      found[2 * i + 1] = upto - mine;
+    }
   __syncthreads();
   auto span_at = [&](uint32_t b) {
     if (!kept) return span_of(p.a.batch, b);
     const int4 v = spans[b];
     return Span{v.x, v.y, v.z};
   };
-  Walk at;
-  at.b = static_cast<uint32_t>(found[0]);
-  at.runs = runs_of(p, span_at(at.b), kRows);
-  unsigned long long skip = begin - found[1];
-  while (skip >= static_cast<unsigned long long>(at.runs.units) * static_cast<unsigned>(at.runs.tiles)) {  // sequences of one thread's share
-    skip -= static_cast<unsigned long long>(at.runs.units) * static_cast<unsigned>(at.runs.tiles);
-    at.runs = runs_of(p, span_at(++at.b), kRows);
-  }
-  const uint32_t unit = static_cast<uint32_t>(skip / static_cast<unsigned>(at.runs.tiles));
-  at.head = unit / at.runs.blocks;
-  at.block = unit % at.runs.blocks;
-  at.tile = at.runs.tile_lo + static_cast<int>(skip % static_cast<unsigned>(at.runs.tiles));
-  at.keys = keys_of(p, at.runs, at.block, kRows);
+  // Walk to tile number x; a run of up to kShort tiles is not cut but belongs to the range it begins in
+  auto locate = [&](unsigned long long& x, int i) {
+    Walk w;
+    w.b = static_cast<uint32_t>(found[2 * i]);
+    w.runs = runs_of(p, span_at(w.b), kRows);
+    unsigned long long skip = x - found[2 * i + 1];
+    while (skip >= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles)) {  // sequences of one thread's share
+      skip -= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles);
+      w.runs = runs_of(p, span_at(++w.b), kRows);
+    }
+    const uint32_t unit = static_cast<uint32_t>(skip / static_cast<unsigned>(w.runs.tiles));
+    int in = static_cast<int>(skip % static_cast<unsigned>(w.runs.tiles));
+    if (w.runs.tiles <= F::kShort) {
+      x -= static_cast<unsigned>(in);
+      in = 0;
+    }
+    w.head = unit / w.runs.blocks;
+    w.block = unit % w.runs.blocks;
+    w.tile = w.runs.tile_lo + in;
+    w.keys = keys_of(p, w.runs, w.block, kRows);
+    return w;
+  };
+  unsigned long long begin = cut[0], end = cut[1];
+  Walk at = locate(begin, 0);
+  if (end < total) locate(end, 1);
+  if (begin >= end) return;
 
   // ---- copies: the warp's tiles, a ring's length ahead --------------------------------------------
   const uint32_t ring = smem_u32(smem + F::kRing) + warp * kStages * F::kTileBytes;
@@ -293,16 +314,28 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
   ahead.tile += static_cast<int>(warp);
   int to_issue = end - begin > warp ? static_cast<int>((end - begin - warp + kWarps - 1) / kWarps) : 0;  // tiles of this warp not passed yet
   uint32_t issued = 0, used = 0;
-  auto issue_next = [&]() {
-    for (; to_issue > 0; ahead.tile += kWarps, --to_issue) {
+  // the next tile to copy: its page number is loaded a tile's time before it is needed
+  bool wanted = false;
+  uint32_t page = 0, key = 0, head_ahead = 0;
+  bool waiting = false;
+  auto look_ahead = [&]() {
+    waiting = false;
+    for (; to_issue > 0 && !waiting; ahead.tile += kWarps, --to_issue) {
       settle(ahead, p, kRows, span_at);
       const int first = ahead.tile * kTile;
       if (first > ahead.keys.last || first + kTile <= ahead.keys.first) continue;
+      key = static_cast<uint32_t>(first) + piece * run;
+      head_ahead = ahead.head;
+      const uint32_t index = key >> p.page_shift;
+      wanted = copies && static_cast<int>(key) <= ahead.keys.last;
+      page = 0xFFFFFFFFu;
+      if (wanted && index < p.a.batch.width) page = static_cast<uint32_t>(__ldg(p.a.batch.pages + static_cast<size_t>(ahead.b) * p.a.batch.width + index));
+      waiting = true;
+    }
+  };
+  auto issue_next = [&]() {
+    if (waiting) {
       const uint32_t stage = issued % kStages, bar = bars + stage * 8;
-      const uint32_t key = static_cast<uint32_t>(first) + piece * run, index = key >> p.page_shift;
-      const bool wanted = copies && static_cast<int>(key) <= ahead.keys.last;
-      uint32_t page = 0xFFFFFFFFu;
-      if (wanted && index < p.a.batch.width) page = static_cast<uint32_t>(p.a.batch.pages[static_cast<size_t>(ahead.b) * p.a.batch.width + index]);
       const bool have = page < p.a.cache.pages;  // a negative number is not
       const uint32_t all = __ballot_sync(0xffffffffu, have), lost = __ballot_sync(0xffffffffu, wanted && !have);
       if (lost) {  // no such page: what it would hold is NaN
@@ -315,17 +348,16 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(all) / 4 * run * (D + 8)) : "memory");
       __syncwarp();
       if (have) {
-        const uint8_t* from = p.a.cache.pool + (static_cast<uint64_t>(page) * p.a.cache.kv_heads + ahead.head) * block_bytes + from_block + (key & (P - 1)) * token_bytes;
+        const uint8_t* from = p.a.cache.pool + (static_cast<uint64_t>(page) * p.a.cache.kv_heads + head_ahead) * block_bytes + from_block + (key & (P - 1)) * token_bytes;
         asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                      ::"r"(ring + stage * F::kTileBytes + to_stage), "l"(from), "r"(run * token_bytes), "r"(bar) : "memory");
       }
       ++issued;
-      ahead.tile += kWarps;
-      --to_issue;
-      return;
+      look_ahead();
     }
   };
   __syncwarp();
+  look_ahead();
   for (int i = 0; i < kStages; ++i) issue_next();
 
   const uint32_t odd = t & 1;  // the order of a thread's tokens in a pair of rows: neighbouring rows fall into different banks
@@ -731,17 +763,15 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       const uint32_t group0 = max(c0, blockIdx.x / kGroup * kGroup), group1 = min(c1, blockIdx.x / kGroup * kGroup + kGroup - 1);
       const uint32_t groups = c1 / kGroup - c0 / kGroup + 1;
       auto last_of = [&](unsigned int* counter, uint32_t count) {
-        __threadfence();
         __syncthreads();
         if (tid == 0) {
-          const unsigned int before = atomicAdd(counter, 1u);
+          unsigned int before;
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
           if (before == count - 1) *counter = 0;
           *arrived = before;
         }
         __syncthreads();
-        const bool is_last = *arrived == count - 1;
-        __threadfence();
-        return is_last;
+        return *arrived == count - 1;
       };
       // joins the parts in slots slot(0 .. count), in order; into `to`, or (null) the output
       auto join = [&](auto slot, uint32_t count, float* to) {
@@ -751,18 +781,36 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
           if (quad >= kQuads) break;
           const int row = quad / (D / 4);
           float m = -INFINITY, total_l = 0.0f, v[4] = {};
-          for (uint32_t j = 0; j < count; ++j) m = fmaxf(m, __ldcg(p.parts + static_cast<size_t>(slot(j)) * F::kPartFloats + kRows * D + row * 2));
-#pragma unroll 4
-          for (uint32_t j = 0; j < count; ++j) {
-            const float* from_part = p.parts + static_cast<size_t>(slot(j)) * F::kPartFloats;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(from_part + kRows * D) + row);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(from_part) + quad);
-            const float keep = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - m);
-            total_l = fmaf(keep, ml.y, total_l);
-            v[0] = fmaf(keep, x.x, v[0]);
-            v[1] = fmaf(keep, x.y, v[1]);
-            v[2] = fmaf(keep, x.z, v[2]);
-            v[3] = fmaf(keep, x.w, v[3]);
+          constexpr uint32_t kBatch = 8;
+          for (uint32_t j0 = 0; j0 < count; j0 += kBatch) {
+            float2 ml[kBatch];
+            float4 x[kBatch];
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+              const float* from_part = p.parts + static_cast<size_t>(slot(min(j0 + j, count - 1))) * F::kPartFloats;
+              ml[j] = __ldcg(reinterpret_cast<const float2*>(from_part + kRows * D) + row);
+              x[j] = __ldcg(reinterpret_cast<const float4*>(from_part) + quad);
+            }
+            float now = m;
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+              if (j0 + j >= count) ml[j] = make_float2(-INFINITY, 0.0f);
+              now = fmaxf(now, ml[j].x);
+            }
+            const float before = m == -INFINITY ? 0.0f : exp2_fast(m - now);
+            m = now;
+            total_l *= before;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] *= before;
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+              const float keep = ml[j].x == -INFINITY ? 0.0f : exp2_fast(ml[j].x - m);
+              total_l = fmaf(keep, ml[j].y, total_l);
+              v[0] = fmaf(keep, x[j].x, v[0]);
+              v[1] = fmaf(keep, x[j].y, v[1]);
+              v[2] = fmaf(keep, x[j].z, v[2]);
+              v[3] = fmaf(keep, x[j].w, v[3]);
+            }
           }
           if (!to) {
             store_row(quad, v, total_l);
@@ -806,7 +854,6 @@ cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
   p.parts = static_cast<float*>(env.workspace);
   p.counters = env.counters;
   p.status = env.status;
-  p.least = 8;
   // a CTA's two parts and those of its groups must fit the scratch; one CTA alone shares no run
   const uint64_t fit = env.workspace ? env.workspace_bytes / (4ull * F::kPartFloats * sizeof(float)) : 0;
   const unsigned grid = static_cast<unsigned>(
