@@ -19,7 +19,7 @@
 //            largest s_j + log2 of s'_j's binade, and moves only when a weight would grow past 2^8 of it: P fits binary16
 //            with its full precision wherever it matters, whatever the size of the values.
 //   output   sum_j P_j (u'_j - 7.5) + sum_j p_j (o'_j + 7.5 s'_j): codes around zero, because sums of many uncentred
-//            ones cancel (70001 keys: 1e-3 of the result was lost); f32 queries add each 32 tokens' sums in registers,
+//            ones cancel (70001 keys: 1e-3 of the result was lost); f32 queries add each tile's sums in registers,
 //            where the tensor core's own chain would truncate.
 //
 // Work: every (sequence, kv head, block of query rows) is a run of tiles of 32 tokens.  All runs of the call, laid end to
@@ -35,7 +35,6 @@
 namespace kq {
 namespace {
 
-constexpr int kTile = 32;            // tokens a warp takes at a time
 constexpr uint32_t kFewWaitLimit = 1u << 22;
 constexpr int kFewTimeout = 40;      // status word: a copy of the cache did not arrive
 
@@ -46,6 +45,11 @@ template <typename T, int D, int NT, bool kPair>
 struct Few {
   static constexpr bool kSplit = sizeof(T) == 4;
   static_assert(kPair || !kSplit, "f32 queries are pairs of parts");
+  // Tokens a warp takes at a time.  What a tile costs whatever its size (the wait, the next copies, the check of M) is a third
+  // of 32 tokens' instructions: 64 of them gain 10 % where registers and shared memory leave room (64 sequences, bf16: 169 -> 152 us),
+  // and lose as much on the wide forms.
+  static constexpr int kTile = NT == 1 && D <= 128 ? 64 : 32;
+  static constexpr int kSubs = kTile / 16;
   static constexpr int kOf = kPair ? 4 : 8;          // query rows of an n-tile
   static constexpr int kRows = kOf * NT;             // ... and of a block
   static constexpr int kWarps = 4;
@@ -57,7 +61,7 @@ struct Few {
   static constexpr int kTileBytes = kTile * (D + 8);
   static constexpr bool kQInRegisters = NT * kSteps <= 16;
   static constexpr int kPartFloats = kRows * (D + 2);  // a partial result in the scratch: sums, M, l
-  static constexpr int kShort = 16;                    // tiles of a run that is not shared by CTAs
+  static constexpr int kShort = 512 / kTile;                    // tiles of a run that is not shared by CTAs
   static constexpr int kSpans = 128;                   // sequences whose lengths are kept in shared memory
 
   static constexpr int kRing = 0;
@@ -132,14 +136,14 @@ struct Runs {
   int tile_lo, tiles;
   uint32_t blocks, units;
 };
-__device__ __forceinline__ Runs runs_of(const FewParams& p, const Span& span, int rows) {
+__device__ __forceinline__ Runs runs_of(const FewParams& p, const Span& span, int rows, int tile) {
   Runs r;
   r.span = span;
   const int first = span.length - span.count;  // position of the first query
   const int window = static_cast<int>(min(p.a.window, 0x7fffffffu));
   const int from = window && first + 1 > window ? first + 1 - window : 0;
-  r.tile_lo = from / kTile;
-  r.tiles = (span.length - 1) / kTile + 1 - r.tile_lo;
+  r.tile_lo = from / tile;
+  r.tiles = (span.length - 1) / tile + 1 - r.tile_lo;
   r.blocks = span.length > 0 ? (static_cast<uint32_t>(span.count) * p.group + rows - 1) / rows : 0;  // idle: no work
   r.units = r.blocks * p.a.cache.kv_heads;
   return r;
@@ -171,13 +175,13 @@ struct Walk {
 };
 // Carries a tile number beyond the run's end into the following runs; false behind the last one.
 template <typename SpanAt>
-__device__ __forceinline__ bool settle(Walk& w, const FewParams& p, int rows, SpanAt span_at) {
+__device__ __forceinline__ bool settle(Walk& w, const FewParams& p, int rows, int tile, SpanAt span_at) {
   while (w.tile >= w.runs.tile_lo + w.runs.tiles || w.runs.units == 0) {
     if (w.runs.units != 0) w.tile -= w.runs.tiles;
     if (w.runs.units == 0 || (++w.block == w.runs.blocks && ++w.head == p.a.cache.kv_heads)) {
       if (++w.b >= p.a.batch.sequences) return false;
       w.tile -= w.runs.units != 0 ? w.runs.tile_lo : 0;
-      w.runs = runs_of(p, span_at(w.b), rows);
+      w.runs = runs_of(p, span_at(w.b), rows, tile);
       w.tile += w.runs.units != 0 ? w.runs.tile_lo : 0;
       w.head = w.block = 0;
     } else if (w.block == w.runs.blocks) {
@@ -191,7 +195,7 @@ __device__ __forceinline__ bool settle(Walk& w, const FewParams& p, int rows, Sp
 template <typename T, int D, int NT, bool kPair>
 __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, kPair>::kCtas) attend_few_kernel(const __grid_constant__ FewParams p) {
   using F = Few<T, D, NT, kPair>;
-  constexpr int kRows = F::kRows, kOf = F::kOf, kWarps = F::kWarps, kStages = F::kStages;
+  constexpr int kRows = F::kRows, kOf = F::kOf, kWarps = F::kWarps, kStages = F::kStages, kTile = F::kTile, kSubs = F::kSubs;
   constexpr bool kSplit = F::kSplit;
   constexpr int kPer = kPair ? 1 : 2;  // query rows of a thread in one n-tile
   extern __shared__ __align__(128) uint8_t smem[];
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
   for (uint32_t b = tid * each; b < min((tid + 1) * each, sequences); ++b) {
     const Span span = span_of(p.a.batch, b);
     if (kept) spans[b] = make_int4(span.first, span.count, span.length, 0);
-    const Runs r = runs_of(p, span, kRows);
+    const Runs r = runs_of(p, span, kRows, kTile);
     mine += static_cast<unsigned long long>(r.units) * static_cast<unsigned>(r.tiles);
     mine_runs += r.units;
     if (span.length == 0 && blockIdx.x == b % gridDim.x)  // an idle sequence's rows are zero
@@ -257,8 +261,8 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
     }
   }
   if (total == 0) return;
-  // equal ranges, of eight tiles at least, or of a run's where those are shorter: then as many CTAs as runs share the work
-  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, min(8ull, (total + runs - 1) / runs));
+  // equal ranges, of 256 tokens at least, or of a run's where those are shorter: then as many CTAs as runs share the work
+  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, min(256ull / kTile, (total + runs - 1) / runs));
   const unsigned long long cut[2] = {blockIdx.x * per, min(blockIdx.x * per + per, total)};
   if (cut[0] >= total) return;
 #pragma unroll
@@ -277,11 +281,11 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
   auto locate = [&](unsigned long long& x, int i) {
     Walk w;
     w.b = static_cast<uint32_t>(found[2 * i]);
-    w.runs = runs_of(p, span_at(w.b), kRows);
+    w.runs = runs_of(p, span_at(w.b), kRows, kTile);
     unsigned long long skip = x - found[2 * i + 1];
     while (skip >= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles)) {  // sequences of one thread's share
       skip -= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles);
-      w.runs = runs_of(p, span_at(++w.b), kRows);
+      w.runs = runs_of(p, span_at(++w.b), kRows, kTile);
     }
     const uint32_t unit = static_cast<uint32_t>(skip / static_cast<unsigned>(w.runs.tiles));
     int in = static_cast<int>(skip % static_cast<unsigned>(w.runs.tiles));
@@ -309,23 +313,23 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
   const bool copies = piece * run < kTile;
   const uint32_t from_block = (array >= 2 ? P * D : 0u) + (array & 1 ? P * token_bytes : 0u);
   const uint32_t to_stage = (array >= 2 ? kTile * D : 0) + ((array & 1 ? kTile : 0) + piece * run) * token_bytes;
-  const uint64_t block_bytes = cache_block_bytes(P, D);
+  const uint32_t block_bytes = static_cast<uint32_t>(cache_block_bytes(P, D)), page_bytes = block_bytes * p.a.cache.kv_heads;  // 1024 heads: 70 MB at most
   Walk ahead = at;
   ahead.tile += static_cast<int>(warp);
   int to_issue = end - begin > warp ? static_cast<int>((end - begin - warp + kWarps - 1) / kWarps) : 0;  // tiles of this warp not passed yet
   uint32_t issued = 0, used = 0;
   // the next tile to copy: its page number is loaded a tile's time before it is needed
   bool wanted = false;
-  uint32_t page = 0, key = 0, head_ahead = 0;
+  uint32_t page = 0, in_page = 0;
   bool waiting = false;
   auto look_ahead = [&]() {
     waiting = false;
     for (; to_issue > 0 && !waiting; ahead.tile += kWarps, --to_issue) {
-      settle(ahead, p, kRows, span_at);
+      settle(ahead, p, kRows, kTile, span_at);
       const int first = ahead.tile * kTile;
       if (first > ahead.keys.last || first + kTile <= ahead.keys.first) continue;
-      key = static_cast<uint32_t>(first) + piece * run;
-      head_ahead = ahead.head;
+      const uint32_t key = static_cast<uint32_t>(first) + piece * run;
+      in_page = ahead.head * block_bytes + from_block + (key & (P - 1)) * token_bytes;
       const uint32_t index = key >> p.page_shift;
       wanted = copies && static_cast<int>(key) <= ahead.keys.last;
       page = 0xFFFFFFFFu;
@@ -340,7 +344,8 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       const uint32_t all = __ballot_sync(0xffffffffu, have), lost = __ballot_sync(0xffffffffu, wanted && !have);
       if (lost) {  // no such page: what it would hold is NaN
         uint32_t* params = reinterpret_cast<uint32_t*>(ring_ptr + stage * F::kTileBytes + kTile * D);
-        if (lost >> (lane / run * 4) & 1) params[lane] = params[kTile + lane] = 0x7E007E00u;
+        for (uint32_t i = lane; i < kTile; i += 32)
+          if (lost >> (i / run * 4) & 1) params[i] = params[kTile + i] = 0x7E007E00u;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
@@ -348,7 +353,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(all) / 4 * run * (D + 8)) : "memory");
       __syncwarp();
       if (have) {
-        const uint8_t* from = p.a.cache.pool + (static_cast<uint64_t>(page) * p.a.cache.kv_heads + head_ahead) * block_bytes + from_block + (key & (P - 1)) * token_bytes;
+        const uint8_t* from = p.a.cache.pool + static_cast<uint64_t>(page) * page_bytes + in_page;
         asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                      ::"r"(ring + stage * F::kTileBytes + to_stage), "l"(from), "r"(run * token_bytes), "r"(bar) : "memory");
       }
@@ -475,10 +480,10 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       __syncwarp();
       const uint8_t* tile = ring_ptr + stage * F::kTileBytes;
       const bool whole = first >= keys.first_all && first + kTile - 1 <= keys.last_all;
-      float s[2][NT][kPer][2];  // [subtile][..][row][token half]
-      uint32_t vp[2][2];        // the values' (scale, offset) of the thread's tokens
+      float s[kSubs][NT][kPer][2];  // [subtile][..][row][token half]
+      uint32_t vp[kSubs][2];        // the values' (scale, offset) of the thread's tokens
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
+      for (int sub = 0; sub < kSubs; ++sub) {
         float acc[NT][4] = {};
         const uint8_t* row0 = tile + (sub * 16 + token_g) * (D / 2);
         const uint8_t* row1 = row0 + 8 * (D / 2);
@@ -522,10 +527,12 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       }
       // the largest binade of the values' scales that a row sees (at least log2 of a scale)
       auto binade_of = [](uint32_t bits) { return static_cast<float>(max(static_cast<int>(bits >> 10), 1) - 14); };
-      const uint32_t scale_bits[4] = {vp[0][0] & 0x7C00u, vp[0][1] & 0x7C00u, vp[1][0] & 0x7C00u, vp[1][1] & 0x7C00u};
       float binade[NT][kPer];
       if (whole) {
-        const float common = binade_of(max(max(scale_bits[0], scale_bits[1]), max(scale_bits[2], scale_bits[3])));
+        uint32_t big = 0;
+#pragma unroll
+        for (int j = 0; j < 2 * kSubs; ++j) big = max(big, vp[j / 2][j % 2] & 0x7C00u);
+        const float common = binade_of(big);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -538,10 +545,10 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
             const float4 c = row_const[n * kOf + t * kPer + i];
             uint32_t big = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2 * kSubs; ++j) {
               const int key = first + j * 8 + static_cast<int>(token_g);
               if (key > __float_as_int(c.z) || key < __float_as_int(c.w)) s[j / 2][n][i][j % 2] = -INFINITY;
-              else big = max(big, scale_bits[j]);
+              else big = max(big, vp[j / 2][j % 2] & 0x7C00u);
             }
             binade[n][i] = binade_of(big);
           }
@@ -553,7 +560,10 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          top[n][i] = fmaxf(fmaxf(s[0][n][i][0], s[0][n][i][1]), fmaxf(s[1][n][i][0], s[1][n][i][1])) + binade[n][i];
+          top[n][i] = fmaxf(s[0][n][i][0], s[0][n][i][1]);
+#pragma unroll
+          for (int sub = 1; sub < kSubs; ++sub) top[n][i] = fmaxf(top[n][i], fmaxf(s[sub][n][i][0], s[sub][n][i][1]));
+          top[n][i] += binade[n][i];
           if constexpr (kSplit) {  // the tile's largest
 #pragma unroll
             for (int o = 4; o < 32; o *= 2) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], o));
@@ -591,10 +601,10 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
         lift[n] = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
         drop[n] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
       }
-      uint32_t bp[2][NT][2];
+      uint32_t bp[kSubs][NT][2];
       auto weigh = [&](auto all_seen) {
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+        for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&vp[sub][half]));
@@ -630,7 +640,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       else weigh(std::false_type());
       float tile_acc[kSplit ? NT : 1][kSplit ? F::kVWords * 4 : 1][4] = {};
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
+      for (int sub = 0; sub < kSubs; ++sub) {
         const uint8_t* v0 = tile + kTile * (D / 2) + sub * 16 * (D / 2) + g * (D / 16);
         uint32_t xa[F::kVWords], xb[F::kVWords], xc[F::kVWords], xd[F::kVWords];
         auto load_v = [&](uint32_t (&x)[F::kVWords], uint32_t token) {
@@ -833,7 +843,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
     __syncthreads();  // q_frag, row_const, merge and warp_stat belong to the next run
     pos += static_cast<unsigned>(stop - at.tile);
     at.tile = stop;
-    if (pos < end) settle(at, p, kRows, span_at);
+    if (pos < end) settle(at, p, kRows, kTile, span_at);
   }
 }
 
