@@ -86,6 +86,7 @@ struct FewParams {
   float* parts;            // [4 * grid][kPartFloats]: two of a CTA, and two of the groups that begin with it
   unsigned int* counters;  // [3 * grid], zero between launches
   int* status;
+  uint32_t beyond;         // sequences of more query rows a kv head are another kernel's
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -144,7 +145,8 @@ __device__ __forceinline__ Runs runs_of(const FewParams& p, const Span& span, in
   const int from = window && first + 1 > window ? first + 1 - window : 0;
   r.tile_lo = from / tile;
   r.tiles = (span.length - 1) / tile + 1 - r.tile_lo;
-  r.blocks = span.length > 0 ? (static_cast<uint32_t>(span.count) * p.group + rows - 1) / rows : 0;  // idle: no work
+  const uint64_t query_rows = static_cast<uint64_t>(span.count) * p.group;
+  r.blocks = span.length > 0 && query_rows <= p.beyond ? static_cast<uint32_t>((query_rows + rows - 1) / rows) : 0;  // idle: no work
   r.units = r.blocks * p.a.cache.kv_heads;
   return r;
 }
@@ -848,7 +850,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
 }
 
 template <typename T, int D, int NT, bool kPair>
-cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
+cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond) {
   using F = Few<T, D, NT, kPair>;
   static_assert(F::kCtas >= 1, "shared memory");
   static_assert(F::kMerge % 16 == 0 && F::kQFrag % 16 == 0 && F::kRowConst % 16 == 0 && F::kScan % 16 == 0 && F::kSpan % 16 == 0 && F::kBars % 8 == 0 &&
@@ -864,6 +866,7 @@ cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
   p.parts = static_cast<float*>(env.workspace);
   p.counters = env.counters;
   p.status = env.status;
+  p.beyond = beyond;
   // a CTA's two parts and those of its groups must fit the scratch; one CTA alone shares no run
   const uint64_t fit = env.workspace ? env.workspace_bytes / (4ull * F::kPartFloats * sizeof(float)) : 0;
   const unsigned grid = static_cast<unsigned>(
@@ -883,37 +886,46 @@ cudaError_t few_as(const LaunchEnv& env, const AttendArgs& a) {
 
 // By the rows that a sequence's new tokens make with one kv head; beyond the widest block, blocks of it.
 template <typename T, int D>
-cudaError_t few_of(const LaunchEnv& env, const AttendArgs& a) {
-  const uint64_t rows = static_cast<uint64_t>(a.batch.most) * (a.heads / a.cache.kv_heads);
-  if (rows <= 4) return few_as<T, D, 1, true>(env, a);
+cudaError_t few_of(const LaunchEnv& env, const AttendArgs& a, uint64_t rows, uint32_t beyond) {
+  if (rows <= 4) return few_as<T, D, 1, true>(env, a, beyond);
   if constexpr (sizeof(T) == 4) {
-    if (rows <= 8 || D > 128) return few_as<T, D, 2, true>(env, a);
-    if constexpr (D <= 128) return few_as<T, D, 4, true>(env, a);
+    if (rows <= 8 || D > 128) return few_as<T, D, 2, true>(env, a, beyond);
+    if constexpr (D <= 128) return few_as<T, D, 4, true>(env, a, beyond);
   } else {
-    if (rows <= 8) return few_as<T, D, 1, false>(env, a);
-    if (rows <= 16 || D > 128) return few_as<T, D, 2, false>(env, a);
-    if constexpr (D <= 128) return few_as<T, D, 4, false>(env, a);
+    if (rows <= 8) return few_as<T, D, 1, false>(env, a, beyond);
+    if (rows <= 16 || D > 128) return few_as<T, D, 2, false>(env, a, beyond);
+    if constexpr (D <= 128) return few_as<T, D, 4, false>(env, a, beyond);
   }
   return cudaErrorInvalidValue;
 }
 
 template <typename T>
-cudaError_t attend_as(const LaunchEnv& env, const AttendArgs& a) {
+cudaError_t few_in(const LaunchEnv& env, const AttendArgs& a, uint64_t rows, uint32_t beyond) {
   switch (a.cache.head_dim) {
-    case 64: return few_of<T, 64>(env, a);
-    case 128: return few_of<T, 128>(env, a);
-    case 256: return few_of<T, 256>(env, a);
+    case 64: return few_of<T, 64>(env, a, rows, beyond);
+    case 128: return few_of<T, 128>(env, a, rows, beyond);
+    case 256: return few_of<T, 256>(env, a, rows, beyond);
     default: return cudaErrorInvalidValue;
   }
 }
 
+// Query rows (of a sequence and kv head) from which on 128-row MMAs are faster.
+constexpr uint32_t kFewRows = 32;
+
 }  // namespace
 
 cudaError_t launch_attend(const LaunchEnv& env, const AttendArgs& a, int* launches) {
-  *launches = 1;
-  if (a.dtype == KQ_F32) return attend_as<float>(env, a);
-  if (a.dtype == KQ_F16) return attend_as<__half>(env, a);
-  return attend_as<__nv_bfloat16>(env, a);
+  // Each sequence is the work of one kernel, by its own rows: a call may hold prompts and single tokens.
+  const uint64_t rows = static_cast<uint64_t>(a.batch.most) * (a.heads / a.cache.kv_heads);
+  const bool many = rows > kFewRows && attend_many_supports(a);
+  const uint32_t beyond = many ? kFewRows : 0xFFFFFFFFu;
+  const uint64_t few = many ? kFewRows : rows;
+  cudaError_t e = a.dtype == KQ_F32   ? few_in<float>(env, a, few, beyond)
+                  : a.dtype == KQ_F16 ? few_in<__half>(env, a, few, beyond)
+                                      : few_in<__nv_bfloat16>(env, a, few, beyond);
+  *launches = many ? 2 : 1;
+  if (e == cudaSuccess && many) e = launch_attend_many(env, a, beyond);
+  return e;
 }
 
 }  // namespace kq

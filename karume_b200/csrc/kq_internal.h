@@ -238,4 +238,7 @@ cudaError_t launch_cache_append(const LaunchEnv& env, const Cache& cache, const 
                                 const void* v, uint64_t v_stride, int dtype, const RopeTable& rope);
 cudaError_t launch_cache_read(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, float* k, float* v);
 cudaError_t launch_attend(const LaunchEnv& env, const AttendArgs& args, int* launches);
+// Its kernel for sequences whose new tokens make more than `beyond` query rows a kv head (kq_attend_many.cu).
+bool attend_many_supports(const AttendArgs& args);
+cudaError_t launch_attend_many(const LaunchEnv& env, const AttendArgs& args, uint32_t beyond);
 }  // namespace kq
