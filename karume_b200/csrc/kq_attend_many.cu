@@ -5,11 +5,11 @@
 //
 // A CTA takes 256 query rows (query and head of one kv head's group, packed: all heads of the group share what is unpacked)
 // and walks over the keys they see in tiles of 128.  Warps:
-//   0-3, 4-7   one row each thread of the first / second 128 rows: scores from tensor memory, weights back into it, and
-//              the sums of the output in registers (what the tensor core adds is one tile's, so a long row does not drift)
-//   8-11       unpack a tile: keys as [token][dim], values transposed as [dim][token], both K-major with 128-byte swizzle
-//   12         issues the MMAs:   S_r = Q_r K^T (both in shared memory),   O_r = P_r V (P in tensor memory, over S)
-//   13         copies the codes and scales of the next tile (bulk copies, page by page)
+//   0-3, 4-7   one row each thread of the first / second 128 rows: scores from tensor memory, weights back into it; f32 queries:
+//              the sums of the output in registers (what the tensor core adds is one tile's, so that a long row does not drift)
+//   four (f32) or eight   unpack a tile: keys as [token][dim], values transposed as [dim][token], both K-major, 128-byte swizzle
+//   one        issues the MMAs:   S_r = Q_r K^T (both in shared memory),   O_r += P_r V (P in tensor memory, over S)
+//   one        copies the codes and scales of the next tile (bulk copies, page by page)
 // The two row blocks take turns: while one's weights are being computed the tensor core works for the other.
 //
 //   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights).
@@ -17,6 +17,7 @@
 //                   codes around zero; scale and offset are applied to the scores and weights in f32.  Queries and weights are
 //                   two binary16 parts each (fixed-point, the low ones multiplied first), 22 bits and more.
 #include <algorithm>
+#include <type_traits>
 
 #include "kq_cache.cuh"
 #include "kq_umma.cuh"
@@ -24,30 +25,39 @@
 namespace kq {
 namespace {
 
-constexpr int kManyThreads = 512;
 constexpr int kKeys = 128;    // of a tile
 constexpr int kBlock = 256;   // query rows of a CTA
 constexpr int kManyTimeout = 50;
+
+enum Bar { kRawKFull, kRawKFree = 2, kRawVFull = 4, kRawVFree = 6, kKFull = 8, kKEmpty, kVFull, kVEmpty = 12, kSFull = 14, kPReady = 16, kOFull = 18, kBarCount = 20 };
 
 template <typename T, int D>
 struct Many {
   static constexpr bool kSplit = sizeof(T) == 4;
   static constexpr int kParts = kSplit ? 2 : 1;
+  // 8 softmax warps, the unpacking ones, MMA, copies.  f32 keeps the output's sums in the softmax warps' registers (192 a thread,
+  // taken from the others, which makes whole groups of four warps); 16-bit ones stay in tensor memory.
+  static constexpr int kUnpackWarps = kSplit ? 4 : 8, kUnpack = kUnpackWarps * 32;
+  static constexpr int kMmaWarp = 8 + kUnpackWarps, kCopyWarp = kMmaWarp + 1;
+  static constexpr int kThreads = kSplit ? 512 : (kCopyWarp + 1) * 32;
   static constexpr int kOperand = 128 * D * 2;             // bytes of 128 rows (or tokens) of D values
-  static constexpr int kBufs = kSplit && D == 128 ? 1 : 2;  // unpacked tiles: as many as fit beside the queries
+  static constexpr bool kFull = kSplit && D == 128;        // the queries leave room for one of everything
+  static constexpr int kVBufs = kFull ? 1 : 2;             // unpacked values; one tile of unpacked keys (needed only while scores are made)
+  static constexpr int kRaws = kFull ? 1 : 2;              // tiles of codes on their way
   static constexpr int kGroup = 4 * D + 16;                // raw values of eight tokens, 16 bytes apart: lanes of eight groups meet no bank twice
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + 2 * kParts * kOperand;
-  static constexpr int kV = kK + kBufs * kOperand;
-  static constexpr int kRawK = kV + kBufs * kOperand;
-  static constexpr int kRawV = kRawK + kKeys * (D / 2);
-  static constexpr int kRawParams = kRawV + 16 * kGroup;   // K, then V (scale, offset)
-  static constexpr int kTable = kRawParams + 2 * kKeys * 4;  // f32: [2][128] (ks, ko, vs, v mid); 16-bit: K pairs, V scales, V offsets
-  static constexpr int kRows = kTable + 2 * kKeys * 16;    // [256] (factor, sum, last key, first key)
+  static constexpr int kV = kK + kOperand;
+  static constexpr int kRaw = kV + kVBufs * kOperand;
+  static constexpr int kRawV = kKeys * (D / 2);            // in a tile of codes: keys, values,
+  static constexpr int kRawParams = kRawV + 16 * kGroup;   // keys' and values' (scale, offset)
+  static constexpr int kRawBytes = kRawParams + 2 * kKeys * 4;
+  static constexpr int kTable = kRaw + kRaws * kRawBytes;  // [2][2][128]: (scale, offset) of keys and values, what is not seen zero
+  static constexpr int kRows = kTable + 4 * kKeys * 4;     // [256] (factor, sum, last key, first key)
   static constexpr int kLost = kRows + kBlock * 16;        // [2] 128 bits: tokens whose value is NaN
   static constexpr int kBinade = kLost + 32;               // [2][4]: largest binade of the values' scales, by warp
   static constexpr int kBars = kBinade + 32;
-  static constexpr int kMisc = kBars + 18 * 8;
+  static constexpr int kMisc = kBars + kBarCount * 8;
   static constexpr int kSmem = kMisc + 64 + 1024;          // the operands start on a multiple of 1024
 };
 
@@ -57,13 +67,13 @@ struct ManyParams {
   int* status;
 };
 
-enum Bar { kRawKFull, kRawKFree, kRawVFull, kRawVFree, kKFull, kKEmpty = 6, kVFull = 8, kVEmpty = 10, kSFull = 12, kPReady = 14, kOFull = 16, kBarCount = 18 };
-
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// a whole number that is more than log2 of a scale (of binary16: no smaller than 2^-24)
+__device__ __forceinline__ float binade_of(float scale) { return static_cast<float>(max(static_cast<int>(__float_as_uint(scale) >> 23) - 126, -24)); }
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -94,16 +104,20 @@ __device__ __forceinline__ void tmem_ld16_done(float (&f)[16]) {
                :
                : "memory");
 }
-// N columns, sixteen at a time: use(column, values), the next ones on their way meanwhile
-template <int N, typename Use>
+// N columns, sixteen at a time: use(column, values), the next ones on their way meanwhile.  kFlat: unrolled, so that the
+// column is a constant (registers are indexed with it); otherwise a loop, for the instruction cache.
+template <int N, bool kFlat, typename Use>
 __device__ __forceinline__ void tmem_columns(uint32_t taddr, Use use) {
   float x[2][16];
   tmem_ld16_begin(taddr, x[0]);
-#pragma unroll
-  for (int c = 0; c < N / 16; ++c) {
-    tmem_ld16_done(x[c & 1]);
-    if (c + 1 < N / 16) tmem_ld16_begin(taddr + (c + 1) * 16, x[(c + 1) & 1]);
-    use(c * 16, x[c & 1]);
+#pragma unroll(kFlat ? N / 32 : 1)
+  for (int c = 0; c < N; c += 32) {
+    tmem_ld16_done(x[0]);
+    tmem_ld16_begin(taddr + c + 16, x[1]);
+    use(c, x[0]);
+    tmem_ld16_done(x[1]);
+    if (c + 32 < N) tmem_ld16_begin(taddr + c + 32, x[0]);
+    use(c + 16, x[1]);
   }
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
@@ -148,9 +162,9 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const fl
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __grid_constant__ ManyParams p) {
+__global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(const __grid_constant__ ManyParams p) {
   using F = Many<T, D>;
-  constexpr int kParts = F::kParts, kBufs = F::kBufs;
+  constexpr int kParts = F::kParts, kVBufs = F::kVBufs, kRaws = F::kRaws;
   constexpr bool kSplit = F::kSplit;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + (1024 - (static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw)) & 1023u)) % 1024;
@@ -168,14 +182,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
   };
 
   if (tid == 0) {
-    umma::mbar_init(bar(kRawKFull), 1);
-    umma::mbar_init(bar(kRawVFull), 1);
-    umma::mbar_init(bar(kRawKFree), 128);
-    umma::mbar_init(bar(kRawVFree), 128);
+    umma::mbar_init(bar(kKFull), F::kUnpack);
+    umma::mbar_init(bar(kKEmpty), 1);
     for (int i = 0; i < 2; ++i) {
-      umma::mbar_init(bar(kKFull + i), 128);
-      umma::mbar_init(bar(kVFull + i), 128);
-      umma::mbar_init(bar(kKEmpty + i), 1);
+      umma::mbar_init(bar(kRawKFull + i), 1);
+      umma::mbar_init(bar(kRawVFull + i), 1);
+      umma::mbar_init(bar(kRawKFree + i), F::kUnpack);
+      umma::mbar_init(bar(kRawVFree + i), F::kUnpack);
+      umma::mbar_init(bar(kVFull + i), F::kUnpack);
       umma::mbar_init(bar(kVEmpty + i), 1);
       umma::mbar_init(bar(kSFull + i), 1);
       umma::mbar_init(bar(kOFull + i), 1);
@@ -191,7 +205,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
   __syncthreads();
 
   // ---- which rows: units are (sequence, block of rows from the last, kv head) ----------------------
-  const uint32_t sequences = p.a.batch.sequences, each = (sequences + kManyThreads - 1) / kManyThreads, heads = p.a.cache.kv_heads;
+  const uint32_t sequences = p.a.batch.sequences, each = (sequences + F::kThreads - 1) / F::kThreads, heads = p.a.cache.kv_heads;
   const auto blocks_of = [&](uint32_t b) {
     const Span s = span_of(p.a.batch, b);
     const uint64_t n = static_cast<uint64_t>(s.count) * p.group;
@@ -205,7 +219,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= static_cast<uint32_t>(o)) upto += v;
   }
-  uint32_t* const scan = reinterpret_cast<uint32_t*>(smem + F::kTable);
+  uint32_t* const scan = reinterpret_cast<uint32_t*>(smem + F::kRows);
   if (lane == 31) scan[warp] = upto;
   __syncthreads();
   for (uint32_t i = 0; i < warp; ++i) upto += scan[i];
@@ -232,7 +246,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
     const uint32_t c = lane % kLanes;
 #pragma unroll 2
-    for (uint32_t r = warp * kAtOnce + lane / kLanes; r < kBlock; r += 16 * kAtOnce) {
+    for (uint32_t r = warp * kAtOnce + lane / kLanes; r < kBlock; r += F::kThreads / 32 * kAtOnce) {
       const int row = row0 + static_cast<int>(r), query = row / static_cast<int>(p.group);
       const bool there = row < n_rows;
       float v[8] = {};
@@ -281,7 +295,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == F::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(tmem_word))), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -292,7 +306,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
 
   if (warp < 8) {
     // ---- softmax and output: a row a thread --------------------------------------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if constexpr (kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const uint32_t wg = warp / 4, lanes = (warp % 4 * 32) << 16;
     const uint32_t t_s = tmem + lanes + wg * 128, t_o = tmem + lanes + 256 + wg * 128;
     const int r = static_cast<int>(tid);
@@ -300,97 +314,144 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     const float factor = rc.x, q_sum = rc.y;
     const int last = __float_as_int(rc.z), from = __float_as_int(rc.w);
     const int last_all = __reduce_min_sync(0xffffffffu, last), from_all = __reduce_max_sync(0xffffffffu, from);
-    float O[D];
+    float O[kSplit ? D : 1];
+    if constexpr (kSplit) {
 #pragma unroll
-    for (int i = 0; i < D; ++i) O[i] = 0.0f;
+      for (int i = 0; i < D; ++i) O[i] = 0.0f;
+    }
+    // Weights are 2^(score - M + kLift).  M is a whole number (what it moves by is an exact power of two) that follows the row's
+    // largest score, f32: and the binade of the values' scales beside it; it moves when a weight (times its value's scale) would
+    // pass 2^14.  So that this is seen before anything is written, sixteen scores are looked at at a time; what was written
+    // of the tile before is then scaled too.  f32 lets M lag by one bit, to keep the fixed-point parts' 22; 16-bit by eight.
+    constexpr float kLift = kSplit ? 13.0f : 6.0f, kLag = kSplit ? 1.0f : 8.0f;
     float M = -INFINITY, l = 0.0f, centre = 0.0f;
     for (int j = 0; j < tiles; ++j) {
       const int first = (tile0 + j) * kKeys;
       const bool whole = first >= from_all && first + kKeys - 1 <= last_all;
       const int sees0 = from - first, sees1 = last - first;  // columns the row sees
-      const float4* table = reinterpret_cast<const float4*>(smem + F::kTable) + (j & 1) * kKeys;
+      const __half2* k_par = reinterpret_cast<const __half2*>(smem + F::kTable) + (j & 1) * 2 * kKeys;
+      const __half2* v_par = k_par + kKeys;
       wait(kSFull + wg, j);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float m = -INFINITY, binade = 0.0f;
+      float binade = 0.0f;
       if constexpr (kSplit) {
         const float* bn = reinterpret_cast<const float*>(smem + F::kBinade) + (j & 1) * 4;
         binade = fmaxf(fmaxf(bn[0], bn[1]), fmaxf(bn[2], bn[3]));
+        if (!whole) {  // ... of what this row sees
+          float big = 0.0f;
+          for (int i = 0; i < kKeys; ++i)
+            if (i >= sees0 && i <= sees1) big = fmaxf(big, __low2float(v_par[i]));
+          binade = binade_of(big);
+        }
       }
-      float vs_big = 0.0f;
-      tmem_columns<kKeys>(t_s, [&](int c, float (&x)[16]) {
-        if constexpr (kSplit) {
+      float limit = M + kLag - binade, shift = M == -INFINITY ? kLift : kLift - M;
+      const auto tile = [&](auto all_seen) {
+        constexpr bool kAll = decltype(all_seen)::value;
+        float x[2][16];
+        const auto sixteen = [&](int c, float (&z)[16], auto begin_next) {
+          float big[8];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float4 k = table[c + i];
-            x[i] = fmaf(x[i], k.x, k.y * q_sum);
-            if (!whole && c + i >= sees0 && c + i <= sees1) vs_big = fmaxf(vs_big, k.z);
-          }
-        }
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) m = fmaxf(m, x[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i >= sees0 && c + i <= sees1) m = fmaxf(m, x[i]);
-        }
-      });
-      if constexpr (kSplit)
-        if (!whole) binade = fmaxf(static_cast<float>(static_cast<int>(__float_as_uint(vs_big) >> 23) - 126), -14.0f);
-      // M: the largest score (f32: and the binade of the values' scales); moves only when a weight would grow past 2^8
-      const float top = m == -INFINITY ? m : m * factor + binade;
-      const bool more = top > M + 8.0f;
-      if (__any_sync(0xffffffffu, more)) {
-        const float keep = !more ? 1.0f : ex2(M - top);
-        if (more) M = top;
-        l *= keep;
-        centre *= keep;
-#pragma unroll
-        for (int i = 0; i < D; ++i) O[i] *= keep;
-      }
-      int up = 0;  // f32: P is lifted to just below 2^14 in each tile, and its sums brought back
-      if constexpr (kSplit) up = top == -INFINITY ? 0 : min(max(14 - static_cast<int>(ceilf(top - M)), 0), 120);
-      const float shift = (M == -INFINITY ? 0.0f : -M) + static_cast<float>(up), drop = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-      float l_tile = 0.0f, centre_tile = 0.0f;
-      tmem_columns<kKeys>(t_s, [&](int c, float (&x)[16]) {
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float w[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float z = x[i + k];
-            float4 t = {};
             if constexpr (kSplit) {
-              t = table[c + i + k];
-              z = fmaf(z, t.x, t.y * q_sum);
+              const float2 k = __half22float2(k_par[c + i]);
+              z[i] = fmaf(z[i], k.x, k.y * q_sum);
             }
-            w[k] = ex2(fmaf(z, factor, shift));
-            if (!whole && (c + i + k < sees0 || c + i + k > sees1)) {
-              w[k] = 0.0f;  // what is not seen may hold anything
-            } else if constexpr (kSplit) {
-              l_tile += w[k];
-              centre_tile = fmaf(w[k], t.w, centre_tile);
-              w[k] *= t.z;
+            if (!kAll && (c + i < sees0 || c + i > sees1)) z[i] = -INFINITY;  // what is not seen may hold anything
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) big[i] = fmaxf(z[i], z[i + 8]);
+#pragma unroll
+          for (int o = 4; o > 0; o /= 2)
+#pragma unroll
+            for (int i = 0; i < o; ++i) big[i] = fmaxf(big[i], big[i + o]);
+          const float top = big[0] * factor;
+          if (__any_sync(0xffffffffu, top > limit)) {
+            const float now = top > limit ? ceilf(top + binade) : M;
+            const float keep = M == -INFINITY ? 0.0f : exp2f(M - now);
+            if (now != -INFINITY) M = now;
+            const bool moved = M != -INFINITY;
+            limit = M + kLag - binade;
+            shift = moved ? kLift - M : kLift;
+            l *= keep;
+            centre *= keep;
+            const __half2 keep2 = __float2half2_rn(keep);
+            for (int at = 0; at < c; at += 16) {
+              float w[16];
+              tmem_ld16_begin(t_s + at, w);
+              tmem_ld16_done(w);
+              uint32_t y[2][8];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w[i]), keep2);
+                y[i / 8][i % 8] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              tmem_st8(t_s + at, y[0]);
+              if constexpr (kSplit) tmem_st8(t_s + at + 8, y[1]);
+            }
+            if constexpr (kSplit) {
+#pragma unroll
+              for (int i = 0; i < D; ++i) O[i] *= keep;
+            } else if (j > 0) {  // the sums of the tiles before, in tensor memory
+              wait(kOFull + wg, j - 1);
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              for (int at = 0; at < D; at += 16) {
+                float w[16];
+                tmem_ld16_begin(t_o + at, w);
+                tmem_ld16_done(w);
+                uint32_t y[2][8];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i / 8][i % 8] = __float_as_uint(w[i] * keep);
+                tmem_st8(t_o + at, y[0]);
+                tmem_st8(t_o + at + 8, y[1]);
+              }
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          }
+          begin_next();
+          uint32_t hi[8], lo[8];
+          float part[4] = {}, mid[4] = {};
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float w[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              w[k] = ex2(fmaf(z[i + k], factor, shift));
+              part[i / 2 % 4] += w[k];
+              if constexpr (kSplit) {
+                const float2 v = __half22float2(v_par[c + i + k]);
+                const bool sees = kAll || (c + i + k >= sees0 && c + i + k <= sees1);
+                mid[i / 2 % 4] = fmaf(w[k], sees ? fmaf(7.5f, v.x, v.y) : 0.0f, mid[i / 2 % 4]);
+                w[k] *= sees ? v.x : 0.0f;
+              }
+            }
+            if constexpr (kSplit) {
+              constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
+              const float h0 = __fsub_rn(__fadd_rn(w[0], kEight), kEight), h1 = __fsub_rn(__fadd_rn(w[1], kEight), kEight);
+              hi[i / 2] = half2_bits(h0, h1);
+              lo[i / 2] = half2_bits(w[0] - h0, w[1] - h1);
             } else {
-              l_tile += w[k];
+              hi[i / 2] = half2_bits(w[0], w[1]);
             }
           }
-          if constexpr (kSplit) {
-            constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
-            const float h0 = __fsub_rn(__fadd_rn(w[0], kEight), kEight), h1 = __fsub_rn(__fadd_rn(w[1], kEight), kEight);
-            hi[i / 2] = half2_bits(h0, h1);
-            lo[i / 2] = half2_bits(w[0] - h0, w[1] - h1);
-          } else {
-            hi[i / 2] = half2_bits(w[0], w[1]);
-          }
+          l += (part[0] + part[1]) + (part[2] + part[3]);
+          if constexpr (kSplit) centre += (mid[0] + mid[1]) + (mid[2] + mid[3]);
+          // sixteen keys' weights go where their scores were: eight columns, and eight for the low parts
+          tmem_st8(t_s + c, hi);
+          if constexpr (kSplit) tmem_st8(t_s + c + 8, lo);
+        };
+        tmem_ld16_begin(t_s, x[0]);
+#pragma unroll 1
+        for (int c = 0; c < kKeys; c += 32) {
+          tmem_ld16_done(x[0]);
+          sixteen(c, x[0], [&] { tmem_ld16_begin(t_s + c + 16, x[1]); });
+          tmem_ld16_done(x[1]);
+          sixteen(c + 16, x[1], [&] {
+            if (c + 32 < kKeys) tmem_ld16_begin(t_s + c + 32, x[0]);
+          });
         }
-        // sixteen keys' weights go where their scores were: eight columns, and eight for the low parts
-        tmem_st8(t_s + c, hi);
-        if constexpr (kSplit) tmem_st8(t_s + c + 8, lo);
-      });
-      l = fmaf(l_tile, drop, l);
-      centre = fmaf(centre_tile, drop, centre);
+      };
+      if (whole) tile(std::true_type());
+      else tile(std::false_type());
       if constexpr (!kSplit) {
         const uint4 lost = *reinterpret_cast<const uint4*>(smem + F::kLost + (j & 1) * 16);
         if (lost.x | lost.y | lost.z | lost.w) {  // values that are NaN entered as zeros: whoever sees one is NaN
@@ -403,55 +464,73 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       umma::mbar_arrive(bar(kPReady + wg));
-      wait(kOFull + wg, j);
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      tmem_columns<D>(t_o, [&](int c, float (&x)[16]) {
+      if constexpr (kSplit) {
+        wait(kOFull + wg, j);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_columns<D, true>(t_o, [&](int c, float (&x)[16]) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) O[c + i] = kSplit ? fmaf(x[i], drop, O[c + i]) : O[c + i] + x[i];
-      });
+          for (int i = 0; i < 16; ++i) O[c + i] += x[i];
+        });
+      }
     }
-    const int row = row0 + r;
-    if (row < n_rows) {
-      const int query = row / static_cast<int>(p.group);
-      T* out = static_cast<T*>(p.a.out) + static_cast<size_t>(span.first + query) * p.a.out_stride +
-               static_cast<size_t>(head * p.group + static_cast<uint32_t>(row - query * static_cast<int>(p.group))) * D;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = row0 + r, query = row / static_cast<int>(p.group);
+    T* const out = static_cast<T*>(p.a.out) + static_cast<size_t>(span.first + query) * p.a.out_stride +
+                   static_cast<size_t>(head * p.group + static_cast<uint32_t>(row - query * static_cast<int>(p.group))) * D;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if constexpr (kSplit) {
 #pragma unroll
       for (int i = 0; i < D; i += 8) {
         float o[8];
-        // f32: the codes' powers of two, even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
+        // the codes' powers of two: even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = kSplit ? fmaf(O[i + k], (k & 1) ? 1048576.0f : 8388608.0f, centre) * inv : O[i + k] * inv;
-        store8(out + i, o);
+        for (int k = 0; k < 8; ++k) o[k] = fmaf(O[i + k], (k & 1) ? 1048576.0f : 8388608.0f, centre) * inv;
+        if (row < n_rows) store8(out + i, o);
       }
+    } else if (tiles == 0) {
+      const float zero[8] = {};
+      if (row < n_rows)
+        for (int i = 0; i < D; i += 8) store8(out + i, zero);
+    } else {
+      wait(kOFull + wg, tiles - 1);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      tmem_columns<D, false>(t_o, [&](int c, float (&x)[16]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= inv;
+        if (row < n_rows) {
+          store8(out + c, x);
+          store8(out + c + 8, x + 8);
+        }
+        __syncwarp();
+      });
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp < 12) {
+    if constexpr (kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp < F::kMmaWarp) {
       // ---- unpacking ---------------------------------------------------------------------------------
       const uint32_t t = tid - 256, w4 = warp - 8;
       constexpr uint32_t kExp = 0x64006400u, k1024 = 0xE400E400u, k16th = 0x2C002C00u, k64 = 0xD400D400u;  // 1024 | x, -1024, 1/16, -64
       constexpr uint32_t kCentre0 = 0x800F800Fu, kCentre1 = 0x80788078u;                                   // -15 2^-24, -7.5 2^-20
-      uint32_t* const k_par = reinterpret_cast<uint32_t*>(smem + F::kTable);                 // 16-bit: (scale, offset) of each key
-      __half* const v_scale = reinterpret_cast<__half*>(smem + F::kTable + 512);
-      __half* const v_offset = v_scale + kKeys;
-      const uint32_t* const raw_params = reinterpret_cast<const uint32_t*>(smem + F::kRawParams);
       bool ok = true;  // after a wait that gave up nothing is handed on: no barrier is arrived on beyond its phase
       for (int j = 0; j < tiles; ++j) {
         const int first = (tile0 + j) * kKeys;
-        const uint32_t buf = j % kBufs;
-        ok = wait(kRawKFull, j) && ok;
-        if (j >= kBufs) wait(kKEmpty + buf, j / kBufs - 1);
-        if (kBufs == 2 && j >= 2) wait(kVEmpty + buf, j / 2 - 1);  // what the softmax warps read of tile j - 2 has been read
-        {
+        const uint32_t buf = j % kVBufs, raw = j % kRaws;
+        const uint8_t* const codes = smem + F::kRaw + raw * F::kRawBytes;
+        uint32_t* const k_par = reinterpret_cast<uint32_t*>(smem + F::kTable) + (j & 1) * 2 * kKeys;  // (scale, offset) of each key; values:
+        __half* const v_scale = reinterpret_cast<__half*>(k_par + kKeys);                          // f32 pairs too, 16-bit scales, then offsets
+        __half* const v_offset = v_scale + kKeys;
+        ok = wait(kRawKFull + raw, j / kRaws) && ok;
+        if (kVBufs == 2 && j >= 2) wait(kVEmpty + buf, j / 2 - 1);  // what the softmax warps read of tile j - 2 has been read
+        if (t < kKeys) {
           const bool seen = first + static_cast<int>(t) <= key_last;
+          const uint32_t* const raw_params = reinterpret_cast<const uint32_t*>(codes + F::kRawParams);
           uint32_t kp = seen ? raw_params[t] : 0u, vp = seen ? raw_params[kKeys + t] : 0u;
-          float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kp)), v = __half22float2(*reinterpret_cast<const __half2*>(&vp));
+          const float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kp)), v = __half22float2(*reinterpret_cast<const __half2*>(&vp));
           if constexpr (kSplit) {
-            reinterpret_cast<float4*>(smem + F::kTable)[(j & 1) * kKeys + t] = make_float4(k.x, k.y, v.x, fmaf(7.5f, v.x, v.y));
-            const int big = __reduce_max_sync(0xffffffffu, static_cast<int>(__float_as_uint(v.x) >> 23) - 126);
-            if (lane == 0) reinterpret_cast<float*>(smem + F::kBinade)[(j & 1) * 4 + w4] = static_cast<float>(max(big, -14));
+            k_par[t] = kp;
+            k_par[kKeys + t] = vp;
+            const uint32_t big = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v.x, 0.0f)));  // not NaN
+            if (lane == 0) reinterpret_cast<float*>(smem + F::kBinade)[(j & 1) * 4 + w4] = binade_of(__uint_as_float(big));
           } else {
             // the largest value must stay finite in binary16: a scale that was rounded up gives one unit back
             if (fmaf(15.0f, k.x, k.y) >= 65520.0f) kp -= 1;
@@ -464,15 +543,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             v_offset[t] = __ushort_as_half(static_cast<unsigned short>(vp >> 16));
           }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (j >= 1) wait(kKEmpty, j - 1);
+        asm volatile("bar.sync 1, %0;" ::"n"(F::kUnpack) : "memory");
         {
           constexpr int kPieces = D / 32;  // 16-byte pieces of a token
           const uint32_t q = t % kPieces;
           const uint32_t swap = D == 128 ? q / 2 * 2 : 0;  // pieces of the second 64 dims in another order: other banks
 #pragma unroll 1
-          for (uint32_t it = 0; it < kPieces; ++it) {
-            const uint32_t row = (it * 128 + t) / kPieces;
-            const uint4 raw = *reinterpret_cast<const uint4*>(smem + F::kRawK + row * (D / 2) + q * 16);
+          for (uint32_t at = t; at < kKeys * kPieces; at += F::kUnpack) {
+            const uint32_t row = at / kPieces;
+            const uint4 raw = *reinterpret_cast<const uint4*>(codes + row * (D / 2) + q * 16);
             const uint32_t x[4] = {swap ? raw.z : raw.x, swap ? raw.w : raw.y, swap ? raw.x : raw.z, swap ? raw.y : raw.w};
             uint32_t s2 = 0, o2 = 0;
             if constexpr (!kSplit) {
@@ -492,23 +572,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                 out.z = hfma2_bits(hadd2_bits((x8 & 0x000F000Fu) | kExp, k1024), s2, o2);
                 out.w = hfma2_bits(hfma2_bits((x8 & 0x00F000F0u) | kExp, k16th, k64), s2, o2);
               }
-              umma::sts128(base + F::kK + buf * F::kOperand + (word / 8) * 16384 + umma::swz(row, word % 8), out);
+              umma::sts128(base + F::kK + (word / 8) * 16384 + umma::swz(row, word % 8), out);
             }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (ok) {
-          umma::mbar_arrive(bar(kKFull + buf));
-          umma::mbar_arrive(bar(kRawKFree));
+          umma::mbar_arrive(bar(kKFull));
+          umma::mbar_arrive(bar(kRawKFree + raw));
         }
-        ok = wait(kRawVFull, j) && ok;
-        if (j >= kBufs) wait(kVEmpty + buf, j / kBufs - 1);
+        ok = wait(kRawVFull + raw, j / kRaws) && ok;
+        if (kVBufs == 1 && j >= 1) wait(kVEmpty, j - 1);
         {
           const uint32_t tg = lane % 8;
 #pragma unroll 1
-          for (uint32_t lin = w4; lin < D / 16; lin += 4) {
+          for (uint32_t lin = warp - 8; lin < D / 16; lin += F::kUnpackWarps) {
             const uint32_t word = lin % (D / 32) * 4 + lane / 8, atom = lin / (D / 32);
-            const uint32_t* from_v = reinterpret_cast<const uint32_t*>(smem + F::kRawV + (atom * 8 + tg) * F::kGroup) + word;
+            const uint32_t* from_v = reinterpret_cast<const uint32_t*>(codes + F::kRawV + (atom * 8 + tg) * F::kGroup) + word;
             uint32_t c01[4], c23[4];  // dims 0..3 / 4..7 of two tokens
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -544,16 +624,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (ok) {
           umma::mbar_arrive(bar(kVFull + buf));
-          umma::mbar_arrive(bar(kRawVFree));
+          umma::mbar_arrive(bar(kRawVFree + raw));
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the 16-bit table is written anew for the next tile
       }
-    } else if (warp == 12) {
+    } else if (warp == F::kMmaWarp) {
       // ---- MMAs ----------------------------------------------------------------------------------------
       const uint32_t leader = umma::elect_lane();
-      const auto scores = [&](int j, uint32_t r) {
-        const uint32_t buf = j % kBufs, d = tmem + r * 128;
-        const uint32_t q = desc_low(base + F::kQ + r * kParts * F::kOperand), k = desc_low(base + F::kK + buf * F::kOperand);
+      const auto scores = [&](uint32_t r) {
+        const uint32_t d = tmem + r * 128, q = desc_low(base + F::kQ + r * kParts * F::kOperand), k = desc_low(base + F::kK);
 #pragma unroll
         for (int part = kParts - 1; part >= 0; --part)
 #pragma unroll
@@ -565,15 +643,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
       if (tiles > 0) {
         wait(kKFull, 0);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        scores(0, 0);
-        scores(0, 1);
+        scores(0);
+        scores(1);
         umma::commit_one(leader, bar(kKEmpty));
       }
       for (int j = 0; j < tiles; ++j) {
-        const uint32_t buf = j % kBufs;
+        const uint32_t buf = j % kVBufs;
         for (uint32_t r = 0; r < 2; ++r) {
           wait(kPReady + r, j);
-          if (r == 0) wait(kVFull + buf, j / kBufs);
+          if (r == 0) wait(kVFull + buf, j / kVBufs);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t v = desc_low(base + F::kV + buf * F::kOperand);
 #pragma unroll
@@ -581,20 +659,20 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
 #pragma unroll
             for (int s = 0; s < kKeys / 16; ++s)
               mma_ts(leader, tmem + 256 + r * 128, tmem + r * 128 + s * 16 + part * 8, v + (s / 4 * (D * 128) + s % 4 * 32) / 16, f16_idesc(D),
-                     part != kParts - 1 || s != 0);
+                     part != kParts - 1 || s != 0 || (!kSplit && j > 0));
           umma::commit_one(leader, bar(kOFull + r));
           if (r == 1) umma::commit_one(leader, bar(kVEmpty + buf));
           if (j + 1 < tiles) {
             if (r == 0) {
-              wait(kKFull + (j + 1) % kBufs, (j + 1) / kBufs);
+              wait(kKFull, j + 1);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
-            scores(j + 1, r);
-            if (r == 1) umma::commit_one(leader, bar(kKEmpty + (j + 1) % kBufs));
+            scores(r);
+            if (r == 1) umma::commit_one(leader, bar(kKEmpty));
           }
         }
       }
-    } else if (warp == 13) {
+    } else if (warp == F::kCopyWarp) {
       // ---- copies --------------------------------------------------------------------------------------
       const uint32_t P = p.a.cache.page_tokens, block_bytes = static_cast<uint32_t>(cache_block_bytes(P, D));
       const int* const pages = p.a.batch.pages + static_cast<size_t>(seq) * p.a.batch.width;
@@ -621,38 +699,39 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         const uint8_t* const block_k = p.a.cache.pool + (static_cast<uint64_t>(page_k) * heads + head) * block_bytes;
         const uint8_t* const block_v = p.a.cache.pool + (static_cast<uint64_t>(page_v) * heads + head) * block_bytes;
         look(j + 1);
-        if (j > 0) ok = wait(kRawKFree, j - 1) && ok;
+        const uint32_t raw = j % kRaws, codes = base + F::kRaw + raw * F::kRawBytes;
+        if (j >= kRaws) ok = wait(kRawKFree + raw, j / kRaws - 1) && ok;
         ok = __all_sync(0xffffffffu, ok);
         const uint32_t n_k = __popc(__ballot_sync(0xffffffffu, have_k)), n_v = __popc(__ballot_sync(0xffffffffu, have_v));
-        if (lane < 8 && !have_k && key_k <= key_last) {  // no such page: what it would hold is NaN
-          uint32_t* params = reinterpret_cast<uint32_t*>(smem + F::kRawParams) + lane * 16;
+        if (ok && lane < 8 && !have_k && key_k <= key_last) {  // no such page: what it would hold is NaN
+          uint32_t* params = reinterpret_cast<uint32_t*>(smem + F::kRaw + raw * F::kRawBytes + F::kRawParams) + lane * 16;
           for (int i = 0; i < 16; ++i) params[i] = params[kKeys + i] = 0x7E007E00u;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         __syncwarp();
         if (!ok) break;  // a wait gave up: nothing more is copied
         if (lane == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar(kRawKFull)), "r"(n_k * 16 * (D / 2 + 8)) : "memory");
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar(kRawKFull + raw)), "r"(n_k * 16 * (D / 2 + 8)) : "memory");
         __syncwarp();
         if (have_k) {
           const uint32_t slot = static_cast<uint32_t>(key_k) & (P - 1);
-          copy(base + F::kRawK + lane * 16 * (D / 2), block_k + slot * (D / 2), 16 * (D / 2), kRawKFull);
-          copy(base + F::kRawParams + lane * 64, block_k + P * D + slot * 4, 64, kRawKFull);
-          copy(base + F::kRawParams + kKeys * 4 + lane * 64, block_k + P * D + (P + slot) * 4, 64, kRawKFull);
+          copy(codes + lane * 16 * (D / 2), block_k + slot * (D / 2), 16 * (D / 2), kRawKFull + raw);
+          copy(codes + F::kRawParams + lane * 64, block_k + P * D + slot * 4, 64, kRawKFull + raw);
+          copy(codes + F::kRawParams + kKeys * 4 + lane * 64, block_k + P * D + (P + slot) * 4, 64, kRawKFull + raw);
         }
-        if (j > 0) ok = wait(kRawVFree, j - 1) && ok;
+        if (j >= kRaws) ok = wait(kRawVFree + raw, j / kRaws - 1) && ok;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar(kRawVFull)), "r"(n_v * 4 * D) : "memory");
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar(kRawVFull + raw)), "r"(n_v * 4 * D) : "memory");
         __syncwarp();
-        if (have_v) copy(base + F::kRawV + lane * F::kGroup, block_v + (P + (static_cast<uint32_t>(key_v) & (P - 1))) * (D / 2), 4 * D, kRawVFull);
+        if (have_v) copy(codes + F::kRawV + lane * F::kGroup, block_v + (P + (static_cast<uint32_t>(key_v) & (P - 1))) * (D / 2), 4 * D, kRawVFull + raw);
       }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == F::kMmaWarp) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
@@ -661,7 +740,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
 template <typename T, int D>
 cudaError_t many_as(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond) {
   using F = Many<T, D>;
-  static_assert(F::kSmem <= 227 * 1024 && F::kTable % 16 == 0 && F::kRows % 16 == 0 && F::kLost % 16 == 0 && F::kBars % 8 == 0 && F::kRawParams % 16 == 0,
+  static_assert(F::kSmem <= 227 * 1024 && F::kTable % 16 == 0 && F::kRows % 16 == 0 && F::kLost % 16 == 0 && F::kBars % 8 == 0 && F::kRawParams % 16 == 0 && F::kRawBytes % 16 == 0,
                 "shared memory and the alignment of its arrays");
   static OncePerDevice once;
   cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_many_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem); });
@@ -678,7 +757,7 @@ cudaError_t many_as(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond) 
   const uint64_t blocks = rows / kBlock + std::min<uint64_t>(a.batch.sequences, rows / (beyond + 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.cache.kv_heads));
-  cfg.blockDim = dim3(kManyThreads);
+  cfg.blockDim = dim3(F::kThreads);
   cfg.dynamicSmemBytes = F::kSmem;
   cfg.stream = env.stream;
   cudaLaunchAttribute attr;
