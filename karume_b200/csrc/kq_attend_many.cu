@@ -7,7 +7,7 @@
 // and walks over the keys they see in tiles of 128.  Warps:
 //   0-3, 4-7   one row each thread of the first / second 128 rows: scores from tensor memory, weights back into it; f32 queries:
 //              the sums of the output in registers (what the tensor core adds is one tile's, so that a long row does not drift)
-//   four (f32) or eight   unpack a tile: keys as [token][dim], values transposed as [dim][token], both K-major, 128-byte swizzle
+//   four (f32) or six     unpack a tile: keys as [token][dim], values transposed as [dim][token], both K-major, 128-byte swizzle
 //   one        issues the MMAs:   S_r = Q_r K^T (both in shared memory),   O_r += P_r V (P in tensor memory, over S)
 //   one        copies the codes and scales of the next tile (bulk copies, page by page)
 // The two row blocks take turns: while one's weights are being computed the tensor core works for the other.
@@ -37,9 +37,10 @@ struct Many {
   static constexpr int kParts = kSplit ? 2 : 1;
   // 8 softmax warps, the unpacking ones, MMA, copies.  f32 keeps the output's sums in the softmax warps' registers (192 a thread,
   // taken from the others, which makes whole groups of four warps); 16-bit ones stay in tensor memory.
-  static constexpr int kUnpackWarps = kSplit ? 4 : 8, kUnpack = kUnpackWarps * 32;
+  static constexpr int kUnpackWarps = kSplit ? 4 : 6, kUnpack = kUnpackWarps * 32;
   static constexpr int kMmaWarp = 8 + kUnpackWarps, kCopyWarp = kMmaWarp + 1;
-  static constexpr int kThreads = kSplit ? 512 : (kCopyWarp + 1) * 32;
+  static constexpr int kThreads = 512;
+  static constexpr int kAtOnce = kSplit ? 16 : 32;         // scores a softmax thread has in hand
   static constexpr int kOperand = 128 * D * 2;             // bytes of 128 rows (or tokens) of D values
   static constexpr bool kFull = kSplit && D == 128;        // the queries leave room for one of everything
   static constexpr int kVBufs = kFull ? 1 : 2;             // unpacked values; one tile of unpacked keys (needed only while scores are made)
@@ -104,6 +105,31 @@ __device__ __forceinline__ void tmem_ld16_done(float (&f)[16]) {
                :
                : "memory");
 }
+// ... and any number of them
+template <int N>
+__device__ __forceinline__ void tmem_ld_begin(uint32_t taddr, float (&f)[N]) {
+  if constexpr (N == 16) {
+    tmem_ld16_begin(taddr, f);
+  } else {
+    static_assert(N == 32, "columns at a time");
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_done(float (&f)[N]) {
+  if constexpr (N == 16) {
+    tmem_ld16_done(f);
+  } else {
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) : : "memory");
+    asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+  }
+}
 // N columns, sixteen at a time: use(column, values), the next ones on their way meanwhile.  kFlat: unrolled, so that the
 // column is a constant (registers are indexed with it); otherwise a loop, for the instruction cache.
 template <int N, bool kFlat, typename Use>
@@ -120,7 +146,7 @@ __device__ __forceinline__ void tmem_columns(uint32_t taddr, Use use) {
     use(c + 16, x[1]);
   }
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
@@ -242,18 +268,20 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   const int tile0 = key_first / kKeys, tiles = key_last < 0 ? 0 : key_last / kKeys + 1 - tile0;
 
   // ---- queries --------------------------------------------------------------------------------------
-  {
-    constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+  const auto stage_queries = [&](auto plain) {
+    constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
     const uint32_t c = lane % kLanes;
 #pragma unroll 2
-    for (uint32_t r = warp * kAtOnce + lane / kLanes; r < kBlock; r += F::kThreads / 32 * kAtOnce) {
-      const int row = row0 + static_cast<int>(r), query = row / static_cast<int>(p.group);
+    for (uint32_t r = warp * kRowsAtOnce + lane / kLanes; r < kBlock; r += F::kThreads / 32 * kRowsAtOnce) {
+      const int row = row0 + static_cast<int>(r), query = min(row, n_rows - 1) / static_cast<int>(p.group);
       const bool there = row < n_rows;
-      float v[8] = {};
-      if (there)
-        load8_rotated(static_cast<const T*>(p.a.q) + static_cast<size_t>(span.first + query) * p.a.q_stride +
-                          static_cast<size_t>(head * p.group + static_cast<uint32_t>(row - query * static_cast<int>(p.group))) * D,
-                      c * 8, p.a.rope, before + query, v);
+      float v[8];
+      const T* from_q = static_cast<const T*>(p.a.q) + static_cast<size_t>(span.first + query) * p.a.q_stride +
+                        static_cast<size_t>(head * p.group + static_cast<uint32_t>(min(row, n_rows - 1) - query * static_cast<int>(p.group))) * D;
+      if constexpr (decltype(plain)::value) load8_rotated_plain(from_q, c * 8, p.a.rope, before + query, v);
+      else load8_rotated(from_q, c * 8, p.a.rope, before + query, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = there ? v[i] : 0.0f;
       float big = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -293,8 +321,10 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
                          : make_float4(factor * exp2f(static_cast<float>(-up)), 0.0f, __int_as_float(last), __int_as_float(from));
       }
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
+  };
+  if (rope_is_plain(p.a.rope)) stage_queries(std::true_type());
+  else stage_queries(std::false_type());
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (warp == F::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(tmem_word))), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -321,8 +351,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     }
     // Weights are 2^(score - M + kLift).  M is a whole number (what it moves by is an exact power of two) that follows the row's
     // largest score, f32: and the binade of the values' scales beside it; it moves when a weight (times its value's scale) would
-    // pass 2^14.  So that this is seen before anything is written, sixteen scores are looked at at a time; what was written
+    // pass 2^14.  So that this is seen before anything is written, a few scores are looked at at a time; what was written
     // of the tile before is then scaled too.  f32 lets M lag by one bit, to keep the fixed-point parts' 22; 16-bit by eight.
+    constexpr int kN = F::kAtOnce;
     constexpr float kLift = kSplit ? 13.0f : 6.0f, kLag = kSplit ? 1.0f : 8.0f;
     float M = -INFINITY, l = 0.0f, centre = 0.0f;
     for (int j = 0; j < tiles; ++j) {
@@ -347,11 +378,11 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       float limit = M + kLag - binade, shift = M == -INFINITY ? kLift : kLift - M;
       const auto tile = [&](auto all_seen) {
         constexpr bool kAll = decltype(all_seen)::value;
-        float x[2][16];
-        const auto sixteen = [&](int c, float (&z)[16], auto begin_next) {
-          float big[8];
+        float x[2][kN];
+        const auto some = [&](int c, float* z, auto begin_next) {
+          float big[kN / 2];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < kN; ++i) {
             if constexpr (kSplit) {
               const float2 k = __half22float2(k_par[c + i]);
               z[i] = fmaf(z[i], k.x, k.y * q_sum);
@@ -359,9 +390,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             if (!kAll && (c + i < sees0 || c + i > sees1)) z[i] = -INFINITY;  // what is not seen may hold anything
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) big[i] = fmaxf(z[i], z[i + 8]);
+          for (int i = 0; i < kN / 2; ++i) big[i] = fmaxf(z[i], z[i + kN / 2]);
 #pragma unroll
-          for (int o = 4; o > 0; o /= 2)
+          for (int o = kN / 4; o > 0; o /= 2)
 #pragma unroll
             for (int i = 0; i < o; ++i) big[i] = fmaxf(big[i], big[i + o]);
           const float top = big[0] * factor;
@@ -408,10 +439,10 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           }
           begin_next();
-          uint32_t hi[8], lo[8];
+          uint32_t hi[kN / 2], lo[kN / 2];
           float part[4] = {}, mid[4] = {};
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
+          for (int i = 0; i < kN; i += 2) {
             float w[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -436,17 +467,20 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
           l += (part[0] + part[1]) + (part[2] + part[3]);
           if constexpr (kSplit) centre += (mid[0] + mid[1]) + (mid[2] + mid[3]);
           // sixteen keys' weights go where their scores were: eight columns, and eight for the low parts
-          tmem_st8(t_s + c, hi);
-          if constexpr (kSplit) tmem_st8(t_s + c + 8, lo);
+#pragma unroll
+          for (int i = 0; i < kN / 16; ++i) {
+            tmem_st8(t_s + c + i * 16, hi + i * 8);
+            if constexpr (kSplit) tmem_st8(t_s + c + i * 16 + 8, lo + i * 8);
+          }
         };
-        tmem_ld16_begin(t_s, x[0]);
+        tmem_ld_begin(t_s, x[0]);
 #pragma unroll 1
-        for (int c = 0; c < kKeys; c += 32) {
-          tmem_ld16_done(x[0]);
-          sixteen(c, x[0], [&] { tmem_ld16_begin(t_s + c + 16, x[1]); });
-          tmem_ld16_done(x[1]);
-          sixteen(c + 16, x[1], [&] {
-            if (c + 32 < kKeys) tmem_ld16_begin(t_s + c + 32, x[0]);
+        for (int c = 0; c < kKeys; c += 2 * kN) {
+          tmem_ld_done(x[0]);
+          some(c, x[0], [&] { tmem_ld_begin(t_s + c + kN, x[1]); });
+          tmem_ld_done(x[1]);
+          some(c + kN, x[1], [&] {
+            if (c + 2 * kN < kKeys) tmem_ld_begin(t_s + c + 2 * kN, x[0]);
           });
         }
       };
