@@ -811,7 +811,7 @@ int kq_rope(kq_ctx* ctx, uint64_t x_dptr, int x_dtype, uint32_t tokens, uint32_t
   if (!x_dptr || !out_dptr || !positions_dptr || !table_dptr || ((x_dptr | out_dptr) & mask) || (positions_dptr & 3u))
     return fail(ctx, KQ_ERR_BAD_ARG, "kq_rope: x, out, positions and the table must be aligned device pointers");
   if (row > 0xffffffffull || x_stride < row || out_stride < row || x_stride > (1ull << 40) || out_stride > (1ull << 40) || tokens > (1u << 30) ||
-      static_cast<uint64_t>(tokens) * row > (1ull << 38))
+      static_cast<uint64_t>(tokens) * row > (1ull << 38) || static_cast<uint64_t>(tokens) * heads > (1ull << 31) - 1)
     return fail(ctx, KQ_ERR_SHAPE, "kq_rope: rows of [%u, %u] do not fit strides %llu and %llu, or are too many", heads, head_dim,
                 (unsigned long long)x_stride, (unsigned long long)out_stride);
   if (x_dptr == out_dptr && x_stride != out_stride) return fail(ctx, KQ_ERR_BAD_ARG, "kq_rope: in place, both strides must be the same");

@@ -39,36 +39,58 @@ struct RopeParams {
   uint32_t tokens, heads, dim;
   uint32_t units;        // runs (or pairs of runs) a head
   uint32_t head_groups;  // threads that share a token's heads for one unit
+  bool wide;             // the table's rows can be read sixteen bytes at a time
 };
+
+template <int N>
+__device__ __forceinline__ void load_angles(const float2* p, bool inside, bool wide, float2 (&cs)[N]) {
+  if (!inside) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) cs[i] = make_float2(quiet_nan(), quiet_nan());
+  } else if (N % 2 == 0 && wide) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i / 2];
+      cs[i] = make_float2(v.x, v.y);
+      if (i + 1 < N) cs[i + 1] = make_float2(v.z, v.w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) cs[i] = p[i];
+  }
+}
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
   using R = Run<T, V>;
-  const uint64_t id = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const uint32_t unit = id % p.units;
-  const uint32_t group = id / p.units % p.head_groups;
-  const uint64_t token = id / (static_cast<uint64_t>(p.units) * p.head_groups);
-  if (token >= p.tokens) return;
+  pdl_launch_dependents();
+  const uint32_t across = min(p.units, static_cast<uint32_t>(kThreads)), slots = kThreads / across;  // (token, head group)s of a block
+  const uint32_t slot = threadIdx.x / across, unit = blockIdx.y * kThreads + threadIdx.x - slot * across;
+  const uint32_t at_slot = blockIdx.x * slots + slot, token = at_slot / p.head_groups, group = at_slot - token * p.head_groups;
+  pdl_wait_prior_grid();
+  if (slot >= slots || unit >= p.units || token >= p.tokens) return;
   const uint32_t half = p.rope.rotary / 2, turning = p.rope.interleaved && V > 1 ? p.rope.rotary / V : half / V;
   const T* x = static_cast<const T*>(p.x) + token * p.x_stride;
   T* out = static_cast<T*>(p.out) + token * p.out_stride;
   if (unit >= turning) {  // behind the rotated part
     const uint32_t at = p.rope.rotary + (unit - turning) * V;
-    if (x != out)
+    if (x != out) {
+#pragma unroll 4
       for (uint32_t h = group; h < p.heads; h += p.head_groups)
-        *reinterpret_cast<R*>(out + h * p.dim + at) = *reinterpret_cast<const R*>(x + h * p.dim + at);
+        *reinterpret_cast<R*>(out + static_cast<size_t>(h) * p.dim + at) = *reinterpret_cast<const R*>(x + static_cast<size_t>(h) * p.dim + at);
+    }
     return;
   }
   const int position = p.positions[token];
   const bool inside = position >= 0 && static_cast<uint32_t>(position) < p.rope.positions;
   const float2* row = p.rope.table + static_cast<size_t>(inside ? position : 0) * half;
-  float2 cs[V];
   if constexpr (V > 1) {
     if (p.rope.interleaved) {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) cs[i] = inside ? row[unit * (V / 2) + i] : make_float2(quiet_nan(), quiet_nan());
+      float2 cs[V / 2];
+      load_angles(row + unit * (V / 2), inside, p.wide, cs);
+#pragma unroll 4
       for (uint32_t h = group; h < p.heads; h += p.head_groups) {
-        const uint32_t at = h * p.dim + unit * V;
+        const size_t at = static_cast<size_t>(h) * p.dim + unit * V;
         R r = *reinterpret_cast<const R*>(x + at);
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
@@ -83,10 +105,11 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
   }
   // runs of V values and what they are paired with: rotary / 2 further on, or (interleaved, one value at a time) the next one
   const uint32_t step = p.rope.interleaved ? 2 : V, pair = p.rope.interleaved ? 1 : half;
-#pragma unroll
-  for (int i = 0; i < V; ++i) cs[i] = inside ? row[unit * V + i] : make_float2(quiet_nan(), quiet_nan());
+  float2 cs[V];
+  load_angles(row + unit * V, inside, p.wide, cs);
+#pragma unroll 4
   for (uint32_t h = group; h < p.heads; h += p.head_groups) {
-    const uint32_t at = h * p.dim + unit * step;
+    const size_t at = static_cast<size_t>(h) * p.dim + unit * step;
     R a = *reinterpret_cast<const R*>(x + at), b = *reinterpret_cast<const R*>(x + at + pair);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -99,14 +122,34 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
   }
 }
 
+// A launch that may begin while its predecessor drains (the kernels wait for it before they read anything).
+template <typename Kernel, typename Params>
+cudaError_t launch_overlapped(const LaunchEnv& env, Kernel kernel, dim3 grid, const Params& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = env.stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = env.overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <typename T, int V>
 cudaError_t rope_as(const LaunchEnv& env, RopeParams& p) {
   const uint32_t half = p.rope.rotary / 2;
   p.units = (p.rope.interleaved && V > 1 ? p.rope.rotary / V : half / V) + (p.dim - p.rope.rotary) / V;
-  p.head_groups = p.heads;
-  const uint64_t threads = static_cast<uint64_t>(p.tokens) * p.units * p.head_groups;
-  rope_kernel<T, V><<<static_cast<unsigned>((threads + kThreads - 1) / kThreads), kThreads, 0, env.stream>>>(p);
-  return cudaGetLastError();
+  p.wide = (reinterpret_cast<uintptr_t>(p.rope.table) & 15u) == 0 && half % 2 == 0;
+  // Heads a thread takes one after the other, the angles in registers: as many as leave the SMs full of threads
+  const uint64_t units = static_cast<uint64_t>(p.tokens) * p.units;
+  uint32_t each = 1;
+  while (each < 8 && each < p.heads && units * (p.heads / (2 * each)) >= static_cast<uint64_t>(env.sm_count) * 2048) each *= 2;
+  p.head_groups = (p.heads + each - 1) / each;
+  const uint32_t across = std::min<uint32_t>(p.units, kThreads), slots = kThreads / across;
+  const dim3 grid(static_cast<unsigned>((static_cast<uint64_t>(p.tokens) * p.head_groups + slots - 1) / slots), (p.units + kThreads - 1) / kThreads);
+  return launch_overlapped(env, rope_kernel<T, V>, grid, p);
 }
 
 // The longest run, up to 16 bytes, that divides the rotated part, the rest of a head and every address.
@@ -148,6 +191,8 @@ __device__ __forceinline__ RowOf row_of(uint64_t row, uint32_t heads) {
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendParams p) {
   constexpr int kLanes = D / 8;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
   const uint32_t lane = threadIdx.x % kLanes;
   const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
   const bool there = row < static_cast<uint64_t>(p.batch.tokens) * 2 * p.cache.kv_heads;
@@ -208,6 +253,8 @@ struct ReadParams {
 template <int D>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadParams p) {
   constexpr int kLanes = D / 8;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
   const uint32_t lane = threadIdx.x % kLanes;
   const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
   if (row >= static_cast<uint64_t>(p.batch.tokens) * 2 * p.cache.kv_heads) return;
@@ -244,19 +291,18 @@ template <typename T>
 cudaError_t append_as(const LaunchEnv& env, const AppendParams& p) {
   const unsigned grid = blocks_for(p.cache, p.batch);
   switch (p.cache.head_dim) {
-    case 64: cache_append_kernel<T, 64><<<grid, kThreads, 0, env.stream>>>(p); break;
-    case 128: cache_append_kernel<T, 128><<<grid, kThreads, 0, env.stream>>>(p); break;
-    case 256: cache_append_kernel<T, 256><<<grid, kThreads, 0, env.stream>>>(p); break;
+    case 64: return launch_overlapped(env, cache_append_kernel<T, 64>, grid, p);
+    case 128: return launch_overlapped(env, cache_append_kernel<T, 128>, grid, p);
+    case 256: return launch_overlapped(env, cache_append_kernel<T, 256>, grid, p);
     default: return cudaErrorInvalidValue;
   }
-  return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_rope(const LaunchEnv& env, const void* x, int dtype, uint32_t tokens, uint32_t heads, uint32_t dim, uint64_t x_stride,
                         const int* positions, const RopeTable& rope, void* out, uint64_t out_stride) {
-  RopeParams p = {x, out, x_stride, out_stride, positions, rope, tokens, heads, dim, 0, 0};
+  RopeParams p = {x, out, x_stride, out_stride, positions, rope, tokens, heads, dim, 0, 0, false};
   if (dtype == KQ_F32) return rope_of<float>(env, p);
   if (dtype == KQ_F16) return rope_of<__half>(env, p);
   return rope_of<__nv_bfloat16>(env, p);
@@ -274,12 +320,11 @@ cudaError_t launch_cache_read(const LaunchEnv& env, const Cache& cache, const Ca
   const ReadParams p = {cache, batch, k, v};
   const unsigned grid = blocks_for(cache, batch);
   switch (cache.head_dim) {
-    case 64: cache_read_kernel<64><<<grid, kThreads, 0, env.stream>>>(p); break;
-    case 128: cache_read_kernel<128><<<grid, kThreads, 0, env.stream>>>(p); break;
-    case 256: cache_read_kernel<256><<<grid, kThreads, 0, env.stream>>>(p); break;
+    case 64: return launch_overlapped(env, cache_read_kernel<64>, grid, p);
+    case 128: return launch_overlapped(env, cache_read_kernel<128>, grid, p);
+    case 256: return launch_overlapped(env, cache_read_kernel<256>, grid, p);
     default: return cudaErrorInvalidValue;
   }
-  return cudaGetLastError();
 }
 
 }  // namespace kq

@@ -55,7 +55,8 @@ def _load_fast() -> None:
         _torch()
         from . import _kqtorch
         _kqtorch.bind(*[ctypes.cast(f, ctypes.c_void_p).value
-                        for f in (L.kq_linear, L.kq_linear_fused, L.kq_quantize_rows, L.kq_linear_a8, L.kq_embedding)])
+                        for f in (L.kq_linear, L.kq_linear_fused, L.kq_quantize_rows, L.kq_linear_a8, L.kq_embedding, L.kq_rope,
+                                  L.kq_cache_append, L.kq_cache_read, L.kq_cache_attention)])
         _fast = _kqtorch
 
 
@@ -417,6 +418,9 @@ class Gpu:
     # -- the attention half of a decoder layer --------------------------------------------------
     def rope(self, x, positions, rope: Rope, out=None):
         """x [tokens, heads, head_dim] (f32 / f16 / bf16, tokens may be strided) rotated to positions (CUDA int32 [tokens])."""
+        done = _fast.rope(self._ctx_addr, x, positions, rope.args, out)
+        if done is not None:
+            return self._done(done)
         torch = _torch()
         tokens, heads, dim = x.shape
         px, stride = _rows(x, heads, dim, "x")
@@ -444,6 +448,10 @@ class Gpu:
 
     def cache_append(self, cache: KvCache, k, v, batch: CacheBatch, rope: "Rope | None" = None) -> None:
         """Stores the new tokens' keys (rotated on the way) and values [tokens, kv_heads, head_dim] in the cache's pages."""
+        done = _fast.cache_append(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, k, v, batch.args,
+                                  rope.args if rope is not None else None)
+        if done is not None:
+            return self._check(done)
         if k.shape[0] != batch.tokens or v.shape[0] != batch.tokens or k.dtype != v.dtype:
             raise KqError(2, f"k and v must be [{batch.tokens}, {cache.kv_heads}, {cache.head_dim}] of one type")
         pk, k_stride = _rows(k, cache.kv_heads, cache.head_dim, "k")
@@ -453,6 +461,9 @@ class Gpu:
 
     def cache_read(self, cache: KvCache, batch: CacheBatch):
         """(k, v) f32 [tokens, kv_heads, head_dim]: what the cache holds for the new tokens of `batch`."""
+        done = _fast.cache_read(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, self.index, batch.args)
+        if done is not None:
+            return self._done(done)
         torch = _torch()
         k, v = (torch.empty((batch.tokens, cache.kv_heads, cache.head_dim), dtype=torch.float32, device=self.device) for _ in range(2))
         self._check(L.kq_cache_read(self._ctx, cache.handle, *batch.args, k.data_ptr(), v.data_ptr()))
@@ -462,6 +473,12 @@ class Gpu:
                         rope: "Rope | None" = None, out=None):
         """Causal attention of q [tokens, heads, head_dim] (f32 / f16 / bf16, rotated on the way) over each sequence's keys
         in the cache, the last `window` of them if given; scale defaults to head_dim^-0.5.  Returns q's type."""
+        if scale is None:
+            scale = cache.head_dim ** -0.5
+        done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window,
+                                     rope.args if rope is not None else None, out)
+        if done is not None:
+            return self._done(done)
         torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
@@ -473,7 +490,7 @@ class Gpu:
             raise KqError(2, "out must have q's type and shape")
         po, out_stride = _rows(out, heads, dim, "out")
         self._check(L.kq_cache_attention(self._ctx, cache.handle, pq, q_stride, _tensor_dtype_code(q), heads, *batch.args, batch.most,
-                                         float(scale if scale is not None else dim ** -0.5), int(window),
+                                         float(scale), int(window),
                                          *(rope.args if rope is not None else _NO_ROPE), po, out_stride))
         return out
 
