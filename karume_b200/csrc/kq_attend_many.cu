@@ -13,8 +13,8 @@
 // The two row blocks take turns: while one's weights are being computed the tensor core works for the other.
 //
 //   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights).
-//   f32 queries     codes enter exactly: keys as the subnormals u 2^-24 and u 2^-20 that their bits already are, values as
-//                   codes around zero; scale and offset are applied to the scores and weights in f32.  Queries and weights are
+//   f32 queries     codes enter exactly, around zero: (2 u - 15) 2^-24 and (u - 7.5) 2^-20, one operation from the subnormals that
+//                   their bits already are; scale and offset are applied to the scores and weights in f32.  Queries and weights are
 //                   two binary16 parts each (fixed-point, the low ones multiplied first), 22 bits and more.
 #include <algorithm>
 #include <type_traits>
@@ -53,19 +53,26 @@ struct Many {
   static constexpr int kRawV = kKeys * (D / 2);            // in a tile of codes: keys, values,
   static constexpr int kRawParams = kRawV + 16 * kGroup;   // keys' and values' (scale, offset)
   static constexpr int kRawBytes = kRawParams + 2 * kKeys * 4;
-  static constexpr int kTable = kRaw + kRaws * kRawBytes;  // [2][2][128]: (scale, offset) of keys and values, what is not seen zero
-  static constexpr int kRows = kTable + 4 * kKeys * 4;     // [256] (factor, sum, last key, first key)
+  // [2] x 16-bit: [2][128] (scale, offset) of keys and values; f32: [4][128] scale and centre of keys, then of values (2^13 scale)
+  static constexpr int kTable = kRaw + kRaws * kRawBytes;
+  static constexpr int kTableBytes = (kSplit ? 4 : 2) * kKeys * 4;
+  static constexpr int kRows = kTable + 2 * kTableBytes;   // [256] (factor, sum, last key, first key)
   static constexpr int kLost = kRows + kBlock * 16;        // [2] 128 bits: tokens whose value is NaN
   static constexpr int kBinade = kLost + 32;               // [2][4]: largest binade of the values' scales, by warp
   static constexpr int kBars = kBinade + 32;
   static constexpr int kMisc = kBars + kBarCount * 8;
-  static constexpr int kSmem = kMisc + 64 + 1024;          // the operands start on a multiple of 1024
+  static constexpr int kPartFloats = kBlock * (D + 2);
+  static constexpr int kUnits = 512;                       // more than these are not shared by CTAs
+  static constexpr int kSmem = kMisc + 96 + 1024;          // the operands start on a multiple of 1024
 };
 
 struct ManyParams {
   AttendArgs a;
   uint32_t group, page_shift, beyond;  // sequences of more than `beyond` query rows a kv head are this kernel's
   int* status;
+  float* parts;            // null: a CTA walks over all keys of its rows.  Else [CTAs][kPartFloats]: sums, then (M, l) of each row
+  unsigned int* counters;  // [units], zero between launches
+  uint32_t ctas;           // that share the keys' tiles evenly
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -75,6 +82,24 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // a whole number that is more than log2 of a scale (of binary16: no smaller than 2^-24)
 __device__ __forceinline__ float binade_of(float scale) { return static_cast<float>(max(static_cast<int>(__float_as_uint(scale) >> 23) - 126, -24)); }
+// two f32 operations as one
+__device__ __forceinline__ uint64_t bits2(float2 v) { return *reinterpret_cast<const uint64_t*>(&v); }
+__device__ __forceinline__ float2 float2_of(uint64_t v) { return *reinterpret_cast<const float2*>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return float2_of(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return float2_of(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return float2_of(r);
+}
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -151,6 +176,26 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
                ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
+// The thread's lane of n columns times `keep`: weights (two binary16 a column) or sums.  Seldom run: a call, so that the loop
+// around it keeps its registers.
+template <bool kHalves>
+__device__ __noinline__ void scale_columns(uint32_t taddr, int n, float keep) {
+  const __half2 keep2 = __float2half2_rn(keep);
+  for (int at = 0; at < n; at += 16) {
+    float w[16];
+    tmem_ld16_begin(taddr + at, w);
+    tmem_ld16_done(w);
+    uint32_t y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w[i]), keep2);
+      y[i] = kHalves ? *reinterpret_cast<const uint32_t*>(&h) : __float_as_uint(w[i] * keep);
+    }
+    tmem_st8(taddr + at, y);
+    tmem_st8(taddr + at + 8, y + 8);
+  }
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 // binary16 operands, f32 accumulators; descriptors by their low words
 __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
   asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
@@ -165,6 +210,17 @@ __device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, 
 __device__ __forceinline__ uint32_t desc_low(uint32_t smem) { return ((smem >> 4) & 0x3FFFu) | (1u << 16); }
 __host__ __device__ constexpr uint32_t f16_idesc(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
 
+__device__ __forceinline__ void load2(const float* p, float& a, float& b) {
+  const float2 v = *reinterpret_cast<const float2*>(p);
+  a = v.x;
+  b = v.y;
+}
+template <typename T>
+__device__ __forceinline__ void load2(const T* p, float& a, float& b) {
+  const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+  a = to_f32(reinterpret_cast<const T*>(&v)[0]);
+  b = to_f32(reinterpret_cast<const T*>(&v)[1]);
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* v);
 template <>
@@ -199,7 +255,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   float4* const rows = reinterpret_cast<float4*>(smem + F::kRows);
   uint32_t* const tmem_word = reinterpret_cast<uint32_t*>(smem + F::kMisc + 16);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + F::kMisc + 20);
-  uint32_t* const found = reinterpret_cast<uint32_t*>(smem + F::kMisc + 24);  // sequence, number in it
+  uint32_t* const found = reinterpret_cast<uint32_t*>(smem + F::kMisc + 24);  // sequence, number in it, part, parts, unit
   const auto bar = [&](int i) { return base + F::kBars + i * 8; };
   const auto wait = [&](int i, uint32_t parity) {
     const bool ok = umma::wait_bounded(bar(i), parity & 1u, abort_flag, p.status, kManyTimeout);
@@ -248,43 +304,198 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   uint32_t* const scan = reinterpret_cast<uint32_t*>(smem + F::kRows);
   if (lane == 31) scan[warp] = upto;
   __syncthreads();
-  for (uint32_t i = 0; i < warp; ++i) upto += scan[i];
-  if (upto - mine <= blockIdx.x && blockIdx.x < upto) {
-    uint32_t b = tid * each, left = blockIdx.x - (upto - mine);
-    for (uint32_t n = blocks_of(b) * heads; left >= n; n = blocks_of(++b) * heads) left -= n;
-    found[0] = b;
-    found[1] = left;
+  uint32_t units = 0;
+  for (uint32_t i = 0; i < F::kThreads / 32; ++i) {
+    if (i < warp) upto += scan[i];
+    units += scan[i];
+  }
+  const int window = static_cast<int>(min(p.a.window, 0x7fffffffu));
+  // the tiles of a unit: first and number
+  const auto tiles_of = [&](uint32_t b, uint32_t number) {
+    const Span s = span_of(p.a.batch, b);
+    const int block = static_cast<int>(blocks_of(b) - 1 - number / heads), n = s.count * static_cast<int>(p.group);
+    const int first = block * kBlock / static_cast<int>(p.group), last = min(block * kBlock + kBlock - 1, n - 1) / static_cast<int>(p.group);
+    const int key_last = s.length - s.count + last, from = s.length - s.count + first + 1 - window;
+    const int tile0 = window && from > 0 ? from / kKeys : 0;
+    return make_int2(tile0, key_last < 0 ? 0 : key_last / kKeys + 1 - tile0);
+  };
+  if (!p.parts) {
+    if (upto - mine <= blockIdx.x && blockIdx.x < upto) {
+      uint32_t b = tid * each, left = blockIdx.x - (upto - mine);
+      for (uint32_t n = blocks_of(b) * heads; left >= n; n = blocks_of(++b) * heads) left -= n;
+      found[0] = b;
+      found[1] = left;
+      found[3] = 1;
+    }
+  } else if (units > 0) {  // parts of units, as many as make the CTAs' shares even
+    uint32_t* const of = reinterpret_cast<uint32_t*>(smem);  // sequence and number of each unit
+    uint32_t at = upto - mine;
+    for (uint32_t b = tid * each; b < min((tid + 1) * each, sequences); ++b)
+      for (uint32_t n = blocks_of(b) * heads, i = 0; i < n; ++i, ++at)
+        if (at < F::kUnits) {
+          of[2 * at] = b;
+          of[2 * at + 1] = i;
+        }
+    __syncthreads();
+    const int mine_tiles = tid < units ? tiles_of(of[2 * tid], of[2 * tid + 1]).y : 0;
+    const int warp_tiles = __reduce_add_sync(0xffffffffu, mine_tiles);
+    __syncthreads();
+    if (lane == 0) scan[warp] = static_cast<uint32_t>(warp_tiles);
+    __syncthreads();
+    int all = 0;
+    for (int i = 0; i < F::kThreads / 32; ++i) all += static_cast<int>(scan[i]);
+    // the smallest share of tiles with which the parts are one wave of CTAs
+    int share = max((all + static_cast<int>(p.ctas) - 1) / static_cast<int>(p.ctas), 2);
+    uint32_t n_parts = 0;
+    for (;; ++share) {
+      n_parts = tid < units ? static_cast<uint32_t>(max((mine_tiles + share - 1) / share, 1)) : 0u;
+      const bool more = __syncthreads_or(n_parts > 1);
+      const uint32_t warp_parts = __reduce_add_sync(0xffffffffu, n_parts);
+      if (lane == 0) scan[warp] = warp_parts;
+      __syncthreads();
+      uint32_t sum = 0;
+      for (int i = 0; i < F::kThreads / 32; ++i) sum += scan[i];
+      __syncthreads();
+      if (sum <= p.ctas || !more) break;
+    }
+    uint32_t to = n_parts;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= static_cast<uint32_t>(o)) to += v;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = to;
+    __syncthreads();
+    for (uint32_t i = 0; i < warp; ++i) to += scan[i];
+    if (to - n_parts <= blockIdx.x && blockIdx.x < to) {
+      found[0] = of[2 * tid];
+      found[1] = of[2 * tid + 1];
+      found[2] = blockIdx.x - (to - n_parts);
+      found[3] = n_parts;
+      found[4] = tid;
+    }
   }
   __syncthreads();
   const uint32_t seq = found[0];
   if (seq == 0xFFFFFFFFu) return;
   const Span span = span_of(p.a.batch, seq);
   const uint32_t blocks = blocks_of(seq), head = found[1] % heads, block = blocks - 1 - found[1] / heads;  // the longest first
+  const uint32_t all_parts = found[3], my_part = all_parts > 1 ? found[2] : 0;
   const int row0 = static_cast<int>(block * kBlock), n_rows = span.count * static_cast<int>(p.group), before = span.length - span.count;
-  const int window = static_cast<int>(min(p.a.window, 0x7fffffffu));
-  const int q_first = row0 / static_cast<int>(p.group), q_last = min(row0 + kBlock - 1, n_rows - 1) / static_cast<int>(p.group);
-  const int key_last = before + q_last;
-  const int key_first = window && before + q_first + 1 > window ? before + q_first + 1 - window : 0;
-  const int tile0 = key_first / kKeys, tiles = key_last < 0 ? 0 : key_last / kKeys + 1 - tile0;
+  const int key_last = before + min(row0 + kBlock - 1, n_rows - 1) / static_cast<int>(p.group);
+  const int2 walk = tiles_of(seq, found[1]);
+  const int part_from = static_cast<int>(static_cast<int64_t>(walk.y) * my_part / all_parts), part_to = static_cast<int>(static_cast<int64_t>(walk.y) * (my_part + 1) / all_parts);
+  const int tile0 = walk.x + part_from, tiles = part_to - part_from;
+  __syncthreads();  // `scan` and the units' list lie where the queries go
 
   // ---- queries --------------------------------------------------------------------------------------
-  const auto stage_queries = [&](auto plain) {
+  const int q_of_row0 = row0 / static_cast<int>(p.group), head_of_row0 = row0 - q_of_row0 * static_cast<int>(p.group);
+  const float inv_group = 1.0f / static_cast<float>(p.group);
+  // query and head of row row0 + r: numbers below 2^17, so that the rounded-down product with the reciprocal is the quotient
+  const auto query_and_head = [&](int r) {
+    const int q = static_cast<int>((static_cast<float>(r + head_of_row0) + 0.5f) * inv_group);
+    return make_int2(q_of_row0 + q, r + head_of_row0 - q * static_cast<int>(p.group));
+  };
+  const auto pointer_of = [&](int2 qh) {
+    return static_cast<const T*>(p.a.q) + static_cast<size_t>(span.first + qh.x) * p.a.q_stride + (head * p.group + static_cast<uint32_t>(qh.y)) * D;
+  };
+  // a row is lifted to just below 2^14
+  const auto lift_of = [](float big) {
+    const int e = static_cast<int>(__float_as_uint(big) >> 23);
+    return big > 0.0f && e < 255 ? min(max(140 - e, -100), 100) : 0;
+  };
+  const auto power = [](int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); };  // |e| up to 126
+  // f32: fixed-point parts; odd dims meet codes eight times as large
+  const auto parts_of = [](float x, bool odd, float& hi, float& lo) {
+    constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
+    const float top = __fsub_rn(__fadd_rn(x, kEight), kEight), down = odd ? 0.125f : 1.0f;
+    hi = top * down;
+    lo = (x - top) * down;
+  };
+  const auto row_constants = [&](uint32_t r, int up, float sum) {
+    const float factor = p.a.scale * 1.4426950408889634f;
+    const bool there = row0 + static_cast<int>(r) < n_rows;
+    const int last = there ? before + query_and_head(static_cast<int>(r)).x : 0x7fffffff;  // rows beyond the end see anything and are not stored
+    const int from = there && window && last + 1 > window ? last + 1 - window : 0;
+    // f32: score = factor 2^(23 - up) (acc scale + centre sum 2^(up - 23))
+    rows[r] = kSplit ? make_float4(factor * power(23 - up), sum * power(up - 23), __int_as_float(last), __int_as_float(from))
+                     : make_float4(factor * power(-up), 0.0f, __int_as_float(last), __int_as_float(from));
+  };
+  if (rope_is_plain(p.a.rope) && p.a.rope.rotary == D) {
+    // Half layout, whole heads: a lane has two pairs of a row, so that the angles are read coalesced (runs of eight dims a lane read them
+    // at a stride of 64 bytes, 9000 clocks a CTA); words of dims (d, d + 4) are put together with the lane two further on.
+    constexpr uint32_t kLanes = D / 4, kRowsAtOnce = 32 / kLanes, kStep = F::kThreads / 32 * kRowsAtOnce, kBatch = 8;
+    static_assert(kBlock % (kStep * kBatch) == 0, "whole batches");
+    const uint32_t c = lane % kLanes;
+    const uint32_t word = (c & 1) * 2 + (c >> 1 & 1);  // of its eight dims' chunk: dims (0, 4), (1, 5), (2, 6), (3, 7) from lanes 0, 2, 1, 3
+#pragma unroll 1
+    for (uint32_t r0 = warp * kRowsAtOnce + lane / kLanes; r0 < kBlock; r0 += kStep * kBatch) {
+      float x[kBatch][4];
+      float4 cs[kBatch];
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k) {
+        const int2 qh = query_and_head(min(static_cast<int>(r0 + k * kStep), n_rows - 1 - row0));
+        const T* from_q = pointer_of(qh);
+        const int position = before + qh.x;
+        const bool inside = position >= 0 && static_cast<uint32_t>(position) < p.a.rope.positions;
+        load2(from_q + 2 * c, x[k][0], x[k][1]);
+        load2(from_q + D / 2 + 2 * c, x[k][2], x[k][3]);
+        cs[k] = reinterpret_cast<const float4*>(p.a.rope.table + static_cast<size_t>(inside ? position : 0) * (D / 2))[c];
+        if (!inside) cs[k].x = cs[k].z = quiet_nan();
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k) {
+        const uint32_t r = r0 + k * kStep;
+        const bool there = row0 + static_cast<int>(r) < n_rows;
+        const float2 a = rotate_pair(x[k][0], x[k][2], make_float2(cs[k].x, cs[k].y)), b = rotate_pair(x[k][1], x[k][3], make_float2(cs[k].z, cs[k].w));
+        float v[4] = {a.x, b.x, a.y, b.y};  // dims 2 c, 2 c + 1, and those half a head on
+        float big = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = there ? v[i] : 0.0f;
+          big = fmaxf(big, fabsf(v[i]));
+          sum += v[i];
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o /= 2) {
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          if constexpr (kSplit) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        const int up = lift_of(big);
+        const float lift = power(up);
+        float hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kSplit) parts_of(v[i] * lift, i & 1, hi[i], lo[i]);
+          else hi[i] = v[i] * lift;
+        }
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float* h = part ? lo : hi;
+            const uint32_t mine2 = half2_bits(h[2 * half], h[2 * half + 1]), other2 = __shfl_xor_sync(0xffffffffu, mine2, 2);
+            const uint32_t out = c & 2 ? __byte_perm(other2, mine2, 0x7632) : __byte_perm(mine2, other2, 0x5410);
+            const uint32_t chunk = half * (D / 16) + c / 4;
+            const uint32_t at = base + F::kQ + ((r / 128) * kParts + part) * F::kOperand + (chunk / 8) * 16384 + umma::swz(r % 128, chunk % 8) + word * 4;
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(out) : "memory");
+          }
+        if (c == 0) row_constants(r, up, sum);
+      }
+    }
+  } else {
     constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
     const uint32_t c = lane % kLanes;
-#pragma unroll 2
+#pragma unroll 1
     for (uint32_t r = warp * kRowsAtOnce + lane / kLanes; r < kBlock; r += F::kThreads / 32 * kRowsAtOnce) {
-      const int row = row0 + static_cast<int>(r), query = min(row, n_rows - 1) / static_cast<int>(p.group);
-      const bool there = row < n_rows;
-      float v[8];
-      const T* from_q = static_cast<const T*>(p.a.q) + static_cast<size_t>(span.first + query) * p.a.q_stride +
-                        static_cast<size_t>(head * p.group + static_cast<uint32_t>(min(row, n_rows - 1) - query * static_cast<int>(p.group))) * D;
-      if constexpr (decltype(plain)::value) load8_rotated_plain(from_q, c * 8, p.a.rope, before + query, v);
-      else load8_rotated(from_q, c * 8, p.a.rope, before + query, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = there ? v[i] : 0.0f;
-      float big = 0.0f, sum = 0.0f;
+      const bool there = row0 + static_cast<int>(r) < n_rows;
+      const int2 qh = query_and_head(min(static_cast<int>(r), n_rows - 1 - row0));
+      float v[8], big = 0.0f, sum = 0.0f;
+      load8_rotated(pointer_of(qh), c * 8, p.a.rope, before + qh.x, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
+        v[i] = there ? v[i] : 0.0f;
         big = fmaxf(big, fabsf(v[i]));
         sum += v[i];
       }
@@ -293,37 +504,21 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
       }
-      const int e = static_cast<int>(__float_as_uint(big) >> 23);
-      const int up = big > 0.0f && e < 255 ? min(max(140 - e, -100), 120) : 0;  // below 2^14
-      const float lift = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+      const int up = lift_of(big);
+      const float lift = power(up);
       float hi[8], lo[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = v[i] * lift;
-        if constexpr (kSplit) {  // odd dims meet codes sixteen times as large
-          const float top = rintf(x * 0.125f) * 8.0f, down = (i & 1) ? 0.0625f : 1.0f;
-          hi[i] = top * down;
-          lo[i] = rintf((x - top) * 256.0f) * (0.00390625f * down);
-        } else {
-          hi[i] = x;
-        }
+        if constexpr (kSplit) parts_of(v[i] * lift, i & 1, hi[i], lo[i]);
+        else hi[i] = v[i] * lift;
       }
       const uint32_t at = base + F::kQ + (r / 128) * kParts * F::kOperand + (c / 8) * 16384 + umma::swz(r % 128, c % 8);
       umma::sts128(at, make_uint4(half2_bits(hi[0], hi[4]), half2_bits(hi[1], hi[5]), half2_bits(hi[2], hi[6]), half2_bits(hi[3], hi[7])));
       if constexpr (kSplit)
         umma::sts128(at + F::kOperand, make_uint4(half2_bits(lo[0], lo[4]), half2_bits(lo[1], lo[5]), half2_bits(lo[2], lo[6]), half2_bits(lo[3], lo[7])));
-      if (c == 0) {
-        const float factor = p.a.scale * 1.4426950408889634f;
-        const int last = there ? before + query : 0x7fffffff;  // rows beyond the end see anything and are not stored
-        const int from = there && window && last + 1 > window ? last + 1 - window : 0;
-        // f32: score = factor 2^(24 - up) (acc ks + ko sum 2^(up - 24))
-        rows[r] = kSplit ? make_float4(factor * exp2f(static_cast<float>(24 - up)), sum * exp2f(static_cast<float>(up - 24)), __int_as_float(last), __int_as_float(from))
-                         : make_float4(factor * exp2f(static_cast<float>(-up)), 0.0f, __int_as_float(last), __int_as_float(from));
-      }
+      if (c == 0) row_constants(r, up, sum);
     }
-  };
-  if (rope_is_plain(p.a.rope)) stage_queries(std::true_type());
-  else stage_queries(std::false_type());
+  }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (warp == F::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(tmem_word))), "r"(512u) : "memory");
@@ -354,14 +549,13 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     // pass 2^14.  So that this is seen before anything is written, a few scores are looked at at a time; what was written
     // of the tile before is then scaled too.  f32 lets M lag by one bit, to keep the fixed-point parts' 22; 16-bit by eight.
     constexpr int kN = F::kAtOnce;
-    constexpr float kLift = kSplit ? 13.0f : 6.0f, kLag = kSplit ? 1.0f : 8.0f;
+    constexpr float kLift = kSplit ? 0.0f : 6.0f, kLag = kSplit ? 1.0f : 8.0f;  // f32: the values' scales carry 2^13
     float M = -INFINITY, l = 0.0f, centre = 0.0f;
     for (int j = 0; j < tiles; ++j) {
       const int first = (tile0 + j) * kKeys;
       const bool whole = first >= from_all && first + kKeys - 1 <= last_all;
       const int sees0 = from - first, sees1 = last - first;  // columns the row sees
-      const __half2* k_par = reinterpret_cast<const __half2*>(smem + F::kTable) + (j & 1) * 2 * kKeys;
-      const __half2* v_par = k_par + kKeys;
+      const float* table = reinterpret_cast<const float*>(smem + F::kTable + (j & 1) * F::kTableBytes);
       wait(kSFull + wg, j);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       float binade = 0.0f;
@@ -371,22 +565,27 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         if (!whole) {  // ... of what this row sees
           float big = 0.0f;
           for (int i = 0; i < kKeys; ++i)
-            if (i >= sees0 && i <= sees1) big = fmaxf(big, __low2float(v_par[i]));
-          binade = binade_of(big);
+            if (i >= sees0 && i <= sees1) big = fmaxf(big, table[2 * kKeys + i]);
+          binade = binade_of(big * (1.0f / 8192.0f));
         }
       }
       float limit = M + kLag - binade, shift = M == -INFINITY ? kLift : kLift - M;
       const auto tile = [&](auto all_seen) {
         constexpr bool kAll = decltype(all_seen)::value;
-        float x[2][kN];
+        float x[kSplit ? 1 : 2][kN];
         const auto some = [&](int c, float* z, auto begin_next) {
           float big[kN / 2];
+          if constexpr (kSplit) {
+#pragma unroll
+            for (int i = 0; i < kN; i += 2) {
+              const float2 k_scale = *reinterpret_cast<const float2*>(table + c + i), k_mid = *reinterpret_cast<const float2*>(table + kKeys + c + i);
+              const float2 s = fma2(make_float2(z[i], z[i + 1]), k_scale, mul2(k_mid, make_float2(q_sum, q_sum)));
+              z[i] = s.x;
+              z[i + 1] = s.y;
+            }
+          }
 #pragma unroll
           for (int i = 0; i < kN; ++i) {
-            if constexpr (kSplit) {
-              const float2 k = __half22float2(k_par[c + i]);
-              z[i] = fmaf(z[i], k.x, k.y * q_sum);
-            }
             if (!kAll && (c + i < sees0 || c + i > sees1)) z[i] = -INFINITY;  // what is not seen may hold anything
           }
 #pragma unroll
@@ -405,67 +604,50 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             shift = moved ? kLift - M : kLift;
             l *= keep;
             centre *= keep;
-            const __half2 keep2 = __float2half2_rn(keep);
-            for (int at = 0; at < c; at += 16) {
-              float w[16];
-              tmem_ld16_begin(t_s + at, w);
-              tmem_ld16_done(w);
-              uint32_t y[2][8];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w[i]), keep2);
-                y[i / 8][i % 8] = *reinterpret_cast<const uint32_t*>(&h);
-              }
-              tmem_st8(t_s + at, y[0]);
-              if constexpr (kSplit) tmem_st8(t_s + at + 8, y[1]);
-            }
+            scale_columns<true>(t_s, c, keep);
             if constexpr (kSplit) {
 #pragma unroll
               for (int i = 0; i < D; ++i) O[i] *= keep;
             } else if (j > 0) {  // the sums of the tiles before, in tensor memory
               wait(kOFull + wg, j - 1);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              for (int at = 0; at < D; at += 16) {
-                float w[16];
-                tmem_ld16_begin(t_o + at, w);
-                tmem_ld16_done(w);
-                uint32_t y[2][8];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) y[i / 8][i % 8] = __float_as_uint(w[i] * keep);
-                tmem_st8(t_o + at, y[0]);
-                tmem_st8(t_o + at + 8, y[1]);
-              }
+              scale_columns<false>(t_o, D, keep);
             }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           }
           begin_next();
           uint32_t hi[kN / 2], lo[kN / 2];
-          float part[4] = {}, mid[4] = {};
+          if constexpr (kSplit) {
+            float2 part = {}, mid = {};
 #pragma unroll
-          for (int i = 0; i < kN; i += 2) {
-            float w[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              w[k] = ex2(fmaf(z[i + k], factor, shift));
-              part[i / 2 % 4] += w[k];
-              if constexpr (kSplit) {
-                const float2 v = __half22float2(v_par[c + i + k]);
-                const bool sees = kAll || (c + i + k >= sees0 && c + i + k <= sees1);
-                mid[i / 2 % 4] = fmaf(w[k], sees ? fmaf(7.5f, v.x, v.y) : 0.0f, mid[i / 2 % 4]);
-                w[k] *= sees ? v.x : 0.0f;
+            for (int i = 0; i < kN; i += 2) {
+              const float2 e = fma2(make_float2(z[i], z[i + 1]), make_float2(factor, factor), make_float2(shift, shift));
+              const float2 w = make_float2(ex2(e.x), ex2(e.y));
+              float2 v_scale = *reinterpret_cast<const float2*>(table + 2 * kKeys + c + i), v_mid = *reinterpret_cast<const float2*>(table + 3 * kKeys + c + i);
+              if (!kAll) {
+                if (c + i < sees0 || c + i > sees1) v_scale.x = v_mid.x = 0.0f;
+                if (c + i + 1 < sees0 || c + i + 1 > sees1) v_scale.y = v_mid.y = 0.0f;
               }
-            }
-            if constexpr (kSplit) {
+              part = add2(part, w);
+              mid = fma2(w, v_mid, mid);
+              const float2 y = mul2(w, v_scale);
               constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
-              const float h0 = __fsub_rn(__fadd_rn(w[0], kEight), kEight), h1 = __fsub_rn(__fadd_rn(w[1], kEight), kEight);
-              hi[i / 2] = half2_bits(h0, h1);
-              lo[i / 2] = half2_bits(w[0] - h0, w[1] - h1);
-            } else {
-              hi[i / 2] = half2_bits(w[0], w[1]);
+              const float2 h = add2(add2(y, make_float2(kEight, kEight)), make_float2(-kEight, -kEight)), low = fma2(h, make_float2(-1.0f, -1.0f), y);
+              hi[i / 2] = half2_bits(h.x, h.y);
+              lo[i / 2] = half2_bits(low.x, low.y);
             }
+            l += part.x + part.y;
+            centre += mid.x + mid.y;
+          } else {
+            float part[4] = {};
+#pragma unroll
+            for (int i = 0; i < kN; i += 2) {
+              const float w0 = ex2(fmaf(z[i], factor, shift)), w1 = ex2(fmaf(z[i + 1], factor, shift));
+              part[i / 2 % 2 * 2] += w0;
+              part[i / 2 % 2 * 2 + 1] += w1;
+              hi[i / 2] = half2_bits(w0, w1);
+            }
+            l += (part[0] + part[1]) + (part[2] + part[3]);
           }
-          l += (part[0] + part[1]) + (part[2] + part[3]);
-          if constexpr (kSplit) centre += (mid[0] + mid[1]) + (mid[2] + mid[3]);
           // sixteen keys' weights go where their scores were: eight columns, and eight for the low parts
 #pragma unroll
           for (int i = 0; i < kN / 16; ++i) {
@@ -473,15 +655,24 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             if constexpr (kSplit) tmem_st8(t_s + c + i * 16 + 8, lo + i * 8);
           }
         };
-        tmem_ld_begin(t_s, x[0]);
+        if constexpr (kSplit) {  // registers are short: one set of scores
 #pragma unroll 1
-        for (int c = 0; c < kKeys; c += 2 * kN) {
-          tmem_ld_done(x[0]);
-          some(c, x[0], [&] { tmem_ld_begin(t_s + c + kN, x[1]); });
-          tmem_ld_done(x[1]);
-          some(c + kN, x[1], [&] {
-            if (c + 2 * kN < kKeys) tmem_ld_begin(t_s + c + 2 * kN, x[0]);
-          });
+          for (int c = 0; c < kKeys; c += kN) {
+            tmem_ld_begin(t_s + c, x[0]);
+            tmem_ld_done(x[0]);
+            some(c, x[0], [] {});
+          }
+        } else {
+          tmem_ld_begin(t_s, x[0]);
+#pragma unroll 1
+          for (int c = 0; c < kKeys; c += 2 * kN) {
+            tmem_ld_done(x[0]);
+            some(c, x[0], [&] { tmem_ld_begin(t_s + c + kN, x[1]); });
+            tmem_ld_done(x[1]);
+            some(c + kN, x[1], [&] {
+              if (c + 2 * kN < kKeys) tmem_ld_begin(t_s + c + 2 * kN, x[0]);
+            });
+          }
         }
       };
       if (whole) tile(std::true_type());
@@ -507,35 +698,78 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         });
       }
     }
-    const int row = row0 + r, query = row / static_cast<int>(p.group);
-    T* const out = static_cast<T*>(p.a.out) + static_cast<size_t>(span.first + query) * p.a.out_stride +
-                   static_cast<size_t>(head * p.group + static_cast<uint32_t>(row - query * static_cast<int>(p.group))) * D;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = row0 + r;
+    const auto out_of = [&](int row_of) {
+      const int query = row_of / static_cast<int>(p.group);
+      return static_cast<T*>(p.a.out) + static_cast<size_t>(span.first + query) * p.a.out_stride +
+             static_cast<size_t>(head * p.group + static_cast<uint32_t>(row_of - query * static_cast<int>(p.group))) * D;
+    };
+    // read again: what was not needed in the loop takes no registers there
+    const uint32_t n_parts = reinterpret_cast<volatile uint32_t*>(found)[3];
+    const bool shared = n_parts > 1;
+    const float inv = shared ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    float* const part = shared ? p.parts + static_cast<size_t>(blockIdx.x) * F::kPartFloats : nullptr;
+    const auto store = [&](int i, const float* o) {
+      if (shared) store8(part + static_cast<size_t>(r) * D + i, o);
+      else if (row < n_rows) store8(out_of(row) + i, o);
+    };
     if constexpr (kSplit) {
 #pragma unroll
       for (int i = 0; i < D; i += 8) {
         float o[8];
-        // the codes' powers of two: even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
+        // powers of two: the weights' 2^13, the codes' even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = fmaf(O[i + k], (k & 1) ? 1048576.0f : 8388608.0f, centre) * inv;
-        if (row < n_rows) store8(out + i, o);
+        for (int k = 0; k < 8; ++k) o[k] = fmaf(O[i + k], (k & 1) ? 128.0f : 1024.0f, centre) * inv;
+        store(i, o);
       }
     } else if (tiles == 0) {
       const float zero[8] = {};
-      if (row < n_rows)
-        for (int i = 0; i < D; i += 8) store8(out + i, zero);
+      for (int i = 0; i < D; i += 8) store(i, zero);
     } else {
       wait(kOFull + wg, tiles - 1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       tmem_columns<D, false>(t_o, [&](int c, float (&x)[16]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= inv;
-        if (row < n_rows) {
-          store8(out + c, x);
-          store8(out + c + 8, x + 8);
-        }
+        store(c, x);
+        store(c + 8, x + 8);
         __syncwarp();
       });
+    }
+    if (shared) {  // the last CTA of the unit joins the parts, in order
+      reinterpret_cast<float2*>(part + kBlock * D)[r] = make_float2(M, l);
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (tid == 0) {
+        unsigned int arrived;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(arrived) : "l"(p.counters + found[4]) : "memory");
+        if (arrived == n_parts - 1) p.counters[found[4]] = 0;
+        found[5] = arrived;
+      }
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (found[5] == n_parts - 1) {
+        const float* const parts = p.parts + static_cast<size_t>(blockIdx.x - found[2]) * F::kPartFloats;
+        for (int at = static_cast<int>(tid); at < kBlock * D / 8; at += 256) {
+          const int of = at / (D / 8), i = at % (D / 8) * 8;
+          if (row0 + of >= n_rows) break;
+          float m = -INFINITY, total = 0.0f, o[8] = {};
+          for (uint32_t k = 0; k < n_parts; ++k) m = fmaxf(m, __ldcg(parts + static_cast<size_t>(k) * F::kPartFloats + kBlock * D + 2 * of));
+#pragma unroll 4
+          for (uint32_t k = 0; k < n_parts; ++k) {
+            const float* from_part = parts + static_cast<size_t>(k) * F::kPartFloats;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(from_part + kBlock * D) + of);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(from_part + static_cast<size_t>(of) * D + i)), y = __ldcg(reinterpret_cast<const float4*>(from_part + static_cast<size_t>(of) * D + i) + 1);
+            const float keep = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
+            const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            total = fmaf(keep, ml.y, total);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = fmaf(keep, v[e], o[e]);
+          }
+          const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] *= scale;
+          store8(out_of(row0 + of) + i, o);
+        }
+      }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   } else {
@@ -550,8 +784,8 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         const int first = (tile0 + j) * kKeys;
         const uint32_t buf = j % kVBufs, raw = j % kRaws;
         const uint8_t* const codes = smem + F::kRaw + raw * F::kRawBytes;
-        uint32_t* const k_par = reinterpret_cast<uint32_t*>(smem + F::kTable) + (j & 1) * 2 * kKeys;  // (scale, offset) of each key; values:
-        __half* const v_scale = reinterpret_cast<__half*>(k_par + kKeys);                          // f32 pairs too, 16-bit scales, then offsets
+        uint32_t* const k_par = reinterpret_cast<uint32_t*>(smem + F::kTable + (j & 1) * F::kTableBytes);  // (scale, offset) of each key;
+        __half* const v_scale = reinterpret_cast<__half*>(k_par + kKeys);                                  // values' scales, then offsets
         __half* const v_offset = v_scale + kKeys;
         ok = wait(kRawKFull + raw, j / kRaws) && ok;
         if (kVBufs == 2 && j >= 2) wait(kVEmpty + buf, j / 2 - 1);  // what the softmax warps read of tile j - 2 has been read
@@ -561,8 +795,11 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
           uint32_t kp = seen ? raw_params[t] : 0u, vp = seen ? raw_params[kKeys + t] : 0u;
           const float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kp)), v = __half22float2(*reinterpret_cast<const __half2*>(&vp));
           if constexpr (kSplit) {
-            k_par[t] = kp;
-            k_par[kKeys + t] = vp;
+            float* const table = reinterpret_cast<float*>(k_par) + t;
+            table[0] = k.x;
+            table[kKeys] = fmaf(7.5f, k.x, k.y);
+            table[2 * kKeys] = v.x * 8192.0f;
+            table[3 * kKeys] = fmaf(7.5f, v.x, v.y);
             const uint32_t big = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v.x, 0.0f)));  // not NaN
             if (lane == 0) reinterpret_cast<float*>(smem + F::kBinade)[(j & 1) * 4 + w4] = binade_of(__uint_as_float(big));
           } else {
@@ -599,7 +836,8 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
               const uint32_t word = q * 4 + (w ^ swap), x8 = x[w] >> 8;
               uint4 out;
               if constexpr (kSplit) {
-                out = make_uint4(x[w] & 0x000F000Fu, x[w] & 0x00F000F0u, x8 & 0x000F000Fu, x8 & 0x00F000F0u);
+                out = make_uint4(hfma2_bits(x[w] & 0x000F000Fu, 0x40004000u, kCentre0), hadd2_bits(x[w] & 0x00F000F0u, kCentre1),
+                                 hfma2_bits(x8 & 0x000F000Fu, 0x40004000u, kCentre0), hadd2_bits(x8 & 0x00F000F0u, kCentre1));
               } else {
                 out.x = hfma2_bits(hadd2_bits((x[w] & 0x000F000Fu) | kExp, k1024), s2, o2);
                 out.y = hfma2_bits(hfma2_bits((x[w] & 0x00F000F0u) | kExp, k16th, k64), s2, o2);
@@ -790,7 +1028,18 @@ cudaError_t many_as(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond) 
   const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * p.group;
   const uint64_t blocks = rows / kBlock + std::min<uint64_t>(a.batch.sequences, rows / (beyond + 1));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.cache.kv_heads));
+  const uint64_t units = blocks * a.cache.kv_heads;
+  // Few units: their keys are shared, so that every SM has its part (a part more for each unit's odd end).
+  p.parts = nullptr;
+  p.counters = env.counters;
+  p.ctas = static_cast<uint32_t>(env.sm_count);
+  uint64_t grid = units;
+  if (units < 2ull * p.ctas && units <= F::kUnits && units <= env.counter_count && env.workspace &&
+      (units + p.ctas) * F::kPartFloats * sizeof(float) <= env.workspace_bytes) {
+    p.parts = static_cast<float*>(env.workspace);
+    grid = units + p.ctas;
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(F::kThreads);
   cfg.dynamicSmemBytes = F::kSmem;
   cfg.stream = env.stream;

@@ -111,28 +111,9 @@ __device__ __forceinline__ void load8_rotated(const T* row, uint32_t at, const R
   }
 }
 
-// The same in straight-line code, for callers with several rows on their way: half layout, rotary a multiple of 16, the
-// table 16-byte aligned (rope_is_plain), a position that may lie outside it.
+// Half layout with angles that can be read sixteen bytes at a time.
 __host__ __device__ __forceinline__ bool rope_is_plain(const RopeTable& rope) {
-  return rope.table && !rope.interleaved && rope.rotary % 16 == 0 && (reinterpret_cast<uintptr_t>(rope.table) & 15u) == 0 && rope.positions > 0;
-}
-template <typename T>
-__device__ __forceinline__ void load8_rotated_plain(const T* row, uint32_t at, const RopeTable& rope, int position, float (&v)[8]) {
-  const uint32_t half = rope.rotary / 2;
-  const bool turns = at < rope.rotary, first = at < half, inside = position >= 0 && static_cast<uint32_t>(position) < rope.positions;
-  float other[8];
-  float4 cs[4];
-  load8(row + at, v);
-  load8(row + (!turns ? at : first ? at + half : at - half), other);
-  const float4* angles = reinterpret_cast<const float4*>(rope.table + static_cast<size_t>(inside ? position : 0) * half + (!turns ? 0 : first ? at : at - half));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) cs[i] = angles[i];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 a = i & 1 ? make_float2(cs[i / 2].z, cs[i / 2].w) : make_float2(cs[i / 2].x, cs[i / 2].y);
-    const float2 y = rotate_pair(first ? v[i] : other[i], first ? other[i] : v[i], a);
-    if (turns) v[i] = inside ? (first ? y.x : y.y) : quiet_nan();
-  }
+  return rope.table && !rope.interleaved && rope.rotary % 4 == 0 && (reinterpret_cast<uintptr_t>(rope.table) & 15u) == 0 && rope.positions > 0;
 }
 
 }  // namespace kq
