@@ -12,8 +12,17 @@ from tests.test_gpu_cache import dev, make_batch
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(scope="module", autouse=True)
+def one_stream():
+    """torch and the library on one stream: what torch makes is there when a kernel reads it."""
+    before = torch.cuda.current_stream()
+    torch.cuda.set_stream(torch.cuda.Stream())
+    yield
+    torch.cuda.set_stream(before)
+
+
 @pytest.fixture(scope="module")
-def gpu():
+def gpu(one_stream):
     import karume_b200 as kb
     g = kb.acquire_gpu(0)
     yield g
@@ -236,4 +245,70 @@ def test_a_recorded_step_follows_the_lengths(gpu):
     gpu.use_stream(torch.cuda.current_stream())
     assert all(torch.equal(a, b) for a, b in replayed) and lengths.tolist() == [40, 20]
     assert all(bool(torch.isfinite(a).all()) for a, _ in replayed)
+    cache.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_many_sequences(gpu, kind):
+    """More sequences than a block has threads, a few of them prompts, some idle; `most` says too little and is still only a hint."""
+    rng = np.random.default_rng(2)
+    lengths = rng.integers(0, 40, 700).tolist()
+    lengths[5], lengths[300], lengths[699] = 500, 130, 77
+    f = Filled(gpu, lengths, 16, 1, 64, seed=8)
+    f.check(kind, [1] * 700, 2)
+    news = [0 if i % 7 == 3 else min(1, n) for i, n in enumerate(lengths)]
+    news[5], news[300], news[699] = 400, 130, 20
+    f.check(kind, news, 2, rotary=64, most=400)
+    f.check(kind, news, 2, most=2)
+    f.check(kind, news, 2, padding=2)
+    f.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_little_scratch(kind):
+    """Too little for parts: fewer CTAs share a run, or none."""
+    import karume_b200 as kb
+    for scratch in (1 << 12, 1 << 18):
+        g = kb.acquire_gpu(0, workspace_bytes=scratch)
+        f = Filled(g, [3000, 100], 64, 1, 128, seed=4)
+        f.check(kind, [1, 1], 4)
+        f.check(kind, [90, 3], 4, rotary=128)
+        f.free()
+        g.destroy()
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """Pages more than 4 GiB into the pool, and an output whose rows are far apart."""
+    import karume_b200 as kb
+    page, dim, heads = 256, 128, 2
+    block = page * (dim + 8)
+    count = (5 << 30) // (block * heads)
+    pool = torch.zeros(count, heads, block, dtype=torch.uint8, device="cuda")
+    cache = gpu.kv_cache(count, page, heads, dim, pool=pool)
+    pages = torch.tensor([[count - 1, 0, count - 2]], dtype=torch.int32, device="cuda")
+    n = 700
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(n, heads, dim, generator=gen, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    lengths, starts = dev(np.array([n], np.int32)), dev(np.array([0, n], np.int32))
+    whole = kb.CacheBatch(pages, lengths, starts, tokens=n)
+    gpu.cache_append(cache, k, v, whole)
+    k, v = gpu.cache_read(cache, whole)
+    for kind, new in (("f32", 1), ("bf16", 1), ("f32", 100), ("bf16", 100)):
+        q = torch.randn(new, 4, dim, generator=gen, device="cuda").to(ref.TYPES[kind])
+        stride = (3 << 30) // q.element_size() if new == 1 else 4 * dim
+        torch.cuda.synchronize()
+        got = gpu.cache_attention(cache, q, kb.CacheBatch(pages, lengths, dev(np.array([0, new], np.int32)), tokens=new))
+        gpu.sync()
+        want, reach, largest = ref.attend(q.double(), k.double(), v.double(), dim ** -0.5, 0)
+        assert bool(((got.double() - want).abs() <= ref.allowed(kind, want, reach, largest)).all()), (kind, new, stride)
+    wide = torch.zeros(3, 1 << 31, dtype=torch.int8, device="cuda").view(torch.float16)  # rows 2 GiB apart
+    q = torch.randn(3, 4, dim, generator=gen, device="cuda").half()
+    out = wide[:, :4 * dim].unflatten(1, (4, dim))
+    torch.cuda.synchronize()
+    batch = kb.CacheBatch(pages, lengths, dev(np.array([0, 3], np.int32)), tokens=3)
+    gpu.cache_attention(cache, q, batch, out=out)
+    near = gpu.cache_attention(cache, q, batch)
+    gpu.sync()
+    assert torch.equal(out, near)
     cache.free()

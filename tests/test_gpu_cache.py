@@ -9,8 +9,17 @@ from tests import cache_reference as ref
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(scope="module", autouse=True)
+def one_stream():
+    """torch and the library on one stream: what torch makes is there when a kernel reads it."""
+    before = torch.cuda.current_stream()
+    torch.cuda.set_stream(torch.cuda.Stream())
+    yield
+    torch.cuda.set_stream(before)
+
+
 @pytest.fixture(scope="module")
-def gpu():
+def gpu(one_stream):
     import karume_b200 as kb
     g = kb.acquire_gpu(0)
     yield g
