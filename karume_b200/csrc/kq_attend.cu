@@ -382,14 +382,24 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
     const Keys keys = at.keys;
 
     // queries: rotated, scaled to binary16's range by a power of two, in the order of the B fragments
-    for (int r = static_cast<int>(warp); r < kRows; r += kWarps) {
-      const int row = static_cast<int>(at.block) * kRows + r, query = row / static_cast<int>(p.group);
+    // (all of a warp's rows asked for before the first is worked on)
+    float loaded[kRows / kWarps][8];
+#pragma unroll
+    for (int i = 0; i < kRows / kWarps; ++i) {
+      const int row = static_cast<int>(at.block) * kRows + static_cast<int>(warp) + i * kWarps, query = row / static_cast<int>(p.group);
       const int head = static_cast<int>(at.head * p.group) + row - query * static_cast<int>(p.group);
-      const bool there = row < q_rows;
-      float v[8] = {};
-      if (there && lane < D / 8)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) loaded[i][e] = 0.0f;
+      if (row < q_rows && lane < D / 8)
         load8_rotated(static_cast<const T*>(p.a.q) + static_cast<size_t>(at.runs.span.first + query) * p.a.q_stride + static_cast<size_t>(head) * D,
-                      lane * 8, p.a.rope, base + query, v);
+                      lane * 8, p.a.rope, base + query, loaded[i]);
+    }
+#pragma unroll
+    for (int i_row = 0; i_row < kRows / kWarps; ++i_row) {
+      const int r = static_cast<int>(warp) + i_row * kWarps;
+      const int query = (static_cast<int>(at.block) * kRows + r) / static_cast<int>(p.group);
+      const bool there = static_cast<int>(at.block) * kRows + r < q_rows;
+      const float (&v)[8] = loaded[i_row];
       float big = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {

@@ -72,22 +72,16 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
   const uint32_t half = p.rope.rotary / 2, turning = p.rope.interleaved && V > 1 ? p.rope.rotary / V : half / V;
   const T* x = static_cast<const T*>(p.x) + token * p.x_stride;
   T* out = static_cast<T*>(p.out) + token * p.out_stride;
-  if (unit >= turning) {  // behind the rotated part
-    const uint32_t at = p.rope.rotary + (unit - turning) * V;
-    if (x != out) {
-#pragma unroll 4
-      for (uint32_t h = group; h < p.heads; h += p.head_groups)
-        *reinterpret_cast<R*>(out + static_cast<size_t>(h) * p.dim + at) = *reinterpret_cast<const R*>(x + static_cast<size_t>(h) * p.dim + at);
-    }
-    return;
-  }
+  // What is behind the rotated part takes the same way and keeps its values: on a way of its own its lanes would wait for the
+  // others of their warp (half of each head rotated: 45 us instead of 33).
+  const bool turns = unit < turning;
   const int position = p.positions[token];
   const bool inside = position >= 0 && static_cast<uint32_t>(position) < p.rope.positions;
   const float2* row = p.rope.table + static_cast<size_t>(inside ? position : 0) * half;
   if constexpr (V > 1) {
     if (p.rope.interleaved) {
       float2 cs[V / 2];
-      load_angles(row + unit * (V / 2), inside, p.wide, cs);
+      load_angles(row + (turns ? unit * (V / 2) : 0), inside, p.wide, cs);
 #pragma unroll 4
       for (uint32_t h = group; h < p.heads; h += p.head_groups) {
         const size_t at = static_cast<size_t>(h) * p.dim + unit * V;
@@ -95,8 +89,8 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
           const float2 y = rotate_pair(to_f32(r.v[i]), to_f32(r.v[i + 1]), cs[i / 2]);
-          r.v[i] = from_f32<T>(y.x);
-          r.v[i + 1] = from_f32<T>(y.y);
+          r.v[i] = turns ? from_f32<T>(y.x) : r.v[i];
+          r.v[i + 1] = turns ? from_f32<T>(y.y) : r.v[i + 1];
         }
         *reinterpret_cast<R*>(out + at) = r;
       }
@@ -104,21 +98,23 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeParams p) {
     }
   }
   // runs of V values and what they are paired with: rotary / 2 further on, or (interleaved, one value at a time) the next one
-  const uint32_t step = p.rope.interleaved ? 2 : V, pair = p.rope.interleaved ? 1 : half;
+  const uint32_t pair = p.rope.interleaved ? 1 : half;
+  const uint32_t first = !turns ? p.rope.rotary + (unit - turning) * V : unit * (p.rope.interleaved ? 2 : V);
   float2 cs[V];
-  load_angles(row + unit * V, inside, p.wide, cs);
+  load_angles(row + (turns ? unit * V : 0), inside, p.wide, cs);
 #pragma unroll 4
   for (uint32_t h = group; h < p.heads; h += p.head_groups) {
-    const size_t at = static_cast<size_t>(h) * p.dim + unit * step;
-    R a = *reinterpret_cast<const R*>(x + at), b = *reinterpret_cast<const R*>(x + at + pair);
+    const size_t at = static_cast<size_t>(h) * p.dim + first;
+    R a = *reinterpret_cast<const R*>(x + at), b = a;
+    if (turns) b = *reinterpret_cast<const R*>(x + at + pair);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float2 y = rotate_pair(to_f32(a.v[i]), to_f32(b.v[i]), cs[i]);
-      a.v[i] = from_f32<T>(y.x);
+      a.v[i] = turns ? from_f32<T>(y.x) : a.v[i];
       b.v[i] = from_f32<T>(y.y);
     }
     *reinterpret_cast<R*>(out + at) = a;
-    *reinterpret_cast<R*>(out + at + pair) = b;
+    if (turns) *reinterpret_cast<R*>(out + at + pair) = b;
   }
 }
 
