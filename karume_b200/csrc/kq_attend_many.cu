@@ -3,14 +3,16 @@
 //
 //   out = sum_j softmax_j(scale q . k_j) v_j,   k_j = u_j s_j + o_j, v_j likewise, codes u in 0..15
 //
-// A CTA takes 256 query rows (query and head of one kv head's group, packed: all heads of the group share what is unpacked)
-// and walks over the keys they see in tiles of 128.  Warps:
-//   0-3, 4-7   one row each thread of the first / second 128 rows: scores from tensor memory, weights back into it; f32 queries:
-//              the sums of the output in registers (what the tensor core adds is one tile's, so that a long row does not drift)
-//   four (f32) or six     unpack a tile: keys as [token][dim], values transposed as [dim][token], both K-major, 128-byte swizzle
-//   one        issues the MMAs:   S_r = Q_r K^T (both in shared memory),   O_r += P_r V (P in tensor memory, over S)
-//   one        copies the codes and scales of the next tile (bulk copies, page by page)
-// The two row blocks take turns: while one's weights are being computed the tensor core works for the other.
+// A CTA takes 256 (f32: 128) query rows, (query, head of one kv head's group) packed: all heads of the group share what is
+// unpacked.  It walks over the keys they see in tiles of 128.  Warps:
+//   0-7    softmax: scores from tensor memory, weights back into it (over the scores)
+//   8-13   unpack a tile: keys as [token][dim], values transposed as [dim][token], both K-major, 128-byte swizzle
+//   14     issues the MMAs:   S = Q K^T (both in shared memory),   O = P V (P in tensor memory)
+//   15     copies the codes and scales of the next tiles (bulk copies, page by page)
+// 16-bit: two blocks of 128 rows, a thread a row; while one block's weights are computed the tensor core works for the other;
+// O is added up in tensor memory.  f32: one block, two threads a row (half of the keys each, then half of the dims); the
+// next tile's scores are made meanwhile; O is one tile's, added in registers, so that a long row does not drift.
+// Few blocks of rows: the tiles of keys of each are shared by several CTAs, and the last one joins their sums in order.
 //
 //   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights).
 //   f32 queries     codes enter exactly, around zero: (2 u - 15) 2^-24 and (u - 7.5) 2^-20, one operation from the subnormals that
@@ -26,29 +28,28 @@ namespace kq {
 namespace {
 
 constexpr int kKeys = 128;    // of a tile
-constexpr int kBlock = 256;   // query rows of a CTA
 constexpr int kManyTimeout = 50;
 
-enum Bar { kRawKFull, kRawKFree = 2, kRawVFull = 4, kRawVFree = 6, kKFull = 8, kKEmpty, kVFull, kVEmpty = 12, kSFull = 14, kPReady = 16, kOFull = 18, kBarCount = 20 };
+enum Bar { kRawKFull, kRawKFree = 2, kRawVFull = 4, kRawVFree = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kSFull = 16, kPReady = 18, kOFull = 20, kBarCount = 22 };
 
 template <typename T, int D>
 struct Many {
   static constexpr bool kSplit = sizeof(T) == 4;
   static constexpr int kParts = kSplit ? 2 : 1;
-  // 8 softmax warps, the unpacking ones, MMA, copies.  f32 keeps the output's sums in the softmax warps' registers (192 a thread,
-  // taken from the others, which makes whole groups of four warps); 16-bit ones stay in tensor memory.
-  static constexpr int kUnpackWarps = kSplit ? 4 : 6, kUnpack = kUnpackWarps * 32;
+  // Query rows of a CTA.  16-bit: two blocks of 128, a softmax thread a row, the blocks taking turns; f32: one block, two threads a
+  // row (half of the keys, then of the dims each: scores and sums stay in registers), the tiles of keys taking turns.
+  static constexpr int kBlock = kSplit ? 128 : 256;
+  static constexpr int kUnpackWarps = 6, kUnpack = kUnpackWarps * 32;
   static constexpr int kMmaWarp = 8 + kUnpackWarps, kCopyWarp = kMmaWarp + 1;
-  static constexpr int kThreads = 512;
-  static constexpr int kAtOnce = kSplit ? 16 : 32;         // scores a softmax thread has in hand
+  static constexpr int kThreads = (kCopyWarp + 1) * 32;
+  static constexpr int kAtOnce = 32;                       // 16-bit: scores a softmax thread has in hand
   static constexpr int kOperand = 128 * D * 2;             // bytes of 128 rows (or tokens) of D values
-  static constexpr bool kFull = kSplit && D == 128;        // the queries leave room for one of everything
-  static constexpr int kVBufs = kFull ? 1 : 2;             // unpacked values; one tile of unpacked keys (needed only while scores are made)
-  static constexpr int kRaws = kFull ? 1 : 2;              // tiles of codes on their way
+  // Unpacked tiles (16-bit: keys are needed only while scores are made) and tiles of codes on their way, as many as fit
+  static constexpr int kKBufs = kSplit ? 2 : 1, kVBufs = 2, kRaws = kSplit && D == 128 ? 1 : 2;
   static constexpr int kGroup = 4 * D + 16;                // raw values of eight tokens, 16 bytes apart: lanes of eight groups meet no bank twice
   static constexpr int kQ = 0;
-  static constexpr int kK = kQ + 2 * kParts * kOperand;
-  static constexpr int kV = kK + kOperand;
+  static constexpr int kK = kQ + 2 * kOperand;              // two blocks, or the two parts of one
+  static constexpr int kV = kK + kKBufs * kOperand;
   static constexpr int kRaw = kV + kVBufs * kOperand;
   static constexpr int kRawV = kKeys * (D / 2);            // in a tile of codes: keys, values,
   static constexpr int kRawParams = kRawV + 16 * kGroup;   // keys' and values' (scale, offset)
@@ -56,10 +57,11 @@ struct Many {
   // [2] x 16-bit: [2][128] (scale, offset) of keys and values; f32: [4][128] scale and centre of keys, then of values (2^13 scale)
   static constexpr int kTable = kRaw + kRaws * kRawBytes;
   static constexpr int kTableBytes = (kSplit ? 4 : 2) * kKeys * 4;
-  static constexpr int kRows = kTable + 2 * kTableBytes;   // [256] (factor, sum, last key, first key)
+  static constexpr int kRows = kTable + 2 * kTableBytes;   // [kBlock] (factor, sum, last key, first key)
   static constexpr int kLost = kRows + kBlock * 16;        // [2] 128 bits: tokens whose value is NaN
-  static constexpr int kBinade = kLost + 32;               // [2][4]: largest binade of the values' scales, by warp
-  static constexpr int kBars = kBinade + 32;
+  static constexpr int kBinade = kLost + 32;               // [2][4]: f32: the largest of 32 values' scales (2^13 scale)
+  static constexpr int kHalves = kBinade + 32;             // f32: [2][2][128] (largest score, largest scale) of each half of a row's keys
+  static constexpr int kBars = kHalves + (kSplit ? 2 * 2 * 128 * 8 : 0);
   static constexpr int kMisc = kBars + kBarCount * 8;
   static constexpr int kPartFloats = kBlock * (D + 2);
   static constexpr int kUnits = 512;                       // more than these are not shared by CTAs
@@ -246,7 +248,7 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const fl
 template <typename T, int D>
 __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(const __grid_constant__ ManyParams p) {
   using F = Many<T, D>;
-  constexpr int kParts = F::kParts, kVBufs = F::kVBufs, kRaws = F::kRaws;
+  constexpr int kParts = F::kParts, kBlock = F::kBlock, kKBufs = F::kKBufs, kVBufs = F::kVBufs, kRaws = F::kRaws;
   constexpr bool kSplit = F::kSplit;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + (1024 - (static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw)) & 1023u)) % 1024;
@@ -264,9 +266,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   };
 
   if (tid == 0) {
-    umma::mbar_init(bar(kKFull), F::kUnpack);
-    umma::mbar_init(bar(kKEmpty), 1);
     for (int i = 0; i < 2; ++i) {
+      umma::mbar_init(bar(kKFull + i), F::kUnpack);
+      umma::mbar_init(bar(kKEmpty + i), 1);
       umma::mbar_init(bar(kRawKFull + i), 1);
       umma::mbar_init(bar(kRawVFull + i), 1);
       umma::mbar_init(bar(kRawKFree + i), F::kUnpack);
@@ -275,7 +277,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       umma::mbar_init(bar(kVEmpty + i), 1);
       umma::mbar_init(bar(kSFull + i), 1);
       umma::mbar_init(bar(kOFull + i), 1);
-      umma::mbar_init(bar(kPReady + i), 128);
+      umma::mbar_init(bar(kPReady + i), kSplit ? 256 : 128);
     }
     *abort_flag = 0;
     found[0] = 0xFFFFFFFFu;
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   if (rope_is_plain(p.a.rope) && p.a.rope.rotary == D) {
     // Half layout, whole heads: a lane has two pairs of a row, so that the angles are read coalesced (runs of eight dims a lane read them
     // at a stride of 64 bytes, 9000 clocks a CTA); words of dims (d, d + 4) are put together with the lane two further on.
-    constexpr uint32_t kLanes = D / 4, kRowsAtOnce = 32 / kLanes, kStep = F::kThreads / 32 * kRowsAtOnce, kBatch = 8;
+    constexpr uint32_t kLanes = D / 4, kRowsAtOnce = 32 / kLanes, kStep = F::kThreads / 32 * kRowsAtOnce, kBatch = kBlock / kStep < 8 ? kBlock / kStep : 8;
     static_assert(kBlock % (kStep * kBatch) == 0, "whole batches");
     const uint32_t c = lane % kLanes;
     const uint32_t word = (c & 1) * 2 + (c >> 1 & 1);  // of its eight dims' chunk: dims (0, 4), (1, 5), (2, 6), (3, 7) from lanes 0, 2, 1, 3
@@ -531,138 +533,186 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
 
   if (warp < 8) {
     // ---- softmax and output: a row a thread --------------------------------------------------------
-    if constexpr (kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if constexpr (kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t wg = warp / 4, lanes = (warp % 4 * 32) << 16;
-    const uint32_t t_s = tmem + lanes + wg * 128, t_o = tmem + lanes + 256 + wg * 128;
-    const int r = static_cast<int>(tid);
+    const int r = static_cast<int>(kSplit ? tid % 128 : tid);
     const float4 rc = rows[r];
     const float factor = rc.x, q_sum = rc.y;
     const int last = __float_as_int(rc.z), from = __float_as_int(rc.w);
     const int last_all = __reduce_min_sync(0xffffffffu, last), from_all = __reduce_max_sync(0xffffffffu, from);
-    float O[kSplit ? D : 1];
-    if constexpr (kSplit) {
-#pragma unroll
-      for (int i = 0; i < D; ++i) O[i] = 0.0f;
-    }
-    // Weights are 2^(score - M + kLift).  M is a whole number (what it moves by is an exact power of two) that follows the row's
-    // largest score, f32: and the binade of the values' scales beside it; it moves when a weight (times its value's scale) would
-    // pass 2^14.  So that this is seen before anything is written, a few scores are looked at at a time; what was written
-    // of the tile before is then scaled too.  f32 lets M lag by one bit, to keep the fixed-point parts' 22; 16-bit by eight.
-    constexpr int kN = F::kAtOnce;
-    constexpr float kLift = kSplit ? 0.0f : 6.0f, kLag = kSplit ? 1.0f : 8.0f;  // f32: the values' scales carry 2^13
+    // Weights are 2^(score - M + lift).  M is a whole number (what it moves by is an exact power of two) that follows the row's
+    // largest score, f32: and the binade of the values' scales beside it; it moves when a weight (times its value's scale)
+    // would pass 2^14.  f32 lets M lag by one bit, to keep the fixed-point parts' 22; 16-bit by eight.
     float M = -INFINITY, l = 0.0f, centre = 0.0f;
-    for (int j = 0; j < tiles; ++j) {
-      const int first = (tile0 + j) * kKeys;
-      const bool whole = first >= from_all && first + kKeys - 1 <= last_all;
-      const int sees0 = from - first, sees1 = last - first;  // columns the row sees
-      const float* table = reinterpret_cast<const float*>(smem + F::kTable + (j & 1) * F::kTableBytes);
-      wait(kSFull + wg, j);
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float binade = 0.0f;
-      if constexpr (kSplit) {
-        const float* bn = reinterpret_cast<const float*>(smem + F::kBinade) + (j & 1) * 4;
-        binade = fmaxf(fmaxf(bn[0], bn[1]), fmaxf(bn[2], bn[3]));
-        if (!whole) {  // ... of what this row sees
-          float big = 0.0f;
-          for (int i = 0; i < kKeys; ++i)
-            if (i >= sees0 && i <= sees1) big = fmaxf(big, table[2 * kKeys + i]);
-          binade = binade_of(big * (1.0f / 8192.0f));
+    float O[kSplit ? D / 2 : 1];
+    if constexpr (kSplit) {
+      // ---- f32: this thread's keys and dims are half wg of the tile's and of the head's -----------------------------
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) O[i] = 0.0f;
+      float2* const halves = reinterpret_cast<float2*>(smem + F::kHalves);
+      float keep_sums = 1.0f;  // what the tile before is still to be scaled by
+      const auto drain = [&](int j, float keep) {
+        wait(kOFull + (j & 1), j / 2);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_columns<D / 2, true>(tmem + lanes + 256 + (j & 1) * 128 + wg * (D / 2), [&](int c, float (&x)[16]) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) O[c + i] = fmaf(x[i], keep, O[c + i]);
+        });
+      };
+      for (int j = 0; j < tiles; ++j) {
+        const int first = (tile0 + j) * kKeys + static_cast<int>(wg) * 64;
+        const bool whole = first >= from_all && first + 63 <= last_all;
+        const int sees0 = from - first, sees1 = last - first;  // of the thread's 64 columns those that the row sees
+        const float* table = reinterpret_cast<const float*>(smem + F::kTable + (j & 1) * F::kTableBytes) + wg * 64;
+        const uint32_t t_s = tmem + lanes + (j & 1) * 128 + wg * 64;
+        wait(kSFull + (j & 1), j / 2);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float z[64];
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) tmem_ld_begin(t_s + c, reinterpret_cast<float (&)[32]>(z[c]));
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) tmem_ld_done(reinterpret_cast<float (&)[32]>(z[c]));
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          const float2 k_scale = *reinterpret_cast<const float2*>(table + i), k_mid = *reinterpret_cast<const float2*>(table + kKeys + i);
+          const float2 s = fma2(make_float2(z[i], z[i + 1]), k_scale, mul2(k_mid, make_float2(q_sum, q_sum)));
+          z[i] = s.x;
+          z[i + 1] = s.y;
         }
+        float scale_seen = 0.0f;
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            if (i < sees0 || i > sees1) z[i] = -INFINITY;  // what is not seen may hold anything
+            else scale_seen = fmaxf(scale_seen, table[2 * kKeys + i]);
+          }
+        } else {
+          const float* bn = reinterpret_cast<const float*>(smem + F::kBinade) + (j & 1) * 4 + wg * 2;  // warps 2 wg, 2 wg + 1 made these keys' scales
+          scale_seen = fmaxf(bn[0], bn[1]);
+        }
+        float big[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) big[i] = fmaxf(fmaxf(z[i], z[i + 16]), fmaxf(z[i + 32], z[i + 48]));
+#pragma unroll
+        for (int o = 8; o > 0; o /= 2)
+#pragma unroll
+          for (int i = 0; i < o; ++i) big[i] = fmaxf(big[i], big[i + o]);
+        // the row's other half
+        halves[((j & 1) * 2 + wg) * 128 + r] = make_float2(big[0], scale_seen);
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        const float2 other = halves[((j & 1) * 2 + (wg ^ 1)) * 128 + r];
+        const float binade = binade_of(fmaxf(scale_seen, other.y) * (1.0f / 8192.0f));
+        const float top = fmaxf(big[0], other.x) * factor + binade;
+        const bool more = top > M + 1.0f;
+        keep_sums = 1.0f;
+        if (__any_sync(0xffffffffu, more)) {
+          const float now = more ? ceilf(top) : M;
+          keep_sums = M == -INFINITY ? 0.0f : exp2f(M - now);
+          M = now;
+          l *= keep_sums;
+          centre *= keep_sums;
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i) O[i] *= keep_sums;
+        }
+        const float shift = M == -INFINITY ? 0.0f : -M;  // the values' scales carry 2^13
+        float2 part = {}, mid = {};
+#pragma unroll
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float2 e = fma2(make_float2(z[c + i], z[c + i + 1]), make_float2(factor, factor), make_float2(shift, shift));
+            const float2 w = make_float2(ex2(e.x), ex2(e.y));
+            float2 v_scale = *reinterpret_cast<const float2*>(table + 2 * kKeys + c + i), v_mid = *reinterpret_cast<const float2*>(table + 3 * kKeys + c + i);
+            if (!whole) {
+              if (c + i < sees0 || c + i > sees1) v_scale.x = v_mid.x = 0.0f;
+              if (c + i + 1 < sees0 || c + i + 1 > sees1) v_scale.y = v_mid.y = 0.0f;
+            }
+            part = add2(part, w);
+            mid = fma2(w, v_mid, mid);
+            const float2 y = mul2(w, v_scale);
+            constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
+            const float2 h = add2(add2(y, make_float2(kEight, kEight)), make_float2(-kEight, -kEight)), low = fma2(h, make_float2(-1.0f, -1.0f), y);
+            hi[i / 2] = half2_bits(h.x, h.y);
+            lo[i / 2] = half2_bits(low.x, low.y);
+          }
+          // sixteen keys' weights go where their scores were: eight columns, and eight for the low parts
+          tmem_st8(t_s + c, hi);
+          tmem_st8(t_s + c + 8, lo);
+        }
+        l += part.x + part.y;
+        centre += mid.x + mid.y;
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        umma::mbar_arrive(bar(kPReady + (j & 1)));
+        if (j > 0) drain(j - 1, keep_sums);
       }
-      float limit = M + kLag - binade, shift = M == -INFINITY ? kLift : kLift - M;
-      const auto tile = [&](auto all_seen) {
-        constexpr bool kAll = decltype(all_seen)::value;
-        float x[kSplit ? 1 : 2][kN];
-        const auto some = [&](int c, float* z, auto begin_next) {
-          float big[kN / 2];
-          if constexpr (kSplit) {
+      if (tiles > 0) drain(tiles - 1, 1.0f);
+      // both halves' weights
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      halves[wg * 128 + r] = make_float2(l, centre);
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      const float2 first_half = halves[r], second_half = halves[128 + r];
+      l = first_half.x + second_half.x;
+      centre = first_half.y + second_half.y;
+    } else {
+      // ---- 16-bit: row r, all keys; the sums stay in tensor memory ------------------------------------------------
+      // So that M's move is seen before anything is written, a few scores are looked at at a time; what was written of the tile before
+      // is then scaled too.
+      constexpr int kN = F::kAtOnce;
+      constexpr float kLift = 6.0f, kLag = 8.0f;
+      const uint32_t t_s = tmem + lanes + wg * 128, t_o = tmem + lanes + 256 + wg * 128;
+      for (int j = 0; j < tiles; ++j) {
+        const int first = (tile0 + j) * kKeys;
+        const bool whole = first >= from_all && first + kKeys - 1 <= last_all;
+        const int sees0 = from - first, sees1 = last - first;  // columns the row sees
+        wait(kSFull + wg, j);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float limit = M + kLag, shift = M == -INFINITY ? kLift : kLift - M;
+        const auto tile = [&](auto all_seen) {
+          constexpr bool kAll = decltype(all_seen)::value;
+          float x[2][kN];
+          const auto some = [&](int c, float* z, auto begin_next) {
+            float big[kN / 2];
 #pragma unroll
-            for (int i = 0; i < kN; i += 2) {
-              const float2 k_scale = *reinterpret_cast<const float2*>(table + c + i), k_mid = *reinterpret_cast<const float2*>(table + kKeys + c + i);
-              const float2 s = fma2(make_float2(z[i], z[i + 1]), k_scale, mul2(k_mid, make_float2(q_sum, q_sum)));
-              z[i] = s.x;
-              z[i + 1] = s.y;
-            }
-          }
+            for (int i = 0; i < kN; ++i)
+              if (!kAll && (c + i < sees0 || c + i > sees1)) z[i] = -INFINITY;  // what is not seen may hold anything
 #pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            if (!kAll && (c + i < sees0 || c + i > sees1)) z[i] = -INFINITY;  // what is not seen may hold anything
-          }
+            for (int i = 0; i < kN / 2; ++i) big[i] = fmaxf(z[i], z[i + kN / 2]);
 #pragma unroll
-          for (int i = 0; i < kN / 2; ++i) big[i] = fmaxf(z[i], z[i + kN / 2]);
+            for (int o = kN / 4; o > 0; o /= 2)
 #pragma unroll
-          for (int o = kN / 4; o > 0; o /= 2)
-#pragma unroll
-            for (int i = 0; i < o; ++i) big[i] = fmaxf(big[i], big[i + o]);
-          const float top = big[0] * factor;
-          if (__any_sync(0xffffffffu, top > limit)) {
-            const float now = top > limit ? ceilf(top + binade) : M;
-            const float keep = M == -INFINITY ? 0.0f : exp2f(M - now);
-            if (now != -INFINITY) M = now;
-            const bool moved = M != -INFINITY;
-            limit = M + kLag - binade;
-            shift = moved ? kLift - M : kLift;
-            l *= keep;
-            centre *= keep;
-            scale_columns<true>(t_s, c, keep);
-            if constexpr (kSplit) {
-#pragma unroll
-              for (int i = 0; i < D; ++i) O[i] *= keep;
-            } else if (j > 0) {  // the sums of the tiles before, in tensor memory
-              wait(kOFull + wg, j - 1);
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              scale_columns<false>(t_o, D, keep);
-            }
-          }
-          begin_next();
-          uint32_t hi[kN / 2], lo[kN / 2];
-          if constexpr (kSplit) {
-            float2 part = {}, mid = {};
-#pragma unroll
-            for (int i = 0; i < kN; i += 2) {
-              const float2 e = fma2(make_float2(z[i], z[i + 1]), make_float2(factor, factor), make_float2(shift, shift));
-              const float2 w = make_float2(ex2(e.x), ex2(e.y));
-              float2 v_scale = *reinterpret_cast<const float2*>(table + 2 * kKeys + c + i), v_mid = *reinterpret_cast<const float2*>(table + 3 * kKeys + c + i);
-              if (!kAll) {
-                if (c + i < sees0 || c + i > sees1) v_scale.x = v_mid.x = 0.0f;
-                if (c + i + 1 < sees0 || c + i + 1 > sees1) v_scale.y = v_mid.y = 0.0f;
+              for (int i = 0; i < o; ++i) big[i] = fmaxf(big[i], big[i + o]);
+            const float top = big[0] * factor;
+            if (__any_sync(0xffffffffu, top > limit)) {
+              const float now = top > limit ? ceilf(top) : M;
+              const float keep = M == -INFINITY ? 0.0f : exp2f(M - now);
+              M = now;
+              limit = M + kLag;
+              shift = M == -INFINITY ? kLift : kLift - M;
+              l *= keep;
+              scale_columns<true>(t_s, c, keep);
+              if (j > 0) {  // the sums of the tiles before
+                wait(kOFull + wg, j - 1);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                scale_columns<false>(t_o, D, keep);
               }
-              part = add2(part, w);
-              mid = fma2(w, v_mid, mid);
-              const float2 y = mul2(w, v_scale);
-              constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
-              const float2 h = add2(add2(y, make_float2(kEight, kEight)), make_float2(-kEight, -kEight)), low = fma2(h, make_float2(-1.0f, -1.0f), y);
-              hi[i / 2] = half2_bits(h.x, h.y);
-              lo[i / 2] = half2_bits(low.x, low.y);
             }
-            l += part.x + part.y;
-            centre += mid.x + mid.y;
-          } else {
+            begin_next();
+            uint32_t w2[kN / 2];
             float part[4] = {};
 #pragma unroll
             for (int i = 0; i < kN; i += 2) {
               const float w0 = ex2(fmaf(z[i], factor, shift)), w1 = ex2(fmaf(z[i + 1], factor, shift));
               part[i / 2 % 2 * 2] += w0;
               part[i / 2 % 2 * 2 + 1] += w1;
-              hi[i / 2] = half2_bits(w0, w1);
+              w2[i / 2] = half2_bits(w0, w1);
             }
             l += (part[0] + part[1]) + (part[2] + part[3]);
-          }
-          // sixteen keys' weights go where their scores were: eight columns, and eight for the low parts
+            // sixteen keys' weights go where their scores were, into eight columns
 #pragma unroll
-          for (int i = 0; i < kN / 16; ++i) {
-            tmem_st8(t_s + c + i * 16, hi + i * 8);
-            if constexpr (kSplit) tmem_st8(t_s + c + i * 16 + 8, lo + i * 8);
-          }
-        };
-        if constexpr (kSplit) {  // registers are short: one set of scores
-#pragma unroll 1
-          for (int c = 0; c < kKeys; c += kN) {
-            tmem_ld_begin(t_s + c, x[0]);
-            tmem_ld_done(x[0]);
-            some(c, x[0], [] {});
-          }
-        } else {
+            for (int i = 0; i < kN / 16; ++i) tmem_st8(t_s + c + i * 16, w2 + i * 8);
+          };
           tmem_ld_begin(t_s, x[0]);
 #pragma unroll 1
           for (int c = 0; c < kKeys; c += 2 * kN) {
@@ -673,11 +723,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
               if (c + 2 * kN < kKeys) tmem_ld_begin(t_s + c + 2 * kN, x[0]);
             });
           }
-        }
-      };
-      if (whole) tile(std::true_type());
-      else tile(std::false_type());
-      if constexpr (!kSplit) {
+        };
+        if (whole) tile(std::true_type());
+        else tile(std::false_type());
         const uint4 lost = *reinterpret_cast<const uint4*>(smem + F::kLost + (j & 1) * 16);
         if (lost.x | lost.y | lost.z | lost.w) {  // values that are NaN entered as zeros: whoever sees one is NaN
           const uint32_t bits[4] = {lost.x, lost.y, lost.z, lost.w};
@@ -685,17 +733,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             if (bits[i / 32] >> (i % 32) & 1) l = quiet_nan();
           __syncwarp();
         }
-      }
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      umma::mbar_arrive(bar(kPReady + wg));
-      if constexpr (kSplit) {
-        wait(kOFull + wg, j);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_columns<D, true>(t_o, [&](int c, float (&x)[16]) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) O[c + i] += x[i];
-        });
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        umma::mbar_arrive(bar(kPReady + wg));
       }
     }
     const int row = row0 + r;
@@ -715,12 +755,12 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     };
     if constexpr (kSplit) {
 #pragma unroll
-      for (int i = 0; i < D; i += 8) {
+      for (int i = 0; i < D / 2; i += 8) {
         float o[8];
         // powers of two: the weights' 2^13, the codes' even dims (2 u - 15) 2^-24, odd ones (u - 7.5) 2^-20
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] = fmaf(O[i + k], (k & 1) ? 128.0f : 1024.0f, centre) * inv;
-        store(i, o);
+        store(static_cast<int>(wg) * (D / 2) + i, o);
       }
     } else if (tiles == 0) {
       const float zero[8] = {};
@@ -728,7 +768,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     } else {
       wait(kOFull + wg, tiles - 1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      tmem_columns<D, false>(t_o, [&](int c, float (&x)[16]) {
+      tmem_columns<D, false>(tmem + lanes + 256 + wg * 128, [&](int c, float (&x)[16]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= inv;
         store(c, x);
@@ -737,7 +777,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       });
     }
     if (shared) {  // the last CTA of the unit joins the parts, in order
-      reinterpret_cast<float2*>(part + kBlock * D)[r] = make_float2(M, l);
+      if (!kSplit || wg == 0) reinterpret_cast<float2*>(part + kBlock * D)[r] = make_float2(M, l);
       asm volatile("bar.sync 2, 256;" ::: "memory");
       if (tid == 0) {
         unsigned int arrived;
@@ -773,7 +813,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   } else {
-    if constexpr (kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp < F::kMmaWarp) {
       // ---- unpacking ---------------------------------------------------------------------------------
       const uint32_t t = tid - 256, w4 = warp - 8;
@@ -782,13 +822,13 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       bool ok = true;  // after a wait that gave up nothing is handed on: no barrier is arrived on beyond its phase
       for (int j = 0; j < tiles; ++j) {
         const int first = (tile0 + j) * kKeys;
-        const uint32_t buf = j % kVBufs, raw = j % kRaws;
+        const uint32_t buf = j % kVBufs, kbuf = j % kKBufs, raw = j % kRaws;
         const uint8_t* const codes = smem + F::kRaw + raw * F::kRawBytes;
         uint32_t* const k_par = reinterpret_cast<uint32_t*>(smem + F::kTable + (j & 1) * F::kTableBytes);  // (scale, offset) of each key;
         __half* const v_scale = reinterpret_cast<__half*>(k_par + kKeys);                                  // values' scales, then offsets
         __half* const v_offset = v_scale + kKeys;
         ok = wait(kRawKFull + raw, j / kRaws) && ok;
-        if (kVBufs == 2 && j >= 2) wait(kVEmpty + buf, j / 2 - 1);  // what the softmax warps read of tile j - 2 has been read
+        if (j >= 2) wait(kVEmpty + buf, j / 2 - 1);  // what the softmax warps read of tile j - 2 has been read
         if (t < kKeys) {
           const bool seen = first + static_cast<int>(t) <= key_last;
           const uint32_t* const raw_params = reinterpret_cast<const uint32_t*>(codes + F::kRawParams);
@@ -801,7 +841,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             table[2 * kKeys] = v.x * 8192.0f;
             table[3 * kKeys] = fmaf(7.5f, v.x, v.y);
             const uint32_t big = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v.x, 0.0f)));  // not NaN
-            if (lane == 0) reinterpret_cast<float*>(smem + F::kBinade)[(j & 1) * 4 + w4] = binade_of(__uint_as_float(big));
+            if (lane == 0) reinterpret_cast<float*>(smem + F::kBinade)[(j & 1) * 4 + w4] = __uint_as_float(big) * 8192.0f;
           } else {
             // the largest value must stay finite in binary16: a scale that was rounded up gives one unit back
             if (fmaf(15.0f, k.x, k.y) >= 65520.0f) kp -= 1;
@@ -814,7 +854,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             v_offset[t] = __ushort_as_half(static_cast<unsigned short>(vp >> 16));
           }
         }
-        if (j >= 1) wait(kKEmpty, j - 1);
+        if (j >= kKBufs) wait(kKEmpty + kbuf, j / kKBufs - 1);
         asm volatile("bar.sync 1, %0;" ::"n"(F::kUnpack) : "memory");
         {
           constexpr int kPieces = D / 32;  // 16-byte pieces of a token
@@ -844,17 +884,16 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
                 out.z = hfma2_bits(hadd2_bits((x8 & 0x000F000Fu) | kExp, k1024), s2, o2);
                 out.w = hfma2_bits(hfma2_bits((x8 & 0x00F000F0u) | kExp, k16th, k64), s2, o2);
               }
-              umma::sts128(base + F::kK + (word / 8) * 16384 + umma::swz(row, word % 8), out);
+              umma::sts128(base + F::kK + kbuf * F::kOperand + (word / 8) * 16384 + umma::swz(row, word % 8), out);
             }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (ok) {
-          umma::mbar_arrive(bar(kKFull));
+          umma::mbar_arrive(bar(kKFull + kbuf));
           umma::mbar_arrive(bar(kRawKFree + raw));
         }
         ok = wait(kRawVFull + raw, j / kRaws) && ok;
-        if (kVBufs == 1 && j >= 1) wait(kVEmpty, j - 1);
         {
           const uint32_t tg = lane % 8;
 #pragma unroll 1
@@ -902,45 +941,71 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     } else if (warp == F::kMmaWarp) {
       // ---- MMAs ----------------------------------------------------------------------------------------
       const uint32_t leader = umma::elect_lane();
-      const auto scores = [&](uint32_t r) {
-        const uint32_t d = tmem + r * 128, q = desc_low(base + F::kQ + r * kParts * F::kOperand), k = desc_low(base + F::kK);
+      // scores into tensor memory's columns at t * 128 (of row block t, or f32: of every other tile), keys from buffer `kbuf`
+      const auto scores = [&](uint32_t t, uint32_t kbuf) {
+        const uint32_t q = desc_low(base + F::kQ + (kSplit ? 0 : t) * F::kOperand), k = desc_low(base + F::kK + kbuf * F::kOperand);
 #pragma unroll
         for (int part = kParts - 1; part >= 0; --part)
 #pragma unroll
           for (int s = 0; s < D / 16; ++s)
-            mma_ss(leader, d, q + (part * F::kOperand + s / 4 * 16384 + s % 4 * 32) / 16, k + (s / 4 * 16384 + s % 4 * 32) / 16, f16_idesc(kKeys),
+            mma_ss(leader, tmem + t * 128, q + (part * F::kOperand + s / 4 * 16384 + s % 4 * 32) / 16, k + (s / 4 * 16384 + s % 4 * 32) / 16, f16_idesc(kKeys),
                    part != kParts - 1 || s != 0);
-        umma::commit_one(leader, bar(kSFull + r));
+        umma::commit_one(leader, bar(kSFull + t));
       };
-      if (tiles > 0) {
-        wait(kKFull, 0);
+      const auto outputs = [&](uint32_t t, uint32_t buf, uint32_t add) {
+        const uint32_t v = desc_low(base + F::kV + buf * F::kOperand);
+#pragma unroll
+        for (int part = kParts - 1; part >= 0; --part)
+#pragma unroll
+          for (int s = 0; s < kKeys / 16; ++s)
+            mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + s * 16 + part * 8, v + (s / 4 * (D * 128) + s % 4 * 32) / 16, f16_idesc(D),
+                   part != kParts - 1 || s != 0 ? 1 : add);
+        umma::commit_one(leader, bar(kOFull + t));
+      };
+      const auto keys_ready = [&](int j) {
+        wait(kKFull + j % kKBufs, j / kKBufs);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        scores(0);
-        scores(1);
-        umma::commit_one(leader, bar(kKEmpty));
-      }
-      for (int j = 0; j < tiles; ++j) {
-        const uint32_t buf = j % kVBufs;
-        for (uint32_t r = 0; r < 2; ++r) {
-          wait(kPReady + r, j);
-          if (r == 0) wait(kVFull + buf, j / kVBufs);
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t v = desc_low(base + F::kV + buf * F::kOperand);
-#pragma unroll
-          for (int part = kParts - 1; part >= 0; --part)
-#pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
-              mma_ts(leader, tmem + 256 + r * 128, tmem + r * 128 + s * 16 + part * 8, v + (s / 4 * (D * 128) + s % 4 * 32) / 16, f16_idesc(D),
-                     part != kParts - 1 || s != 0 || (!kSplit && j > 0));
-          umma::commit_one(leader, bar(kOFull + r));
-          if (r == 1) umma::commit_one(leader, bar(kVEmpty + buf));
+      };
+      if constexpr (kSplit) {
+        // the next tile's scores are made while the softmax works on this one's
+        if (tiles > 0) {
+          keys_ready(0);
+          scores(0, 0);
+          umma::commit_one(leader, bar(kKEmpty));
+        }
+        for (int j = 0; j < tiles; ++j) {
+          const uint32_t t = j & 1;
           if (j + 1 < tiles) {
-            if (r == 0) {
-              wait(kKFull, j + 1);
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            keys_ready(j + 1);
+            scores(t ^ 1, (j + 1) % kKBufs);
+            umma::commit_one(leader, bar(kKEmpty + (j + 1) % kKBufs));
+          }
+          wait(kPReady + t, j / 2);
+          wait(kVFull + t, j / 2);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          outputs(t, t, 0);
+          umma::commit_one(leader, bar(kVEmpty + t));
+        }
+      } else {
+        if (tiles > 0) {
+          keys_ready(0);
+          scores(0, 0);
+          scores(1, 0);
+          umma::commit_one(leader, bar(kKEmpty));
+        }
+        for (int j = 0; j < tiles; ++j) {
+          const uint32_t buf = j % kVBufs;
+          for (uint32_t t = 0; t < 2; ++t) {
+            wait(kPReady + t, j);
+            if (t == 0) wait(kVFull + buf, j / kVBufs);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            outputs(t, buf, j > 0);
+            if (t == 1) umma::commit_one(leader, bar(kVEmpty + buf));
+            if (j + 1 < tiles) {
+              if (t == 0) keys_ready(j + 1);
+              scores(t, (j + 1) % kKBufs);
+              if (t == 1) umma::commit_one(leader, bar(kKEmpty + (j + 1) % kKBufs));
             }
-            scores(r);
-            if (r == 1) umma::commit_one(leader, bar(kKEmpty));
           }
         }
       }
@@ -1026,7 +1091,7 @@ cudaError_t many_as(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond) 
   p.status = env.status;
   // at most so many blocks of rows: full ones, and one begun for each sequence
   const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * p.group;
-  const uint64_t blocks = rows / kBlock + std::min<uint64_t>(a.batch.sequences, rows / (beyond + 1));
+  const uint64_t blocks = rows / F::kBlock + std::min<uint64_t>(a.batch.sequences, rows / (beyond + 1));
   cudaLaunchConfig_t cfg = {};
   const uint64_t units = blocks * a.cache.kv_heads;
   // Few units: their keys are shared, so that every SM has its part (a part more for each unit's odd end).
