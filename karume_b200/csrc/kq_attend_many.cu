@@ -17,7 +17,7 @@
 //   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights).
 //   f32 queries     codes enter exactly, around zero: (2 u - 15) 2^-24 and (u - 7.5) 2^-20, one operation from the subnormals that
 //                   their bits already are; scale and offset are applied to the scores and weights in f32.  Queries and weights are
-//                   two binary16 parts each (fixed-point, the low ones multiplied first), 22 bits and more.
+//                   two binary16 parts each (fixed-point: sums of high parts are exact), 22 bits and more.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,7 +30,7 @@ namespace {
 constexpr int kKeys = 128;    // of a tile
 constexpr int kManyTimeout = 50;
 
-enum Bar { kRawKFull, kRawKFree = 2, kRawVFull = 4, kRawVFree = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kSFull = 16, kPReady = 18, kOFull = 20, kBarCount = 22 };
+enum Bar { kRawKFull, kRawKFree = 2, kRawVFull = 4, kRawVFree = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kSFull = 16, kPReady = 18, kOFull = 20, kLoaded = 21, kBarCount = 22 };
 
 template <typename T, int D>
 struct Many {
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       umma::mbar_init(bar(kVFull + i), F::kUnpack);
       umma::mbar_init(bar(kVEmpty + i), 1);
       umma::mbar_init(bar(kSFull + i), 1);
-      umma::mbar_init(bar(kOFull + i), 1);
+      umma::mbar_init(bar(kOFull + i), kSplit && i == 1 ? 256 : 1);  // f32: one O; the second is kLoaded
       umma::mbar_init(bar(kPReady + i), kSplit ? 256 : 128);
     }
     *abort_flag = 0;
@@ -552,9 +552,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       float2* const halves = reinterpret_cast<float2*>(smem + F::kHalves);
       float keep_sums = 1.0f;  // what the tile before is still to be scaled by
       const auto drain = [&](int j, float keep) {
-        wait(kOFull + (j & 1), j / 2);
+        wait(kOFull, j);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_columns<D / 2, true>(tmem + lanes + 256 + (j & 1) * 128 + wg * (D / 2), [&](int c, float (&x)[16]) {
+        tmem_columns<D / 2, true>(tmem + lanes + 384 + wg * (D / 2), [&](int c, float (&x)[16]) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) O[c + i] = fmaf(x[i], keep, O[c + i]);
         });
@@ -572,6 +572,16 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         for (int c = 0; c < 64; c += 32) tmem_ld_begin(t_s + c, reinterpret_cast<float (&)[32]>(z[c]));
 #pragma unroll
         for (int c = 0; c < 64; c += 32) tmem_ld_done(reinterpret_cast<float (&)[32]>(z[c]));
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {  // the low parts' share
+          float low[32];
+          tmem_ld_begin(tmem + lanes + 256 + wg * 64 + c, low);
+          tmem_ld_done(low);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[c + i] += low[i];
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        umma::mbar_arrive(bar(kLoaded));
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
           const float2 k_scale = *reinterpret_cast<const float2*>(table + i), k_mid = *reinterpret_cast<const float2*>(table + kKeys + i);
@@ -642,10 +652,10 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         }
         l += part.x + part.y;
         centre += mid.x + mid.y;
+        if (j > 0) drain(j - 1, keep_sums);  // before the next sums are made in the same columns
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         umma::mbar_arrive(bar(kPReady + (j & 1)));
-        if (j > 0) drain(j - 1, keep_sums);
       }
       if (tiles > 0) drain(tiles - 1, 1.0f);
       // both halves' weights
@@ -941,26 +951,29 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     } else if (warp == F::kMmaWarp) {
       // ---- MMAs ----------------------------------------------------------------------------------------
       const uint32_t leader = umma::elect_lane();
-      // scores into tensor memory's columns at t * 128 (of row block t, or f32: of every other tile), keys from buffer `kbuf`
+      // scores into tensor memory's columns at t * 128 (of row block t, or f32: of every other tile), keys from buffer `kbuf`; f32: the
+      // queries' low parts into columns of their own: added to the high ones they would be cut off step by step
       const auto scores = [&](uint32_t t, uint32_t kbuf) {
         const uint32_t q = desc_low(base + F::kQ + (kSplit ? 0 : t) * F::kOperand), k = desc_low(base + F::kK + kbuf * F::kOperand);
 #pragma unroll
         for (int part = kParts - 1; part >= 0; --part)
 #pragma unroll
           for (int s = 0; s < D / 16; ++s)
-            mma_ss(leader, tmem + t * 128, q + (part * F::kOperand + s / 4 * 16384 + s % 4 * 32) / 16, k + (s / 4 * 16384 + s % 4 * 32) / 16, f16_idesc(kKeys),
-                   part != kParts - 1 || s != 0);
+            mma_ss(leader, tmem + (part ? 256 : t * 128), q + (part * F::kOperand + s / 4 * 16384 + s % 4 * 32) / 16, k + (s / 4 * 16384 + s % 4 * 32) / 16, f16_idesc(kKeys),
+                   s != 0);
         umma::commit_one(leader, bar(kSFull + t));
       };
       const auto outputs = [&](uint32_t t, uint32_t buf, uint32_t add) {
         const uint32_t v = desc_low(base + F::kV + buf * F::kOperand);
+        // f32: the high parts first, whose sums are exact: products' bits line up with the operands' exponents, and a subnormal's is the
+        // smallest normal one, so a high part's step would cut 2^-19 off a sum that held low ones
 #pragma unroll
-        for (int part = kParts - 1; part >= 0; --part)
+        for (int part = 0; part < kParts; ++part)
 #pragma unroll
           for (int s = 0; s < kKeys / 16; ++s)
-            mma_ts(leader, tmem + 256 + t * 128, tmem + t * 128 + s * 16 + part * 8, v + (s / 4 * (D * 128) + s % 4 * 32) / 16, f16_idesc(D),
-                   part != kParts - 1 || s != 0 ? 1 : add);
-        umma::commit_one(leader, bar(kOFull + t));
+            mma_ts(leader, tmem + (kSplit ? 384 : 256 + t * 128), tmem + t * 128 + s * 16 + part * 8, v + (s / 4 * (D * 128) + s % 4 * 32) / 16, f16_idesc(D),
+                   part != 0 || s != 0 ? 1 : add);
+        umma::commit_one(leader, bar(kOFull + (kSplit ? 0 : t)));
       };
       const auto keys_ready = [&](int j) {
         wait(kKFull + j % kKBufs, j / kKBufs);
@@ -977,6 +990,8 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
           const uint32_t t = j & 1;
           if (j + 1 < tiles) {
             keys_ready(j + 1);
+            wait(kLoaded, j);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             scores(t ^ 1, (j + 1) % kKBufs);
             umma::commit_one(leader, bar(kKEmpty + (j + 1) % kKBufs));
           }
