@@ -637,9 +637,9 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
                 pv[i] *= lift[n];
               }
               uint32_t both;
-              if constexpr (kSplit) {  // fixed-point parts, as the queries'
-                const float hi = rintf(pv[0] * 0.125f) * 8.0f;
-                both = pack_half2(__float2half_rn(hi), __float2half_rn(rintf((pv[0] - hi) * 256.0f) * 0.00390625f));
+              if constexpr (kSplit) {  // the high part: whole numbers (their sums are exact) of eleven bits, so that small weights keep 22 too
+                const float hi = __uint_as_float(__float_as_uint(rintf(pv[0])) & 0xFFFFE000u);
+                both = pack_half2(__float2half_rn(hi), __float2half_rn(pv[0] - hi));
               } else {
                 const __half2 h = __floats2half2_rn(pv[0], kPair ? 0.0f : pv[kPer - 1]);
                 both = *reinterpret_cast<const uint32_t*>(&h);

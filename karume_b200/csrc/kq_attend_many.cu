@@ -340,17 +340,17 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         }
     __syncthreads();
     const int mine_tiles = tid < units ? tiles_of(of[2 * tid], of[2 * tid + 1]).y : 0;
-    const int warp_tiles = __reduce_add_sync(0xffffffffu, mine_tiles);
+    const uint32_t warp_tiles = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(min(mine_tiles, 1 << 22)));
     __syncthreads();
-    if (lane == 0) scan[warp] = static_cast<uint32_t>(warp_tiles);
+    if (lane == 0) scan[warp] = warp_tiles;
     __syncthreads();
-    int all = 0;
-    for (int i = 0; i < F::kThreads / 32; ++i) all += static_cast<int>(scan[i]);
-    // the smallest share of tiles with which the parts are one wave of CTAs
-    int share = max((all + static_cast<int>(p.ctas) - 1) / static_cast<int>(p.ctas), 2);
+    uint32_t all = 0;
+    for (uint32_t i = 0; i < F::kThreads / 32; ++i) all += scan[i];
+    // about the smallest share of tiles with which the parts are one wave of CTAs; more units than CTAs stay whole
+    int share = units > p.ctas ? 1 << 24 : max(static_cast<int>((all + p.ctas - 1) / p.ctas), 2);
     uint32_t n_parts = 0;
-    for (;; ++share) {
-      n_parts = tid < units ? static_cast<uint32_t>(max((mine_tiles + share - 1) / share, 1)) : 0u;
+    for (;; share += share / 16 + 1) {
+      n_parts = tid < units ? min(static_cast<uint32_t>(max((mine_tiles + share - 1) / share, 1)), p.ctas + 1) : 0u;
       const bool more = __syncthreads_or(n_parts > 1);
       const uint32_t warp_parts = __reduce_add_sync(0xffffffffu, n_parts);
       if (lane == 0) scan[warp] = warp_parts;
@@ -641,8 +641,12 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             part = add2(part, w);
             mid = fma2(w, v_mid, mid);
             const float2 y = mul2(w, v_scale);
-            constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
-            const float2 h = add2(add2(y, make_float2(kEight, kEight)), make_float2(-kEight, -kEight)), low = fma2(h, make_float2(-1.0f, -1.0f), y);
+            // the high part: whole numbers (their sums are exact) of eleven bits, so that small weights keep 22 bits too
+            constexpr float kOne = 12582912.0f;  // 1.5 2^23: numbers beside it are whole
+            float2 h = add2(add2(y, make_float2(kOne, kOne)), make_float2(-kOne, -kOne));
+            h.x = __uint_as_float(__float_as_uint(h.x) & 0xFFFFE000u);
+            h.y = __uint_as_float(__float_as_uint(h.y) & 0xFFFFE000u);
+            const float2 low = fma2(h, make_float2(-1.0f, -1.0f), y);
             hi[i / 2] = half2_bits(h.x, h.y);
             lo[i / 2] = half2_bits(low.x, low.y);
           }
