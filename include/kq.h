@@ -362,10 +362,12 @@ KQ_API int kq_cache_free(kq_ctx* ctx, kq_cache cache);
 /* The sequences of a call are device arrays of i32: `page_table` [sequences, table_width] with the pages
  * of each sequence in order, `lengths` [sequences], and `starts` [sequences + 1]: sequence b's new tokens are
  * rows starts[b] .. starts[b + 1] of the call's tensors and its last tokens, lengths[b] counting them.
- * starts == 0: every sequence has one new token, row b.  `most` bounds the new tokens of any sequence (0: not
- * known); it chooses kernels, results do not depend on it.  All of this is read on the device at launch, so
- * that a recorded step can be replayed with other lengths and pages.  A page number outside the pool, or a
- * token beyond table_width pages, is not written and reads as NaN; a sequence may be idle (length 0).
+ * starts == 0: every sequence has one new token, row b.  starts ascend; a row that belongs to no sequence is not
+ * appended, reads as NaN and attends to nothing (zeros).  `most` bounds the new tokens of any sequence (0: not
+ * known); it only chooses kernels, so that their roundings may differ, and a bound that is too low costs time, not
+ * results.  All of this is read on the device at launch, so that a recorded step can be replayed with other lengths
+ * and pages.  A page number outside the pool, or a token beyond table_width pages, is not written and reads as NaN;
+ * a sequence may be idle (length 0).
  *
  * kq_cache_append: k and v are [tokens, kv_heads, head_dim] of `dtype`, k_stride / v_stride elements apart
  * (columns of a fused projection); keys are rotated on the way (table_dptr == 0: not).  Two rows that name the

@@ -14,6 +14,12 @@
 // next tile's scores are made meanwhile; O is one tile's, added in registers, so that a long row does not drift.
 // Few blocks of rows: the tiles of keys of each are shared by several CTAs, and the last one joins their sums in order.
 //
+// Measured: 4096 new tokens behind 904, 32 heads over 8, bfloat16: 305 us (650 TFLOP/s; tensor pipe 32 %, issue slots 50 %).  Of it a tile
+// of 256 rows is 2.6 us of a CTA (the MMAs 1.1): the turn from scores to weights and back, neither the unpacking (left out: 292 us)
+// nor the exponentials (left out: the same) alone; a CTA's beginning and end are 21 us (rows found 1.8, queries 7.2, the first
+// tile's way 4, output 5.9, the next CTA's start 1.8), three to four times an SM; the last CTAs end 27 us after the mean one.
+// Three f32 prompts of up to 777 tokens behind 724, 12 heads over 2: 75 us, four products for one.
+//
 //   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights).
 //   f32 queries     codes enter exactly, around zero: (2 u - 15) 2^-24 and (u - 7.5) 2^-20, one operation from the subnormals that
 //                   their bits already are; scale and offset are applied to the scores and weights in f32.  Queries and weights are
