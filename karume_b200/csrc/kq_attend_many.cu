@@ -16,7 +16,7 @@
 //
 // Measured: 4096 new tokens behind 904, 32 heads over 8, bfloat16: 305 us (650 TFLOP/s; tensor pipe 32 %, issue slots 50 %).  Of it a tile
 // of 256 rows is 2.6 us of a CTA (the MMAs 1.1): the turn from scores to weights and back, neither the unpacking (left out: 292 us)
-// nor the exponentials (left out: the same) alone; a CTA's beginning and end are 21 us (rows found 1.8, queries 7.2, the first
+// nor the exponentials (left out: 307) alone; a CTA's beginning and end are 21 us (rows found 1.8, queries 7.2, the first
 // tile's way 4, output 5.9, the next CTA's start 1.8), three to four times an SM; the last CTAs end 27 us after the mean one.
 // Three f32 prompts of up to 777 tokens behind 724, 12 heads over 2: 75 us, four products for one.
 //
