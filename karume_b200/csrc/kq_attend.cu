@@ -926,7 +926,8 @@ cudaError_t few_in(const LaunchEnv& env, const AttendArgs& a, uint64_t rows, uin
   }
 }
 
-// Query rows (of a sequence and kv head) from which on 128-row MMAs are faster.
+// Query rows (of a sequence and kv head) up to which this kernel is faster than 128-row MMAs.  16 sequences of 4096 tokens, 8 kv heads,
+// this one / the other: bfloat16 16 rows 43 / 95 us, 32 rows 88 / 96, 48 rows 141 / 97; f32 32 rows 104 / 148, 48 rows 147 / 148.
 constexpr uint32_t kFewRows = 32;
 
 }  // namespace
