@@ -788,13 +788,35 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     } else {
       wait(kOFull + wg, tiles - 1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      // Rows go out whole, through the block's queries' memory, which every score has been made of by now: a thread's own row is 16
+      // bytes of 32 rows an instruction.
+      uint8_t* const mine = smem + F::kQ + wg * F::kOperand + warp % 4 * (32 * D * 2);
       tmem_columns<D, false>(tmem + lanes + 256 + wg * 128, [&](int c, float (&x)[16]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= inv;
-        store(c, x);
-        store(c + 8, x + 8);
+        if (shared) {
+          store(c, x);
+          store(c + 8, x + 8);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            store8(reinterpret_cast<T*>(mine + lane * (D * 2) + ((c / 8 + h) ^ (lane & 7)) * 16), x + 8 * h);
+        }
         __syncwarp();
       });
+      if (!shared) {
+        constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;  // of a row; rows an instruction
+#pragma unroll 4
+        for (uint32_t i = lane / kChunks; i < 32; i += kAtOnce) {
+          const uint32_t of = wg * 128 + warp % 4 * 32 + i, chunk = lane % kChunks;
+          if (row0 + static_cast<int>(of) >= n_rows) break;
+          const int2 qh = query_and_head(static_cast<int>(of));
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.a.out) + static_cast<size_t>(span.first + qh.x) * p.a.out_stride +
+                                    static_cast<size_t>(head * p.group + static_cast<uint32_t>(qh.y)) * D + chunk * 8) =
+              *reinterpret_cast<const uint4*>(mine + i * (D * 2) + (chunk ^ (i & 7)) * 16);
+        }
+        __syncwarp();
+      }
     }
     if (shared) {  // the last CTA of the unit joins the parts, in order
       if (!kSplit || wg == 0) reinterpret_cast<float2*>(part + kBlock * D)[r] = make_float2(M, l);
