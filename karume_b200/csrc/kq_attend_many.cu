@@ -14,11 +14,11 @@
 // next tile's scores are made meanwhile; O is one tile's, added in registers, so that a long row does not drift.
 // Few blocks of rows: the tiles of keys of each are shared by several CTAs, and the last one joins their sums in order.
 //
-// Measured: 4096 new tokens behind 904, 32 heads over 8, bfloat16: 305 us (650 TFLOP/s; tensor pipe 32 %, issue slots 50 %).  Of it a tile
-// of 256 rows is 2.6 us of a CTA (the MMAs 1.1): the turn from scores to weights and back, neither the unpacking (left out: 292 us)
-// nor the exponentials (left out: 307) alone; a CTA's beginning and end are 21 us (rows found 1.8, queries 7.2, the first
-// tile's way 4, output 5.9, the next CTA's start 1.8), three to four times an SM; the last CTAs end 27 us after the mean one.
-// Three f32 prompts of up to 777 tokens behind 724, 12 heads over 2: 75 us, four products for one.
+// Measured: 4096 new tokens behind 904, 32 heads over 8, bfloat16: 292 us (680 TFLOP/s; tensor pipe 33 %, issue slots 50 %).  Of it a tile
+// of 256 rows is 2.6 us of a CTA (the MMAs 1.1): the turn from scores to weights and back, neither the unpacking (left out: 292 of 305 us)
+// nor the exponentials (left out: 307) alone; a CTA's beginning and end were 21 us (rows found 1.8, queries 7.2, the first
+// tile's way 4, output 5.9 (2.4 since it leaves in whole rows: 305 -> 293 us), the next CTA's start 1.8), three to four times an SM; the last CTAs end 27 us after the mean one.
+// Three f32 prompts of up to 777 tokens behind 724, 12 heads over 2: 67 us, four products for one.
 //
 //   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights).
 //   f32 queries     codes enter exactly, around zero: (2 u - 15) 2^-24 and (u - 7.5) 2^-20, one operation from the subnormals that
@@ -270,20 +270,31 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     __syncwarp();  // what follows is often an aligned instruction
     return ok;
   };
+  // Each lane has fenced what it did.  f32: one arrival for the warp, since 32 on one word take their turns (three prompts: 75 -> 67 us);
+  // 16-bit, whose warps have longer to the next barrier: each lane its own (4096 new tokens: 293 us, with one 297).
+  constexpr uint32_t kArrivals = kSplit ? 1 : 32;  // of a warp
+  const auto arrive = [&](int i) {
+    if constexpr (kSplit) {
+      __syncwarp();
+      if (lane == 0) umma::mbar_arrive(bar(i));
+    } else {
+      umma::mbar_arrive(bar(i));
+    }
+  };
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      umma::mbar_init(bar(kKFull + i), F::kUnpack);
+      umma::mbar_init(bar(kKFull + i), F::kUnpackWarps * kArrivals);
       umma::mbar_init(bar(kKEmpty + i), 1);
       umma::mbar_init(bar(kRawKFull + i), 1);
       umma::mbar_init(bar(kRawVFull + i), 1);
-      umma::mbar_init(bar(kRawKFree + i), F::kUnpack);
-      umma::mbar_init(bar(kRawVFree + i), F::kUnpack);
-      umma::mbar_init(bar(kVFull + i), F::kUnpack);
+      umma::mbar_init(bar(kRawKFree + i), F::kUnpackWarps * kArrivals);
+      umma::mbar_init(bar(kRawVFree + i), F::kUnpackWarps * kArrivals);
+      umma::mbar_init(bar(kVFull + i), F::kUnpackWarps * kArrivals);
       umma::mbar_init(bar(kVEmpty + i), 1);
       umma::mbar_init(bar(kSFull + i), 1);
-      umma::mbar_init(bar(kOFull + i), kSplit && i == 1 ? 256 : 1);  // f32: one O; the second is kLoaded
-      umma::mbar_init(bar(kPReady + i), kSplit ? 256 : 128);
+      umma::mbar_init(bar(kOFull + i), kSplit && i == 1 ? 8 * kArrivals : 1);  // f32: one O; the second is kLoaded
+      umma::mbar_init(bar(kPReady + i), (kSplit ? 8 : 4) * kArrivals);
     }
     *abort_flag = 0;
     found[0] = 0xFFFFFFFFu;
@@ -587,7 +598,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
           for (int i = 0; i < 32; ++i) z[c + i] += low[i];
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        umma::mbar_arrive(bar(kLoaded));
+        arrive(kLoaded);
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
           const float2 k_scale = *reinterpret_cast<const float2*>(table + i), k_mid = *reinterpret_cast<const float2*>(table + kKeys + i);
@@ -665,7 +676,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         if (j > 0) drain(j - 1, keep_sums);  // before the next sums are made in the same columns
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        umma::mbar_arrive(bar(kPReady + (j & 1)));
+        arrive(kPReady + (j & 1));
       }
       if (tiles > 0) drain(tiles - 1, 1.0f);
       // both halves' weights
@@ -755,7 +766,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        umma::mbar_arrive(bar(kPReady + wg));
+        arrive(kPReady + wg);
       }
     }
     const int row = row0 + r;
@@ -931,9 +942,10 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if constexpr (kSplit) ok = __all_sync(0xffffffffu, ok);
         if (ok) {
-          umma::mbar_arrive(bar(kKFull + kbuf));
-          umma::mbar_arrive(bar(kRawKFree + raw));
+          arrive(kKFull + kbuf);
+          arrive(kRawKFree + raw);
         }
         ok = wait(kRawVFull + raw, j / kRaws) && ok;
         {
@@ -975,9 +987,10 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if constexpr (kSplit) ok = __all_sync(0xffffffffu, ok);
         if (ok) {
-          umma::mbar_arrive(bar(kVFull + buf));
-          umma::mbar_arrive(bar(kRawVFree + raw));
+          arrive(kVFull + buf);
+          arrive(kRawVFree + raw);
         }
       }
     } else if (warp == F::kMmaWarp) {
