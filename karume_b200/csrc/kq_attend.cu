@@ -18,7 +18,7 @@
 //   weight   p_j = 2^(s_j - M), and P = p_j s'_j (s' the value's scale) is what enters the tensor core.  M follows the
 //            largest s_j + log2 of s'_j's binade, and moves only when a weight would grow past 2^8 of it: P fits binary16
 //            with its full precision wherever it matters, whatever the size of the values.  16-bit queries round P to binary16
-//            once (2.9e-4 of the result, where rounding the result alone is 2.1e-4); f32 ones keep two parts of eleven bits.
+//            once (with the rotated queries, 2.9e-4 to 3.9e-4 of an f16 result; its own rounding is 2.1e-4); f32 ones keep two parts of eleven bits.
 //   output   sum_j P_j (u'_j - 7.5) + sum_j p_j (o'_j + 7.5 s'_j): codes around zero, because sums of many uncentred
 //            ones cancel (70001 keys: 1e-3 of the result was lost); f32 queries add each tile's sums in registers,
 //            where the tensor core's own chain would truncate.
