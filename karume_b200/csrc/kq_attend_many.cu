@@ -189,6 +189,7 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
 template <bool kHalves>
 __device__ __noinline__ void scale_columns(uint32_t taddr, int n, float keep) {
   const __half2 keep2 = __float2half2_rn(keep);
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");  // the weights of the keys in front may still be on their way there
   for (int at = 0; at < n; at += 16) {
     float w[16];
     tmem_ld16_begin(taddr + at, w);
