@@ -80,7 +80,11 @@ KQ_API void kq_destroy(kq_ctx* ctx);
 KQ_API const char* kq_last_error(kq_ctx* ctx);
 
 /* Work is enqueued on the context's own stream unless a foreign cudaStream_t is
- * installed here (pass 0 to return to the own stream). */
+ * installed here (pass 0 to return to the own stream).  The own stream and the device's
+ * legacy default stream wait for each other, as CUDA's blocking streams do: what the host
+ * enqueued on the default stream in front of a call is there when its kernels run, and what it
+ * enqueues behind the call sees their results.  Against any other stream the host keeps order
+ * itself: by installing it here, or with events. */
 KQ_API int kq_set_stream(kq_ctx* ctx, uint64_t cuda_stream);
 KQ_API int kq_sync(kq_ctx* ctx);
 

@@ -16,7 +16,8 @@ using kq::Weight;
 
 struct kq_ctx {
   int device = 0;
-  cudaStream_t own_stream = nullptr;
+  cudaStream_t own_stream = nullptr;     // waits for the legacy default stream, and that one for it
+  cudaStream_t record_stream = nullptr;  // what the own stream would run goes here while a graph is recorded
   cudaStream_t stream = nullptr;
   bool overlap = true;
   bool capturing = false;
@@ -496,7 +497,11 @@ int kq_init(int device, uint64_t workspace_bytes, kq_ctx** out) {
   ctx->sm_count = prop.multiProcessorCount;
   ctx->workspace_bytes = workspace_bytes ? workspace_bytes : (256ull << 20);
   ctx->counter_count = 8192;
-  e = cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking);
+  // A host that works on the default stream (torch does unless told otherwise) and hands its tensors to this library has no
+  // stream to install: 0 is the own one.  So the own stream is of the kind that is ordered with the default one on both sides.
+  // Such a stream cannot be recorded while others use the default stream; that goes to one of the other kind.
+  e = cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamDefault);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&ctx->record_stream, cudaStreamNonBlocking);
   if (e == cudaSuccess) e = cudaMalloc(&ctx->workspace, ctx->workspace_bytes);
   if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&ctx->counters), ctx->counter_count * sizeof(unsigned int));
   if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, ctx->counter_count * sizeof(unsigned int));
@@ -544,6 +549,7 @@ void kq_destroy(kq_ctx* ctx) {
   if (ctx->ev_start) cudaEventDestroy(ctx->ev_start);
   if (ctx->ev_stop) cudaEventDestroy(ctx->ev_stop);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
+  if (ctx->record_stream) cudaStreamDestroy(ctx->record_stream);
   delete ctx;
 }
 
@@ -931,7 +937,9 @@ int kq_graph_begin(kq_ctx* ctx) {
   if (!ctx) return KQ_ERR_BAD_ARG;
   if (ctx->capturing || ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_graph_begin: a recording is already open");
   DeviceGuard guard(ctx->device);
-  KQ_CUDA(ctx, cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal));
+  const cudaStream_t on = ctx->stream == ctx->own_stream ? ctx->record_stream : ctx->stream;
+  KQ_CUDA(ctx, cudaStreamBeginCapture(on, cudaStreamCaptureModeThreadLocal));
+  ctx->stream = on;
   ctx->capturing = true;
   ctx->capture_mark = ctx->launches;
   return KQ_OK;
@@ -942,8 +950,10 @@ int kq_graph_end(kq_ctx* ctx, kq_graph* out) {
   if (!ctx->capturing) return fail(ctx, KQ_ERR_STATE, "kq_graph_end without kq_graph_begin");
   DeviceGuard guard(ctx->device);
   ctx->capturing = false;
+  const cudaStream_t recorded = ctx->stream;
+  if (recorded == ctx->record_stream) ctx->stream = ctx->own_stream;
   cudaGraph_t graph = nullptr;
-  KQ_CUDA(ctx, cudaStreamEndCapture(ctx->stream, &graph));
+  KQ_CUDA(ctx, cudaStreamEndCapture(recorded, &graph));
   cudaGraphExec_t exec = nullptr;
   cudaError_t e = cudaGraphInstantiate(&exec, graph, 0);
   cudaGraphDestroy(graph);

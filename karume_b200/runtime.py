@@ -162,7 +162,11 @@ def _rows(t, heads: int, dim: int, name: str):
 
 
 class Gpu:
-    """One CUDA device = one libkq context (the reference's GpuContext)."""
+    """One CUDA device = one libkq context (the reference's GpuContext).
+
+    Calls run on the stream that was torch's current one when the context was made, or that use_stream() installed since.
+    Where that is torch's default stream (or with use_torch_stream=False) they run on the library's own, which waits for the default
+    stream and which the default stream waits for.  Work on any other stream is in no order with the calls: install it first."""
 
     def __init__(self, device: int = 0, workspace_bytes: int = 0, use_torch_stream: bool = True):
         torch = _torch()
