@@ -444,6 +444,7 @@ class Gpu:
         need = int(L.kq_cache_bytes(pages, page_tokens, kv_heads, head_dim))
         if pool is None:
             pool = torch.zeros((pages, kv_heads, need // max(1, pages * kv_heads)), dtype=torch.uint8, device=self.device)
+            torch.cuda.current_stream(self.device).synchronize()  # the first append may run on another stream than torch's current one
         if pool.dtype != torch.uint8 or not pool.is_cuda or not pool.is_contiguous() or pool.numel() < need:
             raise KqError(2, f"the pool must be {need} bytes of contiguous CUDA uint8 memory")
         handle = ctypes.c_uint64(0)

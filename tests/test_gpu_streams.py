@@ -125,3 +125,20 @@ def test_linears_beside_the_default_stream(gpu):
         torch.cuda.synchronize()
         assert torch.equal(seen, want)
     w.free()
+
+
+def test_a_pool_made_on_another_stream_is_there_before_its_first_row(gpu):
+    import karume_b200 as kb
+    k = torch.randn(1, 2, 128, device="cuda")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = kb.CacheBatch(i32([0]), i32(1))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda._sleep(LONG)
+        cache = gpu.kv_cache(1, 64, 2, 128)
+    gpu.cache_append(cache, k, k, batch)
+    torch.cuda.synchronize()
+    held, _ = gpu.cache_read(cache, batch)
+    gpu.sync()
+    assert float((held - k).abs().max()) < 0.5  # a step of these rows is about a third
+    cache.free()
