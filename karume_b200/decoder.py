@@ -30,13 +30,15 @@ class DecoderShape:
 
 class Decoder:
     """`weights` maps "embedding", "head" and "{layer}.{q,k,v,o,gate,up,down}" to resident weights, `norms` "{layer}.1",
-    "{layer}.2" and "final" to f32 tensors [hidden].  Up to `sequences` conversations of up to `longest` tokens; the context
-    must run on a stream of its own or torch's current one (not the legacy default stream, which cannot be recorded)."""
+    "{layer}.2" and "final" to f32 tensors [hidden].  Up to `sequences` conversations of up to `longest` tokens.  Calls are made
+    with torch on the context's stream (on its default one if the context has its own), which is checked: lengths, ids and what
+    a prompt's layers work in are torch's, and nothing else orders the two."""
 
     def __init__(self, gpu: Gpu, shape: DecoderShape, weights: dict, norms: dict, rope: Rope, sequences: int, longest: int,
                  page_tokens: int = 64, window: int = 0):
         import torch
         self.torch, self.gpu, self.shape, self.weights, self.norms, self.rope, self.window = torch, gpu, shape, weights, norms, rope, window
+        self._check_stream()
         width = (longest + page_tokens - 1) // page_tokens
         if longest > rope.positions:
             raise KqError(2, f"the rotation table has {rope.positions} positions, sequences may have {longest}")
@@ -49,6 +51,10 @@ class Decoder:
         self._step = None
         self._step_batch = CacheBatch(self.pages, self.lengths)
         self._step_buffers = self._buffers(sequences)
+
+    def _check_stream(self) -> None:
+        if int(self.torch.cuda.current_stream(self.gpu.device).cuda_stream) != self.gpu.stream:
+            raise KqError(8, "torch's current stream is not the context's: install it with use_stream(), or make the call under the context's")
 
     def _buffers(self, rows: int):
         s, dev = self.shape, self.gpu.device
@@ -87,6 +93,7 @@ class Decoder:
         """Takes `news[b]` more tokens of each sequence b (0: none), packed in `ids` (CUDA int32); returns the logits of each
         sequence's last row [sequences, vocab] (of the rows in front of it where it has none)."""
         torch = self.torch
+        self._check_stream()
         if len(news) != len(self.held) or sum(news) != ids.numel() or ids.numel() == 0:
             raise KqError(2, f"{sum(news)} new tokens announced, {ids.numel()} given")
         if any(n + h > self.longest for n, h in zip(news, self.held)):
@@ -101,6 +108,7 @@ class Decoder:
     def step(self):
         """One token of every sequence, from self.ids (CUDA int32 [sequences]); returns the logits, a buffer that the next
         step writes again."""
+        self._check_stream()
         if any(h + 1 > self.longest for h in self.held):
             raise KqError(2, f"a sequence would grow beyond {self.longest} tokens")
         if self._step is None:

@@ -180,6 +180,7 @@ class Gpu:
             raise KqError(rc, (L.kq_last_error(None) or b"").decode())
         self._ctx = ctx
         self._ctx_addr = ctx.value
+        self.stream = 0  # handle of the stream the calls run on; 0: the library's own
         _load_fast()
         if use_torch_stream:
             self.use_stream(torch.cuda.current_stream(self.device))
@@ -196,7 +197,9 @@ class Gpu:
             raise KqError(rc, (L.kq_last_error(self._ctx) or b"").decode())
 
     def use_stream(self, stream) -> None:
-        self._check(L.kq_set_stream(self._ctx, int(stream.cuda_stream) if stream is not None else 0))
+        handle = int(stream.cuda_stream) if stream is not None else 0
+        self._check(L.kq_set_stream(self._ctx, handle))
+        self.stream = handle
 
     def set_overlap(self, enabled: bool) -> None:
         self._check(L.kq_set_overlap(self._ctx, 1 if enabled else 0))

@@ -142,3 +142,46 @@ def test_a_pool_made_on_another_stream_is_there_before_its_first_row(gpu):
     gpu.sync()
     assert float((held - k).abs().max()) < 0.5  # a step of these rows is about a third
     cache.free()
+
+
+def test_a_decoder_on_the_default_stream_and_refused_on_another(gpu):
+    import os
+    import sys
+    import karume_b200 as kb
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    from generate import small_decoder
+    rng = np.random.default_rng(3)
+    ids = torch.from_numpy(rng.integers(0, 1024, 90).astype(np.int32)).cuda()
+    ones = [torch.from_numpy(rng.integers(0, 1024, 3).astype(np.int32)).cuda() for _ in range(3)]
+
+    def logits_of(d, busy):
+        got = []
+        if busy:
+            torch.cuda._sleep(LONG)
+        got.append(d.prompt(ids + 0, [70, 3, 17]) + 0)
+        for more in ones:
+            if busy:
+                torch.cuda._sleep(LONG // 4)
+            d.ids.copy_(more)
+            got.append(d.step() + 0)
+        torch.cuda.synchronize()
+        assert d.lengths.tolist() == d.held == [73, 6, 20]
+        return got
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        apart = kb.acquire_gpu(0)
+        d = small_decoder(apart, layers=2)
+        want = logits_of(d, False)
+        d.close()
+    apart.destroy()
+    d = small_decoder(gpu, layers=2)
+    assert all(torch.equal(a, b) for a, b in zip(logits_of(d, True), want))
+    with torch.cuda.stream(side):
+        for call in (lambda: d.prompt(ids, [70, 3, 17]), d.step, lambda: small_decoder(gpu, layers=1)):
+            with pytest.raises(kb.KqError) as e:
+                call()
+            assert e.value.status == "KQ_ERR_STATE"
+    assert d.held == [73, 6, 20]
+    d.close()
