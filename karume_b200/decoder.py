@@ -11,6 +11,7 @@ lengths advancing on the device.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass
 
 from .runtime import CacheBatch, Gpu, KqError, Rope
@@ -56,6 +57,31 @@ class Decoder:
         if int(self.torch.cuda.current_stream(self.gpu.device).cuda_stream) != self.gpu.stream:
             raise KqError(8, "torch's current stream is not the context's: install it with use_stream(), or make the call under the context's")
 
+    @contextmanager
+    def _lengths_kept(self):
+        """Where a call fails, the sequences are as long as before; rows that it appended lie behind their ends."""
+        try:
+            yield
+        except BaseException:
+            self.lengths.copy_(self.torch.tensor(self.held, dtype=self.torch.int32))
+            raise
+
+    def _record(self) -> None:
+        self.logits = self.torch.empty((len(self.held), self.shape.vocab), device=self.gpu.device)
+        enqueue = lambda: self._head(self._layers(self._step_buffers, self.ids, self._step_batch), self.logits)  # noqa: E731
+        # once outside the recording, so that scratch has its size: over idle sequences, which changes no page
+        self.lengths.zero_()
+        enqueue()
+        self.gpu.sync()
+        self.gpu.graph_begin()
+        try:
+            enqueue()
+        except BaseException:
+            self.gpu.graph_free(self.gpu.graph_end())  # the context records no longer
+            raise
+        self._step = self.gpu.graph_end()
+        self.lengths.copy_(self.torch.tensor(self.held, dtype=self.torch.int32))
+
     def _buffers(self, rows: int):
         s, dev = self.shape, self.gpu.device
         sizes = dict(x=s.hidden, h=s.hidden, q=s.heads * s.head_dim, k=s.kv_heads * s.head_dim, v=s.kv_heads * s.head_dim,
@@ -98,12 +124,15 @@ class Decoder:
             raise KqError(2, f"{sum(news)} new tokens announced, {ids.numel()} given")
         if any(n + h > self.longest for n, h in zip(news, self.held)):
             raise KqError(2, f"a sequence would grow beyond {self.longest} tokens")
-        self.held = [n + h for n, h in zip(news, self.held)]
+        held = [n + h for n, h in zip(news, self.held)]
         starts = torch.tensor([0] + list(news)).cumsum(0).to(torch.int32).to(self.gpu.device)
-        self.lengths.copy_(torch.tensor(self.held, dtype=torch.int32))
-        hidden = self._layers(self._buffers(ids.numel()), ids, CacheBatch(self.pages, self.lengths, starts, tokens=ids.numel(), most=max(news)))
-        last = (starts[1:] - 1).clamp(min=0).long()
-        return self._head(hidden[last].contiguous())
+        with self._lengths_kept():
+            self.lengths.copy_(torch.tensor(held, dtype=torch.int32))
+            hidden = self._layers(self._buffers(ids.numel()), ids, CacheBatch(self.pages, self.lengths, starts, tokens=ids.numel(), most=max(news)))
+            last = (starts[1:] - 1).clamp(min=0).long()
+            logits = self._head(hidden[last].contiguous())
+        self.held = held
+        return logits
 
     def step(self):
         """One token of every sequence, from self.ids (CUDA int32 [sequences]); returns the logits, a buffer that the next
@@ -111,20 +140,12 @@ class Decoder:
         self._check_stream()
         if any(h + 1 > self.longest for h in self.held):
             raise KqError(2, f"a sequence would grow beyond {self.longest} tokens")
-        if self._step is None:
-            b = self._step_buffers
-            self.logits = self.torch.empty((len(self.held), self.shape.vocab), device=self.gpu.device)
-            # once outside the recording, so that scratch has its size: over idle sequences, which changes no page
-            self.lengths.zero_()
-            self._head(self._layers(b, self.ids, self._step_batch), self.logits)
-            self.gpu.sync()
-            self.gpu.graph_begin()
-            self._head(self._layers(b, self.ids, self._step_batch), self.logits)
-            self._step = self.gpu.graph_end()
-            self.lengths.copy_(self.torch.tensor(self.held, dtype=self.torch.int32))
+        with self._lengths_kept():
+            if self._step is None:
+                self._record()
+            self.lengths += 1
+            self.gpu.graph_launch(self._step)
         self.held = [h + 1 for h in self.held]
-        self.lengths += 1
-        self.gpu.graph_launch(self._step)
         return self.logits
 
     def close(self) -> None:
