@@ -120,8 +120,10 @@ class Decoder:
         sequence's last row [sequences, vocab] (of the rows in front of it where it has none)."""
         torch = self.torch
         self._check_stream()
-        if len(news) != len(self.held) or sum(news) != ids.numel() or ids.numel() == 0:
-            raise KqError(2, f"{sum(news)} new tokens announced, {ids.numel()} given")
+        if len(news) != len(self.held) or min(news) < 0 or sum(news) != ids.numel() or ids.numel() == 0:
+            raise KqError(2, f"{list(news)} new tokens announced for {len(self.held)} sequences, {ids.numel()} given")
+        if ids.dtype != torch.int32 or not ids.is_cuda or not ids.is_contiguous():
+            raise KqError(2, "ids must be a contiguous CUDA int32 tensor")
         if any(n + h > self.longest for n, h in zip(news, self.held)):
             raise KqError(2, f"a sequence would grow beyond {self.longest} tokens")
         held = [n + h for n, h in zip(news, self.held)]

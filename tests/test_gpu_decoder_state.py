@@ -21,6 +21,17 @@ def tokens(n, seed=0):
     return torch.from_numpy(np.random.default_rng(seed).integers(0, 1024, n).astype(np.int32)).cuda()
 
 
+def test_a_prompt_that_is_refused(gpu):  # noqa: F811
+    import karume_b200 as kb
+    d = small(gpu)
+    for ids, news in ((tokens(4), [-1, 3, 2]), (tokens(4), [1, 1, 1]), (tokens(2), [1, 1]), (tokens(600), [600, 0, 0]), (tokens(3).long(), [1, 1, 1]),
+                      (tokens(3).cpu(), [1, 1, 1]), (tokens(0), [0, 0, 0])):
+        with pytest.raises(kb.KqError) as e:
+            d.prompt(ids, news)
+        assert e.value.status == "KQ_ERR_SHAPE" and d.held == d.lengths.tolist() == [0, 0, 0]
+    d.close()
+
+
 def test_calls_that_fail_leave_the_sequences_as_they_were(gpu, monkeypatch):  # noqa: F811
     """The head's weight is missing: behind all layers, in a prompt, outside and inside the recording of a step."""
     a, b = small(gpu), small(gpu)
