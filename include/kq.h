@@ -354,9 +354,9 @@ KQ_API int kq_rope(kq_ctx* ctx, uint64_t x_dptr, int x_dtype, uint32_t tokens, u
  * (64, 128 or 256) values, a key after its rotation, is held as
  *   offset = f16(min x), scale = max(f16((max x - offset) * f32(1 / 15)), 0)
  *   code = clamp(round_ties_even((x - offset) * (1 / scale)), 0, 15), 0 where scale is 0
- * (f32 operations, each rounded) and stands for fround(code * scale + offset).  A row with a NaN or infinity,
- * or beyond binary16's range, is held as NaN.  The handle keeps the pool's address and shape, nothing else:
- * freeing it leaves the pool. */
+ * (f32 operations, each rounded) and stands for fround(code * scale + offset), which reaches beyond binary16.
+ * A row with a NaN or infinity, or whose offset or scale rounds beyond binary16's range, is held as NaN.  The
+ * handle keeps the pool's address and shape, nothing else: freeing it leaves the pool. */
 typedef uint64_t kq_cache; /* opaque handle, 0 is never valid */
 KQ_API uint64_t kq_cache_bytes(uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim);
 KQ_API int kq_cache_create(kq_ctx* ctx, uint64_t pool_dptr, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads,

@@ -20,7 +20,8 @@
 // tile's way 4, output 5.9 (2.4 since it leaves in whole rows: 305 -> 293 us), the next CTA's start 1.8), three to four times an SM; the last CTAs end 27 us after the mean one.
 // Three f32 prompts of up to 777 tokens behind 724, 12 heads over 2: 67 us, four products for one.
 //
-//   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights).
+//   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights); rows beyond
+//                   binary16's range to a sixteenth of it, which scores and weights make up for.
 //   f32 queries     codes enter exactly, around zero: (2 u - 15) 2^-24 and (u - 7.5) 2^-20, one operation from the subnormals that
 //                   their bits already are; scale and offset are applied to the scores and weights in f32.  Queries and weights are
 //                   two binary16 parts each (fixed-point: sums of high parts are exact), 22 bits and more.
@@ -64,8 +65,9 @@ struct Many {
   static constexpr int kTable = kRaw + kRaws * kRawBytes;
   static constexpr int kTableBytes = (kSplit ? 4 : 2) * kKeys * 4;
   static constexpr int kRows = kTable + 2 * kTableBytes;   // [kBlock] (factor, sum, last key, first key)
-  static constexpr int kLost = kRows + kBlock * 16;        // [2] 128 bits: tokens whose value is NaN
-  static constexpr int kBinade = kLost + 32;               // [2][4]: f32: the largest of 32 values' scales (2^13 scale)
+  // [2][3] 128 bits: values that are not finite, or stand for sixteen times what was unpacked; which of these are the latter; keys that are
+  static constexpr int kRare = kRows + kBlock * 16;
+  static constexpr int kBinade = kRare + 96;               // [2][4]: f32: the largest of 32 values' scales (2^13 scale)
   static constexpr int kHalves = kBinade + 32;             // f32: [2][2][128] (largest score, largest scale) of each half of a row's keys
   static constexpr int kBars = kHalves + (kSplit ? 2 * 2 * 128 * 8 : 0);
   static constexpr int kMisc = kBars + kBarCount * 8;
@@ -114,6 +116,10 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 }
 __device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t hadd2_bits(uint32_t a, uint32_t b) {
@@ -202,6 +208,28 @@ __device__ __noinline__ void scale_columns(uint32_t taddr, int n, float keep) {
     }
     tmem_st8(taddr + at, y);
     tmem_st8(taddr + at + 8, y + 8);
+  }
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// The thread's lane: scores (f32, a key a column) or weights (binary16, sixteen keys in eight columns of every sixteen) of the keys
+// in `keys` sixteen times as large.  Seldom run, as above.
+template <bool kHalves>
+__device__ __noinline__ void sixteenfold(uint32_t taddr, const uint32_t* keys) {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+  for (int at = 0; at < kKeys; at += 16) {
+    const uint32_t of = keys[at / 32] >> (at % 32);
+    float w[16];
+    tmem_ld16_begin(taddr + at, w);
+    tmem_ld16_done(w);
+    uint32_t y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t two = of >> (2 * i % 16);
+      const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w[i]), __floats2half2_rn(two & 1 ? 16.0f : 1.0f, two & 2 ? 16.0f : 1.0f));
+      y[i] = kHalves ? *reinterpret_cast<const uint32_t*>(&h) : __float_as_uint(of >> i & 1 ? w[i] * 16.0f : w[i]);
+    }
+    tmem_st8(taddr + at, y);
+    if constexpr (!kHalves) tmem_st8(taddr + at + 8, y + 8);
   }
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -692,7 +720,8 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       // So that M's move is seen before anything is written, a few scores are looked at at a time; what was written of the tile before
       // is then scaled too.
       constexpr int kN = F::kAtOnce;
-      constexpr float kLift = 6.0f, kLag = 8.0f;
+      // The largest weight is 2^(kLift + kLag), and sixteen times that stays below 2^16.
+      constexpr float kLift = 3.0f, kLag = 8.0f;
       const uint32_t t_s = tmem + lanes + wg * 128, t_o = tmem + lanes + 256 + wg * 128;
       for (int j = 0; j < tiles; ++j) {
         const int first = (tile0 + j) * kKeys;
@@ -756,13 +785,17 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             });
           }
         };
+        const uint4 big = *reinterpret_cast<const uint4*>(smem + F::kRare + (j & 1) * 48 + 32);  // (this look and that at `rare`: 4096 new tokens 304 us, without them 300)
+        if (big.x | big.y | big.z | big.w) sixteenfold<false>(t_s, reinterpret_cast<const uint32_t*>(smem + F::kRare + (j & 1) * 48 + 32));
         if (whole) tile(std::true_type());
         else tile(std::false_type());
-        const uint4 lost = *reinterpret_cast<const uint4*>(smem + F::kLost + (j & 1) * 16);
-        if (lost.x | lost.y | lost.z | lost.w) {  // values that are NaN entered as zeros: whoever sees one is NaN
-          const uint32_t bits[4] = {lost.x, lost.y, lost.z, lost.w};
+        const uint4 rare = *reinterpret_cast<const uint4*>(smem + F::kRare + (j & 1) * 48);
+        if (rare.x | rare.y | rare.z | rare.w) {
+          const uint32_t* const bits = reinterpret_cast<const uint32_t*>(smem + F::kRare) + (j & 1) * 12;
+          sixteenfold<true>(t_s, bits + 4);
+          // values that are not finite entered as zeros: whoever sees one is NaN
           for (int i = max(sees0, 0); i <= min(sees1, kKeys - 1); ++i)
-            if (bits[i / 32] >> (i % 32) & 1) l = quiet_nan();
+            if ((bits[i / 32] & ~bits[4 + i / 32]) >> (i % 32) & 1) l = quiet_nan();
           __syncwarp();
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -897,12 +930,21 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             const uint32_t big = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v.x, 0.0f)));  // not NaN
             if (lane == 0) reinterpret_cast<float*>(smem + F::kBinade)[(j & 1) * 4 + w4] = __uint_as_float(big) * 8192.0f;
           } else {
-            // the largest value must stay finite in binary16: a scale that was rounded up gives one unit back
-            if (fmaf(15.0f, k.x, k.y) >= 65520.0f) kp -= 1;
-            if (fmaf(15.0f, v.x, v.y) >= 65520.0f) vp -= 1;
-            const uint32_t lost = __ballot_sync(0xffffffffu, v.x != v.x || v.y != v.y);
-            if (lane == 0) reinterpret_cast<uint32_t*>(smem + F::kLost)[(j & 1) * 4 + w4] = lost;
-            if (v.x != v.x || v.y != v.y) vp = 0;
+            // A row stands for up to 16 * 65504.  Where that rounds to an infinity in binary16 (its scale is one at least then),
+            // a sixteenth is unpacked, and the softmax warps put it right in the key's score or the value's weight.
+            constexpr float kLargest = 65504.0f, kBeyond = 65520.0f;
+            const bool not_finite = !(fabsf(v.x) <= kLargest && fabsf(v.y) <= kLargest);
+            const bool k_big = fabsf(fmaf(15.0f, k.x, k.y)) >= kBeyond, v_big = !not_finite && fabsf(fmaf(15.0f, v.x, v.y)) >= kBeyond;
+            const uint32_t lost = __ballot_sync(0xffffffffu, not_finite), big_keys = __ballot_sync(0xffffffffu, k_big), big_values = __ballot_sync(0xffffffffu, v_big);
+            if (lane == 0) {
+              uint32_t* const rare = reinterpret_cast<uint32_t*>(smem + F::kRare) + (j & 1) * 12 + w4;
+              rare[0] = lost | big_values;
+              rare[4] = big_values;
+              rare[8] = big_keys;
+            }
+            if (k_big) kp = hmul2_bits(kp, k16th);
+            if (v_big) vp = hmul2_bits(vp, k16th);
+            if (not_finite) vp = 0;
             k_par[t] = kp;
             v_scale[t] = __ushort_as_half(static_cast<unsigned short>(vp));
             v_offset[t] = __ushort_as_half(static_cast<unsigned short>(vp >> 16));
@@ -1138,7 +1180,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
 template <typename T, int D>
 cudaError_t many_as(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond) {
   using F = Many<T, D>;
-  static_assert(F::kSmem <= 227 * 1024 && F::kTable % 16 == 0 && F::kRows % 16 == 0 && F::kLost % 16 == 0 && F::kBars % 8 == 0 && F::kRawParams % 16 == 0 && F::kRawBytes % 16 == 0,
+  static_assert(F::kSmem <= 227 * 1024 && F::kTable % 16 == 0 && F::kRows % 16 == 0 && F::kRare % 16 == 0 && F::kBars % 8 == 0 && F::kRawParams % 16 == 0 && F::kRawBytes % 16 == 0,
                 "shared memory and the alignment of its arrays");
   static OncePerDevice once;
   cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_many_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem); });

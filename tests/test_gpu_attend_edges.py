@@ -30,3 +30,68 @@ def test_scores_that_climb_inside_a_tile(gpu, kind, dim, period):  # noqa: F811
     f.check(kind, [100], 4, q_spread=2.0, window=150)
     f.check(kind, [1], 4, q_spread=2.0)
     f.free()
+
+
+def check_within_range(f, kind, new, heads, window=0, q_spread=1.0):
+    """Filled.check for one sequence whose results may leave binary16: both sides end at its largest number there."""
+    import karume_b200 as kb
+    gen = torch.Generator(device="cuda").manual_seed(heads + new)
+    q = (torch.randn(new, heads, f.dim, generator=gen, device="cuda") * q_spread).to(ref.TYPES[kind])
+    batch = kb.CacheBatch(f.pages, f.length, dev(np.array([0, new], np.int32)), tokens=new)
+    got = f.gpu.cache_attention(f.cache, q, batch, window=window)
+    f.gpu.sync()
+    want, reach, largest = ref.attend(q.double(), f.k.double(), f.v.double(), f.dim ** -0.5, window)
+    allowed, got = ref.allowed(kind, want, reach, largest), got.double()
+    assert not bool(torch.isnan(got).any())
+    if kind == "f16":
+        got, want = got.clamp(-65504, 65504), want.clamp(-65504, 65504)
+    off = (got - want).abs()
+    assert bool((off <= allowed).all()), (kind, new, window, float((off / allowed).max()))
+
+
+@KINDS
+@pytest.mark.parametrize("which", ["keys", "values", "both"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_that_stand_for_more_than_binary16(gpu, kind, which, dim):  # noqa: F811
+    """A row's offset and scale are binary16, what it stands for reaches beyond: rows up to 1e5 and 9e5 among ordinary ones, for who
+    sees them and who does not."""
+    def large(f):
+        rng = np.random.default_rng(dim)
+        for at, low, high in ((150, -3e4, 1e5), (151, -65000.0, 66000.0), (300, -65504.0, 9e5), (301, -65504.0, 65530.0)):
+            for rows, wanted in ((f.k, which != "values"), (f.v, which != "keys")):
+                if wanted:
+                    row = rng.uniform(low, high, rows.shape[1:]).astype(np.float32)
+                    row[:, 3], row[:, dim - 2] = low, high
+                    rows[at] = torch.from_numpy(row).cuda()
+
+    f = Filled(gpu, [400], 64, 1, dim, seed=13, spread=0.3, rows=large)
+    assert float(f.v.abs().max()) > 8e5 or which == "keys"
+    q_spread = 0.999 if which == "values" else 1e-5
+    for new, window in ((400, 0), (100, 120), (1, 0)):
+        check_within_range(f, kind, new, 4, window, q_spread)
+    f.free()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_rows_of_infinities_reach_only_those_who_see_them(gpu, kind):  # noqa: F811
+    """A pool that a host filled itself may hold infinite scales and offsets: to who sees them nothing is promised, to others they
+    are nothing."""
+    import karume_b200 as kb
+    n, dim, page = 200, 128, 64
+    f = Filled(gpu, [n], page, 1, dim, seed=14)
+    pool, bad = f.cache.pool, 120
+    at = f.pages[0, bad // page].item()
+    params = pool[at, 0, page * dim:].view(torch.float16).view(2, page, 2)
+    clean = params[:, bad % page].clone()
+    q = torch.randn(n, 4, dim, device="cuda").to(ref.TYPES[kind])
+    batch = kb.CacheBatch(f.pages, f.length, dev(np.array([0, n], np.int32)), tokens=n)
+    want = gpu.cache_attention(f.cache, q, batch, window=50)
+    gpu.sync()
+    for scale, offset in ((math.inf, 0.0), (1.0, -math.inf), (-math.inf, math.inf)):
+        params[:, bad % page] = torch.tensor([scale, offset], dtype=torch.float16, device="cuda")
+        got = gpu.cache_attention(f.cache, q, batch, window=50)
+        gpu.sync()
+        assert torch.equal(got[:bad], want[:bad]) and torch.equal(got[bad + 50:], want[bad + 50:])
+        assert not bool(torch.isfinite(got[bad:bad + 50]).all(-1).any())
+    params[:, bad % page] = clean
+    f.free()
