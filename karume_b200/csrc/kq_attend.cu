@@ -409,30 +409,30 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       const float (&v)[8] = loaded[i_row];
       float big = 0.0f, sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        big = fmaxf(big, fabsf(v[i]));
-        sum += v[i];
-      }
+      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(v[i]));
 #pragma unroll
       for (int o = 16; o > 0; o /= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-      sum = warp_sum(sum);
       // 2^(13 - exponent of the largest): all below 2^14
       const int e = static_cast<int>(__float_as_uint(big) >> 23);
       const int up = big > 0.0f && e < 255 ? min(max(140 - e, -100), 120) : 0;
       const float lift = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+      __half hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = v[i] * lift, down = (i & 1) ? 0.0625f : 1.0f;
+        // f32: fixed-point parts, multiples of 8 and of 2^-8.  Their products with codes are whole multiples too, 22 bits in
+        // all of a row, so that the tensor core (which cuts each product at a place set by the largest) adds them exactly
+        const float top = kSplit ? rintf(x * 0.125f) * 8.0f : x;
+        hi[i] = __float2half_rn(top * down);
+        lo[i] = kSplit ? __float2half_rn(rintf((x - top) * 256.0f) * (0.00390625f * down)) : __ushort_as_half(0);
+        // The offsets meet the queries as they were rounded, like the codes: a rounding then weighs as much as the key, not as the code
+        // times its scale, which in a row with one large value is large everywhere.
+        sum = fmaf(__half2float(hi[i]) + __half2float(lo[i]), (i & 1) ? 16.0f : 1.0f, sum);
+      }
+      sum = warp_sum(sum) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
       if (lane < D / 8) {
         // word W = lane of a key lies with thread tt as its word ww
         const uint32_t tt = D == 64 ? lane / 2 : lane % 16 / 4, ww = D == 64 ? lane % 2 : lane / 16 * 4 + lane % 4;
-        __half hi[8], lo[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x = v[i] * lift, down = (i & 1) ? 0.0625f : 1.0f;
-          // f32: fixed-point parts, multiples of 8 and of 2^-8.  Their products with codes are whole multiples too, 22 bits in
-          // all of a row, so that the tensor core (which cuts each product at a place set by the largest) adds them exactly
-          const float top = kSplit ? rintf(x * 0.125f) * 8.0f : x;
-          hi[i] = __float2half_rn(top * down);
-          lo[i] = kSplit ? __float2half_rn(rintf((x - top) * 256.0f) * (0.00390625f * down)) : __ushort_as_half(0);
-        }
 #pragma unroll
         for (int part = 0; part < (kPair ? 2 : 1); ++part) {
           const uint32_t col = r * (kPair ? 2 : 1) + part, n = col / 8, c = col % 8;

@@ -459,15 +459,16 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     constexpr float kEight = 100663296.0f;  // 1.5 2^26: numbers beside it are multiples of eight
     const float top = __fsub_rn(__fadd_rn(x, kEight), kEight), down = odd ? 0.125f : 1.0f;
     hi = top * down;
-    lo = (x - top) * down;
+    lo = __half2float(__float2half_rn((x - top) * down));
   };
   const auto row_constants = [&](uint32_t r, int up, float sum) {
     const float factor = p.a.scale * 1.4426950408889634f;
     const bool there = row0 + static_cast<int>(r) < n_rows;
     const int last = there ? before + query_and_head(static_cast<int>(r)).x : 0x7fffffff;  // rows beyond the end see anything and are not stored
     const int from = there && window && last + 1 > window ? last + 1 - window : 0;
-    // f32: score = factor 2^(23 - up) (acc scale + centre sum 2^(up - 23))
-    rows[r] = kSplit ? make_float4(factor * power(23 - up), sum * power(up - 23), __int_as_float(last), __int_as_float(from))
+    // f32: score = factor 2^(23 - up) (acc scale + centre sum 2^-23), the sum of the lifted parts as they are multiplied: a rounding
+    // then weighs as much as the key, not as the code times its scale, which in a row with one large value is large everywhere
+    rows[r] = kSplit ? make_float4(factor * power(23 - up), sum * power(-23), __int_as_float(last), __int_as_float(from))
                      : make_float4(factor * power(-up), 0.0f, __int_as_float(last), __int_as_float(from));
   };
   if (rope_is_plain(p.a.rope) && p.a.rope.rotary == D) {
@@ -503,20 +504,24 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
         for (int i = 0; i < 4; ++i) {
           v[i] = there ? v[i] : 0.0f;
           big = fmaxf(big, fabsf(v[i]));
-          sum += v[i];
         }
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o /= 2) {
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-          if constexpr (kSplit) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
+        for (int o = kLanes / 2; o > 0; o /= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
         const int up = lift_of(big);
         const float lift = power(up);
         float hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (kSplit) parts_of(v[i] * lift, i & 1, hi[i], lo[i]);
-          else hi[i] = v[i] * lift;
+          if constexpr (kSplit) {
+            parts_of(v[i] * lift, i & 1, hi[i], lo[i]);
+            sum = fmaf(hi[i] + lo[i], (i & 1) ? 8.0f : 1.0f, sum);
+          } else {
+            hi[i] = v[i] * lift;
+          }
+        }
+        if constexpr (kSplit) {
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
@@ -545,20 +550,24 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       for (int i = 0; i < 8; ++i) {
         v[i] = there ? v[i] : 0.0f;
         big = fmaxf(big, fabsf(v[i]));
-        sum += v[i];
       }
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o /= 2) {
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      }
+      for (int o = kLanes / 2; o > 0; o /= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
       const int up = lift_of(big);
       const float lift = power(up);
       float hi[8], lo[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if constexpr (kSplit) parts_of(v[i] * lift, i & 1, hi[i], lo[i]);
-        else hi[i] = v[i] * lift;
+        if constexpr (kSplit) {
+          parts_of(v[i] * lift, i & 1, hi[i], lo[i]);
+          sum = fmaf(hi[i] + lo[i], (i & 1) ? 8.0f : 1.0f, sum);
+        } else {
+          hi[i] = v[i] * lift;
+        }
+      }
+      if constexpr (kSplit) {
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       }
       const uint32_t at = base + F::kQ + (r / 128) * kParts * F::kOperand + (c / 8) * 16384 + umma::swz(r % 128, c % 8);
       umma::sts128(at, make_uint4(half2_bits(hi[0], hi[4]), half2_bits(hi[1], hi[5]), half2_bits(hi[2], hi[6]), half2_bits(hi[3], hi[7])));

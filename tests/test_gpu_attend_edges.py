@@ -95,3 +95,33 @@ def test_rows_of_infinities_reach_only_those_who_see_them(gpu, kind):  # noqa: F
         assert not bool(torch.isfinite(got[bad:bad + 50]).all(-1).any())
     params[:, bad % page] = clean
     f.free()
+
+
+@KINDS
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_keys_with_one_large_value(gpu, kind, dim):  # noqa: F811
+    """A value far from a key's others makes code times scale as large in every dim. A rotated query that is rounded to binary16
+    must meet the offset as it was rounded: here all dims round the same way (an amplitude a little above one, as scalings for long
+    contexts have it), 2^-11 of the score and not of dim times as much."""
+    import karume_b200 as kb
+    n = 300
+
+    def outliers(f):
+        at = torch.arange(n, device="cuda")
+        f.k.zero_()
+        f.k[at, 0, (5 * at) % dim] = -0.8 * dim * torch.rand(n, generator=torch.Generator(device="cuda").manual_seed(dim), device="cuda")
+
+    f = Filled(gpu, [n], 64, 1, dim, seed=15, rows=outliers)
+    table = torch.zeros(n, dim // 2, 2, device="cuda")
+    table[..., 0] = 1 + 0.45 * 2.0 ** -10  # no angle
+    for new in (1, 5, 100):
+        q = torch.ones(new, 4, dim, device="cuda", dtype=ref.TYPES[kind])
+        batch = kb.CacheBatch(f.pages, f.length, dev(np.array([0, new], np.int32)), tokens=new)
+        got = gpu.cache_attention(f.cache, q, batch, rope=kb.Rope(table))
+        gpu.sync()
+        want, reach, largest = ref.attend(q.double() * table[0, 0, 0].double(), f.k.double(), f.v.double(), dim ** -0.5, 0)
+        off, allowed = (got.double() - want).abs(), ref.allowed(kind, want, reach, largest)
+        assert bool((off <= allowed).all()), (kind, new, float((off / allowed).max()))
+        # keys whose weights count have scores within a few of the largest: 2^-11 of that, and the bounds that Filled.check has
+        assert float(off.norm() / want.norm()) <= {"f32": 1e-5, "f16": 2e-3, "bf16": 5e-3}[kind], (kind, new, float(off.norm() / want.norm()))
+    f.free()
