@@ -127,9 +127,11 @@ class CacheBatch:
             raise KqError(2, f"{self.sequences} sequences need as many lengths and one more starts")
         if starts is not None and tokens <= 0:
             raise KqError(2, "with starts, tokens says how many rows there are")
+        if most < 0:
+            raise KqError(2, f"most {most}: a bound of a sequence's new tokens, 0 if not known")
         self.pages, self.lengths, self.starts = pages, lengths, starts
         self.tokens = int(tokens) if starts is not None else self.sequences
-        self.most = int(most) if starts is not None else 1
+        self.most = min(int(most), self.tokens) if starts is not None else 1
         self.args = (self.sequences, pages.data_ptr(), self.width, lengths.data_ptr(), starts.data_ptr() if starts is not None else 0,
                      self.tokens)
 
@@ -483,6 +485,9 @@ class Gpu:
         in the cache, the last `window` of them if given; scale defaults to head_dim^-0.5.  Returns q's type."""
         if scale is None:
             scale = cache.head_dim ** -0.5
+        if window < 0:
+            raise KqError(2, f"window {window}: a number of keys, 0 for all")
+        window = min(int(window), 0xFFFFFFFF)  # the ABI's number has 32 bits; no sequence is longer
         done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window,
                                      rope.args if rope is not None else None, out)
         if done is not None:
@@ -498,7 +503,7 @@ class Gpu:
             raise KqError(2, "out must have q's type and shape")
         po, out_stride = _rows(out, heads, dim, "out")
         self._check(L.kq_cache_attention(self._ctx, cache.handle, pq, q_stride, _tensor_dtype_code(q), heads, *batch.args, batch.most,
-                                         float(scale), int(window),
+                                         float(scale), window,
                                          *(rope.args if rope is not None else _NO_ROPE), po, out_stride))
         return out
 

@@ -125,3 +125,26 @@ def test_keys_with_one_large_value(gpu, kind, dim):  # noqa: F811
         # keys whose weights count have scores within a few of the largest: 2^-11 of that, and the bounds that Filled.check has
         assert float(off.norm() / want.norm()) <= {"f32": 1e-5, "f16": 2e-3, "bf16": 5e-3}[kind], (kind, new, float(off.norm() / want.norm()))
     f.free()
+
+
+def test_windows_beyond_32_bits_and_below_zero(gpu):  # noqa: F811
+    """A window is a number of keys: one that no sequence reaches hides nothing, whatever its low bits."""
+    import karume_b200 as kb
+    f = Filled(gpu, [300], 64, 1, 64, seed=16)
+    q = torch.randn(1, 4, 64, device="cuda")
+    one, many = kb.CacheBatch(f.pages, f.length), kb.CacheBatch(f.pages, f.length, dev(np.array([0, 40], np.int32)), tokens=40, most=(1 << 32) + 1)
+    for batch, rows in ((one, q), (many, torch.randn(40, 4, 64, device="cuda"))):
+        want = gpu.cache_attention(f.cache, rows, batch)
+        for window in ((1 << 32) + 5, 1 << 32, (1 << 32) - 1, 1 << 31, 1 << 70):
+            got = gpu.cache_attention(f.cache, rows, batch, window=window)
+            gpu.sync()
+            assert torch.equal(got, want), window
+        narrow = gpu.cache_attention(f.cache, rows, batch, window=np.int64(5))
+        gpu.sync()
+        assert not torch.equal(narrow, want)
+        with pytest.raises(kb.KqError) as e:
+            gpu.cache_attention(f.cache, rows, batch, window=-1)
+        assert e.value.status == "KQ_ERR_SHAPE"
+    with pytest.raises(kb.KqError):
+        kb.CacheBatch(f.pages, f.length, many.starts, tokens=40, most=-1)
+    f.free()
