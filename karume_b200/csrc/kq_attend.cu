@@ -616,7 +616,8 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) shift[n][i] = M[n][i] == -INFINITY ? 0.0f : -M[n][i];
-        const int up = kSplit ? min(max(14 - static_cast<int>(ceilf(top[n][0] + shift[n][0])), 0), 120) : 6;
+        // as numbers: a tile in which the row sees nothing has a largest score of -inf
+        const int up = kSplit ? static_cast<int>(fminf(fmaxf(14.0f - ceilf(top[n][0] + shift[n][0]), 0.0f), 120.0f)) : 6;
         lift[n] = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
         drop[n] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
       }
