@@ -491,12 +491,13 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
                        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
           if (!done && (spin & 1023u) == 1023u && *abort_flag) break;
         }
-        if (!done) {
+        if (!__all_sync(0xffffffffu, done)) {
           *abort_flag = 1;
           *reinterpret_cast<volatile int*>(p.status) = kFewTimeout;
+          waiting = false;  // nothing more is copied: the barrier's phase is not over, and may not be arrived on again
+          to_issue = 0;
         }
       }
-      __syncwarp();
       const uint8_t* tile = ring_ptr + stage * F::kTileBytes;
       const bool whole = first >= keys.first_all && first + kTile - 1 <= keys.last_all;
       float s[kSubs][NT][kPer][2];  // [subtile][..][row][token half]
