@@ -37,7 +37,7 @@ namespace {
 constexpr int kKeys = 128;    // of a tile
 constexpr int kManyTimeout = 50;
 
-enum Bar { kRawKFull, kRawKFree = 2, kRawVFull = 4, kRawVFree = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kSFull = 16, kPReady = 18, kOFull = 20, kLoaded = 21, kBarCount = 22 };
+enum Bar { kRawKFull, kRawKFree = 2, kRawVFull = 4, kRawVFree = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kSFull = 16, kPReady = 18, kOFull = 20, kLoaded = 21, kAllDone = 22, kBarCount = 23 };
 
 template <typename T, int D>
 struct Many {
@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       umma::mbar_init(bar(kOFull + i), kSplit && i == 1 ? 8 * kArrivals : 1);  // f32: one O; the second is kLoaded
       umma::mbar_init(bar(kPReady + i), (kSplit ? 8 : 4) * kArrivals);
     }
+    umma::mbar_init(bar(kAllDone), 1);
     *abort_flag = 0;
     found[0] = 0xFFFFFFFFu;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1120,6 +1121,10 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             }
           }
         }
+      }
+      if (__any_sync(0xffffffffu, *abort_flag)) {  // a wait gave up: none may outlive the tensor memory
+        umma::commit_one(leader, bar(kAllDone));
+        wait(kAllDone, 0);
       }
     } else if (warp == F::kCopyWarp) {
       // ---- copies --------------------------------------------------------------------------------------
