@@ -148,3 +148,49 @@ def test_windows_beyond_32_bits_and_below_zero(gpu):  # noqa: F811
     with pytest.raises(kb.KqError):
         kb.CacheBatch(f.pages, f.length, many.starts, tokens=40, most=-1)
     f.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [3, 80])
+def test_query_rows_more_than_4_gib_apart(gpu, kind, new):  # noqa: F811
+    import karume_b200 as kb
+    f = Filled(gpu, [100], 16, 1, 64, seed=17)
+    stride = (5 << 30) // (new - 1)  # bytes: the last row begins 5 GiB behind the first
+    stride -= stride % 16
+    store = torch.zeros(new * stride // 4, device="cuda").view(ref.TYPES[kind])
+    each = stride // store.element_size()
+    near = torch.randn(new, 4, 64, device="cuda").to(ref.TYPES[kind])
+    far = store.as_strided((new, 4, 64), (each, 64, 1))
+    far.copy_(near)
+    batch = kb.CacheBatch(f.pages, f.length, dev(np.array([0, new], np.int32)), tokens=new)
+    for rotary in (0, 64, 20):
+        rope = kb.Rope(dev(kb.rope_table(100, rotary))) if rotary else None
+        got, want = gpu.cache_attention(f.cache, far, batch, rope=rope), gpu.cache_attention(f.cache, near, batch, rope=rope)
+        gpu.sync()
+        assert torch.equal(got, want)
+    f.free()
+
+
+@KINDS
+@pytest.mark.parametrize("dim,mean", [(64, 0.0), (64, 3.0), (128, 3.0)])
+def test_long_sums_that_no_other_block_shares(gpu, kind, dim, mean):  # noqa: F811
+    """So many blocks of rows that each walks over all 70001 keys by itself, 16-bit sums in one chain of the tensor core's accumulators.
+    It cuts a sum at its last bit at every sixteen keys: 2^-23 of it each, all one way where the values have one sign. On top 16-bit
+    results have three roundings of binary16 (2.1e-4 each of the norm) and that of their type."""
+    import karume_b200 as kb
+    n, new, heads, last = 70001, 9600, 8, 40
+
+    def one_sign(f):
+        f.v += mean
+
+    f = Filled(gpu, [n], 64, heads, dim, seed=18, spread=0.3, rows=one_sign)
+    q = torch.randn(new, heads, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(dim)).to(ref.TYPES[kind])
+    got = gpu.cache_attention(f.cache, q, kb.CacheBatch(f.pages, f.length, dev(np.array([0, new], np.int32)), tokens=new))
+    gpu.sync()
+    want, reach, largest = ref.attend(q[-last:].double(), f.k.double(), f.v.double(), dim ** -0.5, 0)
+    off = (got[-last:].double() - want).abs()
+    assert bool((off <= ref.allowed(kind, want, reach, largest)).all())
+    chain = 0.0 if kind == "f32" else n / 16 * 2.0 ** -23
+    bound = {"f32": 1e-5, "f16": 6e-4, "bf16": 2e-3}[kind] + chain
+    assert float(off.norm() / want.norm()) <= bound, (kind, float(off.norm() / want.norm()), bound)
+    f.free()
