@@ -341,7 +341,11 @@ KQ_API int kq_linear_a8(kq_ctx* ctx, kq_weight w, uint64_t xq_i8_dptr, uint64_t 
  * in what it would have rotated, as kq_embedding does for its indices.
  *
  * kq_rope: x is [tokens, heads, head_dim] of x_dtype, consecutive tokens x_stride elements apart;
- * positions is i32 [tokens]; out has x's type and may be x. */
+ * positions is i32 [tokens]; out has x's type and may be x.  x and out need the alignment of their type,
+ * the table eight bytes (here and below).
+ *
+ * None of these calls can be part of a fused plan (KQ_ERR_STATE between kq_plan_begin and kq_plan_end):
+ * record them with kq_graph_begin. */
 enum kq_rope_flags { KQ_ROPE_INTERLEAVED = 1 };
 KQ_API int kq_rope(kq_ctx* ctx, uint64_t x_dptr, int x_dtype, uint32_t tokens, uint32_t heads, uint32_t head_dim,
                    uint64_t x_stride, uint64_t positions_dptr, uint64_t table_dptr, uint32_t table_positions,
@@ -373,6 +377,10 @@ KQ_API int kq_cache_free(kq_ctx* ctx, kq_cache cache);
  * and pages.  A page number outside the pool, or a token beyond table_width pages, is not written and reads as NaN;
  * a sequence may be idle (length 0).
  *
+ * Rows of k, v, q and out are read and written 16 bytes at a time: an address or a stride (in bytes) that is
+ * no multiple of 16, or a stride shorter than a row, is refused (KQ_ERR_BAD_ARG, KQ_ERR_SHAPE), as is a tensor of
+ * indices that is not 4-byte aligned.
+ *
  * kq_cache_append: k and v are [tokens, kv_heads, head_dim] of `dtype`, k_stride / v_stride elements apart
  * (columns of a fused projection); keys are rotated on the way (table_dptr == 0: not).  Two rows that name the
  * same page and slot race.
@@ -382,8 +390,9 @@ KQ_API int kq_cache_free(kq_ctx* ctx, kq_cache cache);
  *   out = sum_j softmax_j(scale * q . k_j) v_j   over the keys j in [window ? max(0, p - window + 1) : 0, p],
  * zeros where there is none.  q is [tokens, heads, head_dim] of q_dtype (heads a multiple of kv_heads; query
  * head h reads kv head h / (heads / kv_heads)), rotated on the way (table_dptr == 0: not); out has q's type.
- * Scores, softmax and sums are f32; f32 queries keep 22 bits or more through the tensor cores, 16-bit
- * ones are multiplied in binary16. */
+ * Scores, softmax and sums are f32; f32 queries keep 22 bits or more through the tensor cores.  For 16-bit ones
+ * rotated queries, weights and (prompts) the keys and values are rounded to binary16 where they are multiplied, and
+ * the sums of a prompt's rows are cut, not rounded, at their last bit at every sixteen keys. */
 KQ_API int kq_cache_append(kq_ctx* ctx, kq_cache cache, uint64_t k_dptr, uint64_t k_stride, uint64_t v_dptr,
                            uint64_t v_stride, int dtype, uint32_t sequences, uint64_t page_table_dptr,
                            uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,

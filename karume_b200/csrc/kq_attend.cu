@@ -14,7 +14,7 @@
 // parts in neighbouring columns (fixed-point, exact sums), and so are their weights; the parts' sums are added in f32.  The weights
 // get from S^T's fragment to the B fragment of P^T by one movmatrix a 8 x 8 block, nothing passes through shared memory.
 //
-//   score    s_j = scale log2(e) (s_j (q . u_j) + o_j sum q)            (base 2, f32)
+//   score    s_j = scale log2(e) (s_j (q . u_j) + o_j sum q)            (base 2, f32; the sum of q as it is multiplied)
 //   weight   p_j = 2^(s_j - M), and P = p_j s'_j (s' the value's scale) is what enters the tensor core.  M follows the
 //            largest s_j + log2 of s'_j's binade, and moves only when a weight would grow past 2^8 of it: P fits binary16
 //            with its full precision wherever it matters, whatever the size of the values.  16-bit queries round P to binary16
@@ -30,10 +30,11 @@
 // several CTAs share leaves partial sums in the scratch; the last CTA of sixteen neighbours joins theirs in order, the last of
 // those groups the groups'.
 //
-// What bounds it: instructions.  A code costs a masked shift, one operation around zero and its share of an MMA, a (row, key) pair an
-// exponential and some ten more; at 64 bfloat16 sequences of 32 heads over 8, up to 16384 tokens, 161 us (4.3 TB/s, issue slots 49 %,
-// DRAM 0.65 of the copy rate) it is these, not the bytes.  16 f32 sequences up to 8190 tokens: 32 us (2.6 TB/s); one sequence of
-// 200003, two kv heads: 27 us; one of 4096: 10.4 us, where the launch, the cut, the queries and the joining are most of it.
+// What bounds it: the latency of its own instructions.  A code costs a masked shift, one operation around zero and its share of an MMA, a
+// (row, key) pair an exponential and some ten more, and two warps a scheduler, which is what registers leave, do not hide how long
+// they take: at 64 bfloat16 sequences of 32 heads over 8, up to 16384 tokens, 160 us (4.3 TB/s, 0.65 of the copy rate), issue slots and the
+// fullest pipe are at 49 %.  16 f32 sequences up to 8190 tokens: 34 us (2.5 TB/s); one sequence of 200003, two kv heads: 29 us;
+// one of 4096: 10.3 us, where the launch, the cut, the queries and the joining are most of it.
 #include <algorithm>
 #include <type_traits>
 
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair>::kThreads, Few<T, D, NT, 
     const int4 v = spans[b];
     return Span{v.x, v.y, v.z};
   };
-  // Walk to tile number x; a run of up to kShort tiles is not cut but belongs to the range it begins in
+  // Walk to tile number x; a run of up to kShort tiles is not cut: a cut inside it moves to its beginning, so it is the later range's
   auto locate = [&](unsigned long long& x, int i) {
     Walk w;
     w.b = static_cast<uint32_t>(found[2 * i]);

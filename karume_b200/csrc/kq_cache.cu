@@ -5,8 +5,8 @@
 //   read    the f32 values that rows stand for
 //
 // All three are bound by memory: a value is read once and written once.  Measured: 8191 tokens of 32 heads of 128, bfloat16, half of
-// each head rotated, 32.7 us (4.2 TB/s; the latency of loads that depend on one another: position, angles, values); one token 3.4 us,
-// a launch.  Ten thousand rows appended and read back, 14.8 us; one row each of 64 sequences 7.7 us, two launches.
+// each head rotated, 32.7 us (4.2 TB/s; the latency of loads that depend on one another: position, angles, values); one token 3.2 us,
+// a launch.  Ten thousand rows appended and read back, 14.8 us; one row each of 64 sequences 7.2 us, two launches.
 #include <algorithm>
 
 #include "kq_cache.cuh"
