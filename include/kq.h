@@ -406,6 +406,40 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
                               uint32_t window, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary,
                               uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride);
 
+/* ---- pages that sequences share ---------------------------------------------------------------
+ * Who has which page of a pool, for hosts whose sequences begin alike, branch, are cut back and end.  A book of pages is
+ * four device arrays of i32, the host's own:
+ *   table   [sequences, width]  each sequence's pages in token order, -1 behind them: a page_table of the calls above
+ *   lengths [sequences]         its tokens; ceil(length / page_tokens) of its row's entries are pages
+ *   refs    [pages]             how many entries name a page; 0: it is free
+ *   report  [4]                 what the last call did: { pages that were missing, pages taken (kq_pages_compact: in use), pairs, 0 }
+ * all -1 and 0 at first.  The calls keep these rules: a page that several sequences name is full, and a last page that is not full
+ * has one name, so that a token is never appended to a page that another sequence reads.  Free pages are taken lowest first, in the
+ * order of sequences and of their pages: the same book and call give the same pages.  Where pages are missing (report[0] says how many)
+ * or a call is refused on the device (report[0] is -1: a parent that is no sequence, more tokens than a row has room for) nothing changes.
+ * The arrays are read on the device, so a recorded step may take pages as it runs.  Scratch of the context: 16 bytes a sequence, 4 a page
+ * (kq_pages_compact: 12) and (kq_pages_fork) 4 an entry; KQ_ERR_UNSUPPORTED where it is too small.
+ *
+ * kq_pages_grow: sequence b gets the pages of its next news[b] tokens (i32 [sequences]; negative: 0) and is that much longer, so that
+ *   kq_cache_append finds room for them.
+ * kq_pages_fork: every sequence b becomes the first min(keep[b], length) tokens of sequence parents[b] (i32 [sequences]; keep_dptr
+ *   == 0: all of them) as it was before the call, all at once: parents[b] = b cuts b back or leaves it, a negative one ends it.  Whole pages are
+ *   shared.  A last page that is not full and is no one else's goes to the lowest b that continues in it; each other one gets a page of its
+ *   own and a pair (the page that it continues, its own) in `pairs`, i32 [sequences, 2], in the order of b, (-1, -1) behind report[2] pairs.
+ * kq_pages_compact: the pages in use move to the lowest numbers: of those beyond as many as are in use the r-th to the r-th free one below, as
+ *   `pairs` (from, to), i32 [pages, 2], (-1, -1) behind report[2] of them; table and refs have the new numbers.
+ * kq_pages_copy: copies page from to page to for the pairs of such a call, in `count` pools (host arrays of addresses and of the bytes of a
+ *   page, multiples of 16: the pool of a kq_cache has kq_cache_bytes(1, ..) a page): the report's number of them, or (report_dptr == 0) all `most`.
+ *   Pairs with a number outside the pool are passed over; one page may be the target of one pair, and not the source of another. */
+KQ_API int kq_pages_grow(kq_ctx* ctx, uint64_t table_dptr, uint32_t sequences, uint32_t width, uint64_t lengths_dptr, uint64_t refs_dptr,
+                         uint32_t pages, uint32_t page_tokens, uint64_t report_dptr, uint64_t news_dptr);
+KQ_API int kq_pages_fork(kq_ctx* ctx, uint64_t table_dptr, uint32_t sequences, uint32_t width, uint64_t lengths_dptr, uint64_t refs_dptr,
+                         uint32_t pages, uint32_t page_tokens, uint64_t report_dptr, uint64_t parents_dptr, uint64_t keep_dptr, uint64_t pairs_dptr);
+KQ_API int kq_pages_compact(kq_ctx* ctx, uint64_t table_dptr, uint32_t sequences, uint32_t width, uint64_t lengths_dptr, uint64_t refs_dptr,
+                            uint32_t pages, uint32_t page_tokens, uint64_t report_dptr, uint64_t pairs_dptr);
+KQ_API int kq_pages_copy(kq_ctx* ctx, uint32_t count, const uint64_t* pool_dptr, const uint64_t* page_bytes, uint32_t pages, uint64_t pairs_dptr,
+                         uint32_t most, uint64_t report_dptr);
+
 /* ---- replayable plans -----------------------------------------------------------
  * Records every kq_* launch between begin and end into a CUDA graph that
  * kq_graph_launch replays.  Replaces the reference's baked plan replay

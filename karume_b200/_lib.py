@@ -74,6 +74,10 @@ SYMBOLS = {
     "kq_cache_read": (_i32, [_vp, _u64, _u32, _u64, _u32, _u64, _u64, _u32, _u64, _u64]),
     "kq_cache_attention": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, ctypes.c_float, _u32,
                                   _u64, _u32, _u32, _u32, _u64, _u64]),
+    "kq_pages_grow": (_i32, [_vp, _u64, _u32, _u32, _u64, _u64, _u32, _u32, _u64, _u64]),
+    "kq_pages_fork": (_i32, [_vp, _u64, _u32, _u32, _u64, _u64, _u32, _u32, _u64, _u64, _u64, _u64]),
+    "kq_pages_compact": (_i32, [_vp, _u64, _u32, _u32, _u64, _u64, _u32, _u32, _u64, _u64]),
+    "kq_pages_copy": (_i32, [_vp, _u32, _pu64, _pu64, _u32, _u64, _u32, _u64]),
     "kq_graph_begin": (_i32, [_vp]),
     "kq_graph_end": (_i32, [_vp, _pu64]),
     "kq_graph_launch": (_i32, [_vp, _u64]),

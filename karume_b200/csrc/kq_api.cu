@@ -465,6 +465,29 @@ int check_batch(kq_ctx* ctx, const char* who, uint32_t sequences, uint64_t pages
   return KQ_OK;
 }
 
+int check_book(kq_ctx* ctx, const char* who, uint64_t table, uint32_t sequences, uint32_t width, uint64_t lengths, uint64_t refs, uint32_t pages,
+               uint32_t page_tokens, uint64_t report, kq::PageBook* out) {
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "%s cannot be recorded into a fused plan (record a graph)", who);
+  if (!is_pow2(page_tokens) || page_tokens < 16 || page_tokens > 256)
+    return fail(ctx, KQ_ERR_SHAPE, "%s: pages of %u tokens: 16, 32, 64, 128 or 256", who, page_tokens);
+  if (!table || !lengths || !refs || !report || ((table | lengths | refs | report) & 3u))
+    return fail(ctx, KQ_ERR_BAD_ARG, "%s: table [sequences, width], lengths [sequences], refs [pages] and report [4] are i32 device arrays", who);
+  if (!sequences || sequences > (1u << 24) || !width || width > (1u << 27) || !pages || pages > (1u << 30))
+    return fail(ctx, KQ_ERR_SHAPE, "%s: %u sequences of up to %u pages, %u pages: 1..2^24, 1..2^27 and 1..2^30", who, sequences, width, pages);
+  *out = kq::PageBook{reinterpret_cast<int*>(table), reinterpret_cast<int*>(lengths), reinterpret_cast<int*>(refs), reinterpret_cast<int*>(report),
+                      sequences, width, pages, 0};
+  while ((1u << out->shift) < page_tokens) ++out->shift;
+  return KQ_OK;
+}
+
+int check_book_scratch(kq_ctx* ctx, const char* who, const kq::PageBook& book, bool fork, bool compact) {
+  const uint64_t need = kq::pages_scratch_bytes(book, fork, compact);
+  if (need > ctx->workspace_bytes || !ctx->workspace)
+    return fail(ctx, KQ_ERR_UNSUPPORTED, "%s: needs %llu bytes of scratch, the context has %llu (kq_init)", who, (unsigned long long)need,
+                (unsigned long long)ctx->workspace_bytes);
+  return KQ_OK;
+}
+
 }  // namespace
 
 namespace kq {
@@ -930,6 +953,76 @@ int kq_cache_attention(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t q_stri
   cudaError_t e = kq::launch_attend(env_of(ctx), a, &launched);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_attention launch");
   ctx->launches += launched;
+  return KQ_OK;
+}
+
+int kq_pages_grow(kq_ctx* ctx, uint64_t table, uint32_t sequences, uint32_t width, uint64_t lengths, uint64_t refs, uint32_t pages, uint32_t page_tokens,
+                  uint64_t report, uint64_t news) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  kq::PageBook book;
+  int rc = check_book(ctx, "kq_pages_grow", table, sequences, width, lengths, refs, pages, page_tokens, report, &book);
+  if (rc == KQ_OK && (!news || (news & 3u))) rc = fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_grow: news [sequences] is an i32 device array");
+  if (rc == KQ_OK) rc = check_book_scratch(ctx, "kq_pages_grow", book, false, false);
+  if (rc != KQ_OK) return rc;
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_pages_grow(env_of(ctx), book, reinterpret_cast<const int*>(news));
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "pages_grow launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+int kq_pages_fork(kq_ctx* ctx, uint64_t table, uint32_t sequences, uint32_t width, uint64_t lengths, uint64_t refs, uint32_t pages, uint32_t page_tokens,
+                  uint64_t report, uint64_t parents, uint64_t keep, uint64_t pairs) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  kq::PageBook book;
+  int rc = check_book(ctx, "kq_pages_fork", table, sequences, width, lengths, refs, pages, page_tokens, report, &book);
+  if (rc == KQ_OK && (!parents || !pairs || ((parents | keep | pairs) & 3u)))
+    rc = fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_fork: parents and keep [sequences] and pairs [sequences, 2] are i32 device arrays");
+  if (rc == KQ_OK) rc = check_book_scratch(ctx, "kq_pages_fork", book, true, false);
+  if (rc != KQ_OK) return rc;
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_pages_fork(env_of(ctx), book, reinterpret_cast<const int*>(parents), reinterpret_cast<const int*>(keep),
+                                        reinterpret_cast<int*>(pairs));
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "pages_fork launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+int kq_pages_compact(kq_ctx* ctx, uint64_t table, uint32_t sequences, uint32_t width, uint64_t lengths, uint64_t refs, uint32_t pages, uint32_t page_tokens,
+                     uint64_t report, uint64_t pairs) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  kq::PageBook book;
+  int rc = check_book(ctx, "kq_pages_compact", table, sequences, width, lengths, refs, pages, page_tokens, report, &book);
+  if (rc == KQ_OK && (!pairs || (pairs & 3u))) rc = fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_compact: pairs [pages, 2] is an i32 device array");
+  if (rc == KQ_OK) rc = check_book_scratch(ctx, "kq_pages_compact", book, false, true);
+  if (rc != KQ_OK) return rc;
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_pages_compact(env_of(ctx), book, reinterpret_cast<int*>(pairs));
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "pages_compact launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+int kq_pages_copy(kq_ctx* ctx, uint32_t count, const uint64_t* pools, const uint64_t* page_bytes, uint32_t pages, uint64_t pairs, uint32_t most,
+                  uint64_t report) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_pages_copy cannot be recorded into a fused plan (record a graph)");
+  if (count && (!pools || !page_bytes)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: null argument");
+  if (pages > (1u << 30) || most > (1u << 30)) return fail(ctx, KQ_ERR_SHAPE, "kq_pages_copy: %u pages, %u pairs: up to 2^30", pages, most);
+  if (!pairs || ((pairs | report) & 3u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: pairs [most, 2] and report [4] are i32 device arrays");
+  for (uint32_t i = 0; i < count; ++i) {
+    if (!pools[i] || (pools[i] & 15u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: pool %u must be a 16-byte aligned device pointer", i);
+    if (!page_bytes[i] || page_bytes[i] % 16 || page_bytes[i] > (1ull << 32))
+      return fail(ctx, KQ_ERR_SHAPE, "kq_pages_copy: pages of pool %u have %llu bytes: a multiple of 16, up to 2^32", i, (unsigned long long)page_bytes[i]);
+  }
+  if (!pages || !most) return KQ_OK;
+  DeviceGuard guard(ctx->device);
+  for (uint32_t i = 0; i < count; i += kq::kPoolsAtOnce) {
+    cudaError_t e = kq::launch_pages_copy(env_of(ctx), std::min(kq::kPoolsAtOnce, count - i), pools + i, page_bytes + i, pages,
+                                          reinterpret_cast<const int*>(pairs), most, reinterpret_cast<const int*>(report));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "pages_copy launch");
+    ctx->launches += 1;
+  }
   return KQ_OK;
 }
 

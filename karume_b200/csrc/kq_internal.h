@@ -242,3 +242,23 @@ cudaError_t launch_attend(const LaunchEnv& env, const AttendArgs& args, int* lau
 bool attend_many_supports(const AttendArgs& args);
 cudaError_t launch_attend_many(const LaunchEnv& env, const AttendArgs& args, uint32_t beyond);
 }  // namespace kq
+
+// ---- pages that sequences share (kq_pages.cu) ----------------------------------------------------
+namespace kq {
+// All pointers on the device.
+struct PageBook {
+  int* table;    // [sequences, width] page numbers, in token order, -1 behind a sequence's pages
+  int* lengths;  // [sequences]
+  int* refs;     // [pages] names that the table has for a page
+  int* report;   // [4] pages that were missing (-1: a refused call), pages taken or in use, pairs, 0
+  uint32_t sequences, width, pages;
+  uint32_t shift;  // log2 of a page's tokens
+};
+constexpr uint32_t kPoolsAtOnce = 128;  // of one launch
+uint64_t pages_scratch_bytes(const PageBook& book, bool fork, bool compact);  // of LaunchEnv::workspace
+cudaError_t launch_pages_grow(const LaunchEnv& env, const PageBook& book, const int* news);
+cudaError_t launch_pages_fork(const LaunchEnv& env, const PageBook& book, const int* parents, const int* keep, int* pairs);
+cudaError_t launch_pages_compact(const LaunchEnv& env, const PageBook& book, int* pairs);
+cudaError_t launch_pages_copy(const LaunchEnv& env, uint32_t count, const uint64_t* pools, const uint64_t* page_bytes, uint32_t pages, const int* pairs,
+                              uint32_t most, const int* report);
+}  // namespace kq

@@ -1,0 +1,534 @@
+// Pages of a paged cache that sequences share: which page belongs to whom, and copies of pages.
+//
+//   grow     every sequence gets the pages that its next tokens need
+//   fork     every sequence becomes the beginning of a sequence, all at once; pages are shared, one that is not full has one owner
+//   compact  the pages in use move to the lowest numbers
+//   copy     the content of pages, in any number of pools
+//
+// The first three work on small arrays of whole numbers, so what bounds them is latency: loads that depend on one another, atomic
+// operations and the barriers between the steps, each of which sees all of the step in front.  One cluster of CTAs does all of a call:
+// its barrier costs a fraction of a launch.  Free pages are those without a name in `refs`, the lowest first: nothing else has to be
+// kept, and which page a call takes does not depend on the order in which its threads run.
+#include <algorithm>
+
+#include "kq_cache.cuh"
+
+namespace kq {
+namespace {
+
+constexpr int kBookThreads = 1024;
+constexpr int kPagesAThread = 4;    // neighbours that a thread looks at when pages are counted
+constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kChunk = 128;    // table entries that a warp takes at a time
+constexpr int kLowest = -0x7fffffff;
+
+struct BookParams {
+  PageBook book;
+  const int* news;     // grow
+  const int* parents;  // fork
+  const int* keep;     // ... null: all
+  int* pairs;          // fork [sequences][2], compact [pages][2]
+  int* list;           // scratch [pages]: free pages in order
+  int* moves;          // scratch [pages]: compact: pages that move, in order
+  int* place;          // scratch [pages]: compact: a moving page's place in `moves`
+  int4* state;         // scratch [sequences]: what a step found, for the steps behind it
+  int* stage;          // scratch [sequences][width]: fork: new rows, until every old one has been read
+};
+
+struct Shared {
+  int totals[2][kMaxCluster];  // of the CTAs, turn about
+  long long warps[32];
+};
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cta_count() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+// All of the call's threads have come here, and see what the others wrote (read past L1, which others' writes do not reach).
+__device__ __forceinline__ void sync_all(uint32_t ctas) {
+  if (ctas == 1) __syncthreads();
+  else cluster_sync_all();
+}
+// In front of the first write into another CTA's shared memory: all of them have begun.
+__device__ __forceinline__ void begin_all(uint32_t ctas) {
+  if (ctas > 1) cluster_sync_all();
+}
+__device__ __forceinline__ int fresh(const int* p) { return __ldcg(p); }
+__device__ __forceinline__ void put_remote(int* local, uint32_t rank, int value) {
+  uint32_t to;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(local))), "r"(rank));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(value) : "memory");
+}
+
+// Sum of the values of the block's threads in front of the calling one; `total`: of all of them.
+template <typename T>
+__device__ __forceinline__ T block_before(Shared& s, T value, T& total) {
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const auto upto_of = [&](T v) {
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const T other = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= static_cast<uint32_t>(o)) v += other;
+    }
+    return v;
+  };
+  const T upto = upto_of(value);
+  if (lane == 31) s.warps[warp] = upto;
+  __syncthreads();
+  const T mine = static_cast<T>(s.warps[lane]), sum = upto_of(mine);
+  total = __shfl_sync(0xffffffffu, sum, 31);
+  const T before = __shfl_sync(0xffffffffu, sum - mine, warp);
+  __syncthreads();  // s.warps belongs to the next sum
+  return before + upto - value;
+}
+__device__ __forceinline__ int block_most(Shared& s, int value) {
+  const int of_warp = __reduce_max_sync(0xffffffffu, value);
+  if (threadIdx.x % 32 == 0) s.warps[threadIdx.x / 32] = of_warp;
+  __syncthreads();
+  const int most = __reduce_max_sync(0xffffffffu, static_cast<int>(s.warps[threadIdx.x % 32]));
+  __syncthreads();
+  return most;
+}
+
+// The cluster's CTAs' totals: those in front of the calling CTA, and of all.  `turn` counts the calls.
+__device__ __forceinline__ int2 cluster_before(Shared& s, int total, uint32_t rank, uint32_t ctas, uint32_t& turn) {
+  if (ctas == 1) {
+    __syncthreads();
+    return make_int2(0, total);
+  }
+  int* const of = s.totals[turn++ & 1];
+  if (threadIdx.x < ctas) put_remote(of + rank, threadIdx.x, total);
+  cluster_sync_all();
+  int2 r = make_int2(0, 0);
+  for (uint32_t i = 0; i < ctas; ++i) {
+    if (i < rank) r.x += of[i];
+    r.y += of[i];
+  }
+  return r;
+}
+
+// Pages of from .. to that are `used` (or not), in order, into list[0 .. limit); returns how many were found (the scan ends with the
+// step that reaches the limit).
+__device__ __forceinline__ int ranked(const BookParams& p, Shared& s, bool used, uint32_t from, uint32_t to, int limit, int* list, uint32_t rank, uint32_t ctas,
+                                      uint32_t& turn) {
+  int found = 0;
+  for (uint32_t base = from; base < to && found < limit; base += ctas * kBookThreads * kPagesAThread) {
+    const uint32_t at = base + (rank * kBookThreads + threadIdx.x) * kPagesAThread;
+    uint32_t is = 0;
+#pragma unroll
+    for (int i = 0; i < kPagesAThread; ++i)
+      if (at + i < to && (fresh(p.book.refs + at + i) != 0) == used) is |= 1u << i;
+    int total;
+    int before = block_before(s, __popc(is), total);
+    const int2 all = cluster_before(s, total, rank, ctas, turn);
+    before += found + all.x;
+    found += all.y;
+#pragma unroll
+    for (int i = 0; i < kPagesAThread; ++i)
+      if (is >> i & 1) {
+        if (before < limit) list[before] = static_cast<int>(at + i);
+        ++before;
+      }
+  }
+  return found;
+}
+
+__device__ __forceinline__ int pages_of(int tokens, uint32_t shift) { return static_cast<int>((static_cast<uint32_t>(tokens) + (1u << shift) - 1) >> shift); }
+// A sequence's tokens, as many as its row has room for.
+__device__ __forceinline__ int length_of(const PageBook& k, uint32_t b) {
+  const uint64_t room = static_cast<uint64_t>(k.width) << k.shift;
+  return static_cast<int>(min(static_cast<uint64_t>(max(k.lengths[b], 0)), min(room, static_cast<uint64_t>(0x7fffffff))));
+}
+__device__ __forceinline__ bool a_page(const PageBook& k, int page) { return static_cast<uint32_t>(page) < k.pages; }
+
+__device__ __forceinline__ void tell(const BookParams& p, int missing, int pages, int pairs) {
+  if (cta_rank() == 0 && threadIdx.x == 0) {
+    p.book.report[0] = missing;
+    p.book.report[1] = pages;
+    p.book.report[2] = pairs;
+    p.book.report[3] = 0;
+  }
+}
+// Every (sequence, chunk of its row up to `entries`) once over the cluster's warps.
+template <typename Use>
+__device__ __forceinline__ void each_chunk(const PageBook& k, uint32_t entries, uint32_t rank, uint32_t ctas, Use use) {
+  const uint32_t chunks = (entries + kChunk - 1) / kChunk, warps = ctas * (kBookThreads / 32);
+  const uint64_t all = static_cast<uint64_t>(k.sequences) * chunks;
+  for (uint64_t u = rank * (kBookThreads / 32) + threadIdx.x / 32; u < all; u += warps) use(static_cast<uint32_t>(u / chunks), static_cast<uint32_t>(u % chunks) * kChunk);
+}
+
+__global__ void __launch_bounds__(kBookThreads, 1) pages_grow_kernel(const BookParams p) {
+  __shared__ Shared s;
+  const uint32_t rank = cta_rank(), ctas = cta_count(), lane = threadIdx.x % 32;
+  uint32_t turn = 0;
+  pdl_launch_dependents();
+  begin_all(ctas);
+  pdl_wait_prior_grid();
+  const PageBook& k = p.book;
+  const uint64_t room = static_cast<uint64_t>(k.width) << k.shift;
+  // what each sequence needs, every CTA for itself
+  long long need = 0;
+  int most = 0;
+  bool bad = false;
+  for (uint32_t b0 = 0; b0 < k.sequences; b0 += kBookThreads) {
+    const uint32_t b = b0 + threadIdx.x;
+    int length = 0, news = 0, held = 0, more = 0;
+    if (b < k.sequences) {
+      length = length_of(k, b);
+      news = max(p.news[b], 0);
+      const uint64_t wanted = static_cast<uint64_t>(length) + static_cast<uint64_t>(news);
+      if (wanted > room || wanted > 0x7fffffffull) bad = true;
+      held = pages_of(length, k.shift);
+      more = bad ? 0 : pages_of(length + news, k.shift) - held;
+    }
+    long long total;
+    const long long before = need + block_before(s, static_cast<long long>(more), total);
+    // (numbers beyond 31 bits are of a call that has too few pages)
+    if (b < k.sequences && b0 / kBookThreads % ctas == rank) p.state[b] = make_int4(length + (bad ? 0 : news), held, more, static_cast<int>(min(before, 0x7fffffffll)));
+    need += total;
+    most = max(most, more);
+  }
+  bad = __syncthreads_or(bad);
+  most = block_most(s, most);
+  if (bad) {
+    tell(p, -1, 0, 0);
+    return;
+  }
+  const int limit = static_cast<int>(min(need, static_cast<long long>(k.pages) + 1));
+  const int found = need ? ranked(p, s, false, 0, k.pages, limit, p.list, rank, ctas, turn) : 0;
+  if (found < need) {
+    tell(p, static_cast<int>(min(need - found, 0x7fffffffll)), 0, 0);
+    return;
+  }
+  sync_all(ctas);  // the list and the states
+  each_chunk(k, static_cast<uint32_t>(most), rank, ctas, [&](uint32_t b, uint32_t from) {
+    const int4 st = __ldcg(p.state + b);
+    for (uint32_t i = from + lane; i < from + kChunk && static_cast<int>(i) < st.z; i += 32) {
+      const int page = fresh(p.list + st.w + i);
+      k.table[static_cast<size_t>(b) * k.width + st.y + i] = page;
+      k.refs[page] = 1;
+    }
+  });
+  for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) k.lengths[b] = __ldcg(p.state + b).x;
+  tell(p, 0, static_cast<int>(need), 0);
+}
+
+// What sequence b becomes: the first n tokens of its parent.
+struct Becomes {
+  int parent, n, old;
+  bool changes;
+};
+__device__ __forceinline__ Becomes becomes(const BookParams& p, uint32_t b) {
+  Becomes r;
+  r.parent = p.parents[b];
+  r.old = length_of(p.book, b);
+  r.n = 0;
+  if (r.parent >= 0) {
+    r.n = static_cast<uint32_t>(r.parent) == b ? r.old : length_of(p.book, static_cast<uint32_t>(r.parent));
+    if (p.keep) r.n = min(r.n, max(p.keep[b], 0));
+  }
+  r.changes = r.parent < 0 ? r.old > 0 : static_cast<uint32_t>(r.parent) != b || r.n < r.old;
+  return r;
+}
+
+__global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookParams p) {
+  __shared__ Shared s;
+  const uint32_t rank = cta_rank(), ctas = cta_count(), lane = threadIdx.x % 32;
+  uint32_t turn = 0;
+  pdl_launch_dependents();
+  begin_all(ctas);
+  pdl_wait_prior_grid();
+  const PageBook& k = p.book;
+  const auto no_pairs = [&](uint32_t from) {
+    for (uint32_t i = 2 * from + rank * kBookThreads + threadIdx.x; i < 2 * k.sequences; i += ctas * kBookThreads) p.pairs[i] = -1;
+  };
+  bool bad = false;
+  int entries = 0;  // of any row that changes, old or new
+  for (uint32_t b = threadIdx.x; b < k.sequences; b += kBookThreads) {
+    if (p.parents[b] >= static_cast<int>(k.sequences)) {
+      bad = true;
+    } else {
+      const Becomes w = becomes(p, b);
+      if (w.changes) entries = max(entries, pages_of(max(w.n, w.old), k.shift));
+    }
+  }
+  bad = __syncthreads_or(bad);
+  entries = block_most(s, entries);
+  if (bad) {
+    tell(p, -1, 0, 0);
+    no_pairs(0);
+    return;
+  }
+  // ---- the names that rows give up, and those of whole pages that they take -------------------------
+  const auto names = [&](int by) {
+    each_chunk(k, static_cast<uint32_t>(entries), rank, ctas, [&](uint32_t b, uint32_t from) {
+      const Becomes w = becomes(p, b);
+      if (!w.changes) return;
+      const bool same = w.parent >= 0 && static_cast<uint32_t>(w.parent) == b;
+      const int whole = w.n >> k.shift, held = pages_of(w.old, k.shift);
+      const int* const mine = k.table + static_cast<size_t>(b) * k.width;
+      const int* const theirs = k.table + static_cast<size_t>(max(w.parent, 0)) * k.width;
+      for (int i = static_cast<int>(from + lane); i < static_cast<int>(from + kChunk); i += 32) {
+        if (i < held && !(same && i < whole)) {
+          const int page = mine[i];
+          if (a_page(k, page)) atomicSub(k.refs + page, by);
+        }
+        if (i < whole && !same) {
+          const int page = theirs[i];
+          if (a_page(k, page)) atomicAdd(k.refs + page, by);
+          p.stage[static_cast<size_t>(b) * k.width + i] = page;
+        }
+      }
+    });
+  };
+  names(1);
+  sync_all(ctas);
+  // ---- last pages that are not full: one that nobody names goes to the lowest sequence ----------------
+  const auto tail_of = [&](const Becomes& w) {
+    return w.changes && (w.n & ((1 << k.shift) - 1)) ? k.table[static_cast<size_t>(w.parent) * k.width + (w.n >> k.shift)] : -1;
+  };
+  for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
+    const int page = tail_of(becomes(p, b));
+    if (a_page(k, page) && fresh(k.refs + page) <= 0) atomicMin(k.refs + page, kLowest + static_cast<int>(b));
+  }
+  sync_all(ctas);
+  int need = 0;
+  for (uint32_t b0 = 0; b0 < k.sequences; b0 += kBookThreads) {
+    const uint32_t b = b0 + threadIdx.x;
+    Becomes w = {};
+    int page = -1, place = -1;
+    if (b < k.sequences) {
+      w = becomes(p, b);
+      page = tail_of(w);
+      if (a_page(k, page)) place = fresh(k.refs + page) == kLowest + static_cast<int>(b) ? -2 : 0;  // takes it over, or needs another
+    }
+    int total;
+    const int before = block_before(s, place == 0 ? 1 : 0, total);
+    if (place == 0) place = need + before;
+    need += total;
+    if (b < k.sequences && b0 / kBookThreads % ctas == rank) p.state[b] = make_int4(w.changes ? w.n : -1, pages_of(w.old, k.shift), page, place);
+  }
+  const int found = need ? ranked(p, s, false, 0, k.pages, need, p.list, rank, ctas, turn) : 0;
+  sync_all(ctas);  // the list, the states; every look at `refs`
+  const bool enough = found >= need;
+  for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
+    const int4 st = __ldcg(p.state + b);
+    if (st.w == -2) k.refs[st.z] = enough ? 1 : 0;
+  }
+  if (!enough) {  // all as it was
+    sync_all(ctas);
+    names(-1);
+    tell(p, need - found, 0, 0);
+    no_pairs(0);
+    return;
+  }
+  // ---- the new rows ---------------------------------------------------------------------------------
+  each_chunk(k, static_cast<uint32_t>(entries), rank, ctas, [&](uint32_t b, uint32_t from) {
+    const int4 st = __ldcg(p.state + b);
+    if (st.x < 0) return;
+    const bool same = p.parents[b] == static_cast<int>(b);
+    const int whole = st.x >> k.shift, all = pages_of(st.x, k.shift);
+    for (int i = static_cast<int>(from + lane); i < static_cast<int>(from + kChunk); i += 32) {
+      int* const entry = k.table + static_cast<size_t>(b) * k.width + i;
+      if (i < whole) {
+        if (!same) *entry = fresh(p.stage + static_cast<size_t>(b) * k.width + i);
+      } else if (i < all) {
+        *entry = st.w >= 0 ? fresh(p.list + st.w) : st.z;
+      } else if (i < st.y) {
+        *entry = -1;
+      }
+    }
+  });
+  for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
+    const int4 st = __ldcg(p.state + b);
+    if (st.x >= 0) k.lengths[b] = st.x;
+    if (st.w >= 0) {
+      const int page = fresh(p.list + st.w);
+      k.refs[page] = 1;
+      p.pairs[2 * st.w] = st.z;
+      p.pairs[2 * st.w + 1] = page;
+    }
+  }
+  no_pairs(static_cast<uint32_t>(need));
+  tell(p, 0, need, need);
+}
+
+__global__ void __launch_bounds__(kBookThreads, 1) pages_compact_kernel(const BookParams p) {
+  __shared__ Shared s;
+  const uint32_t rank = cta_rank(), ctas = cta_count(), lane = threadIdx.x % 32;
+  uint32_t turn = 0;
+  pdl_launch_dependents();
+  begin_all(ctas);
+  pdl_wait_prior_grid();
+  const PageBook& k = p.book;
+  int mine = 0;
+  for (uint32_t i = rank * kBookThreads + threadIdx.x; i < k.pages; i += ctas * kBookThreads) mine += k.refs[i] != 0;
+  int total;
+  block_before(s, mine, total);
+  const uint32_t used = static_cast<uint32_t>(cluster_before(s, total, rank, ctas, turn).y);
+  const int holes = ranked(p, s, false, 0, used, static_cast<int>(used), p.list, rank, ctas, turn);
+  ranked(p, s, true, used, k.pages, holes, p.moves, rank, ctas, turn);  // as many
+  sync_all(ctas);
+  for (uint32_t i = rank * kBookThreads + threadIdx.x; i < k.pages; i += ctas * kBookThreads) {
+    int from = -1, to = -1;
+    if (static_cast<int>(i) < holes) {
+      from = fresh(p.moves + i);
+      to = fresh(p.list + i);
+      k.refs[to] = fresh(k.refs + from);
+      k.refs[from] = 0;
+      p.place[from] = static_cast<int>(i);
+    }
+    p.pairs[2 * i] = from;
+    p.pairs[2 * i + 1] = to;
+  }
+  sync_all(ctas);
+  each_chunk(k, k.width, rank, ctas, [&](uint32_t b, uint32_t first) {
+    const int held = pages_of(length_of(k, b), k.shift);
+    for (int i = static_cast<int>(first + lane); i < static_cast<int>(first + kChunk) && i < held; i += 32) {
+      int* const entry = k.table + static_cast<size_t>(b) * k.width + i;
+      const int page = *entry;
+      if (!a_page(k, page) || static_cast<uint32_t>(page) < used) continue;
+      const int place = fresh(p.place + page);  // a page that the counts do not know has none: anything is there
+      if (static_cast<uint32_t>(place) < static_cast<uint32_t>(holes) && fresh(p.moves + place) == page) *entry = fresh(p.list + place);
+    }
+  });
+  tell(p, 0, static_cast<int>(used), holes);
+}
+
+// ---- copies -----------------------------------------------------------------------------------------
+constexpr int kCopyThreads = 256, kCopyPieces = 4;  // 16-byte pieces a thread has under way
+constexpr uint32_t kPiece = kCopyThreads * kCopyPieces * 16;
+
+struct CopyParams {
+  uint8_t* pool[kPoolsAtOnce];
+  uint64_t bytes[kPoolsAtOnce];  // of a page
+  const int* pairs;
+  const int* report;  // null: all `most` pairs
+  uint32_t pools, pages, most, parts;  // parts that a page is copied in
+};
+
+__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const __grid_constant__ CopyParams p) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const uint32_t count = p.report ? min(static_cast<uint32_t>(max(p.report[2], 0)), p.most) : p.most;
+  const uint64_t all = static_cast<uint64_t>(count) * p.pools * p.parts;
+  for (uint64_t item = blockIdx.x; item < all; item += gridDim.x) {
+    const uint32_t part = static_cast<uint32_t>(item % p.parts);
+    const uint32_t pool = static_cast<uint32_t>(item / p.parts % p.pools);
+    const uint32_t pair = static_cast<uint32_t>(item / p.parts / p.pools);
+    const uint32_t from = static_cast<uint32_t>(p.pairs[2 * pair]), to = static_cast<uint32_t>(p.pairs[2 * pair + 1]);
+    if (from >= p.pages || to >= p.pages || from == to) continue;
+    const uint64_t bytes = p.bytes[pool], each = (bytes / 16 + p.parts - 1) / p.parts;  // in 16-byte pieces
+    const uint64_t begin = part * each, end = min(begin + each, bytes / 16);
+    const uint4* const src = reinterpret_cast<const uint4*>(p.pool[pool] + from * bytes);
+    uint4* const dst = reinterpret_cast<uint4*>(p.pool[pool] + to * bytes);
+    for (uint64_t at = begin + threadIdx.x; at < end; at += kCopyThreads * kCopyPieces) {
+      uint4 v[kCopyPieces];
+#pragma unroll
+      for (int i = 0; i < kCopyPieces; ++i)
+        if (at + i * kCopyThreads < end) v[i] = src[at + i * kCopyThreads];
+#pragma unroll
+      for (int i = 0; i < kCopyPieces; ++i)
+        if (at + i * kCopyThreads < end) dst[at + i * kCopyThreads] = v[i];
+    }
+  }
+}
+
+// One cluster, of one CTA where that has all its work in a step or two.
+uint32_t cluster_for(const PageBook& k) {
+  const uint64_t work = std::max<uint64_t>(k.pages / kPagesAThread, static_cast<uint64_t>(k.sequences) * k.width / 4);
+  return work <= 2 * kBookThreads ? 1u : kMaxCluster;
+}
+
+template <typename Kernel>
+cudaError_t launch_book(const LaunchEnv& env, Kernel kernel, const BookParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  const uint32_t ctas = cluster_for(p.book);
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kBookThreads);
+  cfg.stream = env.stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = env.overlap ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+uint64_t up16(uint64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+}  // namespace
+
+uint64_t pages_scratch_bytes(const PageBook& k, bool fork, bool compact) {
+  return up16(4ull * k.pages) * (compact ? 3 : 1) + 16ull * k.sequences + (fork ? 4ull * k.sequences * k.width : 0);
+}
+
+cudaError_t launch_pages_grow(const LaunchEnv& env, const PageBook& book, const int* news) {
+  BookParams p = {};
+  p.book = book;
+  p.news = news;
+  p.list = static_cast<int*>(env.workspace);
+  p.state = reinterpret_cast<int4*>(static_cast<uint8_t*>(env.workspace) + up16(4ull * book.pages));
+  return launch_book(env, pages_grow_kernel, p);
+}
+
+cudaError_t launch_pages_fork(const LaunchEnv& env, const PageBook& book, const int* parents, const int* keep, int* pairs) {
+  BookParams p = {};
+  p.book = book;
+  p.parents = parents;
+  p.keep = keep;
+  p.pairs = pairs;
+  p.list = static_cast<int*>(env.workspace);
+  p.state = reinterpret_cast<int4*>(static_cast<uint8_t*>(env.workspace) + up16(4ull * book.pages));
+  p.stage = reinterpret_cast<int*>(p.state + book.sequences);
+  return launch_book(env, pages_fork_kernel, p);
+}
+
+cudaError_t launch_pages_compact(const LaunchEnv& env, const PageBook& book, int* pairs) {
+  BookParams p = {};
+  p.book = book;
+  p.pairs = pairs;
+  p.list = static_cast<int*>(env.workspace);
+  p.moves = p.list + up16(4ull * book.pages) / 4;
+  p.place = p.moves + up16(4ull * book.pages) / 4;
+  return launch_book(env, pages_compact_kernel, p);
+}
+
+cudaError_t launch_pages_copy(const LaunchEnv& env, uint32_t count, const uint64_t* pools, const uint64_t* page_bytes, uint32_t pages, const int* pairs,
+                              uint32_t most, const int* report) {
+  CopyParams p;
+  uint64_t largest = 0;
+  for (uint32_t i = 0; i < count; ++i) {
+    p.pool[i] = reinterpret_cast<uint8_t*>(pools[i]);
+    p.bytes[i] = page_bytes[i];
+    largest = std::max(largest, page_bytes[i]);
+  }
+  p.pairs = pairs;
+  p.report = report;
+  p.pools = count;
+  p.pages = pages;
+  p.most = most;
+  p.parts = static_cast<uint32_t>((largest + kPiece - 1) / kPiece);
+  const uint64_t items = static_cast<uint64_t>(most) * count * p.parts;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<uint64_t>(items, static_cast<uint64_t>(env.sm_count) * 8)));
+  cfg.blockDim = dim3(kCopyThreads);
+  cfg.stream = env.stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = env.overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, pages_copy_kernel, p);
+}
+
+}  // namespace kq

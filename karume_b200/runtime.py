@@ -153,6 +153,34 @@ class KvCache:
             self.handle = 0
 
 
+class CachePages:
+    """Which page belongs to whom: table i32 CUDA [sequences, width] (a CacheBatch's pages; -1 behind a sequence's own), lengths i32
+    [sequences], refs i32 [pages] (how many entries name a page) and report i32 [4] of the last call: pages that were missing (then, and
+    with -1 for a refused call, nothing changed), pages taken or in use, pairs, 0.  Gpu.cache_pages makes an empty one."""
+
+    def __init__(self, table, lengths, refs, page_tokens: int, report=None):
+        torch = _torch()
+        if report is None:
+            report = torch.zeros(4, dtype=torch.int32, device=table.device)
+            torch.cuda.current_stream(table.device).synchronize()  # the first call may run on another stream
+        for name, t, dims in (("table", table, 2), ("lengths", lengths, 1), ("refs", refs, 1), ("report", report, 1)):
+            if t.dtype != torch.int32 or not t.is_cuda or t.dim() != dims or not t.is_contiguous():
+                raise KqError(2, f"{name} must be a contiguous CUDA int32 tensor of {dims} dimension(s)")
+        self.sequences, self.width = (int(n) for n in table.shape)
+        if lengths.numel() != self.sequences or report.numel() != 4:
+            raise KqError(2, f"{self.sequences} sequences need as many lengths, a report four numbers")
+        self.table, self.lengths, self.refs, self.report = table, lengths, refs, report
+        self.pages, self.page_tokens = int(refs.numel()), int(page_tokens)
+        self.args = (table.data_ptr(), self.sequences, self.width, lengths.data_ptr(), refs.data_ptr(), self.pages, self.page_tokens, report.data_ptr())
+
+
+def _per_sequence(t, book: CachePages, name: str) -> int:
+    torch = _torch()
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() != book.sequences:
+        raise KqError(2, f"{name} must be a contiguous CUDA int32 tensor [{book.sequences}]")
+    return t.data_ptr()
+
+
 _NO_ROPE = (0, 0, 0, 0)
 
 
@@ -506,6 +534,58 @@ class Gpu:
                                          float(scale), window,
                                          *(rope.args if rope is not None else _NO_ROPE), po, out_stride))
         return out
+
+    # -- pages that sequences share ---------------------------------------------------------------
+    def cache_pages(self, sequences: int, longest: int, pages: int, page_tokens: int) -> CachePages:
+        """An empty book of `pages` pages for `sequences` sequences of up to `longest` tokens."""
+        torch = _torch()
+        width = (int(longest) + page_tokens - 1) // page_tokens
+        book = CachePages(torch.full((sequences, width), -1, dtype=torch.int32, device=self.device), *(
+            torch.zeros(n, dtype=torch.int32, device=self.device) for n in (sequences, pages)), page_tokens)
+        torch.cuda.current_stream(self.device).synchronize()  # the first call may run on another stream than torch's current one
+        return book
+
+    def pages_grow(self, book: CachePages, news) -> None:
+        """Sequence b gets the pages of its next news[b] tokens (CUDA int32) and is that much longer."""
+        self._check(L.kq_pages_grow(self._ctx, *book.args, _per_sequence(news, book, "news")))
+
+    def pages_fork(self, book: CachePages, parents, keep=None):
+        """Every sequence b becomes the first min(keep[b], length) tokens of parents[b] (CUDA int32; negative: it ends), all at once.
+        Returns the pairs [sequences, 2] of pages to copy, for pages_copy."""
+        torch = _torch()
+        pairs = torch.empty((book.sequences, 2), dtype=torch.int32, device=self.device)
+        self._check(L.kq_pages_fork(self._ctx, *book.args, _per_sequence(parents, book, "parents"),
+                                    _per_sequence(keep, book, "keep") if keep is not None else 0, pairs.data_ptr()))
+        return pairs
+
+    def pages_compact(self, book: CachePages):
+        """Moves the pages in use to the lowest numbers; returns the pairs [pages, 2] (from, to), for pages_copy."""
+        torch = _torch()
+        pairs = torch.empty((book.pages, 2), dtype=torch.int32, device=self.device)
+        self._check(L.kq_pages_compact(self._ctx, *book.args, pairs.data_ptr()))
+        return pairs
+
+    def pages_copy(self, book: CachePages, pairs, pools) -> None:
+        """Copies the pages of the book's last fork or compact in every pool: KvCaches, or CUDA tensors whose first axis is the pages."""
+        torch = _torch()
+        if pairs.dtype != torch.int32 or not pairs.is_cuda or not pairs.is_contiguous() or pairs.dim() != 2 or pairs.shape[1] != 2:
+            raise KqError(2, "pairs must be a contiguous CUDA int32 tensor [pairs, 2]")
+        addresses, sizes = [], []
+        for pool in pools:
+            if isinstance(pool, KvCache):
+                pages, each, address = pool.pages, pool.kv_heads * pool.page_tokens * (pool.head_dim + 8), pool.pool.data_ptr()
+            elif not pool.is_cuda or not pool.is_contiguous() or pool.dim() == 0:
+                raise KqError(2, "a pool is a KvCache or a contiguous CUDA tensor [pages, ...]")
+            else:
+                pages, address = int(pool.shape[0]), pool.data_ptr()
+                each = pool.numel() // max(pages, 1) * pool.element_size()
+            if pages < book.pages:
+                raise KqError(2, f"a pool of {pages} pages for a book of {book.pages}")
+            addresses.append(address)
+            sizes.append(each)
+        n = len(addresses)
+        self._check(L.kq_pages_copy(self._ctx, n, (ctypes.c_uint64 * n)(*addresses), (ctypes.c_uint64 * n)(*sizes), book.pages, pairs.data_ptr(),
+                                    pairs.shape[0], book.report.data_ptr()))
 
     # -- replayable plans -------------------------------------------------------
     def graph_begin(self) -> None:
