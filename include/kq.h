@@ -406,6 +406,42 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
                               uint32_t window, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary,
                               uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride);
 
+/* kq_cache_attention_shared: kq_cache_attention for sequences that begin alike, the keys that they have in common read once.  Group g is the
+ * sequences first[g] .. first[g + 1] - 1 (i32 [groups + 1], ascending); their first shared[g] tokens (i32 [groups]) are the same: their
+ * tables name the same pages for them, or (a last page that is not full) copies.  What is shared beyond a sequence's new tokens' beginning counts as
+ * its own; sequences outside the groups, and a group of one, are as in kq_cache_attention.  The same results but for roundings.  The sums over the
+ * common keys take 4 (head_dim + 2) bytes a row and query head of the context's scratch; where that is more than half of it, nothing is read once.
+ *
+ * kq_cache_summarize: for the pages that new tokens of the batch are in (behind their kq_cache_append), what kq_cache_select goes by: codes i8 [pages,
+ * kv_heads, 2, head_dim] and scales f32 [pages, kv_heads, 2], the host's, 16- and 8-byte aligned.  Over the page's tokens up to the sequence's
+ * length, of what the keys stand for, channel by channel, c = (max + min) * 0.5 and r = (max - min) * 0.5 (rounded to f32); both rows
+ * quantised by kq_quantize_rows' rule.  A page with a key that is not finite has codes 0 and scales NaN.
+ * kq_cache_select: for every new token and kv head, up to `budget` pages of its sequence, as ascending indices into its row of the page table, i32
+ * [tokens, kv_heads, budget], -1 behind them: of the pages up to the token's position the first `first`, the last `last` (1 at least, first +
+ * last <= budget), and those with the largest score, ties to the lower index.  The score of a page is the largest over the query heads that
+ * read the kv head of ((a . c) s_c + (|a| . r) s_r) s, each operation rounded to f32, for a query rotated and quantised by the same rule (codes a, scale s);
+ * not a number (a page that is none, a summary or a query that is not finite) counts as the largest.  A row that belongs to no sequence has no pages (-1).
+ * Scratch: 4 * kv_heads * table_width bytes at least (KQ_ERR_UNSUPPORTED).
+ * kq_cache_attention_selected: attention of every new token over the tokens of its selected pages up to its position; `selected` as kq_cache_select
+ * gives it: min(budget, pages up to the position) indices are read, the last of which is the position's own page.  An index outside the table reads
+ * as NaN.  For few rows a sequence: each reads its own pages. */
+KQ_API int kq_cache_attention_shared(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads,
+                                     uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr,
+                                     uint64_t starts_dptr, uint32_t tokens, uint32_t most, uint32_t groups, uint64_t first_dptr,
+                                     uint64_t shared_dptr, float scale, uint32_t window, uint64_t table_dptr, uint32_t table_positions,
+                                     uint32_t rotary, uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride);
+KQ_API int kq_cache_summarize(kq_ctx* ctx, kq_cache cache, uint64_t codes_dptr, uint64_t scales_dptr, uint32_t sequences,
+                              uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens);
+KQ_API int kq_cache_select(kq_ctx* ctx, kq_cache cache, uint64_t codes_dptr, uint64_t scales_dptr, uint64_t q_dptr, uint64_t q_stride,
+                           int q_dtype, uint32_t heads, uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width,
+                           uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens, uint32_t budget, uint32_t first, uint32_t last,
+                           uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags, uint64_t selected_dptr);
+KQ_API int kq_cache_attention_selected(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads,
+                                       uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr,
+                                       uint64_t starts_dptr, uint32_t tokens, uint64_t selected_dptr, uint32_t budget, float scale,
+                                       uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags,
+                                       uint64_t out_dptr, uint64_t out_stride);
+
 /* ---- pages that sequences share ---------------------------------------------------------------
  * Who has which page of a pool, for hosts whose sequences begin alike, branch, are cut back and end.  A book of pages is
  * four device arrays of i32, the host's own:

@@ -74,6 +74,13 @@ SYMBOLS = {
     "kq_cache_read": (_i32, [_vp, _u64, _u32, _u64, _u32, _u64, _u64, _u32, _u64, _u64]),
     "kq_cache_attention": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, ctypes.c_float, _u32,
                                   _u64, _u32, _u32, _u32, _u64, _u64]),
+    "kq_cache_attention_shared": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, _u32, _u64, _u64, ctypes.c_float,
+                                         _u32, _u64, _u32, _u32, _u32, _u64, _u64]),
+    "kq_cache_summarize": (_i32, [_vp, _u64, _u64, _u64, _u32, _u64, _u32, _u64, _u64, _u32]),
+    "kq_cache_select": (_i32, [_vp, _u64, _u64, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, _u32, _u32, _u64, _u32, _u32,
+                               _u32, _u64]),
+    "kq_cache_attention_selected": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u64, _u32, ctypes.c_float, _u64, _u32,
+                                           _u32, _u32, _u64, _u64]),
     "kq_pages_grow": (_i32, [_vp, _u64, _u32, _u32, _u64, _u64, _u32, _u32, _u64, _u64]),
     "kq_pages_fork": (_i32, [_vp, _u64, _u32, _u32, _u64, _u64, _u32, _u32, _u64, _u64, _u64, _u64]),
     "kq_pages_compact": (_i32, [_vp, _u64, _u32, _u32, _u64, _u64, _u32, _u32, _u64, _u64]),

@@ -465,6 +465,43 @@ int check_batch(kq_ctx* ctx, const char* who, uint32_t sequences, uint64_t pages
   return KQ_OK;
 }
 
+// What the forms of kq_cache_attention have in common; with no rows nothing but the handle and the heads is looked at.
+int check_attention(kq_ctx* ctx, const char* who, kq_cache h, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads, uint32_t sequences,
+                    uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens, uint32_t most, float scale,
+                    uint32_t window, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride,
+                    kq::AttendArgs* out) {
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "%s cannot be recorded into a fused plan (record a graph)", who);
+  const kq::Cache* c = find_cache(ctx, h);
+  if (!c) return fail(ctx, KQ_ERR_BAD_ARG, "%s: unknown cache handle", who);
+  if (!heads || heads % c->kv_heads != 0 || heads > 65536)
+    return fail(ctx, KQ_ERR_SHAPE, "%s: %u query heads do not share %u kv heads evenly", who, heads, c->kv_heads);
+  if (!(scale > 0.0f) || !(scale < __builtin_inff())) return fail(ctx, KQ_ERR_BAD_ARG, "%s: scale must be finite and positive", who);
+  if (tokens == 0) return KQ_OK;
+  kq::AttendArgs& a = *out;
+  a.cache = *c;
+  int rc = check_batch(ctx, who, sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr, tokens, most, &a.batch);
+  if (rc == KQ_OK) rc = check_rope(ctx, who, table_dptr, table_positions, rotary, rope_flags, c->head_dim, &a.rope);
+  if (rc == KQ_OK) rc = check_rows(ctx, who, "q", q_dptr, q_stride, q_dtype, heads, c->head_dim);
+  if (rc == KQ_OK) rc = check_rows(ctx, who, "out", out_dptr, out_stride, q_dtype, heads, c->head_dim);
+  if (rc != KQ_OK) return rc;
+  if (static_cast<uint64_t>(tokens) * heads > (1ull << 30)) return fail(ctx, KQ_ERR_SHAPE, "%s: %u rows of %u heads: beyond 2^30", who, tokens, heads);
+  a.q = reinterpret_cast<const void*>(q_dptr);
+  a.out = reinterpret_cast<void*>(out_dptr);
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.dtype = q_dtype;
+  a.heads = heads;
+  a.window = window;
+  a.scale = scale;
+  return KQ_OK;
+}
+
+int check_summaries(kq_ctx* ctx, const char* who, uint64_t codes, uint64_t scales) {
+  if (!codes || !scales || (codes & 15u) || (scales & 7u))
+    return fail(ctx, KQ_ERR_BAD_ARG, "%s: summaries are device arrays: codes [pages, kv_heads, 2, head_dim] 16-byte, scales [pages, kv_heads, 2] 8-byte aligned", who);
+  return KQ_OK;
+}
+
 int check_book(kq_ctx* ctx, const char* who, uint64_t table, uint32_t sequences, uint32_t width, uint64_t lengths, uint64_t refs, uint32_t pages,
                uint32_t page_tokens, uint64_t report, kq::PageBook* out) {
   if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "%s cannot be recorded into a fused plan (record a graph)", who);
@@ -924,34 +961,97 @@ int kq_cache_attention(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t q_stri
                        uint32_t most, float scale, uint32_t window, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary,
                        uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride) {
   if (!ctx) return KQ_ERR_BAD_ARG;
-  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_cache_attention cannot be recorded into a fused plan (record a graph)");
-  const kq::Cache* c = find_cache(ctx, h);
-  if (!c) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_attention: unknown cache handle");
-  if (!heads || heads % c->kv_heads != 0 || heads > 65536)
-    return fail(ctx, KQ_ERR_SHAPE, "kq_cache_attention: %u query heads do not share %u kv heads evenly", heads, c->kv_heads);
-  if (!(scale > 0.0f) || !(scale < __builtin_inff())) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_attention: scale must be finite and positive");
-  if (tokens == 0) return KQ_OK;
   kq::AttendArgs a;
-  a.cache = *c;
-  int rc = check_batch(ctx, "kq_cache_attention", sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr, tokens, most, &a.batch);
-  if (rc == KQ_OK) rc = check_rope(ctx, "kq_cache_attention", table_dptr, table_positions, rotary, rope_flags, c->head_dim, &a.rope);
-  if (rc == KQ_OK) rc = check_rows(ctx, "kq_cache_attention", "q", q_dptr, q_stride, q_dtype, heads, c->head_dim);
-  if (rc == KQ_OK) rc = check_rows(ctx, "kq_cache_attention", "out", out_dptr, out_stride, q_dtype, heads, c->head_dim);
-  if (rc != KQ_OK) return rc;
-  if (static_cast<uint64_t>(tokens) * heads > (1ull << 30))
-    return fail(ctx, KQ_ERR_SHAPE, "kq_cache_attention: %u rows of %u heads: beyond 2^30", tokens, heads);
-  a.q = reinterpret_cast<const void*>(q_dptr);
-  a.out = reinterpret_cast<void*>(out_dptr);
-  a.q_stride = q_stride;
-  a.out_stride = out_stride;
-  a.dtype = q_dtype;
-  a.heads = heads;
-  a.window = window;
-  a.scale = scale;
+  const int rc = check_attention(ctx, "kq_cache_attention", h, q_dptr, q_stride, q_dtype, heads, sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr,
+                                 tokens, most, scale, window, table_dptr, table_positions, rotary, rope_flags, out_dptr, out_stride, &a);
+  if (rc != KQ_OK || tokens == 0) return rc;
   DeviceGuard guard(ctx->device);
   int launched = 0;
   cudaError_t e = kq::launch_attend(env_of(ctx), a, &launched);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_attention launch");
+  ctx->launches += launched;
+  return KQ_OK;
+}
+
+int kq_cache_attention_shared(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads, uint32_t sequences,
+                              uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,
+                              uint32_t most, uint32_t groups, uint64_t first_dptr, uint64_t shared_dptr, float scale, uint32_t window,
+                              uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  kq::AttendArgs a;
+  const int rc = check_attention(ctx, "kq_cache_attention_shared", h, q_dptr, q_stride, q_dtype, heads, sequences, page_table_dptr, table_width, lengths_dptr,
+                                 starts_dptr, tokens, most, scale, window, table_dptr, table_positions, rotary, rope_flags, out_dptr, out_stride, &a);
+  if (rc != KQ_OK || tokens == 0) return rc;
+  if (groups && (!first_dptr || !shared_dptr || ((first_dptr | shared_dptr) & 3u)))
+    return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_attention_shared: first [groups + 1] and shared [groups] are i32 device arrays");
+  if (groups > sequences) return fail(ctx, KQ_ERR_SHAPE, "kq_cache_attention_shared: %u groups of %u sequences", groups, sequences);
+  DeviceGuard guard(ctx->device);
+  const kq::SharedArgs sh = {reinterpret_cast<const int*>(first_dptr), reinterpret_cast<const int*>(shared_dptr), groups, nullptr, nullptr};
+  int launched = 0;
+  cudaError_t e = groups ? kq::launch_attend_shared(env_of(ctx), a, sh, &launched) : kq::launch_attend(env_of(ctx), a, &launched);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_attention_shared launch");
+  ctx->launches += launched;
+  return KQ_OK;
+}
+
+int kq_cache_attention_selected(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads, uint32_t sequences,
+                                uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,
+                                uint64_t selected_dptr, uint32_t budget, float scale, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary,
+                                uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  kq::AttendArgs a;
+  const int rc = check_attention(ctx, "kq_cache_attention_selected", h, q_dptr, q_stride, q_dtype, heads, sequences, page_table_dptr, table_width, lengths_dptr,
+                                 starts_dptr, tokens, 1, scale, 0, table_dptr, table_positions, rotary, rope_flags, out_dptr, out_stride, &a);
+  if (rc != KQ_OK || tokens == 0) return rc;
+  if (!selected_dptr || (selected_dptr & 3u) || !budget || budget > (1u << 20))
+    return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_attention_selected: selected [tokens, kv_heads, budget] is an i32 device array, budget 1..2^20");
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_attend_selected(env_of(ctx), a, kq::SelectedArgs{reinterpret_cast<const int*>(selected_dptr), budget});
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_attention_selected launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+int kq_cache_summarize(kq_ctx* ctx, kq_cache h, uint64_t codes_dptr, uint64_t scales_dptr, uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width,
+                       uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_cache_summarize cannot be recorded into a fused plan (record a graph)");
+  const kq::Cache* c = find_cache(ctx, h);
+  if (!c) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_summarize: unknown cache handle");
+  if (tokens == 0) return KQ_OK;
+  kq::CacheBatch batch;
+  int rc = check_batch(ctx, "kq_cache_summarize", sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr, tokens, 0, &batch);
+  if (rc == KQ_OK) rc = check_summaries(ctx, "kq_cache_summarize", codes_dptr, scales_dptr);
+  if (rc != KQ_OK) return rc;
+  if (static_cast<uint64_t>(tokens) * c->kv_heads > (1ull << 33)) return fail(ctx, KQ_ERR_SHAPE, "kq_cache_summarize: %u rows of %u heads: beyond 2^33", tokens, c->kv_heads);
+  DeviceGuard guard(ctx->device);
+  cudaError_t e = kq::launch_summarize(env_of(ctx), *c, batch, kq::Summaries{reinterpret_cast<uint8_t*>(codes_dptr), reinterpret_cast<float*>(scales_dptr)});
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_summarize launch");
+  ctx->launches += 1;
+  return KQ_OK;
+}
+
+int kq_cache_select(kq_ctx* ctx, kq_cache h, uint64_t codes_dptr, uint64_t scales_dptr, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads,
+                    uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,
+                    uint32_t budget, uint32_t first, uint32_t last, uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags,
+                    uint64_t selected_dptr) {
+  if (!ctx) return KQ_ERR_BAD_ARG;
+  kq::AttendArgs a;
+  int rc = check_attention(ctx, "kq_cache_select", h, q_dptr, q_stride, q_dtype, heads, sequences, page_table_dptr, table_width, lengths_dptr, starts_dptr, tokens,
+                           1, 1.0f, 0, table_dptr, table_positions, rotary, rope_flags, q_dptr, q_stride, &a);
+  if (rc == KQ_OK && tokens) rc = check_summaries(ctx, "kq_cache_select", codes_dptr, scales_dptr);
+  if (rc != KQ_OK || tokens == 0) return rc;
+  if (!selected_dptr || (selected_dptr & 3u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_select: selected [tokens, kv_heads, budget] is an i32 device array");
+  if (!budget || budget > (1u << 20) || !last || static_cast<uint64_t>(first) + last > budget)
+    return fail(ctx, KQ_ERR_SHAPE, "kq_cache_select: %u pages, the first %u and the last %u of them always: 1..2^20, at least the last one, no more than all", budget, first, last);
+  if (!ctx->workspace || kq::select_scratch_bytes(a) > ctx->workspace_bytes)
+    return fail(ctx, KQ_ERR_UNSUPPORTED, "kq_cache_select: needs %llu bytes of scratch, the context has %llu (kq_init)", (unsigned long long)kq::select_scratch_bytes(a),
+                (unsigned long long)ctx->workspace_bytes);
+  DeviceGuard guard(ctx->device);
+  int launched = 0;
+  cudaError_t e = kq::launch_select(env_of(ctx), a, kq::Summaries{reinterpret_cast<uint8_t*>(codes_dptr), reinterpret_cast<float*>(scales_dptr)}, budget, first, last,
+                                    reinterpret_cast<int*>(selected_dptr), &launched);
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_select launch");
   ctx->launches += launched;
   return KQ_OK;
 }

@@ -1,0 +1,50 @@
+// Attention of sequences that begin alike: the keys that a group of them has in common are read once.
+//
+//   out = (2^(M - m) O + 2^(M' - m) O') / (2^(M - m) l + 2^(M' - m) l'),   m = max(M, M')
+//
+// for the sums (M, l, O) over the common keys and (M', l', O') over a sequence's own: l sums 2^(s - M), O the same times the values.
+// Two launches over the same call: the first makes groups sequences of their own, whose rows are all their members' new ones and whose
+// keys are the common ones, and leaves (M, l, O) in the scratch; the second walks over the keys behind them and joins.
+#include "kq_attend_few.cuh"
+
+namespace kq {
+
+bool attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, const SharedArgs& sh, cudaError_t* e);
+cudaError_t attend_shared_rest_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
+
+cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, SharedArgs sh, int* launches) {
+  const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, floats = rows * (a.cache.head_dim + 2);
+  // The sums take the end of the scratch.  Where they would take more than half of it, every sequence walks over all of its keys.
+  if (!env.workspace || floats * sizeof(float) + 16 > env.workspace_bytes / 2) return launch_attend(env, a, launches);
+  LaunchEnv in = env;
+  in.workspace_bytes = (env.workspace_bytes - floats * sizeof(float)) / 16 * 16;
+  sh.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(env.workspace) + in.workspace_bytes);
+  sh.stats = reinterpret_cast<float2*>(sh.sums + rows * a.cache.head_dim);
+  *launches = 0;
+  const uint64_t group = a.heads / a.cache.kv_heads;
+  cudaError_t e = cudaSuccess;
+  for (uint32_t g = 0; g < sh.groups && e == cudaSuccess; g += 128) {
+    SharedArgs some = sh;
+    some.first += g;
+    some.tokens += g;
+    some.groups = std::min(sh.groups - g, 128u);
+    if (!attend_shared_prefix_many(in, a, some, &e)) {
+      FewParams p = few_params(in, a, 0xFFFFFFFFu);
+      p.prefix = true;
+      p.sh = some;
+      e = launch_few<kShared>(in, p, (a.batch.tokens + sh.groups - 1) / sh.groups * group);
+    }
+    *launches += 1;
+  }
+  if (e != cudaSuccess) return e;
+  const uint64_t own = static_cast<uint64_t>(a.batch.most) * group;
+  const bool many = own > kFewRows && attend_many_supports(a);
+  FewParams p = few_params(in, a, many ? kFewRows : 0xFFFFFFFFu);
+  p.sh = sh;
+  e = launch_few<kShared>(in, p, many ? kFewRows : own);
+  if (e == cudaSuccess && many) e = attend_shared_rest_many(in, a, kFewRows, sh);
+  *launches += many ? 2 : 1;
+  return e;
+}
+
+}  // namespace kq

@@ -53,6 +53,68 @@ __device__ __forceinline__ uint32_t sequence_of(const CacheBatch& batch, uint32_
   return lo;
 }
 
+// Position of the sequence's token that row `row` of the call is, and how many tokens the sequence has in front of its new ones.
+__device__ __forceinline__ int2 place_of_row(const CacheBatch& batch, uint32_t row) {
+  const Span s = span_of(batch, sequence_of(batch, row));
+  const int before = s.length - s.count;
+  return make_int2(before + static_cast<int>(row) - s.first, max(before, 0));
+}
+
+// ---- sequences that begin alike ---------------------------------------------------------------
+__device__ __forceinline__ uint32_t first_of_group(const CacheBatch& batch, const SharedArgs& sh, uint32_t g) {
+  return min(static_cast<uint32_t>(max(__ldg(sh.first + g), 0)), batch.sequences - 1);
+}
+// How many keys sequence b has in common with its group, all of them in front of its new tokens; 0 where it is in none.
+__device__ __forceinline__ int common_keys(const CacheBatch& batch, const SharedArgs& sh, uint32_t b, const Span& span) {
+  uint32_t lo = 0, hi = sh.groups;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (__ldg(sh.first + mid) <= static_cast<int>(b)) lo = mid;
+    else hi = mid;
+  }
+  if (__ldg(sh.first + lo) > static_cast<int>(b) || __ldg(sh.first + lo + 1) <= static_cast<int>(b)) return 0;
+  return min(max(__ldg(sh.tokens + lo), 0), max(span.length - span.count, 0));
+}
+// By a warp: the new rows of group g's sequences (first, number), the keys that any of them has in common, the first of these that a row
+// sees; every: first and last of the keys that all the rows see.
+__device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const SharedArgs& sh, uint32_t g, int window, int2& every) {
+  const int sequences = static_cast<int>(batch.sequences), tokens = static_cast<int>(batch.tokens);
+  const int b0 = min(max(__ldg(sh.first + g), 0), sequences), b1 = min(max(__ldg(sh.first + g + 1), b0), sequences);
+  const int row0 = min(batch.starts ? max(batch.starts[b0], 0) : b0, tokens), row1 = min(max(batch.starts ? batch.starts[b1] : b1, row0), tokens);
+  int least = 0x7fffffff, far = 0, last = -1;
+  for (int b = b0 + static_cast<int>(threadIdx.x % 32); b < b1; b += 32) {
+    const Span s = span_of(batch, static_cast<uint32_t>(b));
+    if (s.count == 0) continue;
+    least = min(least, s.length - s.count);
+    far = max(far, s.length - s.count);
+    last = max(last, s.length - 1);
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  far = __reduce_max_sync(0xffffffffu, far);
+  last = __reduce_max_sync(0xffffffffu, last);
+  const int keys = min(max(__ldg(sh.tokens + g), 0), far);
+  // (a window may hide all of them: one is walked over all the same, so that the rows' sums are written)
+  const int from = window && least >= window ? min(least - window + 1, max(keys - 1, 0)) : 0;
+  every = make_int2(window && last >= window ? last - window + 1 : 0, min(keys, max(least, 0)) - 1);
+  return make_int4(row0, row1 - row0, keys, from);
+}
+
+// ---- rows that attend to selected pages -------------------------------------------------------
+// (sequence, position, keys, 0): the pages in the list's order, the last one up to the position; no keys where the row is no sequence's.
+__device__ __forceinline__ int4 selected_row(const AttendArgs& a, const SelectedArgs& sel, uint32_t row) {
+  const uint32_t b = sequence_of(a.batch, row);
+  const Span s = span_of(a.batch, b);
+  const int in = static_cast<int>(row) - s.first, position = s.length - s.count + in;
+  if (in < 0 || in >= s.count || position < 0) return make_int4(static_cast<int>(b), position, 0, 0);
+  const int page_tokens = static_cast<int>(a.cache.page_tokens), pages = static_cast<int>(min(sel.budget, static_cast<uint32_t>(position / page_tokens) + 1));
+  return make_int4(static_cast<int>(b), position, (pages - 1) * page_tokens + position % page_tokens + 1, 0);
+}
+// The number of the row's index-th page for a kv head; no page's where the list or the table has none.
+__device__ __forceinline__ uint32_t selected_page(const AttendArgs& a, const SelectedArgs& sel, uint32_t row, uint32_t head, int sequence, uint32_t index) {
+  const uint32_t at = static_cast<uint32_t>(__ldg(sel.pages + (static_cast<size_t>(row) * a.cache.kv_heads + head) * sel.budget + index));
+  return at < a.batch.width ? static_cast<uint32_t>(__ldg(a.batch.pages + static_cast<size_t>(sequence) * a.batch.width + at)) : 0xFFFFFFFFu;
+}
+
 // The rotation of one pair, every product and sum rounded to f32 (what a key is held as does not depend on the kernel).
 __device__ __forceinline__ float2 rotate_pair(float x0, float x1, float2 cs) {
   return make_float2(__fsub_rn(__fmul_rn(x0, cs.x), __fmul_rn(x1, cs.y)), __fadd_rn(__fmul_rn(x1, cs.x), __fmul_rn(x0, cs.y)));

@@ -232,6 +232,18 @@ struct AttendArgs {
   uint32_t heads, window;
   float scale;
 };
+// Groups of neighbouring sequences that begin with the same tokens (device arrays), and what their rows' sums over those are.
+struct SharedArgs {
+  const int* first;   // [groups + 1] first sequence of each
+  const int* tokens;  // [groups]
+  uint32_t groups;
+  float* sums;        // [tokens of the call][heads][head_dim], not divided yet
+  float2* stats;      // [tokens of the call][heads] (exponent of two that the weights are relative to, their sum)
+};
+struct SelectedArgs {
+  const int* pages;  // [tokens of the call][kv_heads][budget] indices of a sequence's pages, ascending
+  uint32_t budget;
+};
 cudaError_t launch_rope(const LaunchEnv& env, const void* x, int dtype, uint32_t tokens, uint32_t heads, uint32_t dim, uint64_t x_stride,
                         const int* positions, const RopeTable& rope, void* out, uint64_t out_stride);
 cudaError_t launch_cache_append(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, const void* k, uint64_t k_stride,
@@ -240,6 +252,18 @@ cudaError_t launch_cache_read(const LaunchEnv& env, const Cache& cache, const Ca
 cudaError_t launch_attend(const LaunchEnv& env, const AttendArgs& args, int* launches);
 // Its kernel for sequences whose new tokens make more than `beyond` query rows a kv head (kq_attend_many.cu).
 bool attend_many_supports(const AttendArgs& args);
+// Sequences that begin alike (kq_attend_shared.cu); rows that attend to selected pages (kq_attend_selected.cu).
+cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& args, SharedArgs shared, int* launches);
+cudaError_t launch_attend_selected(const LaunchEnv& env, const AttendArgs& args, const SelectedArgs& selected);
+// Summaries of pages and the selection by them (kq_select.cu); args.q's rows select, args.out is not used.
+struct Summaries {
+  uint8_t* codes;  // [pages][kv_heads][2][head_dim] int8
+  float* scales;   // [pages][kv_heads][2]
+};
+cudaError_t launch_summarize(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, const Summaries& to);
+uint64_t select_scratch_bytes(const AttendArgs& args);  // at least so much of LaunchEnv::workspace
+cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& args, const Summaries& from, uint32_t budget, uint32_t first, uint32_t last, int* out,
+                          int* launches);
 cudaError_t launch_attend_many(const LaunchEnv& env, const AttendArgs& args, uint32_t beyond);
 }  // namespace kq
 

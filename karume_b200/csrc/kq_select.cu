@@ -1,0 +1,379 @@
+// Which pages of a long sequence a query attends to: a summary of each page's keys, a cheap score of it, the pages with the largest.
+//
+//   summary  of a page and kv head, over the page's tokens, for each channel: c = (max + min) / 2, r = (max - min) / 2 of what the keys
+//            stand for; both rows as 8-bit codes with a scale, by kq_quantize_rows' rule
+//   score    a query held likewise (codes a, scale s): s ((a . c) s_c + (|a| . r) s_r), which bounds s a . k over the page's keys;
+//            the largest of the query heads that share the kv head
+//   select   the first and last pages and, up to the budget, those with the largest scores, ties to the lower page
+//
+// The dot products are of whole numbers, up to 127 * 127 * 256, which f32 holds exactly, and each of the few roundings behind them is
+// part of the definition: which pages are selected does not depend on the order of any sum.
+#include <algorithm>
+
+#include "kq_cache.cuh"
+
+namespace kq {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kTiny = 1.17549435e-38f;
+
+__device__ __forceinline__ float scale_of(float largest) { return fmaxf(__fmul_rn(largest, 1.0f / 127.0f), kTiny); }
+__device__ __forceinline__ int code_of(float x, float scale) { return static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.0f), 127.0f)); }
+__device__ __forceinline__ uint32_t pack4(const int* v) {
+  return static_cast<uint32_t>(v[0] & 255) | static_cast<uint32_t>(v[1] & 255) << 8 | static_cast<uint32_t>(v[2] & 255) << 16 | static_cast<uint32_t>(v[3]) << 24;
+}
+
+// ---- summaries ------------------------------------------------------------------------------
+struct SummaryParams {
+  Cache cache;
+  CacheBatch batch;
+  Summaries to;
+};
+
+// A warp for each (new token, kv head); those whose token is not the first of the call in its page have nothing to do.
+template <int D>
+__global__ void __launch_bounds__(kThreads) summarize_kernel(const SummaryParams p) {
+  constexpr int kLanes = D / 8, kTokens = 32 / kLanes;  // lanes of a token (eight channels each), tokens at a time
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const uint32_t lane = threadIdx.x % 32, heads = p.cache.kv_heads;
+  const uint64_t at = (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / 32;
+  if (at >= static_cast<uint64_t>(p.batch.tokens) * heads) return;
+  const uint32_t row = static_cast<uint32_t>(at / heads), head = static_cast<uint32_t>(at % heads), b = sequence_of(p.batch, row);
+  const Span span = span_of(p.batch, b);
+  const int in = static_cast<int>(row) - span.first, position = span.length - span.count + in;
+  const int P = static_cast<int>(p.cache.page_tokens);
+  if (in < 0 || in >= span.count || position < 0 || (in != 0 && position % P != 0)) return;
+  const uint32_t index = static_cast<uint32_t>(position / P);
+  const uint8_t* const block = cache_block(p.cache, p.batch, b, index, head);
+  if (!block) return;
+  const int tokens = min(P, span.length - static_cast<int>(index) * P);
+  const uint32_t channel = lane % kLanes * 8;
+  float low[8], high[8];
+  bool lost = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    low[i] = INFINITY;
+    high[i] = -INFINITY;
+  }
+#pragma unroll 8
+  for (int t = static_cast<int>(lane / kLanes); t < tokens; t += kTokens) {
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(block + t * (D / 2) + channel / 2);
+    const float2 so = __half22float2(*reinterpret_cast<const __half2*>(block + P * D + t * 4));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = fmaf(static_cast<float>(word >> (4 * i) & 15u), so.x, so.y);
+      low[i] = fminf(low[i], x);
+      high[i] = fmaxf(high[i], x);
+    }
+    lost |= !(fabsf(so.x) <= 65504.0f && fabsf(so.y) <= 65504.0f);
+  }
+  float most_c = 0.0f, most_r = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int o = kLanes; o < 32; o *= 2) {
+      low[i] = fminf(low[i], __shfl_xor_sync(0xffffffffu, low[i], o));
+      high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], o));
+    }
+    const float c = __fmul_rn(__fadd_rn(high[i], low[i]), 0.5f), r = __fmul_rn(__fsub_rn(high[i], low[i]), 0.5f);
+    low[i] = c;
+    high[i] = r;
+    most_c = fmaxf(most_c, fabsf(c));
+    most_r = fmaxf(most_r, r);
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o *= 2) {
+    most_c = fmaxf(most_c, __shfl_xor_sync(0xffffffffu, most_c, o));
+    most_r = fmaxf(most_r, __shfl_xor_sync(0xffffffffu, most_r, o));
+  }
+  lost = __any_sync(0xffffffffu, lost);  // a key that is NaN, or of an infinite scale: nothing can be said of the page
+  const float scale_c = scale_of(most_c), scale_r = scale_of(most_r);
+  if (lane >= kLanes) return;
+  int c[8], r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = lost ? 0 : code_of(low[i], scale_c);
+    r[i] = lost ? 0 : code_of(high[i], scale_r);
+  }
+  const size_t of = (static_cast<size_t>(block - p.cache.pool) / cache_block_bytes(p.cache.page_tokens, D)) * 2;  // page * heads + head, twice
+  *reinterpret_cast<uint2*>(p.to.codes + of * D + channel) = make_uint2(pack4(c), pack4(c + 4));
+  *reinterpret_cast<uint2*>(p.to.codes + (of + 1) * D + channel) = make_uint2(pack4(r), pack4(r + 4));
+  if (lane == 0) {
+    p.to.scales[of] = lost ? quiet_nan() : scale_c;
+    p.to.scales[of + 1] = lost ? quiet_nan() : scale_r;
+  }
+}
+
+// ---- scores ---------------------------------------------------------------------------------
+struct SelectParams {
+  AttendArgs a;
+  Summaries from;
+  uint32_t group, budget, first, last;
+  uint32_t row0, rows;  // rows of this launch
+  uint32_t chunks;      // blocks that share a row's pages
+  uint32_t* keys;       // [rows][kv_heads][table width]
+  int* out;             // [tokens][kv_heads][budget]
+};
+
+constexpr int kScoreWarps = 4, kScorePages = 64;  // pages of a block: sixteen a warp at a time
+constexpr uint32_t kAlways = 0xFFFFFFFFu, kUnknown = 0xFFFFFFFEu;
+
+// A number that is larger where the score is; not a number: larger than any.
+__device__ __forceinline__ uint32_t key_of(float score) {
+  const uint32_t bits = __float_as_uint(__fadd_rn(score, 0.0f));  // one zero
+  if (score != score) return kUnknown;
+  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The pages up to a row's position, or 0 where the row is no sequence's; and the sequence.
+__device__ __forceinline__ int2 pages_of_row(const AttendArgs& a, uint32_t row) {
+  const uint32_t b = sequence_of(a.batch, row);
+  const Span s = span_of(a.batch, b);
+  const int in = static_cast<int>(row) - s.first, position = s.length - s.count + in;
+  if (in < 0 || in >= s.count || position < 0) return make_int2(0, static_cast<int>(b));
+  return make_int2(static_cast<int>(min(static_cast<uint32_t>(position) / a.cache.page_tokens + 1, a.batch.width)), static_cast<int>(b));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_constant__ SelectParams p) {
+  constexpr int kHeads = 8;  // columns of an MMA
+  __shared__ __align__(16) uint8_t codes[2][kHeads][D + 16];  // a, |a| (rows 16 bytes apart from a multiple of 128: lanes of eight rows meet no bank twice)
+  __shared__ float scales[kHeads];
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4, heads = p.a.cache.kv_heads;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const uint32_t chunk = blockIdx.x % p.chunks, at = blockIdx.x / p.chunks, head = at % heads, row = p.row0 + at / heads;
+  const int2 of = pages_of_row(p.a, row);
+  const int pages = of.x, first = static_cast<int>(chunk) * kScorePages;
+  if (first >= pages || pages <= static_cast<int>(p.budget)) return;  // all are taken
+  uint32_t* const keys = p.keys + (static_cast<size_t>(at) / heads * heads + head) * p.a.batch.width;
+  const int position = place_of_row(p.a.batch, row).x;
+  float best[2] = {-INFINITY, -INFINITY};
+  bool unknown[2] = {false, false};
+  const int base = first + static_cast<int>(warp) * 16;
+  for (uint32_t h0 = 0; h0 < p.group; h0 += kHeads) {
+    if (h0) __syncthreads();
+    for (uint32_t h = warp; h < kHeads; h += kScoreWarps) {  // a query head a warp
+      float x[8] = {};
+      if (h0 + h < p.group && lane < D / 8)
+        load8_rotated(static_cast<const T*>(p.a.q) + static_cast<size_t>(row) * p.a.q_stride + static_cast<size_t>(head * p.group + h0 + h) * D, lane * 8, p.a.rope,
+                      position, x);
+      float most = 0.0f;
+      bool lost = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        most = fmaxf(most, fabsf(x[i]));
+        lost |= !(fabsf(x[i]) < INFINITY);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      lost = __any_sync(0xffffffffu, lost);
+      const float scale = scale_of(most);
+      int a[8], m[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] = lost ? 0 : code_of(x[i], scale);
+        m[i] = abs(a[i]);
+      }
+      if (lane < D / 8) {
+        *reinterpret_cast<uint2*>(&codes[0][h][lane * 8]) = make_uint2(pack4(a), pack4(a + 4));
+        *reinterpret_cast<uint2*>(&codes[1][h][lane * 8]) = make_uint2(pack4(m), pack4(m + 4));
+      }
+      if (lane == 0) scales[h] = lost ? quiet_nan() : scale;
+    }
+    __syncthreads();
+    if (base >= pages) continue;
+    // sixteen pages: rows g and g + 8 of the MMA, sixteen channels of 64 a lane; the order of the channels is the queries' too
+    int acc[2][4] = {};
+    float2 by[2];
+    const uint8_t* rows[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int index = base + static_cast<int>(g) + i * 8;
+      const uint32_t page = index < pages ? static_cast<uint32_t>(__ldg(p.a.batch.pages + static_cast<size_t>(of.y) * p.a.batch.width + index)) : 0xFFFFFFFFu;
+      const bool there = page < p.a.cache.pages;
+      const size_t place = (static_cast<size_t>(there ? page : 0) * heads + head) * 2;
+      rows[i] = p.from.codes + place * D + t * 16;
+      by[i] = there ? __ldg(reinterpret_cast<const float2*>(p.from.scales + place)) : make_float2(quiet_nan(), quiet_nan());
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(rows[0] + which * D + j * 64)), y = __ldg(reinterpret_cast<const uint4*>(rows[1] + which * D + j * 64));
+        const uint4 q = *reinterpret_cast<const uint4*>(&codes[which][g][j * 64 + t * 16]);
+        mma_s8(acc[which], x.x, y.x, x.y, y.y, q.x, q.y);
+        mma_s8(acc[which], x.z, y.z, x.w, y.w, q.z, q.w);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t h = 2 * t + k;
+        if (h0 + h >= p.group) continue;
+        const float sum = __fadd_rn(__fmul_rn(static_cast<float>(acc[0][2 * i + k]), by[i].x), __fmul_rn(static_cast<float>(acc[1][2 * i + k]), by[i].y));
+        const float score = __fmul_rn(sum, scales[h]);
+        unknown[i] |= score != score;
+        best[i] = fmaxf(best[i], score);
+      }
+  }
+  if (base >= pages) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 1; o < 4; o *= 2) {
+      best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], o));
+      unknown[i] |= __shfl_xor_sync(0xffffffffu, static_cast<int>(unknown[i]), o) != 0;
+    }
+    const int index = base + static_cast<int>(g) + i * 8;
+    if (t == 0 && index < pages)
+      keys[index] = index < static_cast<int>(p.first) || index >= pages - static_cast<int>(p.last) ? kAlways : unknown[i] ? kUnknown : key_of(best[i]);
+  }
+}
+
+// ---- the largest ----------------------------------------------------------------------------
+// A block for each (row, kv head): the budget-th largest key, digit by digit, then the pages above it in order.
+constexpr int kKept = 8192;  // keys in shared memory
+
+__global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectParams p) {
+  __shared__ uint32_t kept[kKept];
+  __shared__ uint32_t count[256];
+  __shared__ uint32_t warps[kThreads / 32], chosen[2];
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, heads = p.a.cache.kv_heads;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
+  const uint32_t row = p.row0 + blockIdx.x / heads;
+  const uint32_t pages = static_cast<uint32_t>(pages_of_row(p.a, row).x);
+  int* const out = p.out + (static_cast<size_t>(row) * heads + blockIdx.x % heads) * p.budget;
+  if (pages <= p.budget) {
+    for (uint32_t i = tid; i < p.budget; i += kThreads) out[i] = i < pages ? static_cast<int>(i) : -1;
+    return;
+  }
+  const uint32_t* const keys = p.keys + static_cast<size_t>(blockIdx.x) * p.a.batch.width;
+  const auto key = [&](uint32_t i) { return i < kKept ? kept[i] : __ldcg(keys + i); };
+  for (uint32_t i = tid; i < min(pages, static_cast<uint32_t>(kKept)); i += kThreads) kept[i] = __ldcg(keys + i);
+  uint32_t digits = 0, left = p.budget;  // the digits found so far; how many of the keys that begin with them are taken
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    count[tid] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < pages; i += kThreads) {
+      const uint32_t k = key(i);
+      if (shift == 24 || k >> (shift + 8) == digits) atomicAdd(&count[k >> shift & 255u], 1u);
+    }
+    __syncthreads();
+    // keys of larger digits: a sum from the top
+    const uint32_t mine = count[255 - tid];
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= static_cast<uint32_t>(o)) upto += v;
+    }
+    if (lane == 31) warps[warp] = upto;
+    __syncthreads();
+    for (uint32_t i = 0; i < warp; ++i) upto += warps[i];
+    if (upto - mine < left && left <= upto) {
+      chosen[0] = 255 - tid;
+      chosen[1] = left - (upto - mine);
+    }
+    __syncthreads();
+    digits = digits << 8 | chosen[0];
+    left = chosen[1];
+  }
+  uint32_t before = 0, equal = 0;
+  for (uint32_t i0 = 0; i0 < pages; i0 += kThreads) {
+    const uint32_t i = i0 + tid, k = i < pages ? key(i) : 0u;
+    const bool above = i < pages && k > digits, same = i < pages && k == digits;
+    // both counts of the threads in front, sixteen bits each
+    const uint32_t mine = (above ? 1u : 0u) | (same ? 0x10000u : 0u);
+    const uint32_t a = __ballot_sync(0xffffffffu, above), s = __ballot_sync(0xffffffffu, same), in_front = (1u << lane) - 1;
+    if (lane == 0) warps[warp] = __popc(a) | __popc(s) << 16;
+    __syncthreads();
+    uint32_t sum = __popc(a & in_front) | __popc(s & in_front) << 16, all = 0;
+    for (uint32_t w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) sum += warps[w];
+      all += warps[w];
+    }
+    __syncthreads();
+    const uint32_t equal_before = equal + (sum >> 16);
+    if (mine) {
+      const uint32_t to = before + (sum & 0xFFFFu) + min(equal_before, left);
+      if (above || equal_before < left) out[to] = static_cast<int>(i);
+    }
+    before += all & 0xFFFFu;
+    equal += all >> 16;
+  }
+}
+
+template <typename Kernel, typename Params>
+cudaError_t launch_after(const LaunchEnv& env, Kernel kernel, uint64_t grid, int threads, const Params& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = env.stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = env.overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T>
+cudaError_t score_as(const LaunchEnv& env, const SelectParams& p) {
+  const uint64_t grid = static_cast<uint64_t>(p.rows) * p.a.cache.kv_heads * p.chunks;
+  switch (p.a.cache.head_dim) {
+    case 64: return launch_after(env, score_kernel<T, 64>, grid, kScoreWarps * 32, p);
+    case 128: return launch_after(env, score_kernel<T, 128>, grid, kScoreWarps * 32, p);
+    case 256: return launch_after(env, score_kernel<T, 256>, grid, kScoreWarps * 32, p);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_summarize(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, const Summaries& to) {
+  const SummaryParams p = {cache, batch, to};
+  const uint64_t grid = (static_cast<uint64_t>(batch.tokens) * cache.kv_heads * 32 + kThreads - 1) / kThreads;
+  switch (cache.head_dim) {
+    case 64: return launch_after(env, summarize_kernel<64>, grid, kThreads, p);
+    case 128: return launch_after(env, summarize_kernel<128>, grid, kThreads, p);
+    case 256: return launch_after(env, summarize_kernel<256>, grid, kThreads, p);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+uint64_t select_scratch_bytes(const AttendArgs& a) { return 4ull * a.cache.kv_heads * a.batch.width; }
+
+cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& a, const Summaries& from, uint32_t budget, uint32_t first, uint32_t last, int* out, int* launches) {
+  SelectParams p;
+  p.a = a;
+  p.from = from;
+  p.group = a.heads / a.cache.kv_heads;
+  p.budget = budget;
+  p.first = first;
+  p.last = last;
+  p.keys = static_cast<uint32_t*>(env.workspace);
+  p.out = out;
+  p.chunks = (a.batch.width + kScorePages - 1) / kScorePages;
+  *launches = 0;
+  // as many rows at a time as have room in the scratch and in a grid
+  const uint64_t room = std::min<uint64_t>(env.workspace_bytes / select_scratch_bytes(a), ((1ull << 31) - 1) / (static_cast<uint64_t>(a.cache.kv_heads) * p.chunks));
+  for (uint32_t row = 0; row < a.batch.tokens; row += p.rows) {
+    p.row0 = row;
+    p.rows = static_cast<uint32_t>(std::min<uint64_t>(a.batch.tokens - row, std::max<uint64_t>(room, 1)));
+    cudaError_t e = a.dtype == KQ_F32 ? score_as<float>(env, p) : a.dtype == KQ_F16 ? score_as<__half>(env, p) : score_as<__nv_bfloat16>(env, p);
+    if (e == cudaSuccess) e = launch_after(env, select_kernel, static_cast<uint64_t>(p.rows) * a.cache.kv_heads, kThreads, p);
+    if (e != cudaSuccess) return e;
+    *launches += 2;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace kq

@@ -153,6 +153,40 @@ class KvCache:
             self.handle = 0
 
 
+class SharedPrefixes:
+    """Sequences that begin alike: first i32 CUDA [groups + 1] (group g is the sequences first[g] .. first[g + 1] - 1) and tokens i32 [groups],
+    how many tokens the sequences of each have in common at their beginning, in the same pages or copies of them."""
+
+    def __init__(self, first, tokens):
+        torch = _torch()
+        for name, t in (("first", first), ("tokens", tokens)):
+            if t.dtype != torch.int32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
+                raise KqError(2, f"{name} must be a contiguous CUDA int32 tensor of one dimension")
+        self.groups = int(tokens.numel())
+        if first.numel() != self.groups + 1:
+            raise KqError(2, f"{self.groups} groups have {self.groups + 1} boundaries, not {first.numel()}")
+        self.first, self.tokens = first, tokens
+        self.args = (self.groups, first.data_ptr(), tokens.data_ptr())
+
+
+class CacheSummaries:
+    """What Gpu.cache_select goes by: codes int8 CUDA [pages, kv_heads, 2, head_dim] and scales f32 [pages, kv_heads, 2] of each page's keys
+    (channels' middles and half spreads), kept up by Gpu.cache_summarize.  Gpu.cache_summaries makes them for a cache."""
+
+    def __init__(self, codes, scales):
+        torch = _torch()
+        if codes.dtype != torch.int8 or scales.dtype != torch.float32 or not (codes.is_cuda and scales.is_cuda) or codes.dim() != 4 or scales.dim() != 3 or \
+                tuple(scales.shape) != tuple(codes.shape[:3]) or codes.shape[2] != 2 or not (codes.is_contiguous() and scales.is_contiguous()):
+            raise KqError(2, "summaries are contiguous CUDA tensors: codes int8 [pages, kv_heads, 2, head_dim], scales f32 [pages, kv_heads, 2]")
+        self.codes, self.scales = codes, scales
+        self.args = (codes.data_ptr(), scales.data_ptr())
+
+    def check(self, cache: "KvCache") -> None:
+        shape = tuple(self.codes.shape)
+        if shape[0] < cache.pages or shape[1] != cache.kv_heads or shape[3] != cache.head_dim:
+            raise KqError(2, f"summaries {list(shape)} are not those of {cache.pages} pages of {cache.kv_heads} heads of {cache.head_dim}")
+
+
 class CachePages:
     """Which page belongs to whom: table i32 CUDA [sequences, width] (a CacheBatch's pages; -1 behind a sequence's own), lengths i32
     [sequences], refs i32 [pages] (how many entries name a page) and report i32 [4] of the last call: pages that were missing (then, and
@@ -508,18 +542,21 @@ class Gpu:
         return k, v
 
     def cache_attention(self, cache: KvCache, q, batch: CacheBatch, scale: "float | None" = None, window: int = 0,
-                        rope: "Rope | None" = None, out=None):
+                        rope: "Rope | None" = None, out=None, shared: "SharedPrefixes | None" = None, selected=None):
         """Causal attention of q [tokens, heads, head_dim] (f32 / f16 / bf16, rotated on the way) over each sequence's keys
-        in the cache, the last `window` of them if given; scale defaults to head_dim^-0.5.  Returns q's type."""
+        in the cache, the last `window` of them if given; scale defaults to head_dim^-0.5.  Returns q's type.
+        shared: what groups of the sequences have in common is read once.  selected: each row sees the tokens of the pages that
+        cache_select chose for it."""
         if scale is None:
             scale = cache.head_dim ** -0.5
         if window < 0:
             raise KqError(2, f"window {window}: a number of keys, 0 for all")
         window = min(int(window), 0xFFFFFFFF)  # the ABI's number has 32 bits; no sequence is longer
-        done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window,
-                                     rope.args if rope is not None else None, out)
-        if done is not None:
-            return self._done(done)
+        if shared is None and selected is None:
+            done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window,
+                                         rope.args if rope is not None else None, out)
+            if done is not None:
+                return self._done(done)
         torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
@@ -530,9 +567,54 @@ class Gpu:
         elif out.dtype != q.dtype or out.shape != q.shape:
             raise KqError(2, "out must have q's type and shape")
         po, out_stride = _rows(out, heads, dim, "out")
-        self._check(L.kq_cache_attention(self._ctx, cache.handle, pq, q_stride, _tensor_dtype_code(q), heads, *batch.args, batch.most,
-                                         float(scale), window,
-                                         *(rope.args if rope is not None else _NO_ROPE), po, out_stride))
+        head = (self._ctx, cache.handle, pq, q_stride, _tensor_dtype_code(q), heads, *batch.args)
+        tail = (*(rope.args if rope is not None else _NO_ROPE), po, out_stride)
+        if selected is not None:
+            if window or shared is not None:
+                raise KqError(2, "selected pages are all that a row sees: no window, no shared prefixes")
+            if selected.dtype != torch.int32 or not selected.is_cuda or not selected.is_contiguous() or selected.dim() != 3 or \
+                    tuple(selected.shape[:2]) != (batch.tokens, cache.kv_heads):
+                raise KqError(2, f"selected must be a contiguous CUDA int32 tensor [{batch.tokens}, {cache.kv_heads}, budget]")
+            self._check(L.kq_cache_attention_selected(*head, selected.data_ptr(), selected.shape[2], float(scale), *tail))
+        elif shared is not None:
+            self._check(L.kq_cache_attention_shared(*head, batch.most, *shared.args, float(scale), window, *tail))
+        else:
+            self._check(L.kq_cache_attention(*head, batch.most, float(scale), window, *tail))
+        return out
+
+    # -- pages that a query selects ---------------------------------------------------------------
+    def cache_summaries(self, cache: KvCache) -> CacheSummaries:
+        """Empty summaries for the pages of a cache."""
+        torch = _torch()
+        shape = (cache.pages, cache.kv_heads, 2)
+        made = CacheSummaries(torch.zeros((*shape, cache.head_dim), dtype=torch.int8, device=self.device), torch.zeros(shape, device=self.device))
+        torch.cuda.current_stream(self.device).synchronize()  # the first call may run on another stream than torch's current one
+        return made
+
+    def cache_summarize(self, cache: KvCache, summaries: CacheSummaries, batch: CacheBatch) -> None:
+        """Brings the summaries of the pages that the batch's new tokens are in up to date (behind cache_append)."""
+        summaries.check(cache)
+        self._check(L.kq_cache_summarize(self._ctx, cache.handle, *summaries.args, *batch.args))
+
+    def cache_select(self, cache: KvCache, summaries: CacheSummaries, q, batch: CacheBatch, budget: int, first: int = 1, last: int = 1,
+                     rope: "Rope | None" = None, out=None):
+        """Up to `budget` pages for every row of q [tokens, heads, head_dim] and kv head, int32 [tokens, kv_heads, budget]: ascending indices into
+        the sequence's pages, -1 behind them; always the first `first` and the last `last` ones, then those whose summaries promise most."""
+        torch = _torch()
+        summaries.check(cache)
+        heads, dim = int(q.shape[1]), cache.head_dim
+        if q.shape[0] != batch.tokens:
+            raise KqError(2, f"q must have {batch.tokens} rows")
+        if min(budget, first, last) < 0:
+            raise KqError(2, f"{budget} pages, the first {first} and the last {last}: no negative numbers")
+        pq, q_stride = _rows(q, heads, dim, "q")
+        shape = (batch.tokens, cache.kv_heads, int(budget))
+        if out is None:
+            out = torch.empty(shape, dtype=torch.int32, device=q.device)
+        elif out.dtype != torch.int32 or not out.is_cuda or not out.is_contiguous() or tuple(out.shape) != shape:
+            raise KqError(2, f"out must be a contiguous CUDA int32 tensor {list(shape)}")
+        self._check(L.kq_cache_select(self._ctx, cache.handle, *summaries.args, pq, q_stride, _tensor_dtype_code(q), heads, *batch.args, budget, first, last,
+                                      *(rope.args if rope is not None else _NO_ROPE), out.data_ptr()))
         return out
 
     # -- pages that sequences share ---------------------------------------------------------------
