@@ -845,19 +845,19 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
       if constexpr (kMode == kShared) {
         const size_t of = static_cast<size_t>(at.runs.span.first + query) * p.a.heads + static_cast<size_t>(head);
         if (prefix) {
-          __stcg(reinterpret_cast<float4*>(p.sh.sums + of * D) + quad % (D / 4), make_float4(v[0], v[1], v[2], v[3]));
-          if (quad % (D / 4) == 0) __stcg(p.sh.stats + of, make_float2(m, total_l));
+          const uint4 place = whole_place(p.sh, p.a, of);
+          __stcg(reinterpret_cast<float4*>(p.sh.scratch) + place.x + quad % (D / 4), make_float4(v[0], v[1], v[2], v[3]));
+          if (quad % (D / 4) == 0) {
+            __stcg(reinterpret_cast<float2*>(p.sh.scratch) + place.y, make_float2(m, total_l));
+            __stcg(p.sh.places + of, place);
+          }
           return;
         }
         if (at.runs.low > 0) {  // with what the row sees of the common keys
-          const float2 other = __ldcg(p.sh.stats + of);
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(p.sh.sums + of * D) + quad % (D / 4));
-          const float top = fmaxf(m, other.x);
-          const float mine = m == -INFINITY ? 0.0f : exp2_fast(m - top), theirs = other.x == -INFINITY ? 0.0f : exp2_fast(other.x - top);
-          total_l = fmaf(theirs, other.y, mine * total_l);
+          float all[4] = {v[0], v[1], v[2], v[3]};
+          join_common(p.sh, of, quad % (D / 4), m, total_l, all);
           const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-          const float o[4] = {fmaf(theirs, x.x, mine * v[0]) * inv, fmaf(theirs, x.y, mine * v[1]) * inv, fmaf(theirs, x.z, mine * v[2]) * inv,
-                              fmaf(theirs, x.w, mine * v[3]) * inv};
+          const float o[4] = {all[0] * inv, all[1] * inv, all[2] * inv, all[3] * inv};
           store4(static_cast<T*>(p.a.out) + static_cast<size_t>(at.runs.span.first + query) * p.a.out_stride + static_cast<size_t>(head) * D + quad % (D / 4) * 4, o);
           return;
         }

@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     };
     // read again: what was not needed in the loop takes no registers there
     const uint32_t n_parts = reinterpret_cast<volatile uint32_t*>(found)[3];
-    const bool shared = n_parts > 1;
+    const bool shared = n_parts > 1 || (kGroups && prefix && p.parts);  // sums over common keys stay in parts
     const float inv = shared || (kGroups && (prefix || common > 0)) ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
     float* const part = shared ? p.parts + static_cast<size_t>(blockIdx.x) * F::kPartFloats : nullptr;
     // Of the sums in the scratch of row `row_of`, their place; and what a row's own weights count beside them: (own, theirs), divided by all.
@@ -873,30 +873,31 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       const int query = row_of / static_cast<int>(p.group);
       return static_cast<size_t>(span.first + query) * p.a.heads + head * p.group + static_cast<uint32_t>(row_of - query * static_cast<int>(p.group));
     };
-    const auto beside = [&](size_t of, float m, float total) {
-      const float2 other = __ldcg(p.sh.stats + of);
-      const float top = fmaxf(m, other.x), mine = m == -INFINITY ? 0.0f : exp2f(m - top), theirs = other.x == -INFINITY ? 0.0f : exp2f(other.x - top);
-      const float all = fmaf(theirs, other.y, mine * total), inv = all == 0.0f ? 0.0f : 1.0f / all;
-      return make_float2(mine * inv, theirs * inv);
-    };
     constexpr float kLifted = kSplit ? 0.0f : 3.0f;  // 16-bit weights and sums are so many powers of two larger than M says
     // eight values of a row that is complete, with its M and sum of weights
     const auto finish = [&](int row_of, int i, float m, float total, const float* o) {
       if constexpr (kGroups) {
         const size_t of = sums_of(row_of);
         if (prefix) {
-          __stcg(reinterpret_cast<float4*>(p.sh.sums + of * D + i), make_float4(o[0], o[1], o[2], o[3]));
-          __stcg(reinterpret_cast<float4*>(p.sh.sums + of * D + i) + 1, make_float4(o[4], o[5], o[6], o[7]));
-          if (i == 0) __stcg(p.sh.stats + of, make_float2(m - kLifted, total));
+          const uint4 place = whole_place(p.sh, p.a, of);
+          __stcg(reinterpret_cast<float4*>(p.sh.scratch) + place.x + i / 4, make_float4(o[0], o[1], o[2], o[3]));
+          __stcg(reinterpret_cast<float4*>(p.sh.scratch) + place.x + i / 4 + 1, make_float4(o[4], o[5], o[6], o[7]));
+          if (i == 0) {
+            __stcg(reinterpret_cast<float2*>(p.sh.scratch) + place.y, make_float2(m - kLifted, total));
+            __stcg(p.sh.places + of, place);
+          }
           return;
         }
         if (common > 0) {
-          const float2 by = beside(of, m - kLifted, total);
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(p.sh.sums + of * D + i)), y = __ldcg(reinterpret_cast<const float4*>(p.sh.sums + of * D + i) + 1);
-          const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
           float z[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) z[e] = fmaf(by.y, v[e], by.x * o[e]);
+          for (int half = 0; half < 8; half += 4) {
+            float top = m - kLifted, all = total, v[4] = {o[half], o[half + 1], o[half + 2], o[half + 3]};
+            join_common(p.sh, of, (i + half) / 4, top, all, v);
+            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[half + e] = v[e] * inv;
+          }
           store8(out_of(row_of) + i, z);
           return;
         }
@@ -966,7 +967,19 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       }
     }
     if (shared) {  // the last CTA of the unit joins the parts, in order
-      if (!kSplit || wg == 0) reinterpret_cast<float2*>(part + kBlock * D)[r] = make_float2(M, l);
+      if (!kSplit || wg == 0) {
+        if constexpr (kGroups) {
+          if (prefix) {
+            reinterpret_cast<float2*>(part + kBlock * D)[r] = make_float2(M - kLifted, l);
+            const size_t at = static_cast<size_t>(p.parts - p.sh.scratch) + static_cast<size_t>(blockIdx.x) * F::kPartFloats;
+            if (my_part == 0 && row < n_rows)
+              __stcg(p.sh.places + sums_of(row), make_uint4(static_cast<uint32_t>(at / 4 + r * (D / 4)), static_cast<uint32_t>((at + kBlock * D) / 2 + r), F::kPartFloats, n_parts));
+          }
+        }
+        if (!prefix) reinterpret_cast<float2*>(part + kBlock * D)[r] = make_float2(M, l);
+      }
+    }
+    if (shared && !prefix) {
       asm volatile("bar.sync 2, 256;" ::: "memory");
       if (tid == 0) {
         unsigned int arrived;

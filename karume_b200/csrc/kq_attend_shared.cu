@@ -13,13 +13,19 @@ bool attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, const 
 cudaError_t attend_shared_rest_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 
 cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, SharedArgs sh, int* launches) {
-  const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, floats = rows * (a.cache.head_dim + 2);
-  // The sums take the end of the scratch.  Where they would take more than half of it, every sequence walks over all of its keys.
-  if (!env.workspace || floats * sizeof(float) + 16 > env.workspace_bytes / 2) return launch_attend(env, a, launches);
-  LaunchEnv in = env;
-  in.workspace_bytes = (env.workspace_bytes - floats * sizeof(float)) / 16 * 16;
-  sh.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(env.workspace) + in.workspace_bytes);
-  sh.stats = reinterpret_cast<float2*>(sh.sums + rows * a.cache.head_dim);
+  // The end of the scratch: a place for each row, and its sums where they are in one part; in front of it the parts of the sums over common
+  // keys, a third of the rest.  Where the rows would take more than half of it, every sequence walks over all of its keys.
+  const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, each = 16 + 4ull * (a.cache.head_dim + 2);
+  if (!env.workspace || rows * each + 64 > env.workspace_bytes / 2) return launch_attend(env, a, launches);
+  uint8_t* const base = static_cast<uint8_t*>(env.workspace);
+  const uint64_t left = (env.workspace_bytes - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
+  sh.scratch = static_cast<float*>(env.workspace);
+  sh.places = reinterpret_cast<uint4*>(base + left);
+  sh.sums = (left + rows * 16) / 4;
+  LaunchEnv in = env, parts = env;
+  in.workspace_bytes = own;
+  parts.workspace = base + own;
+  parts.workspace_bytes = left - own;
   *launches = 0;
   const uint64_t group = a.heads / a.cache.kv_heads;
   cudaError_t e = cudaSuccess;
@@ -28,20 +34,20 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
     some.first += g;
     some.tokens += g;
     some.groups = std::min(sh.groups - g, 128u);
-    if (!attend_shared_prefix_many(in, a, some, &e)) {
-      FewParams p = few_params(in, a, 0xFFFFFFFFu);
+    if (!attend_shared_prefix_many(parts, a, some, &e)) {
+      FewParams p = few_params(parts, a, 0xFFFFFFFFu);
       p.prefix = true;
       p.sh = some;
-      e = launch_few<kShared>(in, p, (a.batch.tokens + sh.groups - 1) / sh.groups * group);
+      e = launch_few<kShared>(parts, p, (a.batch.tokens + sh.groups - 1) / sh.groups * group);
     }
     *launches += 1;
   }
   if (e != cudaSuccess) return e;
-  const uint64_t own = static_cast<uint64_t>(a.batch.most) * group;
-  const bool many = own > kFewRows && attend_many_supports(a);
+  const uint64_t mine = static_cast<uint64_t>(a.batch.most) * group;
+  const bool many = mine > kFewRows && attend_many_supports(a);
   FewParams p = few_params(in, a, many ? kFewRows : 0xFFFFFFFFu);
   p.sh = sh;
-  e = launch_few<kShared>(in, p, many ? kFewRows : own);
+  e = launch_few<kShared>(in, p, many ? kFewRows : mine);
   if (e == cudaSuccess && many) e = attend_shared_rest_many(in, a, kFewRows, sh);
   *launches += many ? 2 : 1;
   return e;

@@ -99,6 +99,49 @@ __device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const Sha
   return make_int4(row0, row1 - row0, keys, from);
 }
 
+// Four of the sums of a row, not divided yet, relative to 2^m, and the sum of its weights: joined with what the row sees of the common keys.
+__device__ __forceinline__ void join_common(const SharedArgs& sh, size_t row, int quad, float& m, float& total, float (&v)[4]) {
+  const uint4 at = __ldcg(sh.places + row);
+  const float4* const sums = reinterpret_cast<const float4*>(sh.scratch) + at.x + quad;
+  const float2* const stats = reinterpret_cast<const float2*>(sh.scratch) + at.y;
+  constexpr uint32_t kBatch = 8;
+  for (uint32_t j0 = 0; j0 < at.w; j0 += kBatch) {
+    float2 ml[kBatch];
+    float4 x[kBatch];
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      const size_t part = static_cast<size_t>(min(j0 + j, at.w - 1)) * at.z;
+      ml[j] = __ldcg(stats + part / 2);
+      x[j] = __ldcg(sums + part / 4);
+    }
+    float now = m;
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      if (j0 + j >= at.w) ml[j] = make_float2(-INFINITY, 0.0f);
+      now = fmaxf(now, ml[j].x);
+    }
+    const float before = m == -INFINITY ? 0.0f : exp2f(m - now);
+    m = now;
+    total *= before;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= before;
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      const float keep = ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - m);
+      total = fmaf(keep, ml[j].y, total);
+      v[0] = fmaf(keep, x[j].x, v[0]);
+      v[1] = fmaf(keep, x[j].y, v[1]);
+      v[2] = fmaf(keep, x[j].z, v[2]);
+      v[3] = fmaf(keep, x[j].w, v[3]);
+    }
+  }
+}
+// Where a row's sums go that are no part, and its pair.
+__device__ __forceinline__ uint4 whole_place(const SharedArgs& sh, const AttendArgs& a, size_t row) {
+  const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, dim = a.cache.head_dim;
+  return make_uint4(static_cast<uint32_t>((sh.sums + row * dim) / 4), static_cast<uint32_t>((sh.sums + rows * dim) / 2 + row), 0u, 1u);
+}
+
 // ---- rows that attend to selected pages -------------------------------------------------------
 // (sequence, position, keys, 0): the pages in the list's order, the last one up to the position; no keys where the row is no sequence's.
 __device__ __forceinline__ int4 selected_row(const AttendArgs& a, const SelectedArgs& sel, uint32_t row) {

@@ -232,13 +232,17 @@ struct AttendArgs {
   uint32_t heads, window;
   float scale;
 };
-// Groups of neighbouring sequences that begin with the same tokens (device arrays), and what their rows' sums over those are.
+// Groups of neighbouring sequences that begin with the same tokens (device arrays), and where their rows' sums over those are: in parts, by
+// the CTAs that shared the keys, which are joined where a row is finished (by the CTA that walked over an eighth of a group's last keys,
+// 16 parts of 128 rows took 50 us).
 struct SharedArgs {
   const int* first;   // [groups + 1] first sequence of each
   const int* tokens;  // [groups]
   uint32_t groups;
-  float* sums;        // [tokens of the call][heads][head_dim], not divided yet
-  float2* stats;      // [tokens of the call][heads] (exponent of two that the weights are relative to, their sum)
+  float* scratch;
+  uint4* places;      // [tokens of the call][heads]: first part's sums in `scratch` (of four floats), its (exponent of two that the weights are
+                      // relative to, their sum) (of two), floats between parts, parts
+  uint64_t sums;      // where in `scratch` a kernel that has no parts leaves a row's sums [tokens][heads][head_dim], and behind them the pairs
 };
 struct SelectedArgs {
   const int* pages;  // [tokens of the call][kv_heads][budget] indices of a sequence's pages, ascending

@@ -57,17 +57,27 @@ __global__ void __launch_bounds__(kThreads) summarize_kernel(const SummaryParams
     low[i] = INFINITY;
     high[i] = -INFINITY;
   }
-#pragma unroll 8
-  for (int t = static_cast<int>(lane / kLanes); t < tokens; t += kTokens) {
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(block + t * (D / 2) + channel / 2);
-    const float2 so = __half22float2(*reinterpret_cast<const __half2*>(block + P * D + t * 4));
+  // sixteen tokens' loads of a lane at a time (behind one another they take 0.5 us each)
+  constexpr int kBatch = 16;
+  for (int t0 = static_cast<int>(lane / kLanes); t0 < tokens; t0 += kBatch * kTokens) {
+    uint32_t words[kBatch], params[kBatch];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = fmaf(static_cast<float>(word >> (4 * i) & 15u), so.x, so.y);
-      low[i] = fminf(low[i], x);
-      high[i] = fmaxf(high[i], x);
+    for (int k = 0; k < kBatch; ++k) {
+      const int t = min(t0 + k * kTokens, tokens - 1);  // the last one again changes nothing
+      words[k] = *reinterpret_cast<const uint32_t*>(block + t * (D / 2) + channel / 2);
+      params[k] = *reinterpret_cast<const uint32_t*>(block + P * D + t * 4);
     }
-    lost |= !(fabsf(so.x) <= 65504.0f && fabsf(so.y) <= 65504.0f);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&params[k]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = fmaf(static_cast<float>(words[k] >> (4 * i) & 15u), so.x, so.y);
+        low[i] = fminf(low[i], x);
+        high[i] = fmaxf(high[i], x);
+      }
+      lost |= !(fabsf(so.x) <= 65504.0f && fabsf(so.y) <= 65504.0f);
+    }
   }
   float most_c = 0.0f, most_r = 0.0f;
 #pragma unroll
@@ -112,12 +122,13 @@ struct SelectParams {
   Summaries from;
   uint32_t group, budget, first, last;
   uint32_t row0, rows;  // rows of this launch
-  uint32_t chunks;      // blocks that share a row's pages
+  uint32_t chunks;      // blocks that share a row's pages,
+  uint32_t turns;       // kScorePages of them each, so often
   uint32_t* keys;       // [rows][kv_heads][table width]
   int* out;             // [tokens][kv_heads][budget]
 };
 
-constexpr int kScoreWarps = 4, kScorePages = 64;  // pages of a block: sixteen a warp at a time
+constexpr int kScoreWarps = 8, kScorePages = 16 * kScoreWarps;  // pages that a block takes at a time: sixteen a warp
 constexpr uint32_t kAlways = 0xFFFFFFFFu, kUnknown = 0xFFFFFFFEu;
 
 // A number that is larger where the score is; not a number: larger than any.
@@ -141,7 +152,7 @@ __device__ __forceinline__ int2 pages_of_row(const AttendArgs& a, uint32_t row) 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 2 : 3) score_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kHeads = 8;  // columns of an MMA
   __shared__ __align__(16) uint8_t codes[2][kHeads][D + 16];  // a, |a| (rows 16 bytes apart from a multiple of 128: lanes of eight rows meet no bank twice)
   __shared__ float scales[kHeads];
@@ -150,90 +161,103 @@ __global__ void __launch_bounds__(kScoreWarps * 32) score_kernel(const __grid_co
   pdl_wait_prior_grid();
   const uint32_t chunk = blockIdx.x % p.chunks, at = blockIdx.x / p.chunks, head = at % heads, row = p.row0 + at / heads;
   const int2 of = pages_of_row(p.a, row);
-  const int pages = of.x, first = static_cast<int>(chunk) * kScorePages;
+  const int pages = of.x, first = static_cast<int>(chunk * p.turns) * kScorePages;
   if (first >= pages || pages <= static_cast<int>(p.budget)) return;  // all are taken
-  uint32_t* const keys = p.keys + (static_cast<size_t>(at) / heads * heads + head) * p.a.batch.width;
-  const int position = place_of_row(p.a.batch, row).x;
-  float best[2] = {-INFINITY, -INFINITY};
-  bool unknown[2] = {false, false};
-  const int base = first + static_cast<int>(warp) * 16;
-  for (uint32_t h0 = 0; h0 < p.group; h0 += kHeads) {
-    if (h0) __syncthreads();
-    for (uint32_t h = warp; h < kHeads; h += kScoreWarps) {  // a query head a warp
-      float x[8] = {};
-      if (h0 + h < p.group && lane < D / 8)
-        load8_rotated(static_cast<const T*>(p.a.q) + static_cast<size_t>(row) * p.a.q_stride + static_cast<size_t>(head * p.group + h0 + h) * D, lane * 8, p.a.rope,
-                      position, x);
-      float most = 0.0f;
-      bool lost = false;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        most = fmaxf(most, fabsf(x[i]));
-        lost |= !(fabsf(x[i]) < INFINITY);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      lost = __any_sync(0xffffffffu, lost);
-      const float scale = scale_of(most);
-      int a[8], m[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] = lost ? 0 : code_of(x[i], scale);
-        m[i] = abs(a[i]);
-      }
-      if (lane < D / 8) {
-        *reinterpret_cast<uint2*>(&codes[0][h][lane * 8]) = make_uint2(pack4(a), pack4(a + 4));
-        *reinterpret_cast<uint2*>(&codes[1][h][lane * 8]) = make_uint2(pack4(m), pack4(m + 4));
-      }
-      if (lane == 0) scales[h] = lost ? quiet_nan() : scale;
-    }
-    __syncthreads();
-    if (base >= pages) continue;
-    // sixteen pages: rows g and g + 8 of the MMA, sixteen channels of 64 a lane; the order of the channels is the queries' too
-    int acc[2][4] = {};
-    float2 by[2];
-    const uint8_t* rows[2];
+  uint32_t* const keys = p.keys + static_cast<size_t>(at) * p.a.batch.width;
+  const int* const table = p.a.batch.pages + static_cast<size_t>(of.y) * p.a.batch.width;
+  // sixteen pages: rows g and g + 8 of the MMA, sixteen channels of 64 a lane; the order of the channels is the queries' too
+  constexpr int kWide = D / 64;
+  uint4 x[2][2][kWide];  // [row][c, r][channels]
+  float2 by[2];
+  const auto load = [&](int base) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int index = base + static_cast<int>(g) + i * 8;
-      const uint32_t page = index < pages ? static_cast<uint32_t>(__ldg(p.a.batch.pages + static_cast<size_t>(of.y) * p.a.batch.width + index)) : 0xFFFFFFFFu;
+      const uint32_t page = index < pages ? static_cast<uint32_t>(__ldg(table + index)) : 0xFFFFFFFFu;
       const bool there = page < p.a.cache.pages;
       const size_t place = (static_cast<size_t>(there ? page : 0) * heads + head) * 2;
-      rows[i] = p.from.codes + place * D + t * 16;
       by[i] = there ? __ldg(reinterpret_cast<const float2*>(p.from.scales + place)) : make_float2(quiet_nan(), quiet_nan());
+#pragma unroll
+      for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) x[i][which][j] = __ldg(reinterpret_cast<const uint4*>(p.from.codes + (place + which) * D + t * 16 + j * 64));
+    }
+  };
+  int base = first + static_cast<int>(warp) * 16;
+  load(base);  // while the queries are worked on
+  const int position = place_of_row(p.a.batch, row).x;
+  const uint32_t blocks = (p.group + kHeads - 1) / kHeads;
+  float best[2];
+  bool unknown[2];
+  for (uint32_t turn = 0; turn < p.turns; ++turn, base += kScorePages) {
+    if (turn) load(base);
+    best[0] = best[1] = -INFINITY;
+    unknown[0] = unknown[1] = false;
+    for (uint32_t h0 = 0; h0 < p.group; h0 += kHeads) {
+      if (turn == 0 || blocks > 1) {
+        if (turn || h0) __syncthreads();
+        for (uint32_t h = warp; h < kHeads; h += kScoreWarps) {  // a query head a warp
+          float v[8] = {};
+          if (h0 + h < p.group && lane < D / 8)
+            load8_rotated(static_cast<const T*>(p.a.q) + static_cast<size_t>(row) * p.a.q_stride + static_cast<size_t>(head * p.group + h0 + h) * D, lane * 8, p.a.rope,
+                          position, v);
+          float most = 0.0f;
+          bool lost = false;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            most = fmaxf(most, fabsf(v[i]));
+            lost |= !(fabsf(v[i]) < INFINITY);
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          lost = __any_sync(0xffffffffu, lost);
+          const float scale = scale_of(most);
+          int a[8], m[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            a[i] = lost ? 0 : code_of(v[i], scale);
+            m[i] = abs(a[i]);
+          }
+          if (lane < D / 8) {
+            *reinterpret_cast<uint2*>(&codes[0][h][lane * 8]) = make_uint2(pack4(a), pack4(a + 4));
+            *reinterpret_cast<uint2*>(&codes[1][h][lane * 8]) = make_uint2(pack4(m), pack4(m + 4));
+          }
+          if (lane == 0) scales[h] = lost ? quiet_nan() : scale;
+        }
+        __syncthreads();
+      }
+      int acc[2][4] = {};
+#pragma unroll
+      for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) {
+          const uint4 q = *reinterpret_cast<const uint4*>(&codes[which][g][j * 64 + t * 16]);
+          mma_s8(acc[which], x[0][which][j].x, x[1][which][j].x, x[0][which][j].y, x[1][which][j].y, q.x, q.y);
+          mma_s8(acc[which], x[0][which][j].z, x[1][which][j].z, x[0][which][j].w, x[1][which][j].w, q.z, q.w);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t h = 2 * t + k;
+          if (h0 + h >= p.group) continue;
+          const float sum = __fadd_rn(__fmul_rn(static_cast<float>(acc[0][2 * i + k]), by[i].x), __fmul_rn(static_cast<float>(acc[1][2 * i + k]), by[i].y));
+          const float score = __fmul_rn(sum, scales[h]);
+          unknown[i] |= score != score;
+          best[i] = fmaxf(best[i], score);
+        }
     }
 #pragma unroll
-    for (int which = 0; which < 2; ++which)
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int j = 0; j < D / 64; ++j) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(rows[0] + which * D + j * 64)), y = __ldg(reinterpret_cast<const uint4*>(rows[1] + which * D + j * 64));
-        const uint4 q = *reinterpret_cast<const uint4*>(&codes[which][g][j * 64 + t * 16]);
-        mma_s8(acc[which], x.x, y.x, x.y, y.y, q.x, q.y);
-        mma_s8(acc[which], x.z, y.z, x.w, y.w, q.z, q.w);
+      for (int o = 1; o < 4; o *= 2) {
+        best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], o));
+        unknown[i] |= __shfl_xor_sync(0xffffffffu, static_cast<int>(unknown[i]), o) != 0;
       }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t h = 2 * t + k;
-        if (h0 + h >= p.group) continue;
-        const float sum = __fadd_rn(__fmul_rn(static_cast<float>(acc[0][2 * i + k]), by[i].x), __fmul_rn(static_cast<float>(acc[1][2 * i + k]), by[i].y));
-        const float score = __fmul_rn(sum, scales[h]);
-        unknown[i] |= score != score;
-        best[i] = fmaxf(best[i], score);
-      }
-  }
-  if (base >= pages) return;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int o = 1; o < 4; o *= 2) {
-      best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], o));
-      unknown[i] |= __shfl_xor_sync(0xffffffffu, static_cast<int>(unknown[i]), o) != 0;
+      const int index = base + static_cast<int>(g) + i * 8;
+      if (t == 0 && index < pages)
+        keys[index] = index < static_cast<int>(p.first) || index >= pages - static_cast<int>(p.last) ? kAlways : unknown[i] ? kUnknown : key_of(best[i]);
     }
-    const int index = base + static_cast<int>(g) + i * 8;
-    if (t == 0 && index < pages)
-      keys[index] = index < static_cast<int>(p.first) || index >= pages - static_cast<int>(p.last) ? kAlways : unknown[i] ? kUnknown : key_of(best[i]);
   }
 }
 
@@ -361,7 +385,10 @@ cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& a, const Summa
   p.last = last;
   p.keys = static_cast<uint32_t*>(env.workspace);
   p.out = out;
-  p.chunks = (a.batch.width + kScorePages - 1) / kScorePages;
+  // a block quantises its queries once: it takes more pages where there are blocks enough for all SMs, eight each
+  const uint64_t blocks = static_cast<uint64_t>(a.batch.tokens) * a.cache.kv_heads, most = (a.batch.width + kScorePages - 1) / kScorePages;
+  p.turns = static_cast<uint32_t>(std::min<uint64_t>({std::max<uint64_t>(blocks * most / (8ull * env.sm_count), 1), most, 8}));
+  p.chunks = static_cast<uint32_t>((most + p.turns - 1) / p.turns);
   *launches = 0;
   // as many rows at a time as have room in the scratch and in a grid
   const uint64_t room = std::min<uint64_t>(env.workspace_bytes / select_scratch_bytes(a), ((1ull << 31) - 1) / (static_cast<uint64_t>(a.cache.kv_heads) * p.chunks));

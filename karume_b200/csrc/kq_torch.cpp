@@ -35,6 +35,25 @@ using AppendFn = int (*)(void*, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t
 using ReadFn = int (*)(void*, uint64_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint64_t, uint64_t);
 using AttendFn = int (*)(void*, uint64_t, uint64_t, uint64_t, int, uint32_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, float,
                          uint32_t, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t, uint64_t);
+using AttendSharedFn = int (*)(void*, uint64_t, uint64_t, uint64_t, int, uint32_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, uint32_t,
+                               uint64_t, uint64_t, float, uint32_t, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t, uint64_t);
+using AttendSelectedFn = int (*)(void*, uint64_t, uint64_t, uint64_t, int, uint32_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint64_t, uint32_t,
+                                 float, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t, uint64_t);
+using SummarizeFn = int (*)(void*, uint64_t, uint64_t, uint64_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t);
+using SelectFn = int (*)(void*, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, int, uint32_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t,
+                         uint32_t, uint32_t, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t);
+using GrowFn = int (*)(void*, uint64_t, uint32_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, uint64_t, uint64_t);
+using ForkFn = int (*)(void*, uint64_t, uint32_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, uint64_t, uint64_t, uint64_t, uint64_t);
+using CompactFn = int (*)(void*, uint64_t, uint32_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, uint64_t, uint64_t);
+using CopyFn = int (*)(void*, uint32_t, const uint64_t*, const uint64_t*, uint32_t, uint64_t, uint32_t, uint64_t);
+AttendSharedFn g_attend_shared = nullptr;
+AttendSelectedFn g_attend_selected = nullptr;
+SummarizeFn g_summarize = nullptr;
+SelectFn g_select = nullptr;
+GrowFn g_grow = nullptr;
+ForkFn g_fork = nullptr;
+CompactFn g_compact = nullptr;
+CopyFn g_copy = nullptr;
 LinearFn g_linear = nullptr;
 FusedFn g_fused = nullptr;
 QuantizeFn g_quantize = nullptr;
@@ -82,8 +101,8 @@ int without_gil(Call call) {
 }
 
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 9) {
-    PyErr_SetString(PyExc_TypeError, "bind takes nine addresses");
+  if (n != 17) {
+    PyErr_SetString(PyExc_TypeError, "bind takes seventeen addresses");
     return nullptr;
   }
   g_linear = reinterpret_cast<LinearFn>(PyLong_AsVoidPtr(a[0]));
@@ -95,6 +114,14 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_append = reinterpret_cast<AppendFn>(PyLong_AsVoidPtr(a[6]));
   g_read = reinterpret_cast<ReadFn>(PyLong_AsVoidPtr(a[7]));
   g_attend = reinterpret_cast<AttendFn>(PyLong_AsVoidPtr(a[8]));
+  g_attend_shared = reinterpret_cast<AttendSharedFn>(PyLong_AsVoidPtr(a[9]));
+  g_attend_selected = reinterpret_cast<AttendSelectedFn>(PyLong_AsVoidPtr(a[10]));
+  g_summarize = reinterpret_cast<SummarizeFn>(PyLong_AsVoidPtr(a[11]));
+  g_select = reinterpret_cast<SelectFn>(PyLong_AsVoidPtr(a[12]));
+  g_grow = reinterpret_cast<GrowFn>(PyLong_AsVoidPtr(a[13]));
+  g_fork = reinterpret_cast<ForkFn>(PyLong_AsVoidPtr(a[14]));
+  g_compact = reinterpret_cast<CompactFn>(PyLong_AsVoidPtr(a[15]));
+  g_copy = reinterpret_cast<CopyFn>(PyLong_AsVoidPtr(a[16]));
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -303,33 +330,198 @@ PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return r;
 }
 
+// The queries and the output of an attention call, made where none is given; false: not of the plain form.
+struct Rows {
+  const at::Tensor *q = nullptr, *given = nullptr;
+  at::Tensor made;
+  int type = -1;
+  int64_t heads = 0;
+  uint64_t pq = 0, po = 0, q_stride = 0, out_stride = 0;
+  bool of(PyObject* queries, PyObject* out, int64_t tokens, int64_t dim) {
+    if (!tensor_of(queries, &q) || (out != Py_None && !tensor_of(out, &given))) return false;
+    type = dtype_code(*q);
+    if (type < 0 || q->dim() != 3 || q->numel() == 0) return false;
+    heads = q->size(1);
+    if (given == nullptr) made = at::detail::empty_cuda(q->sizes(), q->scalar_type(), q->device(), c10::nullopt);
+    const at::Tensor& o = given != nullptr ? *given : made;
+    if (o.scalar_type() != q->scalar_type() || !rows_of(*q, tokens, heads, dim, &q_stride) || !rows_of(o, tokens, heads, dim, &out_stride)) return false;
+    pq = ptr(*q);
+    po = ptr(o);
+    return true;
+  }
+  PyObject* result(PyObject* out) { return given != nullptr ? Py_NewRef(out) : THPVariable_Wrap(std::move(made)); }
+};
+
 // cache_attention(ctx, handle, dim, q, batch args, most, scale, window, rope args, out)
 PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-  const at::Tensor *q, *given = nullptr;
-  uint64_t batch[6], table[4], q_stride, out_stride;
-  if (nargs != 10 || a[0] == Py_None || !tensor_of(a[3], &q) || !numbers_of(a[4], batch) || !numbers_of(a[8], table) ||
-      (a[9] != Py_None && !tensor_of(a[9], &given)))
-    KQ_NONE;
-  const int type = dtype_code(*q);
-  const int64_t dim = PyLong_AsLongLong(a[2]), tokens = static_cast<int64_t>(batch[5]);
-  if (type < 0 || q->dim() != 3 || q->numel() == 0) KQ_NONE;
-  const int64_t heads = q->size(1);
-  at::Tensor made;
-  if (given == nullptr) made = at::detail::empty_cuda(q->sizes(), q->scalar_type(), q->device(), c10::nullopt);
-  const at::Tensor& out = given != nullptr ? *given : made;
-  if (out.scalar_type() != q->scalar_type() || !rows_of(*q, tokens, heads, dim, &q_stride) || !rows_of(out, tokens, heads, dim, &out_stride)) KQ_NONE;
+  uint64_t batch[6], table[4];
+  Rows r;
+  if (nargs != 10 || a[0] == Py_None || !numbers_of(a[4], batch) || !numbers_of(a[8], table)) KQ_NONE;
+  if (!r.of(a[3], a[9], static_cast<int64_t>(batch[5]), PyLong_AsLongLong(a[2]))) KQ_NONE;
   void* ctx = PyLong_AsVoidPtr(a[0]);
-  const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]), pq = ptr(*q), po = ptr(out);
+  const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]);
   const uint32_t most = u32(PyLong_AsUnsignedLong(a[5])), window = u32(PyLong_AsUnsignedLong(a[7]));
   const float scale = static_cast<float>(PyFloat_AsDouble(a[6]));
   if (PyErr_Occurred()) return nullptr;
   const int rc = without_gil([&] {
-    return g_attend(ctx, handle, pq, q_stride, type, u32(heads), u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5]), most, scale, window,
-                    table[0], u32(table[1]), u32(table[2]), u32(table[3]), po, out_stride);
+    return g_attend(ctx, handle, r.pq, r.q_stride, r.type, u32(r.heads), u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5]), most, scale, window,
+                    table[0], u32(table[1]), u32(table[2]), u32(table[3]), r.po, r.out_stride);
+  });
+  return rc != 0 ? status_of(rc) : r.result(a[9]);
+}
+
+// cache_attention_shared(ctx, handle, dim, q, batch args, most, shared args, scale, window, rope args, out)
+PyObject* cache_attention_shared(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t batch[6], table[4], groups[3];
+  Rows r;
+  if (nargs != 11 || a[0] == Py_None || !numbers_of(a[4], batch) || !numbers_of(a[6], groups) || !numbers_of(a[9], table)) KQ_NONE;
+  if (!r.of(a[3], a[10], static_cast<int64_t>(batch[5]), PyLong_AsLongLong(a[2]))) KQ_NONE;
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]);
+  const uint32_t most = u32(PyLong_AsUnsignedLong(a[5])), window = u32(PyLong_AsUnsignedLong(a[8]));
+  const float scale = static_cast<float>(PyFloat_AsDouble(a[7]));
+  if (PyErr_Occurred()) return nullptr;
+  const int rc = without_gil([&] {
+    return g_attend_shared(ctx, handle, r.pq, r.q_stride, r.type, u32(r.heads), u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5]), most,
+                           u32(groups[0]), groups[1], groups[2], scale, window, table[0], u32(table[1]), u32(table[2]), u32(table[3]), r.po, r.out_stride);
+  });
+  return rc != 0 ? status_of(rc) : r.result(a[10]);
+}
+
+// cache_attention_selected(ctx, handle, kv_heads, dim, q, batch args, selected, scale, rope args, out)
+PyObject* cache_attention_selected(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t batch[6], table[4];
+  const at::Tensor* selected;
+  Rows r;
+  if (nargs != 10 || a[0] == Py_None || !numbers_of(a[5], batch) || !numbers_of(a[8], table) || !tensor_of(a[6], &selected)) KQ_NONE;
+  const int64_t tokens = static_cast<int64_t>(batch[5]);
+  if (selected->scalar_type() != at::kInt || !plain(*selected) || selected->dim() != 3 || selected->size(0) != tokens ||
+      selected->size(1) != PyLong_AsLongLong(a[2]) || selected->size(2) == 0 || !r.of(a[4], a[9], tokens, PyLong_AsLongLong(a[3])))
+    KQ_NONE;
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]), ps = ptr(*selected);
+  const float scale = static_cast<float>(PyFloat_AsDouble(a[7]));
+  const uint32_t budget = u32(static_cast<uint64_t>(selected->size(2)));
+  if (PyErr_Occurred()) return nullptr;
+  const int rc = without_gil([&] {
+    return g_attend_selected(ctx, handle, r.pq, r.q_stride, r.type, u32(r.heads), u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5]), ps, budget,
+                             scale, table[0], u32(table[1]), u32(table[2]), u32(table[3]), r.po, r.out_stride);
+  });
+  return rc != 0 ? status_of(rc) : r.result(a[9]);
+}
+
+// cache_summarize(ctx, handle, summaries args, batch args): 0, or the status
+PyObject* cache_summarize(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t of[2], batch[6];
+  if (nargs != 4 || a[0] == Py_None || !numbers_of(a[2], of) || !numbers_of(a[3], batch)) KQ_NONE;
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]);
+  if (PyErr_Occurred()) return nullptr;
+  return status_of(without_gil([&] { return g_summarize(ctx, handle, of[0], of[1], u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5])); }));
+}
+
+// cache_select(ctx, handle, kv_heads, dim, summaries args, q, batch args, budget, first, last, rope args, out)
+PyObject* cache_select(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t of[2], batch[6], table[4], q_stride;
+  const at::Tensor *q, *given = nullptr;
+  if (nargs != 12 || a[0] == Py_None || !numbers_of(a[4], of) || !tensor_of(a[5], &q) || !numbers_of(a[6], batch) || !numbers_of(a[10], table) ||
+      (a[11] != Py_None && !tensor_of(a[11], &given)))
+    KQ_NONE;
+  const int64_t tokens = static_cast<int64_t>(batch[5]), kv_heads = PyLong_AsLongLong(a[2]), dim = PyLong_AsLongLong(a[3]);
+  const int64_t budget = PyLong_AsLongLong(a[7]), first = PyLong_AsLongLong(a[8]), last = PyLong_AsLongLong(a[9]);
+  const int type = dtype_code(*q);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    KQ_NONE;
+  }
+  if (type < 0 || q->dim() != 3 || q->numel() == 0 || !rows_of(*q, tokens, q->size(1), dim, &q_stride) || budget <= 0 || budget > (1 << 20) || first < 0 ||
+      first > budget || last < 0 || last > budget)
+    KQ_NONE;
+  const int64_t shape[3] = {tokens, kv_heads, budget};
+  if (given != nullptr && (given->scalar_type() != at::kInt || !plain(*given) || given->sizes() != at::IntArrayRef(shape))) KQ_NONE;
+  at::Tensor made;
+  if (given == nullptr) made = at::detail::empty_cuda(shape, at::kInt, q->device(), c10::nullopt);
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]), pq = ptr(*q), po = ptr(given != nullptr ? *given : made);
+  const uint32_t heads = u32(static_cast<uint64_t>(q->size(1)));
+  if (PyErr_Occurred()) return nullptr;
+  const int rc = without_gil([&] {
+    return g_select(ctx, handle, of[0], of[1], pq, q_stride, type, heads, u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5]),
+                    static_cast<uint32_t>(budget), static_cast<uint32_t>(first), static_cast<uint32_t>(last), table[0], u32(table[1]), u32(table[2]), u32(table[3]), po);
   });
   if (rc != 0) return status_of(rc);
-  if (given != nullptr) return Py_NewRef(a[9]);
+  if (given != nullptr) return Py_NewRef(a[11]);
   return THPVariable_Wrap(std::move(made));
+}
+
+// ---- books of pages: (table, sequences, width, lengths, refs, pages, page_tokens, report) -----------------
+// An i32 array with a number for each sequence.
+bool each_sequence(PyObject* o, const uint64_t (&book)[8], uint64_t* address) {
+  const at::Tensor* t;
+  if (!tensor_of(o, &t) || t->scalar_type() != at::kInt || !plain(*t) || static_cast<uint64_t>(t->numel()) != book[1]) return false;
+  *address = ptr(*t);
+  return true;
+}
+at::Tensor pairs_for(uint64_t count, int64_t device) {
+  const int64_t shape[2] = {static_cast<int64_t>(count), 2};
+  return at::detail::empty_cuda(shape, at::kInt, at::Device(at::kCUDA, static_cast<at::DeviceIndex>(device)), c10::nullopt);
+}
+
+// pages_grow(ctx, book args, news): 0, or the status
+PyObject* pages_grow(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t k[8], news;
+  if (nargs != 3 || a[0] == Py_None || !numbers_of(a[1], k) || !each_sequence(a[2], k, &news)) KQ_NONE;
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  return status_of(without_gil([&] { return g_grow(ctx, k[0], u32(k[1]), u32(k[2]), k[3], k[4], u32(k[5]), u32(k[6]), k[7], news); }));
+}
+
+// pages_fork(ctx, book args, parents, keep, device index) -> pairs
+PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t k[8], parents, keep = 0;
+  if (nargs != 5 || a[0] == Py_None || !numbers_of(a[1], k) || !each_sequence(a[2], k, &parents) || (a[3] != Py_None && !each_sequence(a[3], k, &keep))) KQ_NONE;
+  at::Tensor pairs = pairs_for(k[1], PyLong_AsLongLong(a[4]));
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  const uint64_t to = ptr(pairs);
+  const int rc = without_gil([&] { return g_fork(ctx, k[0], u32(k[1]), u32(k[2]), k[3], k[4], u32(k[5]), u32(k[6]), k[7], parents, keep, to); });
+  return rc != 0 ? status_of(rc) : THPVariable_Wrap(std::move(pairs));
+}
+
+// pages_compact(ctx, book args, device index) -> pairs
+PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t k[8];
+  if (nargs != 3 || a[0] == Py_None || !numbers_of(a[1], k)) KQ_NONE;
+  at::Tensor pairs = pairs_for(k[5], PyLong_AsLongLong(a[2]));
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  const uint64_t to = ptr(pairs);
+  const int rc = without_gil([&] { return g_compact(ctx, k[0], u32(k[1]), u32(k[2]), k[3], k[4], u32(k[5]), u32(k[6]), k[7], to); });
+  return rc != 0 ? status_of(rc) : THPVariable_Wrap(std::move(pairs));
+}
+
+// pages_copy(ctx, book args, pairs, pools): tensors, or caches' page_args (pages, bytes of one, address); 0, or the status
+PyObject* pages_copy(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  uint64_t k[8];
+  const at::Tensor *pairs, *t;
+  if (nargs != 4 || a[0] == Py_None || !numbers_of(a[1], k) || !tensor_of(a[2], &pairs) || !PyList_CheckExact(a[3])) KQ_NONE;
+  if (pairs->scalar_type() != at::kInt || !plain(*pairs) || pairs->dim() != 2 || pairs->size(1) != 2 || pairs->size(0) >= (1 << 30)) KQ_NONE;
+  const Py_ssize_t count = PyList_GET_SIZE(a[3]);
+  c10::SmallVector<uint64_t, 128> pools(count), bytes(count);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    PyObject* o = PyList_GET_ITEM(a[3], i);
+    uint64_t of[3];
+    if (tensor_of(o, &t)) {
+      if (!plain(*t) || t->dim() == 0 || static_cast<uint64_t>(t->size(0)) < k[5]) KQ_NONE;
+      bytes[i] = static_cast<uint64_t>(t->numel() / t->size(0)) * t->element_size();
+      pools[i] = ptr(*t);
+    } else {
+      if (!PyTuple_CheckExact(o) || !numbers_of(o, of) || of[0] < k[5]) KQ_NONE;
+      bytes[i] = of[1];
+      pools[i] = of[2];
+    }
+  }
+  void* ctx = PyLong_AsVoidPtr(a[0]);
+  const uint64_t pp = ptr(*pairs);
+  const uint32_t most = static_cast<uint32_t>(pairs->size(0));
+  return status_of(without_gil([&] { return g_copy(ctx, static_cast<uint32_t>(count), pools.data(), bytes.data(), u32(k[5]), pp, most, k[7]); }));
 }
 
 // CPython's frames have no handlers: what is thrown in a call must not leave it.
@@ -346,7 +538,8 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t nargs) {
 #define KQ_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {KQ_METHOD(bind),      KQ_METHOD(linear),    KQ_METHOD(linear_fused), KQ_METHOD(quantize_rows),
                          KQ_METHOD(linear_a8), KQ_METHOD(embedding), KQ_METHOD(rope),   KQ_METHOD(cache_append), KQ_METHOD(cache_read),
-                         KQ_METHOD(cache_attention), {nullptr, nullptr, 0, nullptr}};
+                         KQ_METHOD(cache_attention), KQ_METHOD(cache_attention_shared), KQ_METHOD(cache_attention_selected), KQ_METHOD(cache_summarize),
+                         KQ_METHOD(cache_select), KQ_METHOD(pages_grow), KQ_METHOD(pages_fork), KQ_METHOD(pages_compact), KQ_METHOD(pages_copy), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kqtorch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

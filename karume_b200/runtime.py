@@ -56,7 +56,8 @@ def _load_fast() -> None:
         from . import _kqtorch
         _kqtorch.bind(*[ctypes.cast(f, ctypes.c_void_p).value
                         for f in (L.kq_linear, L.kq_linear_fused, L.kq_quantize_rows, L.kq_linear_a8, L.kq_embedding, L.kq_rope,
-                                  L.kq_cache_append, L.kq_cache_read, L.kq_cache_attention)])
+                                  L.kq_cache_append, L.kq_cache_read, L.kq_cache_attention, L.kq_cache_attention_shared, L.kq_cache_attention_selected,
+                                  L.kq_cache_summarize, L.kq_cache_select, L.kq_pages_grow, L.kq_pages_fork, L.kq_pages_compact, L.kq_pages_copy)])
         _fast = _kqtorch
 
 
@@ -147,6 +148,9 @@ class KvCache:
     kv_heads: int
     head_dim: int
 
+    def __post_init__(self):
+        self.page_args = (self.pages, self.kv_heads * self.page_tokens * (self.head_dim + 8), self.pool.data_ptr())
+
     def free(self) -> None:
         if self.handle:
             self.gpu._check(L.kq_cache_free(self.gpu._ctx, self.handle))
@@ -181,10 +185,12 @@ class CacheSummaries:
         self.codes, self.scales = codes, scales
         self.args = (codes.data_ptr(), scales.data_ptr())
 
+        self.shape = tuple(int(n) for n in codes.shape)
+
     def check(self, cache: "KvCache") -> None:
-        shape = tuple(self.codes.shape)
-        if shape[0] < cache.pages or shape[1] != cache.kv_heads or shape[3] != cache.head_dim:
-            raise KqError(2, f"summaries {list(shape)} are not those of {cache.pages} pages of {cache.kv_heads} heads of {cache.head_dim}")
+        pages, heads, _, dim = self.shape
+        if pages < cache.pages or heads != cache.kv_heads or dim != cache.head_dim:
+            raise KqError(2, f"summaries {list(self.shape)} are not those of {cache.pages} pages of {cache.kv_heads} heads of {cache.head_dim}")
 
 
 class CachePages:
@@ -552,11 +558,17 @@ class Gpu:
         if window < 0:
             raise KqError(2, f"window {window}: a number of keys, 0 for all")
         window = min(int(window), 0xFFFFFFFF)  # the ABI's number has 32 bits; no sequence is longer
+        angles = rope.args if rope is not None else None
         if shared is None and selected is None:
-            done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window,
-                                         rope.args if rope is not None else None, out)
-            if done is not None:
-                return self._done(done)
+            done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window, angles, out)
+        elif selected is None:
+            done = _fast.cache_attention_shared(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, shared.args, scale, window, angles, out)
+        elif window or shared is not None:
+            raise KqError(2, "selected pages are all that a row sees: no window, no shared prefixes")
+        else:
+            done = _fast.cache_attention_selected(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, q, batch.args, selected, scale, angles, out)
+        if done is not None:
+            return self._done(done)
         torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
@@ -570,8 +582,6 @@ class Gpu:
         head = (self._ctx, cache.handle, pq, q_stride, _tensor_dtype_code(q), heads, *batch.args)
         tail = (*(rope.args if rope is not None else _NO_ROPE), po, out_stride)
         if selected is not None:
-            if window or shared is not None:
-                raise KqError(2, "selected pages are all that a row sees: no window, no shared prefixes")
             if selected.dtype != torch.int32 or not selected.is_cuda or not selected.is_contiguous() or selected.dim() != 3 or \
                     tuple(selected.shape[:2]) != (batch.tokens, cache.kv_heads):
                 raise KqError(2, f"selected must be a contiguous CUDA int32 tensor [{batch.tokens}, {cache.kv_heads}, budget]")
@@ -594,14 +604,21 @@ class Gpu:
     def cache_summarize(self, cache: KvCache, summaries: CacheSummaries, batch: CacheBatch) -> None:
         """Brings the summaries of the pages that the batch's new tokens are in up to date (behind cache_append)."""
         summaries.check(cache)
+        done = _fast.cache_summarize(self._ctx_addr, cache.handle, summaries.args, batch.args)
+        if done is not None:
+            return self._check(done)
         self._check(L.kq_cache_summarize(self._ctx, cache.handle, *summaries.args, *batch.args))
 
     def cache_select(self, cache: KvCache, summaries: CacheSummaries, q, batch: CacheBatch, budget: int, first: int = 1, last: int = 1,
                      rope: "Rope | None" = None, out=None):
         """Up to `budget` pages for every row of q [tokens, heads, head_dim] and kv head, int32 [tokens, kv_heads, budget]: ascending indices into
         the sequence's pages, -1 behind them; always the first `first` and the last `last` ones, then those whose summaries promise most."""
-        torch = _torch()
         summaries.check(cache)
+        done = _fast.cache_select(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, summaries.args, q, batch.args, budget, first, last,
+                                  rope.args if rope is not None else None, out)
+        if done is not None:
+            return self._done(done)
+        torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
             raise KqError(2, f"q must have {batch.tokens} rows")
@@ -629,11 +646,17 @@ class Gpu:
 
     def pages_grow(self, book: CachePages, news) -> None:
         """Sequence b gets the pages of its next news[b] tokens (CUDA int32) and is that much longer."""
+        done = _fast.pages_grow(self._ctx_addr, book.args, news)
+        if done is not None:
+            return self._check(done)
         self._check(L.kq_pages_grow(self._ctx, *book.args, _per_sequence(news, book, "news")))
 
     def pages_fork(self, book: CachePages, parents, keep=None):
         """Every sequence b becomes the first min(keep[b], length) tokens of parents[b] (CUDA int32; negative: it ends), all at once.
         Returns the pairs [sequences, 2] of pages to copy, for pages_copy."""
+        done = _fast.pages_fork(self._ctx_addr, book.args, parents, keep, self.index)
+        if done is not None:
+            return self._done(done)
         torch = _torch()
         pairs = torch.empty((book.sequences, 2), dtype=torch.int32, device=self.device)
         self._check(L.kq_pages_fork(self._ctx, *book.args, _per_sequence(parents, book, "parents"),
@@ -642,6 +665,9 @@ class Gpu:
 
     def pages_compact(self, book: CachePages):
         """Moves the pages in use to the lowest numbers; returns the pairs [pages, 2] (from, to), for pages_copy."""
+        done = _fast.pages_compact(self._ctx_addr, book.args, self.index)
+        if done is not None:
+            return self._done(done)
         torch = _torch()
         pairs = torch.empty((book.pages, 2), dtype=torch.int32, device=self.device)
         self._check(L.kq_pages_compact(self._ctx, *book.args, pairs.data_ptr()))
@@ -649,13 +675,17 @@ class Gpu:
 
     def pages_copy(self, book: CachePages, pairs, pools) -> None:
         """Copies the pages of the book's last fork or compact in every pool: KvCaches, or CUDA tensors whose first axis is the pages."""
+        pools = [pool.page_args if isinstance(pool, KvCache) else pool for pool in pools]
+        done = _fast.pages_copy(self._ctx_addr, book.args, pairs, pools)
+        if done is not None:
+            return self._check(done)
         torch = _torch()
         if pairs.dtype != torch.int32 or not pairs.is_cuda or not pairs.is_contiguous() or pairs.dim() != 2 or pairs.shape[1] != 2:
             raise KqError(2, "pairs must be a contiguous CUDA int32 tensor [pairs, 2]")
         addresses, sizes = [], []
         for pool in pools:
-            if isinstance(pool, KvCache):
-                pages, each, address = pool.pages, pool.kv_heads * pool.page_tokens * (pool.head_dim + 8), pool.pool.data_ptr()
+            if isinstance(pool, tuple):
+                pages, each, address = pool
             elif not pool.is_cuda or not pool.is_contiguous() or pool.dim() == 0:
                 raise KqError(2, "a pool is a KvCache or a contiguous CUDA tensor [pages, ...]")
             else:
