@@ -28,13 +28,15 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
   parts.workspace_bytes = left - own;
   *launches = 0;
   const uint64_t group = a.heads / a.cache.kv_heads;
+  LaunchEnv alone = parts;  // groups that come in turns: none may leave its parts where the next one's go
+  if (sh.groups > 128) alone.workspace = nullptr;
   cudaError_t e = cudaSuccess;
   for (uint32_t g = 0; g < sh.groups && e == cudaSuccess; g += 128) {
     SharedArgs some = sh;
     some.first += g;
     some.tokens += g;
     some.groups = std::min(sh.groups - g, 128u);
-    if (!attend_shared_prefix_many(parts, a, some, &e)) {
+    if (!attend_shared_prefix_many(alone, a, some, &e)) {
       FewParams p = few_params(parts, a, 0xFFFFFFFFu);
       p.prefix = true;
       p.sh = some;

@@ -35,7 +35,10 @@ struct BookParams {
   int* stage;          // scratch [sequences][width]: fork: new rows, until every old one has been read
 };
 
+constexpr uint32_t kKept = 1024;  // sequences whose numbers are kept in shared memory
+
 struct Shared {
+  int4 kept[kKept];
   int totals[2][kMaxCluster];  // of the CTAs, turn about
   long long warps[32];
 };
@@ -237,6 +240,13 @@ __device__ __forceinline__ Becomes becomes(const BookParams& p, uint32_t b) {
   return r;
 }
 
+// (for the first kKept sequences, from where the block has put it)
+__device__ __forceinline__ Becomes becomes_again(const BookParams& p, const Shared& s, uint32_t b) {
+  if (b >= kKept) return becomes(p, b);
+  const int4 v = s.kept[b];
+  return Becomes{v.x, v.y, v.z, v.w != 0};
+}
+
 __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookParams p) {
   __shared__ Shared s;
   const uint32_t rank = cta_rank(), ctas = cta_count(), lane = threadIdx.x % 32;
@@ -255,6 +265,7 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
       bad = true;
     } else {
       const Becomes w = becomes(p, b);
+      if (b < kKept) s.kept[b] = make_int4(w.parent, w.n, w.old, w.changes);
       if (w.changes) entries = max(entries, pages_of(max(w.n, w.old), k.shift));
     }
   }
@@ -268,22 +279,26 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
   // ---- the names that rows give up, and those of whole pages that they take -------------------------
   const auto names = [&](int by) {
     each_chunk(k, static_cast<uint32_t>(entries), rank, ctas, [&](uint32_t b, uint32_t from) {
-      const Becomes w = becomes(p, b);
+      const Becomes w = becomes_again(p, s, b);
       if (!w.changes) return;
       const bool same = w.parent >= 0 && static_cast<uint32_t>(w.parent) == b;
       const int whole = w.n >> k.shift, held = pages_of(w.old, k.shift);
       const int* const mine = k.table + static_cast<size_t>(b) * k.width;
       const int* const theirs = k.table + static_cast<size_t>(max(w.parent, 0)) * k.width;
-      for (int i = static_cast<int>(from + lane); i < static_cast<int>(from + kChunk); i += 32) {
-        if (i < held && !(same && i < whole)) {
-          const int page = mine[i];
-          if (a_page(k, page)) atomicSub(k.refs + page, by);
-        }
-        if (i < whole && !same) {
-          const int page = theirs[i];
-          if (a_page(k, page)) atomicAdd(k.refs + page, by);
-          p.stage[static_cast<size_t>(b) * k.width + i] = page;
-        }
+      constexpr int kEach = kChunk / 32;
+      int given[kEach], taken[kEach];  // all loads first
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const int i = static_cast<int>(from + lane) + 32 * j;
+        given[j] = i < held && !(same && i < whole) ? mine[i] : -1;
+        taken[j] = i < whole && !same ? theirs[i] : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const int i = static_cast<int>(from + lane) + 32 * j;
+        if (a_page(k, given[j])) atomicSub(k.refs + given[j], by);
+        if (a_page(k, taken[j])) atomicAdd(k.refs + taken[j], by);
+        if (i < whole && !same) p.stage[static_cast<size_t>(b) * k.width + i] = taken[j];
       }
     });
   };
@@ -294,7 +309,7 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
     return w.changes && (w.n & ((1 << k.shift) - 1)) ? k.table[static_cast<size_t>(w.parent) * k.width + (w.n >> k.shift)] : -1;
   };
   for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
-    const int page = tail_of(becomes(p, b));
+    const int page = tail_of(becomes_again(p, s, b));
     if (a_page(k, page) && fresh(k.refs + page) <= 0) atomicMin(k.refs + page, kLowest + static_cast<int>(b));
   }
   sync_all(ctas);
@@ -304,7 +319,7 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
     Becomes w = {};
     int page = -1, place = -1;
     if (b < k.sequences) {
-      w = becomes(p, b);
+      w = becomes_again(p, s, b);
       page = tail_of(w);
       if (a_page(k, page)) place = fresh(k.refs + page) == kLowest + static_cast<int>(b) ? -2 : 0;  // takes it over, or needs another
     }
@@ -402,41 +417,99 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_compact_kernel(const Bo
 }
 
 // ---- copies -----------------------------------------------------------------------------------------
-constexpr int kCopyThreads = 256, kCopyPieces = 4;  // 16-byte pieces a thread has under way
-constexpr uint32_t kPiece = kCopyThreads * kCopyPieces * 16;
+// Bulk copies into shared memory and out of it, a warp with a ring of stages: no registers, and what is under way does not depend on how
+// many threads an SM holds.  Of 96 KB a CTA, two CTAs an SM, half is on its way in.
+constexpr uint32_t kPiece = 16384, kStages = 6, kAhead = 3;
+constexpr uint32_t kCopySmem = kStages * kPiece + 256;
+constexpr uint32_t kCopyWaitLimit = 1u << 22;
+constexpr int kCopyTimeout = 60;  // status word: a piece did not arrive
 
 struct CopyParams {
   uint8_t* pool[kPoolsAtOnce];
   uint64_t bytes[kPoolsAtOnce];  // of a page
   const int* pairs;
   const int* report;  // null: all `most` pairs
-  uint32_t pools, pages, most, parts;  // parts that a page is copied in
+  int* status;
+  uint32_t pools, pages, most, parts;  // parts that a page is copied in, kPiece or less each
 };
 
-__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const __grid_constant__ CopyParams p) {
+__global__ void __launch_bounds__(32) pages_copy_kernel(const __grid_constant__ CopyParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint64_t* const targets = reinterpret_cast<uint64_t*>(smem + kStages * kPiece);
+  uint32_t* const sizes = reinterpret_cast<uint32_t*>(targets + kStages);
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), bars = base + kStages * kPiece + 128, lane = threadIdx.x;
+  if (lane < kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + lane * 8) : "memory");
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
   pdl_launch_dependents();
   pdl_wait_prior_grid();
   const uint32_t count = p.report ? min(static_cast<uint32_t>(max(p.report[2], 0)), p.most) : p.most;
   const uint64_t all = static_cast<uint64_t>(count) * p.pools * p.parts;
-  for (uint64_t item = blockIdx.x; item < all; item += gridDim.x) {
-    const uint32_t part = static_cast<uint32_t>(item % p.parts);
-    const uint32_t pool = static_cast<uint32_t>(item / p.parts % p.pools);
-    const uint32_t pair = static_cast<uint32_t>(item / p.parts / p.pools);
-    const uint32_t from = static_cast<uint32_t>(p.pairs[2 * pair]), to = static_cast<uint32_t>(p.pairs[2 * pair + 1]);
-    if (from >= p.pages || to >= p.pages || from == to) continue;
-    const uint64_t bytes = p.bytes[pool], each = (bytes / 16 + p.parts - 1) / p.parts;  // in 16-byte pieces
-    const uint64_t begin = part * each, end = min(begin + each, bytes / 16);
-    const uint4* const src = reinterpret_cast<const uint4*>(p.pool[pool] + from * bytes);
-    uint4* const dst = reinterpret_cast<uint4*>(p.pool[pool] + to * bytes);
-    for (uint64_t at = begin + threadIdx.x; at < end; at += kCopyThreads * kCopyPieces) {
-      uint4 v[kCopyPieces];
-#pragma unroll
-      for (int i = 0; i < kCopyPieces; ++i)
-        if (at + i * kCopyThreads < end) v[i] = src[at + i * kCopyThreads];
-#pragma unroll
-      for (int i = 0; i < kCopyPieces; ++i)
-        if (at + i * kCopyThreads < end) dst[at + i * kCopyThreads] = v[i];
+  uint32_t n = 0;     // pieces asked for
+  uint32_t done = 0;  // pieces handed on
+  bool ok = true;
+  // piece `done`, which has arrived: on its way out
+  const auto hand_on = [&] {
+    const uint32_t stage = done % kStages, bar = bars + stage * 8, parity = done / kStages & 1;
+    uint32_t here = 0;
+    for (uint32_t spin = 0; spin < kCopyWaitLimit && !here; ++spin)
+      asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(here) : "r"(bar), "r"(parity) : "memory");
+    if (!here) {
+      ok = false;
+      *reinterpret_cast<volatile int*>(p.status) = kCopyTimeout;
+      return;
     }
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(targets[stage]), "r"(base + stage * kPiece), "r"(sizes[stage]) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    ++done;
+  };
+  for (uint64_t item0 = blockIdx.x; item0 < all; item0 += 32ull * gridDim.x) {
+    // thirty-two pieces' addresses, a lane each
+    const uint64_t item = item0 + static_cast<uint64_t>(lane) * gridDim.x;
+    uint64_t from_at = 0, to_at = 0;
+    uint32_t bytes = 0;
+    if (item < all) {
+      const uint32_t part = static_cast<uint32_t>(item % p.parts);
+      const uint64_t of = item / p.parts;
+      const uint32_t pool = static_cast<uint32_t>(of % p.pools), pair = static_cast<uint32_t>(of / p.pools);
+      const uint32_t from = static_cast<uint32_t>(p.pairs[2 * pair]), to = static_cast<uint32_t>(p.pairs[2 * pair + 1]);
+      if (from < p.pages && to < p.pages && from != to) {
+        const uint64_t size = p.bytes[pool], each = (size / 16 + p.parts - 1) / p.parts * 16, begin = min(part * each, size);
+        bytes = static_cast<uint32_t>(min(each, size - begin));
+        from_at = reinterpret_cast<uint64_t>(p.pool[pool]) + from * size + begin;
+        to_at = reinterpret_cast<uint64_t>(p.pool[pool]) + to * size + begin;
+      }
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, bytes != 0); left; left &= left - 1) {
+      const int l = __ffs(left) - 1;
+      const uint64_t src = __shfl_sync(0xffffffffu, from_at, l), dst = __shfl_sync(0xffffffffu, to_at, l);
+      const uint32_t size = __shfl_sync(0xffffffffu, bytes, l);
+      if (lane == 0 && ok) {
+        if (n - done >= kAhead) hand_on();
+        if (ok) {
+          const uint32_t stage = n % kStages, bar = bars + stage * 8;
+          asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStages - kAhead) : "memory");  // what the stage held has left it
+          targets[stage] = dst;
+          sizes[stage] = size;
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(size) : "memory");
+          asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(base + stage * kPiece), "l"(src), "r"(size), "r"(bar)
+                       : "memory");
+          ++n;
+        }
+      }
+    }
+  }
+  if (lane == 0) {
+    while (ok && done < n) hand_on();
+    // behind a wait that gave up: the pieces on their way in are waited for once more each, so that none lands in another block's memory
+    for (uint32_t i = done; !ok && i < n; ++i) {
+      uint32_t here = 0;
+      for (uint32_t spin = 0; spin < kCopyWaitLimit && !here; ++spin)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(here) : "r"(bars + i % kStages * 8), "r"(i / kStages & 1) : "memory");
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 }
 
@@ -505,6 +578,9 @@ cudaError_t launch_pages_compact(const LaunchEnv& env, const PageBook& book, int
 
 cudaError_t launch_pages_copy(const LaunchEnv& env, uint32_t count, const uint64_t* pools, const uint64_t* page_bytes, uint32_t pages, const int* pairs,
                               uint32_t most, const int* report) {
+  static OncePerDevice once;
+  cudaError_t e = once.run([] { return cudaFuncSetAttribute(pages_copy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCopySmem); });
+  if (e != cudaSuccess) return e;
   CopyParams p;
   uint64_t largest = 0;
   for (uint32_t i = 0; i < count; ++i) {
@@ -514,14 +590,16 @@ cudaError_t launch_pages_copy(const LaunchEnv& env, uint32_t count, const uint64
   }
   p.pairs = pairs;
   p.report = report;
+  p.status = env.status;
   p.pools = count;
   p.pages = pages;
   p.most = most;
   p.parts = static_cast<uint32_t>((largest + kPiece - 1) / kPiece);
   const uint64_t items = static_cast<uint64_t>(most) * count * p.parts;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<uint64_t>(items, static_cast<uint64_t>(env.sm_count) * 8)));
-  cfg.blockDim = dim3(kCopyThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<uint64_t>(items, static_cast<uint64_t>(env.sm_count) * 2)));
+  cfg.blockDim = dim3(32);
+  cfg.dynamicSmemBytes = kCopySmem;
   cfg.stream = env.stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -15,7 +15,6 @@
 namespace kq {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kTiny = 1.17549435e-38f;
 
 __device__ __forceinline__ float scale_of(float largest) { return fmaxf(__fmul_rn(largest, 1.0f / 127.0f), kTiny); }
@@ -29,90 +28,111 @@ struct SummaryParams {
   Cache cache;
   CacheBatch batch;
   Summaries to;
+  uint32_t each;  // new tokens of a block
 };
 
-// A warp for each (new token, kv head); those whose token is not the first of the call in its page have nothing to do.
+// A block for each kv head and `each` new tokens: those that are the first of the call in their page, one after the other.  Its warps share
+// a page's tokens, all of whose loads are under way together: one warp for a page took 11 us for what takes 6.
+constexpr int kSummaryThreads = 128;
+
 template <int D>
-__global__ void __launch_bounds__(kThreads) summarize_kernel(const SummaryParams p) {
-  constexpr int kLanes = D / 8, kTokens = 32 / kLanes;  // lanes of a token (eight channels each), tokens at a time
+__global__ void __launch_bounds__(kSummaryThreads) summarize_kernel(const SummaryParams p) {
+  constexpr int kLanes = D / 8, kTokens = kSummaryThreads / kLanes;  // threads of a token (eight channels each), tokens at a time
+  constexpr int kWarps = kSummaryThreads / 32;
+  __shared__ float ends[kWarps][2][D];
   pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const uint32_t lane = threadIdx.x % 32, heads = p.cache.kv_heads;
-  const uint64_t at = (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / 32;
-  if (at >= static_cast<uint64_t>(p.batch.tokens) * heads) return;
-  const uint32_t row = static_cast<uint32_t>(at / heads), head = static_cast<uint32_t>(at % heads), b = sequence_of(p.batch, row);
-  const Span span = span_of(p.batch, b);
-  const int in = static_cast<int>(row) - span.first, position = span.length - span.count + in;
+  const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32, heads = p.cache.kv_heads, head = blockIdx.x % heads, first_row = blockIdx.x / heads * p.each;
   const int P = static_cast<int>(p.cache.page_tokens);
-  if (in < 0 || in >= span.count || position < 0 || (in != 0 && position % P != 0)) return;
-  const uint32_t index = static_cast<uint32_t>(position / P);
-  const uint8_t* const block = cache_block(p.cache, p.batch, b, index, head);
-  if (!block) return;
-  const int tokens = min(P, span.length - static_cast<int>(index) * P);
-  const uint32_t channel = lane % kLanes * 8;
-  float low[8], high[8];
-  bool lost = false;
+  for (uint32_t row = first_row; row < min(first_row + p.each, p.batch.tokens); ++row) {  // (the same for all threads)
+    const uint32_t b = sequence_of(p.batch, row);
+    const Span span = span_of(p.batch, b);
+    const int in = static_cast<int>(row) - span.first, position = span.length - span.count + in;
+    if (in < 0 || in >= span.count || position < 0 || (in != 0 && position % P != 0)) continue;
+    const uint32_t index = static_cast<uint32_t>(position / P);
+    const uint8_t* const block = cache_block(p.cache, p.batch, b, index, head);
+    if (!block) continue;
+    const int tokens = min(P, span.length - static_cast<int>(index) * P);
+    const uint32_t channel = tid % kLanes * 8;
+    float low[8], high[8];
+    bool lost = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    low[i] = INFINITY;
-    high[i] = -INFINITY;
-  }
-  // sixteen tokens' loads of a lane at a time (behind one another they take 0.5 us each)
-  constexpr int kBatch = 16;
-  for (int t0 = static_cast<int>(lane / kLanes); t0 < tokens; t0 += kBatch * kTokens) {
-    uint32_t words[kBatch], params[kBatch];
+    for (int i = 0; i < 8; ++i) {
+      low[i] = INFINITY;
+      high[i] = -INFINITY;
+    }
+    constexpr int kBatch = 8;
+    for (int t0 = static_cast<int>(tid / kLanes); t0 < tokens; t0 += kBatch * kTokens) {
+      uint32_t words[kBatch], params[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int t = min(t0 + k * kTokens, tokens - 1);  // the last one again changes nothing
-      words[k] = *reinterpret_cast<const uint32_t*>(block + t * (D / 2) + channel / 2);
-      params[k] = *reinterpret_cast<const uint32_t*>(block + P * D + t * 4);
+      for (int k = 0; k < kBatch; ++k) {
+        const int t = min(t0 + k * kTokens, tokens - 1);  // the last one again changes nothing
+        words[k] = __ldg(reinterpret_cast<const uint32_t*>(block + t * (D / 2) + channel / 2));
+        params[k] = __ldg(reinterpret_cast<const uint32_t*>(block + P * D + t * 4));
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&params[k]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          constexpr float kWhole = 8388608.0f;  // 2^23: a code in its last bits
+          const float u = __uint_as_float((words[k] >> (4 * i) & 15u) | 0x4B000000u) - kWhole;
+          const float x = fmaf(u, so.x, so.y);
+          low[i] = fminf(low[i], x);
+          high[i] = fmaxf(high[i], x);
+        }
+        lost |= !(fabsf(so.x) <= 65504.0f && fabsf(so.y) <= 65504.0f);
+      }
     }
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&params[k]));
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int o = kLanes; o < 32; o *= 2) {
+        low[i] = fminf(low[i], __shfl_xor_sync(0xffffffffu, low[i], o));
+        high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], o));
+      }
+    if (lane < kLanes)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = fmaf(static_cast<float>(words[k] >> (4 * i) & 15u), so.x, so.y);
-        low[i] = fminf(low[i], x);
-        high[i] = fmaxf(high[i], x);
+        ends[warp][0][channel + i] = low[i];
+        ends[warp][1][channel + i] = high[i];
       }
-      lost |= !(fabsf(so.x) <= 65504.0f && fabsf(so.y) <= 65504.0f);
+    lost = __syncthreads_or(lost);  // a key that is NaN, or of an infinite scale: nothing can be said of the page
+    if (warp == 0) {
+      float most_c = 0.0f, most_r = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float least = ends[0][0][channel + i], most = ends[0][1][channel + i];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+          least = fminf(least, ends[w][0][channel + i]);
+          most = fmaxf(most, ends[w][1][channel + i]);
+        }
+        low[i] = __fmul_rn(__fadd_rn(most, least), 0.5f);
+        high[i] = __fmul_rn(__fsub_rn(most, least), 0.5f);
+        most_c = fmaxf(most_c, fabsf(low[i]));
+        most_r = fmaxf(most_r, high[i]);
+      }
+#pragma unroll
+      for (int o = 1; o < kLanes; o *= 2) {
+        most_c = fmaxf(most_c, __shfl_xor_sync(0xffffffffu, most_c, o));
+        most_r = fmaxf(most_r, __shfl_xor_sync(0xffffffffu, most_r, o));
+      }
+      const float scale_c = scale_of(most_c), scale_r = scale_of(most_r);
+      if (lane < kLanes) {
+        int c[8], r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          c[i] = lost ? 0 : code_of(low[i], scale_c);
+          r[i] = lost ? 0 : code_of(high[i], scale_r);
+        }
+        const size_t of = (static_cast<size_t>(block - p.cache.pool) / cache_block_bytes(p.cache.page_tokens, D)) * 2;  // page * heads + head, twice
+        *reinterpret_cast<uint2*>(p.to.codes + of * D + channel) = make_uint2(pack4(c), pack4(c + 4));
+        *reinterpret_cast<uint2*>(p.to.codes + (of + 1) * D + channel) = make_uint2(pack4(r), pack4(r + 4));
+        if (lane == 0) *reinterpret_cast<float2*>(p.to.scales + of) = lost ? make_float2(quiet_nan(), quiet_nan()) : make_float2(scale_c, scale_r);
+      }
     }
-  }
-  float most_c = 0.0f, most_r = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-#pragma unroll
-    for (int o = kLanes; o < 32; o *= 2) {
-      low[i] = fminf(low[i], __shfl_xor_sync(0xffffffffu, low[i], o));
-      high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], o));
-    }
-    const float c = __fmul_rn(__fadd_rn(high[i], low[i]), 0.5f), r = __fmul_rn(__fsub_rn(high[i], low[i]), 0.5f);
-    low[i] = c;
-    high[i] = r;
-    most_c = fmaxf(most_c, fabsf(c));
-    most_r = fmaxf(most_r, r);
-  }
-#pragma unroll
-  for (int o = 1; o < kLanes; o *= 2) {
-    most_c = fmaxf(most_c, __shfl_xor_sync(0xffffffffu, most_c, o));
-    most_r = fmaxf(most_r, __shfl_xor_sync(0xffffffffu, most_r, o));
-  }
-  lost = __any_sync(0xffffffffu, lost);  // a key that is NaN, or of an infinite scale: nothing can be said of the page
-  const float scale_c = scale_of(most_c), scale_r = scale_of(most_r);
-  if (lane >= kLanes) return;
-  int c[8], r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = lost ? 0 : code_of(low[i], scale_c);
-    r[i] = lost ? 0 : code_of(high[i], scale_r);
-  }
-  const size_t of = (static_cast<size_t>(block - p.cache.pool) / cache_block_bytes(p.cache.page_tokens, D)) * 2;  // page * heads + head, twice
-  *reinterpret_cast<uint2*>(p.to.codes + of * D + channel) = make_uint2(pack4(c), pack4(c + 4));
-  *reinterpret_cast<uint2*>(p.to.codes + (of + 1) * D + channel) = make_uint2(pack4(r), pack4(r + 4));
-  if (lane == 0) {
-    p.to.scales[of] = lost ? quiet_nan() : scale_c;
-    p.to.scales[of + 1] = lost ? quiet_nan() : scale_r;
+    __syncthreads();  // `ends` belongs to the next page
   }
 }
 
@@ -169,11 +189,18 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 2 : 3) score_kern
   constexpr int kWide = D / 64;
   uint4 x[2][2][kWide];  // [row][c, r][channels]
   float2 by[2];
-  const auto load = [&](int base) {
+  uint32_t number[2];  // of the pages that are loaded next
+  const auto look = [&](int base) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int index = base + static_cast<int>(g) + i * 8;
-      const uint32_t page = index < pages ? static_cast<uint32_t>(__ldg(table + index)) : 0xFFFFFFFFu;
+      number[i] = index < pages ? static_cast<uint32_t>(__ldg(table + index)) : 0xFFFFFFFFu;
+    }
+  };
+  const auto load = [&] {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t page = number[i];
       const bool there = page < p.a.cache.pages;
       const size_t place = (static_cast<size_t>(there ? page : 0) * heads + head) * 2;
       by[i] = there ? __ldg(reinterpret_cast<const float2*>(p.from.scales + place)) : make_float2(quiet_nan(), quiet_nan());
@@ -184,13 +211,18 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 2 : 3) score_kern
     }
   };
   int base = first + static_cast<int>(warp) * 16;
-  load(base);  // while the queries are worked on
+  look(base);
+  load();  // while the queries are worked on
+  look(base + kScorePages);
   const int position = place_of_row(p.a.batch, row).x;
   const uint32_t blocks = (p.group + kHeads - 1) / kHeads;
   float best[2];
   bool unknown[2];
   for (uint32_t turn = 0; turn < p.turns; ++turn, base += kScorePages) {
-    if (turn) load(base);
+    if (turn) {
+      load();
+      look(base + kScorePages);
+    }
     best[0] = best[1] = -INFINITY;
     unknown[0] = unknown[1] = false;
     for (uint32_t h0 = 0; h0 < p.group; h0 += kHeads) {
@@ -265,6 +297,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 2 : 3) score_kern
 // A block for each (row, kv head): the budget-th largest key, digit by digit, then the pages above it in order.
 constexpr int kKept = 8192;  // keys in shared memory
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectParams p) {
   __shared__ uint32_t kept[kKept];
   __shared__ uint32_t count[256];
@@ -284,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   for (uint32_t i = tid; i < min(pages, static_cast<uint32_t>(kKept)); i += kThreads) kept[i] = __ldcg(keys + i);
   uint32_t digits = 0, left = p.budget;  // the digits found so far; how many of the keys that begin with them are taken
   for (int shift = 24; shift >= 0; shift -= 8) {
-    count[tid] = 0;
+    if (tid < 256) count[tid] = 0;
     __syncthreads();
     for (uint32_t i = tid; i < pages; i += kThreads) {
       const uint32_t k = key(i);
@@ -292,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     }
     __syncthreads();
     // keys of larger digits: a sum from the top
-    const uint32_t mine = count[255 - tid];
+    const uint32_t mine = tid < 256 ? count[255 - tid] : 0;
     uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -301,8 +334,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     }
     if (lane == 31) warps[warp] = upto;
     __syncthreads();
-    for (uint32_t i = 0; i < warp; ++i) upto += warps[i];
-    if (upto - mine < left && left <= upto) {
+    for (uint32_t i = 0; i < min(warp, 8u); ++i) upto += warps[i];
+    if (tid < 256 && upto - mine < left && left <= upto) {
       chosen[0] = 255 - tid;
       chosen[1] = left - (upto - mine);
     }
@@ -363,12 +396,13 @@ cudaError_t score_as(const LaunchEnv& env, const SelectParams& p) {
 }  // namespace
 
 cudaError_t launch_summarize(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, const Summaries& to) {
-  const SummaryParams p = {cache, batch, to};
-  const uint64_t grid = (static_cast<uint64_t>(batch.tokens) * cache.kv_heads * 32 + kThreads - 1) / kThreads;
+  // one token each: every one has a page; else one of sixteen, or less
+  const SummaryParams p = {cache, batch, to, batch.starts ? 4u : 1u};
+  const uint64_t grid = (static_cast<uint64_t>(batch.tokens) + p.each - 1) / p.each * cache.kv_heads;
   switch (cache.head_dim) {
-    case 64: return launch_after(env, summarize_kernel<64>, grid, kThreads, p);
-    case 128: return launch_after(env, summarize_kernel<128>, grid, kThreads, p);
-    case 256: return launch_after(env, summarize_kernel<256>, grid, kThreads, p);
+    case 64: return launch_after(env, summarize_kernel<64>, grid, kSummaryThreads, p);
+    case 128: return launch_after(env, summarize_kernel<128>, grid, kSummaryThreads, p);
+    case 256: return launch_after(env, summarize_kernel<256>, grid, kSummaryThreads, p);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -385,9 +419,9 @@ cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& a, const Summa
   p.last = last;
   p.keys = static_cast<uint32_t*>(env.workspace);
   p.out = out;
-  // a block quantises its queries once: it takes more pages where there are blocks enough for all SMs, eight each
+  // a block quantises its queries once: it takes more pages where there are blocks enough for all SMs, three each at a time
   const uint64_t blocks = static_cast<uint64_t>(a.batch.tokens) * a.cache.kv_heads, most = (a.batch.width + kScorePages - 1) / kScorePages;
-  p.turns = static_cast<uint32_t>(std::min<uint64_t>({std::max<uint64_t>(blocks * most / (8ull * env.sm_count), 1), most, 8}));
+  p.turns = static_cast<uint32_t>(std::min<uint64_t>({std::max<uint64_t>((blocks * most + 3ull * env.sm_count - 1) / (3ull * env.sm_count), 1), most, 16}));
   p.chunks = static_cast<uint32_t>((most + p.turns - 1) / p.turns);
   *launches = 0;
   // as many rows at a time as have room in the scratch and in a grid
@@ -396,7 +430,9 @@ cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& a, const Summa
     p.row0 = row;
     p.rows = static_cast<uint32_t>(std::min<uint64_t>(a.batch.tokens - row, std::max<uint64_t>(room, 1)));
     cudaError_t e = a.dtype == KQ_F32 ? score_as<float>(env, p) : a.dtype == KQ_F16 ? score_as<__half>(env, p) : score_as<__nv_bfloat16>(env, p);
-    if (e == cudaSuccess) e = launch_after(env, select_kernel, static_cast<uint64_t>(p.rows) * a.cache.kv_heads, kThreads, p);
+    // a thousand pages and more: 1024 threads (3126 pages: 11 -> 8 us)
+    const uint64_t lists = static_cast<uint64_t>(p.rows) * a.cache.kv_heads;
+    if (e == cudaSuccess) e = a.batch.width > 1024 ? launch_after(env, select_kernel<1024>, lists, 1024, p) : launch_after(env, select_kernel<256>, lists, 256, p);
     if (e != cudaSuccess) return e;
     *launches += 2;
   }

@@ -622,8 +622,8 @@ class Gpu:
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
             raise KqError(2, f"q must have {batch.tokens} rows")
-        if min(budget, first, last) < 0:
-            raise KqError(2, f"{budget} pages, the first {first} and the last {last}: no negative numbers")
+        if not (0 < budget <= 1 << 20 and 0 <= first <= budget and 0 <= last <= budget):
+            raise KqError(2, f"{budget} pages, the first {first} and the last {last} of them always: 1..2^20, no more than all")
         pq, q_stride = _rows(q, heads, dim, "q")
         shape = (batch.tokens, cache.kv_heads, int(budget))
         if out is None:
