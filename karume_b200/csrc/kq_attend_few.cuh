@@ -79,6 +79,10 @@ struct Few {
   static constexpr bool kQInRegisters = NT * kSteps <= 16;
   static constexpr int kPartFloats = kRows * (D + 2);  // a partial result in the scratch: sums, M, l
   static constexpr int kShort = 512 / kTile;                    // tiles of a run that is not shared by CTAs
+  // What a run costs whatever its length (its queries, joining its warps, what it has in common: 5 to 6 us), in tiles: a range of the list is
+  // cut by both.  (64 sequences of up to 1024 tokens behind common ones, by tiles alone: the last CTA ended after 45 us, the mean one after 26.)
+  // Whole sequences are cut by tiles, and selections, which are alike.
+  static constexpr int kHead = kMode == kShared ? 640 / kTile : 0;
   static constexpr int kSpans = 128;                   // sequences whose lengths are kept in shared memory
 
   static constexpr int kRing = 0;
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
     if (kept && !prefix) spans[b] = item;
     const Runs r = runs_of<kMode>(p, item, b, kRows, kTile);
     const Span span = r.span;
-    mine += static_cast<unsigned long long>(r.units) * static_cast<unsigned>(r.tiles);
+    mine += static_cast<unsigned long long>(r.units) * static_cast<unsigned>(r.tiles + F::kHead);
     mine_runs += r.units;
     if (!prefix && span.length == 0 && blockIdx.x == b % gridDim.x)  // an idle sequence's rows are zero
       for (int i = 0; i < span.count; ++i)
@@ -358,17 +362,18 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
     w.b = static_cast<uint32_t>(found[2 * i]);
     w.runs = runs_of<kMode>(p, item_at(w.b), w.b, kRows, kTile);
     unsigned long long skip = x - found[2 * i + 1];
-    while (skip >= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles)) {  // sequences of one thread's share
-      skip -= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles);
+    while (skip >= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles + F::kHead)) {  // sequences of one thread's share
+      skip -= static_cast<unsigned long long>(w.runs.units) * static_cast<unsigned>(w.runs.tiles + F::kHead);
       ++w.b;
       w.runs = runs_of<kMode>(p, item_at(w.b), w.b, kRows, kTile);
     }
-    const uint32_t unit = static_cast<uint32_t>(skip / static_cast<unsigned>(w.runs.tiles));
-    int in = static_cast<int>(skip % static_cast<unsigned>(w.runs.tiles));
-    if (w.runs.tiles <= F::kShort) {
+    const uint32_t unit = static_cast<uint32_t>(skip / static_cast<unsigned>(w.runs.tiles + F::kHead));
+    int in = static_cast<int>(skip % static_cast<unsigned>(w.runs.tiles + F::kHead));
+    if (w.runs.tiles <= F::kShort || in <= F::kHead) {
       x -= static_cast<unsigned>(in);
-      in = 0;
+      in = F::kHead;
     }
+    in -= F::kHead;
     w.head = unit / w.runs.blocks;
     w.block = unit % w.runs.blocks;
     w.tile = w.runs.tile_lo + in;
@@ -392,7 +397,20 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
   const uint32_t block_bytes = static_cast<uint32_t>(cache_block_bytes(P, D)), page_bytes = block_bytes * p.a.cache.kv_heads;  // 1024 heads: 70 MB at most
   Walk ahead = at;
   ahead.tile += static_cast<int>(warp);
-  int to_issue = end - begin > warp ? static_cast<int>((end - begin - warp + kWarps - 1) / kWarps) : 0;  // tiles of this warp not passed yet
+  unsigned long long range = end - begin;  // tiles of the range: without what runs cost
+  if constexpr (F::kHead > 0) {
+    Walk w = at;
+    range = 0;
+    for (unsigned long long pos = begin; pos < end;) {
+      const unsigned head = w.tile == w.runs.tile_lo ? F::kHead : 0;
+      const unsigned in_run = min(static_cast<unsigned>(w.runs.tile_lo + w.runs.tiles - w.tile), static_cast<unsigned>(end - pos - head));
+      range += in_run;
+      pos += head + in_run;
+      w.tile += static_cast<int>(in_run);
+      if (pos < end) settle<kMode>(w, p, items, kRows, kTile, all, item_at);
+    }
+  }
+  int to_issue = range > warp ? static_cast<int>((range - warp + kWarps - 1) / kWarps) : 0;  // tiles of this warp not passed yet
   uint32_t issued = 0, used = 0;
   // the next tile to copy: its page number is loaded a tile's time before it is needed
   bool wanted = false;
@@ -453,9 +471,11 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
   constexpr uint32_t kCentre1 = 0x80788078u;  // -7.5 2^-20, twice
 
   // ---- run by run --------------------------------------------------------------------------------
+  unsigned long long passed = 0;  // tiles of the range
   for (unsigned long long pos = begin; pos < end;) {
     const int run_end = at.runs.tile_lo + at.runs.tiles;
-    const int stop = static_cast<int>(min(static_cast<unsigned long long>(run_end), at.tile + (end - pos)));
+    const unsigned head_of_run = at.tile == at.runs.tile_lo ? F::kHead : 0;  // at a run's beginning
+    const int stop = static_cast<int>(min(static_cast<unsigned long long>(run_end), at.tile + (end - pos - head_of_run)));
     const int q_rows = at.runs.span.count * static_cast<int>(p.group);
     const int base = kMode == kSelected ? at.runs.position : at.runs.span.length - at.runs.span.count;
     const Keys keys = at.keys;
@@ -565,7 +585,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
     constexpr int kHold = kSplit ? 2 : 4, kSide = kSplit ? 1 : 2;  // row i's dims are [i] and [kSide + i]
     float O[NT][F::kVWords * 4][kHold] = {};
 
-    const int ahead_of = static_cast<int>((pos - begin) % kWarps);
+    const int ahead_of = static_cast<int>((F::kHead > 0 ? passed : pos - begin) % kWarps);
     for (int tile_at = at.tile + (static_cast<int>(warp) + kWarps - ahead_of) % kWarps; tile_at < stop; tile_at += kWarps) {
       const int first = tile_at * kTile;
       if (first > keys.last || first + kTile <= keys.first) continue;
@@ -834,7 +854,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
     constexpr int kQuads = kRows * D / 4;  // outputs of the block, by four
     constexpr int kLoops = (kQuads + F::kThreads - 1) / F::kThreads;
     const bool complete = at.tile == at.runs.tile_lo && stop == run_end;
-    const unsigned long long run_begin = pos - static_cast<unsigned>(at.tile - at.runs.tile_lo);
+    const unsigned long long run_begin = pos + head_of_run - static_cast<unsigned>(at.tile - at.runs.tile_lo);  // its first tile's place
     const uint32_t c0 = static_cast<uint32_t>(run_begin / per), c1 = static_cast<uint32_t>((run_begin + static_cast<unsigned>(at.runs.tiles) - 1) / per);
     auto slot_of = [&](uint32_t c) { return c == c0 ? 2 * c0 + 1 : 2 * c; };  // a CTA's last run goes on, or its first came from before
     float* part = p.parts + static_cast<size_t>(slot_of(blockIdx.x)) * F::kPartFloats;
@@ -969,7 +989,8 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
       }
     }
     __syncthreads();  // q_frag, row_const, merge and warp_stat belong to the next run
-    pos += static_cast<unsigned>(stop - at.tile);
+    pos += head_of_run + static_cast<unsigned>(stop - at.tile);
+    passed += static_cast<unsigned>(stop - at.tile);
     at.tile = stop;
     if (pos < end) settle<kMode>(at, p, items, kRows, kTile, all, item_at);
   }

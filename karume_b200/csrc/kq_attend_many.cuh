@@ -477,8 +477,17 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     const int q = static_cast<int>((static_cast<float>(r + head_of_row0) + 0.5f) * inv_group);
     return make_int2(q_of_row0 + q, r + head_of_row0 - q * static_cast<int>(p.group));
   };
-  const auto position_of = [&](int query) {
-    if (prefix) return place_of_row(p.a.batch, static_cast<uint32_t>(span.first + query)).x;
+  // Groups: where each row of the block is, looked up by a thread each (by the lanes that load a row it took 6 of 14 us)
+  if (prefix) {
+    for (uint32_t r = tid; r < kBlock; r += F::kThreads) {
+      const int2 qh = query_and_head(min(static_cast<int>(r), n_rows - 1 - row0));
+      const int2 place = place_of_row(p.a.batch, static_cast<uint32_t>(span.first + qh.x));
+      rows[r] = make_float4(__int_as_float(place.x), __int_as_float(place.y), 0.0f, 0.0f);
+    }
+    __syncthreads();
+  }
+  const auto position_of = [&](uint32_t r, int query) {
+    if (prefix) return __float_as_int(rows[r].x);
     return before + query;
   };
   const auto pointer_of = [&](int2 qh) {
@@ -504,9 +513,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     int from = there && window && last + 1 > window ? last + 1 - window : 0;
     if constexpr (kGroups) {
       if (prefix && there) {
-        const int2 place = place_of_row(p.a.batch, static_cast<uint32_t>(span.first + query_and_head(static_cast<int>(r)).x));
-        last = min(place.y, span.length) - 1;
-        from = window && place.x + 1 > window ? place.x + 1 - window : 0;
+        const int position = __float_as_int(rows[r].x);
+        last = min(__float_as_int(rows[r].y), span.length) - 1;
+        from = window && position + 1 > window ? position + 1 - window : 0;
       } else if (there) {
         from = max(from, common);
       }
@@ -531,7 +540,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       for (uint32_t k = 0; k < kBatch; ++k) {
         const int2 qh = query_and_head(min(static_cast<int>(r0 + k * kStep), n_rows - 1 - row0));
         const T* from_q = pointer_of(qh);
-        const int position = position_of(qh.x);
+        const int position = position_of(r0 + k * kStep, qh.x);
         const bool inside = position >= 0 && static_cast<uint32_t>(position) < p.a.rope.positions;
         load2(from_q + 2 * c, x[k][0], x[k][1]);
         load2(from_q + D / 2 + 2 * c, x[k][2], x[k][3]);
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       const bool there = row0 + static_cast<int>(r) < n_rows;
       const int2 qh = query_and_head(min(static_cast<int>(r), n_rows - 1 - row0));
       float v[8], big = 0.0f, sum = 0.0f;
-      load8_rotated(pointer_of(qh), c * 8, p.a.rope, position_of(qh.x), v);
+      load8_rotated(pointer_of(qh), c * 8, p.a.rope, position_of(r, qh.x), v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         v[i] = there ? v[i] : 0.0f;
@@ -939,6 +948,24 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       // Rows go out whole, through the block's queries' memory, which every score has been made of by now: a thread's own row is 16
       // bytes of 32 rows an instruction.
       uint8_t* const mine = smem + F::kQ + wg * F::kOperand + warp % 4 * (32 * D * 2);
+      if (kGroups && prefix && shared) {  // sums in f32: half of a row at a time
+        constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;
+        for (int half = 0; half < 2; ++half) {
+          tmem_columns<D / 2, false>(tmem + lanes + 256 + wg * 128 + half * (D / 2), [&](int c, float (&x)[16]) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              *reinterpret_cast<float4*>(mine + lane * (D * 2) + ((c / 4 + h) ^ (lane & 7)) * 16) = make_float4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
+            __syncwarp();
+          });
+#pragma unroll 4
+          for (uint32_t i = lane / kChunks; i < 32; i += kAtOnce) {
+            const uint32_t chunk = lane % kChunks;
+            *reinterpret_cast<float4*>(part + static_cast<size_t>(wg * 128 + warp % 4 * 32 + i) * D + half * (D / 2) + chunk * 4) =
+                *reinterpret_cast<const float4*>(mine + i * (D * 2) + (chunk ^ (i & 7)) * 16);
+          }
+          __syncwarp();
+        }
+      } else
       tmem_columns<D, false>(tmem + lanes + 256 + wg * 128, [&](int c, float (&x)[16]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= inv;

@@ -104,7 +104,7 @@ __device__ __forceinline__ void join_common(const SharedArgs& sh, size_t row, in
   const uint4 at = __ldcg(sh.places + row);
   const float4* const sums = reinterpret_cast<const float4*>(sh.scratch) + at.x + quad;
   const float2* const stats = reinterpret_cast<const float2*>(sh.scratch) + at.y;
-  constexpr uint32_t kBatch = 8;
+  constexpr uint32_t kBatch = 12;
   for (uint32_t j0 = 0; j0 < at.w; j0 += kBatch) {
     float2 ml[kBatch];
     float4 x[kBatch];
