@@ -576,6 +576,15 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
         factor[n][i] = c.x;
         offset[n][i] = c.y;
       }
+    // what the one row of a thread has in common: its place is there when the row is finished
+    uint4 place_ahead = {};
+    if constexpr (kMode == kShared && kRows * D / 4 <= F::kThreads) {
+      const int row = static_cast<int>(at.block) * kRows + static_cast<int>(tid) / (D / 4);
+      if (!prefix && at.runs.low > 0 && static_cast<int>(tid) < kRows * D / 4 && row < q_rows) {
+        const int query = row / static_cast<int>(p.group);
+        place_ahead = __ldcg(p.sh.places + static_cast<size_t>(at.runs.span.first + query) * p.a.heads + at.head * p.group + static_cast<uint32_t>(row - query * static_cast<int>(p.group)));
+      }
+    }
     float M[NT][kPer], l[NT][kPer] = {}, centre[NT][kPer] = {};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -875,7 +884,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
         }
         if (at.runs.low > 0) {  // with what the row sees of the common keys
           float all[4] = {v[0], v[1], v[2], v[3]};
-          join_common(p.sh, of, quad % (D / 4), m, total_l, all);
+          join_common(p.sh, kLoops == 1 ? place_ahead : __ldcg(p.sh.places + of), quad % (D / 4), m, total_l, all);
           const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
           const float o[4] = {all[0] * inv, all[1] * inv, all[2] * inv, all[3] * inv};
           store4(static_cast<T*>(p.a.out) + static_cast<size_t>(at.runs.span.first + query) * p.a.out_stride + static_cast<size_t>(head) * D + quad % (D / 4) * 4, o);

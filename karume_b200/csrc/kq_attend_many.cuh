@@ -470,6 +470,13 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   __syncthreads();  // `scan` and the units' list lie where the queries go
 
   // ---- queries --------------------------------------------------------------------------------------
+  // kGroups: the copying warp is on its way to the first tiles meanwhile; the others meet without it.
+  constexpr uint32_t kAskers = kGroups ? F::kCopyWarp : F::kThreads / 32;
+  const bool asks = !kGroups || warp != F::kCopyWarp;
+  const auto meet = [&] {
+    if constexpr (!kGroups) __syncthreads();
+    else if (asks) asm volatile("bar.sync 4, %0;" ::"n"(F::kCopyWarp * 32) : "memory");
+  };
   const int q_of_row0 = row0 / static_cast<int>(p.group), head_of_row0 = row0 - q_of_row0 * static_cast<int>(p.group);
   const float inv_group = 1.0f / static_cast<float>(p.group);
   // query and head of row row0 + r: numbers below 2^17, so that the rounded-down product with the reciprocal is the quotient
@@ -484,7 +491,8 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
       const int2 place = place_of_row(p.a.batch, static_cast<uint32_t>(span.first + qh.x));
       rows[r] = make_float4(__int_as_float(place.x), __int_as_float(place.y), 0.0f, 0.0f);
     }
-    __syncthreads();
+    static_assert(!kGroups || kBlock <= F::kCopyWarp * 32, "rows of the warps that meet");
+    meet();
   }
   const auto position_of = [&](uint32_t r, int query) {
     if (prefix) return __float_as_int(rows[r].x);
@@ -528,54 +536,61 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   if (rope_is_plain(p.a.rope) && p.a.rope.rotary == D) {
     // Half layout, whole heads: a lane has two pairs of a row, so that the angles are read coalesced (runs of eight dims a lane read them
     // at a stride of 64 bytes, 9000 clocks a CTA); words of dims (d, d + 4) are put together with the lane two further on.
-    constexpr uint32_t kLanes = D / 4, kRowsAtOnce = 32 / kLanes, kStep = F::kThreads / 32 * kRowsAtOnce, kBatch = kBlock / kStep < 8 ? kBlock / kStep : 8;
-    static_assert(kBlock % (kStep * kBatch) == 0, "whole batches");
+    constexpr uint32_t kLanes = D / 4, kRowsAtOnce = 32 / kLanes, kStep = kAskers * kRowsAtOnce, kEach = (kBlock + kStep - 1) / kStep;
+    constexpr uint32_t kTurns = (kEach + 8) / 9, kBatch = (kEach + kTurns - 1) / kTurns;  // rows a lane has at a time
+    static_assert(kBatch <= kLanes, "a lane for the constants of each row");
     const uint32_t c = lane % kLanes;
     const uint32_t word = (c & 1) * 2 + (c >> 1 & 1);  // of its eight dims' chunk: dims (0, 4), (1, 5), (2, 6), (3, 7) from lanes 0, 2, 1, 3
 #pragma unroll 1
-    for (uint32_t r0 = warp * kRowsAtOnce + lane / kLanes; r0 < kBlock; r0 += kStep * kBatch) {
-      float x[kBatch][4];
+    for (uint32_t r0 = warp * kRowsAtOnce + lane / kLanes, turn = 0; asks && turn < kTurns; r0 += kStep * kBatch, ++turn) {
+      float x[kBatch][4], big[kBatch], sum[kBatch];
       float4 cs[kBatch];
 #pragma unroll
       for (uint32_t k = 0; k < kBatch; ++k) {
-        const int2 qh = query_and_head(min(static_cast<int>(r0 + k * kStep), n_rows - 1 - row0));
+        const uint32_t r = min(r0 + k * kStep, static_cast<uint32_t>(kBlock) - 1);
+        const int2 qh = query_and_head(min(static_cast<int>(r), n_rows - 1 - row0));
         const T* from_q = pointer_of(qh);
-        const int position = position_of(r0 + k * kStep, qh.x);
+        const int position = position_of(r, qh.x);
         const bool inside = position >= 0 && static_cast<uint32_t>(position) < p.a.rope.positions;
         load2(from_q + 2 * c, x[k][0], x[k][1]);
         load2(from_q + D / 2 + 2 * c, x[k][2], x[k][3]);
         cs[k] = reinterpret_cast<const float4*>(p.a.rope.table + static_cast<size_t>(inside ? position : 0) * (D / 2))[c];
         if (!inside) cs[k].x = cs[k].z = quiet_nan();
       }
+      // (step by step for all rows, so that one row's shuffles do not wait for another's)
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k) {
+        const bool there = row0 + static_cast<int>(r0 + k * kStep) < n_rows;
+        const float2 a = rotate_pair(x[k][0], x[k][2], make_float2(cs[k].x, cs[k].y)), b = rotate_pair(x[k][1], x[k][3], make_float2(cs[k].z, cs[k].w));
+        // dims 2 c, 2 c + 1, and those half a head on
+        x[k][0] = there ? a.x : 0.0f;
+        x[k][1] = there ? b.x : 0.0f;
+        x[k][2] = there ? a.y : 0.0f;
+        x[k][3] = there ? b.y : 0.0f;
+        big[k] = fmaxf(fmaxf(fabsf(x[k][0]), fabsf(x[k][1])), fmaxf(fabsf(x[k][2]), fabsf(x[k][3])));
+        sum[k] = 0.0f;
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o /= 2)
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k) big[k] = fmaxf(big[k], __shfl_xor_sync(0xffffffffu, big[k], o));
+      int my_up = 0;
+      float my_sum = 0.0f;
 #pragma unroll
       for (uint32_t k = 0; k < kBatch; ++k) {
         const uint32_t r = r0 + k * kStep;
-        const bool there = row0 + static_cast<int>(r) < n_rows;
-        const float2 a = rotate_pair(x[k][0], x[k][2], make_float2(cs[k].x, cs[k].y)), b = rotate_pair(x[k][1], x[k][3], make_float2(cs[k].z, cs[k].w));
-        float v[4] = {a.x, b.x, a.y, b.y};  // dims 2 c, 2 c + 1, and those half a head on
-        float big = 0.0f, sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = there ? v[i] : 0.0f;
-          big = fmaxf(big, fabsf(v[i]));
-        }
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o /= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        const int up = lift_of(big);
+        const int up = lift_of(big[k]);
         const float lift = power(up);
+        if (c == k) my_up = up;
         float hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (kSplit) {
-            parts_of(v[i] * lift, i & 1, hi[i], lo[i]);
-            sum = fmaf(hi[i] + lo[i], (i & 1) ? 8.0f : 1.0f, sum);
+            parts_of(x[k][i] * lift, i & 1, hi[i], lo[i]);
+            sum[k] = fmaf(hi[i] + lo[i], (i & 1) ? 8.0f : 1.0f, sum[k]);
           } else {
-            hi[i] = v[i] * lift;
+            hi[i] = x[k][i] * lift;
           }
-        }
-        if constexpr (kSplit) {
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
@@ -586,16 +601,25 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
             const uint32_t out = c & 2 ? __byte_perm(other2, mine2, 0x7632) : __byte_perm(mine2, other2, 0x5410);
             const uint32_t chunk = half * (D / 16) + c / 4;
             const uint32_t at = base + F::kQ + ((r / 128) * kParts + part) * F::kOperand + (chunk / 8) * 16384 + umma::swz(r % 128, chunk % 8) + word * 4;
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(out) : "memory");
+            if (kBlock % (kStep * kBatch) == 0 || r < kBlock) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(out) : "memory");
           }
-        if (c == 0) row_constants(r, up, sum);
       }
+      if constexpr (kSplit) {
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o /= 2)
+#pragma unroll
+          for (uint32_t k = 0; k < kBatch; ++k) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+          if (c == k) my_sum = sum[k];
+      }
+      if (c < kBatch && r0 + c * kStep < kBlock) row_constants(r0 + c * kStep, my_up, my_sum);
     }
   } else {
     constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
     const uint32_t c = lane % kLanes;
 #pragma unroll 1
-    for (uint32_t r = warp * kRowsAtOnce + lane / kLanes; r < kBlock; r += F::kThreads / 32 * kRowsAtOnce) {
+    for (uint32_t r = warp * kRowsAtOnce + lane / kLanes; asks && r - lane / kLanes < kBlock; r += kAskers * kRowsAtOnce) {
       const bool there = row0 + static_cast<int>(r) < n_rows;
       const int2 qh = query_and_head(min(static_cast<int>(r), n_rows - 1 - row0));
       float v[8], big = 0.0f, sum = 0.0f;
@@ -636,9 +660,9 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  meet();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_word;
+  const uint32_t tmem = asks ? *tmem_word : 0;
 
   if (warp < 8) {
     // ---- softmax and output: a row a thread --------------------------------------------------------
@@ -898,11 +922,12 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
           return;
         }
         if (common > 0) {
+          const uint4 place = __ldcg(p.sh.places + of);
           float z[8];
 #pragma unroll
           for (int half = 0; half < 8; half += 4) {
             float top = m - kLifted, all = total, v[4] = {o[half], o[half + 1], o[half + 2], o[half + 3]};
-            join_common(p.sh, of, (i + half) / 4, top, all, v);
+            join_common(p.sh, place, (i + half) / 4, top, all, v);
             const float inv = all == 0.0f ? 0.0f : 1.0f / all;
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[half + e] = v[e] * inv;

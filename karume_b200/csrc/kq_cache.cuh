@@ -99,9 +99,14 @@ __device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const Sha
   return make_int4(row0, row1 - row0, keys, from);
 }
 
-// Four of the sums of a row, not divided yet, relative to 2^m, and the sum of its weights: joined with what the row sees of the common keys.
-__device__ __forceinline__ void join_common(const SharedArgs& sh, size_t row, int quad, float& m, float& total, float (&v)[4]) {
-  const uint4 at = __ldcg(sh.places + row);
+__device__ __forceinline__ float power_of_two(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Four of the sums of a row, not divided yet, relative to 2^m, and the sum of its weights: joined with what the row sees of the common keys,
+// which is at the row's place `at`.
+__device__ __forceinline__ void join_common(const SharedArgs& sh, const uint4& at, int quad, float& m, float& total, float (&v)[4]) {
   const float4* const sums = reinterpret_cast<const float4*>(sh.scratch) + at.x + quad;
   const float2* const stats = reinterpret_cast<const float2*>(sh.scratch) + at.y;
   constexpr uint32_t kBatch = 12;
@@ -120,14 +125,14 @@ __device__ __forceinline__ void join_common(const SharedArgs& sh, size_t row, in
       if (j0 + j >= at.w) ml[j] = make_float2(-INFINITY, 0.0f);
       now = fmaxf(now, ml[j].x);
     }
-    const float before = m == -INFINITY ? 0.0f : exp2f(m - now);
+    const float before = m == -INFINITY ? 0.0f : power_of_two(m - now);
     m = now;
     total *= before;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] *= before;
 #pragma unroll
     for (uint32_t j = 0; j < kBatch; ++j) {
-      const float keep = ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - m);
+      const float keep = ml[j].x == -INFINITY ? 0.0f : power_of_two(ml[j].x - m);
       total = fmaf(keep, ml[j].y, total);
       v[0] = fmaf(keep, x[j].x, v[0]);
       v[1] = fmaf(keep, x[j].y, v[1]);
