@@ -409,8 +409,11 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
 /* kq_cache_attention_shared: kq_cache_attention for sequences that begin alike, the keys that they have in common read once.  Group g is the
  * sequences first[g] .. first[g + 1] - 1 (i32 [groups + 1], ascending); their first shared[g] tokens (i32 [groups]) are the same: their
  * tables name the same pages for them, or (a last page that is not full) copies.  What is shared beyond a sequence's new tokens' beginning counts as
- * its own; sequences outside the groups, and a group of one, are as in kq_cache_attention.  The same results but for roundings.  The sums over the
- * common keys take 4 (head_dim + 2) bytes a row and query head of the context's scratch; where that is more than half of it, nothing is read once.
+ * its own; sequences outside the groups, and a group of one, are as in kq_cache_attention.  The same results but for roundings.  Reading
+ * once takes a launch more and joins every row's sums, reading often hits L2: `least` is how many bytes (tokens in common x members but one
+ * x kv_heads (head_dim + 8), as the device arrays say) have to be saved for it, 0 for always, KQ_SHARED_AUTO for what measured faster.  The sums
+ * over the common keys take 4 (head_dim + 6) bytes a row and query head of the context's scratch; where that is more than half of it, nothing is
+ * read once.
  *
  * kq_cache_summarize: for the pages that new tokens of the batch are in (behind their kq_cache_append), what kq_cache_select goes by: codes i8 [pages,
  * kv_heads, 2, head_dim] and scales f32 [pages, kv_heads, 2], the host's, 16- and 8-byte aligned.  Over the page's tokens up to the sequence's
@@ -425,10 +428,11 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
  * kq_cache_attention_selected: attention of every new token over the tokens of its selected pages up to its position; `selected` as kq_cache_select
  * gives it: min(budget, pages up to the position) indices are read, the last of which is the position's own page.  An index outside the table reads
  * as NaN.  For few rows a sequence: each reads its own pages. */
+#define KQ_SHARED_AUTO 0xFFFFFFFFFFFFFFFFull
 KQ_API int kq_cache_attention_shared(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads,
                                      uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr,
                                      uint64_t starts_dptr, uint32_t tokens, uint32_t most, uint32_t groups, uint64_t first_dptr,
-                                     uint64_t shared_dptr, float scale, uint32_t window, uint64_t table_dptr, uint32_t table_positions,
+                                     uint64_t shared_dptr, uint64_t least, float scale, uint32_t window, uint64_t table_dptr, uint32_t table_positions,
                                      uint32_t rotary, uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride);
 KQ_API int kq_cache_summarize(kq_ctx* ctx, kq_cache cache, uint64_t codes_dptr, uint64_t scales_dptr, uint32_t sequences,
                               uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens);

@@ -74,8 +74,8 @@ SYMBOLS = {
     "kq_cache_read": (_i32, [_vp, _u64, _u32, _u64, _u32, _u64, _u64, _u32, _u64, _u64]),
     "kq_cache_attention": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, ctypes.c_float, _u32,
                                   _u64, _u32, _u32, _u32, _u64, _u64]),
-    "kq_cache_attention_shared": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, _u32, _u64, _u64, ctypes.c_float,
-                                         _u32, _u64, _u32, _u32, _u32, _u64, _u64]),
+    "kq_cache_attention_shared": (_i32, [_vp, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, _u32, _u64, _u64, _u64,
+                                         ctypes.c_float, _u32, _u64, _u32, _u32, _u32, _u64, _u64]),
     "kq_cache_summarize": (_i32, [_vp, _u64, _u64, _u64, _u32, _u64, _u32, _u64, _u64, _u32]),
     "kq_cache_select": (_i32, [_vp, _u64, _u64, _u64, _u64, _u64, _i32, _u32, _u32, _u64, _u32, _u64, _u64, _u32, _u32, _u32, _u32, _u64, _u32, _u32,
                                _u32, _u64]),

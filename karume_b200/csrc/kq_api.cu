@@ -975,7 +975,7 @@ int kq_cache_attention(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t q_stri
 
 int kq_cache_attention_shared(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads, uint32_t sequences,
                               uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr, uint64_t starts_dptr, uint32_t tokens,
-                              uint32_t most, uint32_t groups, uint64_t first_dptr, uint64_t shared_dptr, float scale, uint32_t window,
+                              uint32_t most, uint32_t groups, uint64_t first_dptr, uint64_t shared_dptr, uint64_t least, float scale, uint32_t window,
                               uint64_t table_dptr, uint32_t table_positions, uint32_t rotary, uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride) {
   if (!ctx) return KQ_ERR_BAD_ARG;
   kq::AttendArgs a;
@@ -986,7 +986,11 @@ int kq_cache_attention_shared(kq_ctx* ctx, kq_cache h, uint64_t q_dptr, uint64_t
     return fail(ctx, KQ_ERR_BAD_ARG, "kq_cache_attention_shared: first [groups + 1] and shared [groups] are i32 device arrays");
   if (groups > sequences) return fail(ctx, KQ_ERR_SHAPE, "kq_cache_attention_shared: %u groups of %u sequences", groups, sequences);
   DeviceGuard guard(ctx->device);
-  const kq::SharedArgs sh = {reinterpret_cast<const int*>(first_dptr), reinterpret_cast<const int*>(shared_dptr), groups, nullptr, nullptr};
+  kq::SharedArgs sh = {};
+  sh.first = reinterpret_cast<const int*>(first_dptr);
+  sh.tokens = reinterpret_cast<const int*>(shared_dptr);
+  sh.groups = groups;
+  sh.least = least;
   int launched = 0;
   cudaError_t e = groups ? kq::launch_attend_shared(env_of(ctx), a, sh, &launched) : kq::launch_attend(env_of(ctx), a, &launched);
   if (e != cudaSuccess) return cuda_fail(ctx, e, "cache_attention_shared launch");

@@ -281,6 +281,8 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
 
   // ---- this CTA's range of the list --------------------------------------------------------------
   const bool prefix = kMode == kShared && p.prefix;
+  const bool sharing = kMode != kShared || worth_sharing(p.a, p.sh);
+  if (prefix && !sharing) return;
   const uint32_t items = kMode == kSelected ? p.a.batch.tokens : prefix ? p.sh.groups : p.a.batch.sequences, each = (items + F::kThreads - 1) / F::kThreads;
   const bool kept = items <= F::kSpans;
   if constexpr (kMode == kShared) {
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
   auto make_item = [&](uint32_t b) {
     if constexpr (kMode == kSelected) return selected_row(p.a, p.sel, b);
     const Span span = span_of(p.a.batch, b);
-    return make_int4(span.first, span.count, span.length, kMode == kShared ? common_keys(p.a.batch, p.sh, b, span) : 0);
+    return make_int4(span.first, span.count, span.length, kMode == kShared && sharing ? common_keys(p.a.batch, p.sh, b, span) : 0);
   };
   auto item_at = [&](uint32_t b) { return kept ? spans[b] : make_item(b); };
   unsigned long long mine = 0;

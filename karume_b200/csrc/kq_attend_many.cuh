@@ -346,7 +346,8 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   __syncthreads();
 
   // ---- which rows: units are (sequence, block of rows from the last, kv head) ----------------------
-  const bool prefix = kGroups && p.prefix;
+  const bool prefix = kGroups && p.prefix, sharing = kGroups && worth_sharing(p.a, p.sh);
+  if (prefix && !sharing) return;
   const uint32_t sequences = prefix ? p.sh.groups : p.a.batch.sequences, each = (sequences + F::kThreads - 1) / F::kThreads, heads = p.a.cache.kv_heads;
   int4* const groups = reinterpret_cast<int4*>(smem + F::kRaw);  // until the codes come
   static_assert(kGroupsAtOnce * 16 <= F::kRawBytes, "the groups' place");
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     const int key_last = s.length - s.count + last, from = s.length - s.count + first + 1 - window;
     int tile0 = window && from > 0 ? from / kKeys : 0;
     if constexpr (kGroups) {
-      tile0 = max(tile0, common_keys(p.a.batch, p.sh, b, s) / kKeys);
+      if (sharing) tile0 = max(tile0, common_keys(p.a.batch, p.sh, b, s) / kKeys);
       if (key_last / kKeys < tile0) return make_int2(tile0, 0);
     }
     return make_int2(tile0, key_last < 0 ? 0 : key_last / kKeys + 1 - tile0);
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   const uint32_t seq = found[0];
   if (seq == 0xFFFFFFFFu) return;
   const Span span = rows_of(seq);
-  const int common = kGroups && !prefix ? common_keys(p.a.batch, p.sh, seq, span) : 0;
+  const int common = kGroups && !prefix && sharing ? common_keys(p.a.batch, p.sh, seq, span) : 0;
   const uint32_t blocks = blocks_of(seq), head = found[1] % heads, block = blocks - 1 - found[1] / heads;  // the longest first
   const uint32_t all_parts = found[3], my_part = all_parts > 1 ? found[2] : 0;
   const int row0 = static_cast<int>(block * kBlock), n_rows = span.count * static_cast<int>(p.group), before = span.length - span.count;

@@ -12,10 +12,26 @@ namespace kq {
 bool attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, const SharedArgs& sh, cudaError_t* e);
 cudaError_t attend_shared_rest_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 
+// Bytes that are read once instead of often, from which on that is faster: without it they come from L2 mostly, with it there is a launch more
+// and every row's sums are joined.  bfloat16, 32 heads over 8, this way / the other: 64 sequences behind 2048 common tokens (140 MB saved) 52 / 48 us,
+// behind 4096 (281 MB) 55 / 75, behind 32768 (2.2 GB) 103 / 449; f32, 12 over 2: 16 behind 4096 (17 MB) 46 / 26, behind 32768 (134 MB) 64 / 69.
+constexpr uint64_t kWorth = 150ull << 20;
+// Sequences of so many query rows a kv head fill the tensor cores' blocks of rows by themselves: 16 of up to 300 new tokens behind 16384, 4 heads a
+// kv head, bfloat16 1511 / 1045 us; 8 of up to 100 behind 32768, 497 / 648.
+constexpr uint64_t kAlone = 512;
+
 cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, SharedArgs sh, int* launches) {
   // The end of the scratch: a place for each row, and its sums where they are in one part; in front of it the parts of the sums over common
   // keys, a third of the rest.  Where the rows would take more than half of it, every sequence walks over all of its keys.
   const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, each = 16 + 4ull * (a.cache.head_dim + 2);
+  // What a call can save at most; then what it does save, as the lengths say on the device.
+  const uint64_t most = static_cast<uint64_t>(a.batch.sequences) * a.batch.width * cache_block_bytes(a.cache.page_tokens, a.cache.head_dim) * a.cache.kv_heads;
+  const uint64_t group = a.heads / a.cache.kv_heads;
+  if (sh.least == KQ_SHARED_AUTO) sh.least = static_cast<uint64_t>(a.batch.tokens) * group / a.batch.sequences > kAlone ? ~0ull : kWorth;
+  if (most < sh.least) return launch_attend(env, a, launches);
+  sh.all_first = sh.first;
+  sh.all_tokens = sh.tokens;
+  sh.all_groups = sh.groups;
   if (!env.workspace || rows * each + 64 > env.workspace_bytes / 2) return launch_attend(env, a, launches);
   uint8_t* const base = static_cast<uint8_t*>(env.workspace);
   const uint64_t left = (env.workspace_bytes - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
@@ -27,7 +43,6 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
   parts.workspace = base + own;
   parts.workspace_bytes = left - own;
   *launches = 0;
-  const uint64_t group = a.heads / a.cache.kv_heads;
   LaunchEnv alone = parts;  // groups that come in turns: none may leave its parts where the next one's go
   if (sh.groups > 128) alone.workspace = nullptr;
   cudaError_t e = cudaSuccess;

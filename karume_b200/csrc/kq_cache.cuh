@@ -61,6 +61,19 @@ __device__ __forceinline__ int2 place_of_row(const CacheBatch& batch, uint32_t r
 }
 
 // ---- sequences that begin alike ---------------------------------------------------------------
+// By a warp: whether reading what the groups have in common once saves enough (the other way re-reads it, mostly from L2).
+__device__ __forceinline__ bool worth_sharing(const AttendArgs& a, const SharedArgs& sh) {
+  unsigned long long keys = 0;
+  for (uint32_t g = threadIdx.x % 32; g < sh.all_groups; g += 32) {
+    const long long members = static_cast<long long>(__ldg(sh.all_first + g + 1)) - __ldg(sh.all_first + g);
+    unsigned tokens = static_cast<unsigned>(max(__ldg(sh.all_tokens + g), 0));
+    if (a.window) tokens = min(tokens, a.window);
+    if (members > 1) keys += static_cast<unsigned long long>(members - 1) * tokens;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) keys += __shfl_xor_sync(0xffffffffu, keys, o);
+  return keys * (a.cache.kv_heads * (a.cache.head_dim + 8u)) >= sh.least;
+}
 __device__ __forceinline__ uint32_t first_of_group(const CacheBatch& batch, const SharedArgs& sh, uint32_t g) {
   return min(static_cast<uint32_t>(max(__ldg(sh.first + g), 0)), batch.sequences - 1);
 }

@@ -239,6 +239,10 @@ struct SharedArgs {
   const int* first;   // [groups + 1] first sequence of each
   const int* tokens;  // [groups]
   uint32_t groups;
+  const int* all_first;  // of the whole call, where the above are some of its groups
+  const int* all_tokens;
+  uint32_t all_groups;
+  uint64_t least;     // bytes that reading common keys once has to save, else nothing is common
   float* scratch;
   uint4* places;      // [tokens of the call][heads]: first part's sums in `scratch` (of four floats), its (exponent of two that the weights are
                       // relative to, their sum) (of two), floats between parts, parts

@@ -36,7 +36,7 @@ using ReadFn = int (*)(void*, uint64_t, uint32_t, uint64_t, uint32_t, uint64_t, 
 using AttendFn = int (*)(void*, uint64_t, uint64_t, uint64_t, int, uint32_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, float,
                          uint32_t, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t, uint64_t);
 using AttendSharedFn = int (*)(void*, uint64_t, uint64_t, uint64_t, int, uint32_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, uint32_t,
-                               uint64_t, uint64_t, float, uint32_t, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t, uint64_t);
+                               uint64_t, uint64_t, uint64_t, float, uint32_t, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t, uint64_t);
 using AttendSelectedFn = int (*)(void*, uint64_t, uint64_t, uint64_t, int, uint32_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t, uint64_t, uint32_t,
                                  float, uint64_t, uint32_t, uint32_t, uint32_t, uint64_t, uint64_t);
 using SummarizeFn = int (*)(void*, uint64_t, uint64_t, uint64_t, uint32_t, uint64_t, uint32_t, uint64_t, uint64_t, uint32_t);
@@ -372,7 +372,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 
 // cache_attention_shared(ctx, handle, dim, q, batch args, most, shared args, scale, window, rope args, out)
 PyObject* cache_attention_shared(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-  uint64_t batch[6], table[4], groups[3];
+  uint64_t batch[6], table[4], groups[4];
   Rows r;
   if (nargs != 11 || a[0] == Py_None || !numbers_of(a[4], batch) || !numbers_of(a[6], groups) || !numbers_of(a[9], table)) KQ_NONE;
   if (!r.of(a[3], a[10], static_cast<int64_t>(batch[5]), PyLong_AsLongLong(a[2]))) KQ_NONE;
@@ -383,7 +383,7 @@ PyObject* cache_attention_shared(PyObject*, PyObject* const* a, Py_ssize_t nargs
   if (PyErr_Occurred()) return nullptr;
   const int rc = without_gil([&] {
     return g_attend_shared(ctx, handle, r.pq, r.q_stride, r.type, u32(r.heads), u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5]), most,
-                           u32(groups[0]), groups[1], groups[2], scale, window, table[0], u32(table[1]), u32(table[2]), u32(table[3]), r.po, r.out_stride);
+                           u32(groups[0]), groups[1], groups[2], groups[3], scale, window, table[0], u32(table[1]), u32(table[2]), u32(table[3]), r.po, r.out_stride);
   });
   return rc != 0 ? status_of(rc) : r.result(a[10]);
 }

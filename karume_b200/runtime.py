@@ -37,6 +37,8 @@ class KqError(RuntimeError):
         super().__init__(f"{self.status}: {message}")
 
 
+KQ_SHARED_AUTO = (1 << 64) - 1
+
 _NP_DTYPES = {np.dtype(np.float32): KQ_F32, np.dtype(np.float16): KQ_F16}
 
 
@@ -159,9 +161,10 @@ class KvCache:
 
 class SharedPrefixes:
     """Sequences that begin alike: first i32 CUDA [groups + 1] (group g is the sequences first[g] .. first[g + 1] - 1) and tokens i32 [groups],
-    how many tokens the sequences of each have in common at their beginning, in the same pages or copies of them."""
+    how many tokens the sequences of each have in common at their beginning, in the same pages or copies of them.  least: how many bytes
+    reading those once has to save for a call to do so (0: always; None: what measured faster)."""
 
-    def __init__(self, first, tokens):
+    def __init__(self, first, tokens, least: "int | None" = None):
         torch = _torch()
         for name, t in (("first", first), ("tokens", tokens)):
             if t.dtype != torch.int32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
@@ -169,8 +172,10 @@ class SharedPrefixes:
         self.groups = int(tokens.numel())
         if first.numel() != self.groups + 1:
             raise KqError(2, f"{self.groups} groups have {self.groups + 1} boundaries, not {first.numel()}")
+        if least is not None and not 0 <= least < KQ_SHARED_AUTO:
+            raise KqError(2, f"least {least}: a number of bytes")
         self.first, self.tokens = first, tokens
-        self.args = (self.groups, first.data_ptr(), tokens.data_ptr())
+        self.args = (self.groups, first.data_ptr(), tokens.data_ptr(), KQ_SHARED_AUTO if least is None else int(least))
 
 
 class CacheSummaries:

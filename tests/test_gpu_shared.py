@@ -77,7 +77,7 @@ class Groups:
 
     def prefixes(self, first=None, common=None):
         import karume_b200 as kb
-        return kb.SharedPrefixes(i32(first or self.first), i32(common or self.common))
+        return kb.SharedPrefixes(i32(first or self.first), i32(common or self.common), least=0)
 
     def call(self, kind, news, heads, window=0, rotary=0, interleaved=False, scale=None, strided=False, padding=0, prefixes=None, gpu=None, cache=None, most=0):
         import karume_b200 as kb
@@ -237,6 +237,40 @@ def test_little_scratch(gpu):  # noqa: F811
     g.free()
 
 
+def test_what_reading_once_has_to_save(gpu):  # noqa: F811
+    """Less saved than asked for: every sequence reads its own, as without groups; by what the device arrays say, in a recorded call too."""
+    import karume_b200 as kb
+    g = Groups(gpu, [(300, [5, 30, 1, 9]), (64, [70, 3])], 16, 2, 64, seed=9)
+    saved = (3 * 300 + 64) * 2 * 72
+    for heads in (8, 80):
+        q, batch = torch.randn(6, heads, 64, device="cuda"), kb.CacheBatch(g.table, g.length)
+        alone, once = (gpu.cache_attention(g.cache, q, batch, shared=s) for s in (None, g.prefixes()))
+        gpu.sync()
+        assert not torch.equal(alone, once)
+        for least, want in ((None, alone), (saved, once), (1, once), (1 << 40, alone)):
+            got = gpu.cache_attention(g.cache, q, batch, shared=kb.SharedPrefixes(g.prefixes().first, g.prefixes().tokens, least=least))
+            gpu.sync()
+            assert torch.equal(got, want), least
+        prefixes, out = kb.SharedPrefixes(g.prefixes().first, g.prefixes().tokens, least=saved), torch.zeros_like(q)
+        gpu.sync()
+        gpu.graph_begin()
+        gpu.cache_attention(g.cache, q, batch, shared=prefixes, out=out)
+        graph = gpu.graph_end()
+        for common, want in (([300, 64], once), ([299, 64], None), ([0, 64], None), ([300, 64], once)):
+            prefixes.tokens.copy_(i32(common))
+            gpu.graph_launch(graph)
+            gpu.sync()
+            g.check("f32", [1] * 6, heads, prefixes=prefixes)
+            assert want is None or torch.equal(out, want)
+        # below what is asked for, the sums are those of whole sequences but for where the work is cut
+        prefixes.tokens.copy_(i32([299, 64]))
+        gpu.graph_launch(graph)
+        gpu.sync()
+        assert float((out - alone).norm() / alone.norm()) < 1e-6
+        gpu.graph_free(graph)
+    g.free()
+
+
 def test_recorded_calls_follow_the_lengths_and_share_scratch(gpu):  # noqa: F811
     import karume_b200 as kb
     g = Groups(gpu, [(300, [50, 30, 10, 90]), (128, [70, 13])], 16, 2, 64, seed=7)
@@ -281,5 +315,8 @@ def test_refusals(gpu):  # noqa: F811
     assert torch.equal(nothing, gpu.cache_attention(g.cache, q, batch))
     tail = (1.0, 0, 0, 0, 0, 0, q.data_ptr(), 256)
     for groups, first, common in ((1, 0, good.tokens.data_ptr()), (1, good.first.data_ptr(), 0), (1, good.first.data_ptr() + 2, good.tokens.data_ptr())):
-        assert kb.lib.kq_cache_attention_shared(gpu._ctx, g.cache.handle, q.data_ptr(), 256, 0, 4, *batch.args, 1, groups, first, common, *tail) == 1
+        assert kb.lib.kq_cache_attention_shared(gpu._ctx, g.cache.handle, q.data_ptr(), 256, 0, 4, *batch.args, 1, groups, first, common, 0, *tail) == 1
+    for least in (-1, (1 << 64) - 1, 1 << 70):
+        with pytest.raises(kb.KqError):
+            kb.SharedPrefixes(good.first, good.tokens, least=least)
     g.free()
