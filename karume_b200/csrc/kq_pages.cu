@@ -19,6 +19,8 @@ namespace {
 constexpr int kBookThreads = 1024;
 constexpr int kPagesAThread = 4;    // neighbours that a thread looks at when pages are counted
 constexpr uint32_t kMaxCluster = 8;
+constexpr int kFew = 8;             // table entries that a thread takes
+constexpr int kOneThreads = 1 << 30;  // beside a row's pages: such a one
 constexpr uint32_t kChunk = 128;    // table entries that a warp takes at a time
 constexpr int kLowest = -0x7fffffff;
 
@@ -266,7 +268,8 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
     } else {
       const Becomes w = becomes(p, b);
       if (b < kKept) s.kept[b] = make_int4(w.parent, w.n, w.old, w.changes);
-      if (w.changes) entries = max(entries, pages_of(max(w.n, w.old), k.shift));
+      const bool cut = w.parent >= 0 && static_cast<uint32_t>(w.parent) == b && pages_of(w.old, k.shift) - (w.n >> k.shift) <= kFew;
+      if (w.changes && !cut) entries = max(entries, pages_of(max(w.n, w.old), k.shift));
     }
   }
   bad = __syncthreads_or(bad);
@@ -277,10 +280,24 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
     return;
   }
   // ---- the names that rows give up, and those of whole pages that they take -------------------------
+  // A row that gives up its last few pages only is one thread's (a warp looks at all of a row: 256 rows of 500 pages, cut by one each, took
+  // 5 us more); `entries` is of the others.
+  const auto few_given = [&](const Becomes& w, uint32_t b) {
+    return w.changes && w.parent >= 0 && static_cast<uint32_t>(w.parent) == b && pages_of(w.old, k.shift) - (w.n >> k.shift) <= kFew;
+  };
   const auto names = [&](int by) {
+    for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
+      const Becomes w = becomes_again(p, s, b);
+      if (!few_given(w, b)) continue;
+      const int whole = w.n >> k.shift, held = pages_of(w.old, k.shift);
+      for (int i = whole; i < held; ++i) {
+        const int page = k.table[static_cast<size_t>(b) * k.width + i];
+        if (a_page(k, page)) atomicSub(k.refs + page, by);
+      }
+    }
     each_chunk(k, static_cast<uint32_t>(entries), rank, ctas, [&](uint32_t b, uint32_t from) {
       const Becomes w = becomes_again(p, s, b);
-      if (!w.changes) return;
+      if (!w.changes || few_given(w, b) || static_cast<int>(from) >= pages_of(max(w.n, w.old), k.shift)) return;
       const bool same = w.parent >= 0 && static_cast<uint32_t>(w.parent) == b;
       const int whole = w.n >> k.shift, held = pages_of(w.old, k.shift);
       const int* const mine = k.table + static_cast<size_t>(b) * k.width;
@@ -327,7 +344,7 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
     const int before = block_before(s, place == 0 ? 1 : 0, total);
     if (place == 0) place = need + before;
     need += total;
-    if (b < k.sequences && b0 / kBookThreads % ctas == rank) p.state[b] = make_int4(w.changes ? w.n : -1, pages_of(w.old, k.shift), page, place);
+    if (b < k.sequences && b0 / kBookThreads % ctas == rank) p.state[b] = make_int4(w.changes ? w.n : -1, pages_of(w.old, k.shift) | (few_given(w, b) ? kOneThreads : 0), page, place);
   }
   const int found = need ? ranked(p, s, false, 0, k.pages, need, p.list, rank, ctas, turn) : 0;
   sync_all(ctas);  // the list, the states; every look at `refs`
@@ -347,8 +364,9 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
   each_chunk(k, static_cast<uint32_t>(entries), rank, ctas, [&](uint32_t b, uint32_t from) {
     const int4 st = __ldcg(p.state + b);
     if (st.x < 0) return;
-    const bool same = p.parents[b] == static_cast<int>(b);
     const int whole = st.x >> k.shift, all = pages_of(st.x, k.shift);
+    if ((st.y & kOneThreads) || static_cast<int>(from) >= max(all, st.y)) return;
+    const bool same = (b < kKept ? s.kept[b].x : p.parents[b]) == static_cast<int>(b);
     for (int i = static_cast<int>(from + lane); i < static_cast<int>(from + kChunk); i += 32) {
       int* const entry = k.table + static_cast<size_t>(b) * k.width + i;
       if (i < whole) {
@@ -362,6 +380,10 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
   });
   for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
     const int4 st = __ldcg(p.state + b);
+    if (st.x >= 0 && (st.y & kOneThreads)) {
+      for (int i = st.x >> k.shift; i < (st.y & ~kOneThreads); ++i)
+        k.table[static_cast<size_t>(b) * k.width + i] = i < pages_of(st.x, k.shift) ? (st.w >= 0 ? fresh(p.list + st.w) : st.z) : -1;
+    }
     if (st.x >= 0) k.lengths[b] = st.x;
     if (st.w >= 0) {
       const int page = fresh(p.list + st.w);

@@ -148,7 +148,7 @@ struct SelectParams {
   int* out;             // [tokens][kv_heads][budget]
 };
 
-constexpr int kScoreWarps = 8, kScorePages = 16 * kScoreWarps;  // pages that a block takes at a time: sixteen a warp
+constexpr int kScoreWarps = 4, kScorePages = 16 * kScoreWarps;  // pages that a block takes at a time: sixteen a warp
 constexpr uint32_t kAlways = 0xFFFFFFFFu, kUnknown = 0xFFFFFFFEu;
 
 // A number that is larger where the score is; not a number: larger than any.
@@ -172,7 +172,7 @@ __device__ __forceinline__ int2 pages_of_row(const AttendArgs& a, uint32_t row) 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 2 : 3) score_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 4 : 6) score_kernel(const __grid_constant__ SelectParams p) {
   constexpr int kHeads = 8;  // columns of an MMA
   __shared__ __align__(16) uint8_t codes[2][kHeads][D + 16];  // a, |a| (rows 16 bytes apart from a multiple of 128: lanes of eight rows meet no bank twice)
   __shared__ float scales[kHeads];
@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 2 : 3) score_kern
     for (uint32_t h0 = 0; h0 < p.group; h0 += kHeads) {
       if (turn == 0 || blocks > 1) {
         if (turn || h0) __syncthreads();
-        for (uint32_t h = warp; h < kHeads; h += kScoreWarps) {  // a query head a warp
+        for (uint32_t h = warp; h < min(static_cast<uint32_t>(kHeads), p.group - h0); h += kScoreWarps) {  // a query head a warp (other columns hold anything)
           float v[8] = {};
-          if (h0 + h < p.group && lane < D / 8)
+          if (lane < D / 8)
             load8_rotated(static_cast<const T*>(p.a.q) + static_cast<size_t>(row) * p.a.q_stride + static_cast<size_t>(head * p.group + h0 + h) * D, lane * 8, p.a.rope,
                           position, v);
           float most = 0.0f;
@@ -352,11 +352,14 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     const uint32_t a = __ballot_sync(0xffffffffu, above), s = __ballot_sync(0xffffffffu, same), in_front = (1u << lane) - 1;
     if (lane == 0) warps[warp] = __popc(a) | __popc(s) << 16;
     __syncthreads();
-    uint32_t sum = __popc(a & in_front) | __popc(s & in_front) << 16, all = 0;
-    for (uint32_t w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) sum += warps[w];
-      all += warps[w];
+    uint32_t sum = __popc(a & in_front) | __popc(s & in_front) << 16, upto = lane < kThreads / 32 ? warps[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < kThreads / 32; o *= 2) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= static_cast<uint32_t>(o)) upto += v;
     }
+    const uint32_t all = __shfl_sync(0xffffffffu, upto, kThreads / 32 - 1), front = __shfl_sync(0xffffffffu, upto, warp > 0 ? warp - 1 : 0);
+    if (warp > 0) sum += front;
     __syncthreads();
     const uint32_t equal_before = equal + (sum >> 16);
     if (mine) {
@@ -419,9 +422,10 @@ cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& a, const Summa
   p.last = last;
   p.keys = static_cast<uint32_t*>(env.workspace);
   p.out = out;
-  // a block quantises its queries once: it takes more pages where there are blocks enough for all SMs, three each at a time
+  // a block quantises its queries once: it takes more pages where there are blocks enough for all SMs, six each at a time (64 rows, 8 kv heads,
+  // 320 pages each: two waves of blocks of eight warps 26 us, one of four warps 19)
   const uint64_t blocks = static_cast<uint64_t>(a.batch.tokens) * a.cache.kv_heads, most = (a.batch.width + kScorePages - 1) / kScorePages;
-  p.turns = static_cast<uint32_t>(std::min<uint64_t>({std::max<uint64_t>((blocks * most + 3ull * env.sm_count - 1) / (3ull * env.sm_count), 1), most, 16}));
+  p.turns = static_cast<uint32_t>(std::min<uint64_t>({std::max<uint64_t>((blocks * most + 6ull * env.sm_count - 1) / (6ull * env.sm_count), 1), most, 32}));
   p.chunks = static_cast<uint32_t>((most + p.turns - 1) / p.turns);
   *launches = 0;
   // as many rows at a time as have room in the scratch and in a grid
