@@ -40,7 +40,9 @@ struct BookParams {
 constexpr uint32_t kKept = 1024;  // sequences whose numbers are kept in shared memory
 
 struct Shared {
-  int4 kept[kKept];
+  int4 kept[kKept];   // what a sequence becomes,
+  int tail[kKept];    // its last page where that is not full,
+  int4 state[kKept];  // what a step found, for the steps behind it (beyond kKept: in the scratch)
   int totals[2][kMaxCluster];  // of the CTAs, turn about
   long long warps[32];
 };
@@ -161,6 +163,11 @@ __device__ __forceinline__ void tell(const BookParams& p, int missing, int pages
   }
 }
 // Every (sequence, chunk of its row up to `entries`) once over the cluster's warps.
+__device__ __forceinline__ void put_state(const BookParams& p, Shared& s, uint32_t b, bool mine, const int4& v) {
+  if (b < kKept) s.state[b] = v;  // every CTA for itself
+  else if (mine) p.state[b] = v;
+}
+__device__ __forceinline__ int4 state_of(const BookParams& p, const Shared& s, uint32_t b) { return b < kKept ? s.state[b] : __ldcg(p.state + b); }
 template <typename Use>
 __device__ __forceinline__ void each_chunk(const PageBook& k, uint32_t entries, uint32_t rank, uint32_t ctas, Use use) {
   const uint32_t chunks = (entries + kChunk - 1) / kChunk, warps = ctas * (kBookThreads / 32);
@@ -195,7 +202,7 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_grow_kernel(const BookP
     long long total;
     const long long before = need + block_before(s, static_cast<long long>(more), total);
     // (numbers beyond 31 bits are of a call that has too few pages)
-    if (b < k.sequences && b0 / kBookThreads % ctas == rank) p.state[b] = make_int4(length + (bad ? 0 : news), held, more, static_cast<int>(min(before, 0x7fffffffll)));
+    if (b < k.sequences) put_state(p, s, b, b0 / kBookThreads % ctas == rank, make_int4(length + (bad ? 0 : news), held, more, static_cast<int>(min(before, 0x7fffffffll))));
     need += total;
     most = max(most, more);
   }
@@ -213,14 +220,14 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_grow_kernel(const BookP
   }
   sync_all(ctas);  // the list and the states
   each_chunk(k, static_cast<uint32_t>(most), rank, ctas, [&](uint32_t b, uint32_t from) {
-    const int4 st = __ldcg(p.state + b);
+    const int4 st = state_of(p, s, b);
     for (uint32_t i = from + lane; i < from + kChunk && static_cast<int>(i) < st.z; i += 32) {
       const int page = fresh(p.list + st.w + i);
       k.table[static_cast<size_t>(b) * k.width + st.y + i] = page;
       k.refs[page] = 1;
     }
   });
-  for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) k.lengths[b] = __ldcg(p.state + b).x;
+  for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) k.lengths[b] = state_of(p, s, b).x;
   tell(p, 0, static_cast<int>(need), 0);
 }
 
@@ -325,8 +332,10 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
   const auto tail_of = [&](const Becomes& w) {
     return w.changes && (w.n & ((1 << k.shift) - 1)) ? k.table[static_cast<size_t>(w.parent) * k.width + (w.n >> k.shift)] : -1;
   };
+  for (uint32_t b = threadIdx.x; b < min(k.sequences, kKept); b += kBookThreads) s.tail[b] = tail_of(becomes_again(p, s, b));
+  __syncthreads();
   for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
-    const int page = tail_of(becomes_again(p, s, b));
+    const int page = b < kKept ? s.tail[b] : tail_of(becomes_again(p, s, b));
     if (a_page(k, page) && fresh(k.refs + page) <= 0) atomicMin(k.refs + page, kLowest + static_cast<int>(b));
   }
   sync_all(ctas);
@@ -337,20 +346,21 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
     int page = -1, place = -1;
     if (b < k.sequences) {
       w = becomes_again(p, s, b);
-      page = tail_of(w);
+      page = b < kKept ? s.tail[b] : tail_of(w);
       if (a_page(k, page)) place = fresh(k.refs + page) == kLowest + static_cast<int>(b) ? -2 : 0;  // takes it over, or needs another
     }
     int total;
     const int before = block_before(s, place == 0 ? 1 : 0, total);
     if (place == 0) place = need + before;
     need += total;
-    if (b < k.sequences && b0 / kBookThreads % ctas == rank) p.state[b] = make_int4(w.changes ? w.n : -1, pages_of(w.old, k.shift) | (few_given(w, b) ? kOneThreads : 0), page, place);
+    if (b < k.sequences)
+      put_state(p, s, b, b0 / kBookThreads % ctas == rank, make_int4(w.changes ? w.n : -1, pages_of(w.old, k.shift) | (few_given(w, b) ? kOneThreads : 0), page, place));
   }
   const int found = need ? ranked(p, s, false, 0, k.pages, need, p.list, rank, ctas, turn) : 0;
   sync_all(ctas);  // the list, the states; every look at `refs`
   const bool enough = found >= need;
   for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
-    const int4 st = __ldcg(p.state + b);
+    const int4 st = state_of(p, s, b);
     if (st.w == -2) k.refs[st.z] = enough ? 1 : 0;
   }
   if (!enough) {  // all as it was
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
   }
   // ---- the new rows ---------------------------------------------------------------------------------
   each_chunk(k, static_cast<uint32_t>(entries), rank, ctas, [&](uint32_t b, uint32_t from) {
-    const int4 st = __ldcg(p.state + b);
+    const int4 st = state_of(p, s, b);
     if (st.x < 0) return;
     const int whole = st.x >> k.shift, all = pages_of(st.x, k.shift);
     if ((st.y & kOneThreads) || static_cast<int>(from) >= max(all, st.y)) return;
@@ -379,7 +389,7 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_fork_kernel(const BookP
     }
   });
   for (uint32_t b = rank * kBookThreads + threadIdx.x; b < k.sequences; b += ctas * kBookThreads) {
-    const int4 st = __ldcg(p.state + b);
+    const int4 st = state_of(p, s, b);
     if (st.x >= 0 && (st.y & kOneThreads)) {
       for (int i = st.x >> k.shift; i < (st.y & ~kOneThreads); ++i)
         k.table[static_cast<size_t>(b) * k.width + i] = i < pages_of(st.x, k.shift) ? (st.w >= 0 ? fresh(p.list + st.w) : st.z) : -1;
@@ -440,8 +450,9 @@ __global__ void __launch_bounds__(kBookThreads, 1) pages_compact_kernel(const Bo
 
 // ---- copies -----------------------------------------------------------------------------------------
 // Bulk copies into shared memory and out of it, a warp with a ring of stages: no registers, and what is under way does not depend on how
-// many threads an SM holds.  Of 96 KB a CTA, two CTAs an SM, half is on its way in.
-constexpr uint32_t kPiece = 16384, kStages = 6, kAhead = 3;
+// many threads an SM holds.  Of 96 KB a CTA, two CTAs an SM, a third is on its way in, the rest on its way out: 1660 pages of 69,632 bytes in
+// eight pools 290 us (6.37 TB/s, 0.97 of the copy rate); half and half 320, 32 KB pieces and one CTA 296.
+constexpr uint32_t kPiece = 16384, kStages = 6, kAhead = 2;
 constexpr uint32_t kCopySmem = kStages * kPiece + 256;
 constexpr uint32_t kCopyWaitLimit = 1u << 22;
 constexpr int kCopyTimeout = 60;  // status word: a piece did not arrive

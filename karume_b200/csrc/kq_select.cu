@@ -144,12 +144,98 @@ struct SelectParams {
   uint32_t row0, rows;  // rows of this launch
   uint32_t chunks;      // blocks that share a row's pages,
   uint32_t turns;       // kScorePages of them each, so often
+  unsigned int* arrived;  // fused: [rows][kv_heads] blocks that have made their scores, zero between launches; else null
   uint32_t* keys;       // [rows][kv_heads][table width]
   int* out;             // [tokens][kv_heads][budget]
 };
 
-constexpr int kScoreWarps = 4, kScorePages = 16 * kScoreWarps;  // pages that a block takes at a time: sixteen a warp
+// ---- the largest ----------------------------------------------------------------------------
+// By a block: the budget-th largest key, digit by digit, then the pages above it in order.
 constexpr uint32_t kAlways = 0xFFFFFFFFu, kUnknown = 0xFFFFFFFEu;
+constexpr uint32_t kFusedPages = 1024;  // a list of so many is the work of the block that made its last scores
+
+template <int kThreads, int kKept>
+struct Largest {
+  uint32_t kept[kKept];  // the first keys; the others are read again
+  uint32_t count[256];
+  uint32_t warps[kThreads / 32], chosen[2];
+};
+template <int kThreads, int kKept>
+__device__ __forceinline__ void select_largest(Largest<kThreads, kKept>& s, const uint32_t* keys, uint32_t pages, uint32_t budget, int* out) {
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const auto key = [&](uint32_t i) { return i < kKept ? s.kept[i] : __ldcg(keys + i); };
+  for (uint32_t i = tid; i < min(pages, static_cast<uint32_t>(kKept)); i += kThreads) s.kept[i] = __ldcg(keys + i);
+  uint32_t digits = 0, left = budget;  // the digits found so far; how many of the keys that begin with them are taken
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (uint32_t i = tid; i < 256; i += kThreads) s.count[i] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < pages; i += kThreads) {
+      const uint32_t k = key(i);
+      if (shift == 24 || k >> (shift + 8) == digits) atomicAdd(&s.count[k >> shift & 255u], 1u);
+    }
+    __syncthreads();
+    // keys of larger digits: a sum from the top
+    // (two digits a thread in blocks of 128)
+    constexpr uint32_t kDigits = kThreads < 256 ? 256 / kThreads : 1;
+    uint32_t mine = 0;
+#pragma unroll
+    for (uint32_t d = 0; d < kDigits; ++d)
+      if (tid < 256) mine += s.count[255 - tid * kDigits - d];
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= static_cast<uint32_t>(o)) upto += v;
+    }
+    if (lane == 31) s.warps[warp] = upto;
+    __syncthreads();
+    for (uint32_t i = 0; i < min(warp, 8u); ++i) upto += s.warps[i];
+    if (tid < 256 && upto - mine < left && left <= upto) {
+      uint32_t above = upto - mine;
+#pragma unroll
+      for (uint32_t d = 0; d < kDigits; ++d) {
+        const uint32_t n = s.count[255 - tid * kDigits - d];
+        if (above < left && left <= above + n) {
+          s.chosen[0] = 255 - tid * kDigits - d;
+          s.chosen[1] = left - above;
+        }
+        above += n;
+      }
+    }
+    __syncthreads();
+    digits = digits << 8 | s.chosen[0];
+    left = s.chosen[1];
+  }
+  uint32_t before = 0, equal = 0;
+  for (uint32_t i0 = 0; i0 < pages; i0 += kThreads) {
+    const uint32_t i = i0 + tid, k = i < pages ? key(i) : 0u;
+    const bool above = i < pages && k > digits, same = i < pages && k == digits;
+    // both counts of the threads in front, sixteen bits each
+    const uint32_t mine = (above ? 1u : 0u) | (same ? 0x10000u : 0u);
+    const uint32_t a = __ballot_sync(0xffffffffu, above), e = __ballot_sync(0xffffffffu, same), in_front = (1u << lane) - 1;
+    if (lane == 0) s.warps[warp] = __popc(a) | __popc(e) << 16;
+    __syncthreads();
+    uint32_t sum = __popc(a & in_front) | __popc(e & in_front) << 16, upto = lane < kThreads / 32 ? s.warps[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < kThreads / 32; o *= 2) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= static_cast<uint32_t>(o)) upto += v;
+    }
+    const uint32_t all = __shfl_sync(0xffffffffu, upto, kThreads / 32 - 1), front = __shfl_sync(0xffffffffu, upto, warp > 0 ? warp - 1 : 0);
+    if (warp > 0) sum += front;
+    __syncthreads();
+    const uint32_t equal_before = equal + (sum >> 16);
+    if (mine) {
+      const uint32_t to = before + (sum & 0xFFFFu) + min(equal_before, left);
+      if (above || equal_before < left) out[to] = static_cast<int>(i);
+    }
+    before += all & 0xFFFFu;
+    equal += all >> 16;
+  }
+}
+
+// ---- and the scores' kernel ----------------------------------------------------------------------
+constexpr int kScoreWarps = 4, kScorePages = 16 * kScoreWarps;  // pages that a block takes at a time: sixteen a warp
 
 // A number that is larger where the score is; not a number: larger than any.
 __device__ __forceinline__ uint32_t key_of(float score) {
@@ -176,13 +262,21 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 4 : 6) score_kern
   constexpr int kHeads = 8;  // columns of an MMA
   __shared__ __align__(16) uint8_t codes[2][kHeads][D + 16];  // a, |a| (rows 16 bytes apart from a multiple of 128: lanes of eight rows meet no bank twice)
   __shared__ float scales[kHeads];
+  __shared__ Largest<kScoreWarps * 32, kFusedPages> largest;
+  __shared__ unsigned int arrivals;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4, heads = p.a.cache.kv_heads;
   pdl_launch_dependents();
   pdl_wait_prior_grid();
   const uint32_t chunk = blockIdx.x % p.chunks, at = blockIdx.x / p.chunks, head = at % heads, row = p.row0 + at / heads;
   const int2 of = pages_of_row(p.a, row);
   const int pages = of.x, first = static_cast<int>(chunk * p.turns) * kScorePages;
-  if (first >= pages || pages <= static_cast<int>(p.budget)) return;  // all are taken
+  int* const out = p.out + (static_cast<size_t>(row) * heads + head) * p.budget;
+  if (pages <= static_cast<int>(p.budget)) {  // all are taken
+    if (p.arrived && chunk == 0)
+      for (uint32_t i = threadIdx.x; i < p.budget; i += kScoreWarps * 32) out[i] = static_cast<int>(i) < pages ? static_cast<int>(i) : -1;
+    return;
+  }
+  if (first >= pages) return;
   uint32_t* const keys = p.keys + static_cast<size_t>(at) * p.a.batch.width;
   const int* const table = p.a.batch.pages + static_cast<size_t>(of.y) * p.a.batch.width;
   // sixteen pages: rows g and g + 8 of the MMA, sixteen channels of 64 a lane; the order of the channels is the queries' too
@@ -291,84 +385,35 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 4 : 6) score_kern
         keys[index] = index < static_cast<int>(p.first) || index >= pages - static_cast<int>(p.last) ? kAlways : unknown[i] ? kUnknown : key_of(best[i]);
     }
   }
+  if (!p.arrived) return;
+  // the block that is the last one of the row's selects
+  const unsigned int blocks_here = (static_cast<uint32_t>(pages) + p.turns * kScorePages - 1) / (p.turns * kScorePages);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned int* const counter = p.arrived + at;
+    unsigned int before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    if (before == blocks_here - 1) *counter = 0;
+    arrivals = before;
+  }
+  __syncthreads();
+  if (arrivals == blocks_here - 1) select_largest(largest, keys, static_cast<uint32_t>(pages), p.budget, out);
 }
-
-// ---- the largest ----------------------------------------------------------------------------
-// A block for each (row, kv head): the budget-th largest key, digit by digit, then the pages above it in order.
-constexpr int kKept = 8192;  // keys in shared memory
 
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectParams p) {
-  __shared__ uint32_t kept[kKept];
-  __shared__ uint32_t count[256];
-  __shared__ uint32_t warps[kThreads / 32], chosen[2];
-  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32, heads = p.a.cache.kv_heads;
+  __shared__ Largest<kThreads, 8192> s;
+  const uint32_t heads = p.a.cache.kv_heads;
   pdl_launch_dependents();
   pdl_wait_prior_grid();
   const uint32_t row = p.row0 + blockIdx.x / heads;
   const uint32_t pages = static_cast<uint32_t>(pages_of_row(p.a, row).x);
   int* const out = p.out + (static_cast<size_t>(row) * heads + blockIdx.x % heads) * p.budget;
   if (pages <= p.budget) {
-    for (uint32_t i = tid; i < p.budget; i += kThreads) out[i] = i < pages ? static_cast<int>(i) : -1;
+    for (uint32_t i = threadIdx.x; i < p.budget; i += kThreads) out[i] = i < pages ? static_cast<int>(i) : -1;
     return;
   }
-  const uint32_t* const keys = p.keys + static_cast<size_t>(blockIdx.x) * p.a.batch.width;
-  const auto key = [&](uint32_t i) { return i < kKept ? kept[i] : __ldcg(keys + i); };
-  for (uint32_t i = tid; i < min(pages, static_cast<uint32_t>(kKept)); i += kThreads) kept[i] = __ldcg(keys + i);
-  uint32_t digits = 0, left = p.budget;  // the digits found so far; how many of the keys that begin with them are taken
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) count[tid] = 0;
-    __syncthreads();
-    for (uint32_t i = tid; i < pages; i += kThreads) {
-      const uint32_t k = key(i);
-      if (shift == 24 || k >> (shift + 8) == digits) atomicAdd(&count[k >> shift & 255u], 1u);
-    }
-    __syncthreads();
-    // keys of larger digits: a sum from the top
-    const uint32_t mine = tid < 256 ? count[255 - tid] : 0;
-    uint32_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= static_cast<uint32_t>(o)) upto += v;
-    }
-    if (lane == 31) warps[warp] = upto;
-    __syncthreads();
-    for (uint32_t i = 0; i < min(warp, 8u); ++i) upto += warps[i];
-    if (tid < 256 && upto - mine < left && left <= upto) {
-      chosen[0] = 255 - tid;
-      chosen[1] = left - (upto - mine);
-    }
-    __syncthreads();
-    digits = digits << 8 | chosen[0];
-    left = chosen[1];
-  }
-  uint32_t before = 0, equal = 0;
-  for (uint32_t i0 = 0; i0 < pages; i0 += kThreads) {
-    const uint32_t i = i0 + tid, k = i < pages ? key(i) : 0u;
-    const bool above = i < pages && k > digits, same = i < pages && k == digits;
-    // both counts of the threads in front, sixteen bits each
-    const uint32_t mine = (above ? 1u : 0u) | (same ? 0x10000u : 0u);
-    const uint32_t a = __ballot_sync(0xffffffffu, above), s = __ballot_sync(0xffffffffu, same), in_front = (1u << lane) - 1;
-    if (lane == 0) warps[warp] = __popc(a) | __popc(s) << 16;
-    __syncthreads();
-    uint32_t sum = __popc(a & in_front) | __popc(s & in_front) << 16, upto = lane < kThreads / 32 ? warps[lane] : 0;
-#pragma unroll
-    for (int o = 1; o < kThreads / 32; o *= 2) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= static_cast<uint32_t>(o)) upto += v;
-    }
-    const uint32_t all = __shfl_sync(0xffffffffu, upto, kThreads / 32 - 1), front = __shfl_sync(0xffffffffu, upto, warp > 0 ? warp - 1 : 0);
-    if (warp > 0) sum += front;
-    __syncthreads();
-    const uint32_t equal_before = equal + (sum >> 16);
-    if (mine) {
-      const uint32_t to = before + (sum & 0xFFFFu) + min(equal_before, left);
-      if (above || equal_before < left) out[to] = static_cast<int>(i);
-    }
-    before += all & 0xFFFFu;
-    equal += all >> 16;
-  }
+  select_largest(s, p.keys + static_cast<size_t>(blockIdx.x) * p.a.batch.width, pages, p.budget, out);
 }
 
 template <typename Kernel, typename Params>
@@ -429,16 +474,20 @@ cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& a, const Summa
   p.chunks = static_cast<uint32_t>((most + p.turns - 1) / p.turns);
   *launches = 0;
   // as many rows at a time as have room in the scratch and in a grid
-  const uint64_t room = std::min<uint64_t>(env.workspace_bytes / select_scratch_bytes(a), ((1ull << 31) - 1) / (static_cast<uint64_t>(a.cache.kv_heads) * p.chunks));
+  const bool fused = a.batch.width <= kFusedPages;
+  uint64_t room = std::min<uint64_t>(env.workspace_bytes / select_scratch_bytes(a), ((1ull << 31) - 1) / (static_cast<uint64_t>(a.cache.kv_heads) * p.chunks));
+  if (fused) room = std::min<uint64_t>(room, env.counter_count / a.cache.kv_heads);
+  p.arrived = fused && env.counter_count >= a.cache.kv_heads ? env.counters : nullptr;
   for (uint32_t row = 0; row < a.batch.tokens; row += p.rows) {
     p.row0 = row;
     p.rows = static_cast<uint32_t>(std::min<uint64_t>(a.batch.tokens - row, std::max<uint64_t>(room, 1)));
     cudaError_t e = a.dtype == KQ_F32 ? score_as<float>(env, p) : a.dtype == KQ_F16 ? score_as<__half>(env, p) : score_as<__nv_bfloat16>(env, p);
-    // a thousand pages and more: 1024 threads (3126 pages: 11 -> 8 us)
-    const uint64_t lists = static_cast<uint64_t>(p.rows) * a.cache.kv_heads;
-    if (e == cudaSuccess) e = a.batch.width > 1024 ? launch_after(env, select_kernel<1024>, lists, 1024, p) : launch_after(env, select_kernel<256>, lists, 256, p);
+    *launches += 1;
     if (e != cudaSuccess) return e;
-    *launches += 2;
+    if (p.arrived) continue;
+    e = launch_after(env, select_kernel<1024>, static_cast<uint64_t>(p.rows) * a.cache.kv_heads, 1024, p);
+    *launches += 1;
+    if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
