@@ -25,16 +25,19 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
   // keys, a third of the rest.  Where the rows would take more than half of it, every sequence walks over all of its keys.
   const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, each = 16 + 4ull * (a.cache.head_dim + 2);
   // What a call can save at most; then what it does save, as the lengths say on the device.
-  const uint64_t most = static_cast<uint64_t>(a.batch.sequences) * a.batch.width * cache_block_bytes(a.cache.page_tokens, a.cache.head_dim) * a.cache.kv_heads;
+  const double most = static_cast<double>(a.batch.sequences) * a.batch.width * static_cast<double>(cache_block_bytes(a.cache.page_tokens, a.cache.head_dim)) *
+                      a.cache.kv_heads;
   const uint64_t group = a.heads / a.cache.kv_heads;
   if (sh.least == KQ_SHARED_AUTO) sh.least = static_cast<uint64_t>(a.batch.tokens) * group / a.batch.sequences > kAlone ? ~0ull : kWorth;
-  if (most < sh.least) return launch_attend(env, a, launches);
+  if (most < static_cast<double>(sh.least)) return launch_attend(env, a, launches);
   sh.all_first = sh.first;
   sh.all_tokens = sh.tokens;
   sh.all_groups = sh.groups;
-  if (!env.workspace || rows * each + 64 > env.workspace_bytes / 2) return launch_attend(env, a, launches);
+  // (Places count in pairs of floats, so no more than 32 GB of the scratch is used.)
+  const uint64_t scratch = std::min<uint64_t>(env.workspace_bytes, 32ull << 30);
+  if (!env.workspace || rows * each + 64 > scratch / 2) return launch_attend(env, a, launches);
   uint8_t* const base = static_cast<uint8_t*>(env.workspace);
-  const uint64_t left = (env.workspace_bytes - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
+  const uint64_t left = (scratch - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
   sh.scratch = static_cast<float*>(env.workspace);
   sh.places = reinterpret_cast<uint4*>(base + left);
   sh.sums = (left + rows * 16) / 4;

@@ -337,14 +337,16 @@ struct Rows {
   int type = -1;
   int64_t heads = 0;
   uint64_t pq = 0, po = 0, q_stride = 0, out_stride = 0;
-  bool of(PyObject* queries, PyObject* out, int64_t tokens, int64_t dim) {
+  // device: the context's, or -1 for any
+  bool of(PyObject* queries, PyObject* out, int64_t tokens, int64_t dim, int64_t device = -1) {
     if (!tensor_of(queries, &q) || (out != Py_None && !tensor_of(out, &given))) return false;
     type = dtype_code(*q);
     if (type < 0 || q->dim() != 3 || q->numel() == 0) return false;
     heads = q->size(1);
+    if (!rows_of(*q, tokens, heads, dim, &q_stride) || (device >= 0 && q->get_device() != device)) return false;
     if (given == nullptr) made = at::detail::empty_cuda(q->sizes(), q->scalar_type(), q->device(), c10::nullopt);
     const at::Tensor& o = given != nullptr ? *given : made;
-    if (o.scalar_type() != q->scalar_type() || !rows_of(*q, tokens, heads, dim, &q_stride) || !rows_of(o, tokens, heads, dim, &out_stride)) return false;
+    if (o.scalar_type() != q->scalar_type() || !rows_of(o, tokens, heads, dim, &out_stride)) return false;
     pq = ptr(*q);
     po = ptr(o);
     return true;
@@ -370,12 +372,12 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return rc != 0 ? status_of(rc) : r.result(a[9]);
 }
 
-// cache_attention_shared(ctx, handle, dim, q, batch args, most, shared args, scale, window, rope args, out)
+// cache_attention_shared(ctx, handle, dim, q, batch args, most, shared args, scale, window, rope args, out, device index)
 PyObject* cache_attention_shared(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   uint64_t batch[6], table[4], groups[4];
   Rows r;
-  if (nargs != 11 || a[0] == Py_None || !numbers_of(a[4], batch) || !numbers_of(a[6], groups) || !numbers_of(a[9], table)) KQ_NONE;
-  if (!r.of(a[3], a[10], static_cast<int64_t>(batch[5]), PyLong_AsLongLong(a[2]))) KQ_NONE;
+  if (nargs != 12 || a[0] == Py_None || !numbers_of(a[4], batch) || !numbers_of(a[6], groups) || !numbers_of(a[9], table)) KQ_NONE;
+  if (!r.of(a[3], a[10], static_cast<int64_t>(batch[5]), PyLong_AsLongLong(a[2]), PyLong_AsLongLong(a[11]))) KQ_NONE;
   void* ctx = PyLong_AsVoidPtr(a[0]);
   const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]);
   const uint32_t most = u32(PyLong_AsUnsignedLong(a[5])), window = u32(PyLong_AsUnsignedLong(a[8]));
@@ -388,15 +390,17 @@ PyObject* cache_attention_shared(PyObject*, PyObject* const* a, Py_ssize_t nargs
   return rc != 0 ? status_of(rc) : r.result(a[10]);
 }
 
-// cache_attention_selected(ctx, handle, kv_heads, dim, q, batch args, selected, scale, rope args, out)
+// cache_attention_selected(ctx, handle, kv_heads, dim, q, batch args, selected, scale, rope args, out, device index)
 PyObject* cache_attention_selected(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   uint64_t batch[6], table[4];
   const at::Tensor* selected;
   Rows r;
-  if (nargs != 10 || a[0] == Py_None || !numbers_of(a[5], batch) || !numbers_of(a[8], table) || !tensor_of(a[6], &selected)) KQ_NONE;
+  if (nargs != 11 || a[0] == Py_None || !numbers_of(a[5], batch) || !numbers_of(a[8], table) || !tensor_of(a[6], &selected)) KQ_NONE;
+  const int64_t device = PyLong_AsLongLong(a[10]);
   const int64_t tokens = static_cast<int64_t>(batch[5]);
   if (selected->scalar_type() != at::kInt || !plain(*selected) || selected->dim() != 3 || selected->size(0) != tokens ||
-      selected->size(1) != PyLong_AsLongLong(a[2]) || selected->size(2) == 0 || !r.of(a[4], a[9], tokens, PyLong_AsLongLong(a[3])))
+      selected->size(1) != PyLong_AsLongLong(a[2]) || selected->size(2) == 0 || selected->get_device() != device ||
+      !r.of(a[4], a[9], tokens, PyLong_AsLongLong(a[3]), device))
     KQ_NONE;
   void* ctx = PyLong_AsVoidPtr(a[0]);
   const uint64_t handle = PyLong_AsUnsignedLongLong(a[1]), ps = ptr(*selected);
@@ -420,20 +424,21 @@ PyObject* cache_summarize(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return status_of(without_gil([&] { return g_summarize(ctx, handle, of[0], of[1], u32(batch[0]), batch[1], u32(batch[2]), batch[3], batch[4], u32(batch[5])); }));
 }
 
-// cache_select(ctx, handle, kv_heads, dim, summaries args, q, batch args, budget, first, last, rope args, out)
+// cache_select(ctx, handle, kv_heads, dim, summaries args, q, batch args, budget, first, last, rope args, out, device index)
 PyObject* cache_select(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   uint64_t of[2], batch[6], table[4], q_stride;
   const at::Tensor *q, *given = nullptr;
-  if (nargs != 12 || a[0] == Py_None || !numbers_of(a[4], of) || !tensor_of(a[5], &q) || !numbers_of(a[6], batch) || !numbers_of(a[10], table) ||
+  if (nargs != 13 || a[0] == Py_None || !numbers_of(a[4], of) || !tensor_of(a[5], &q) || !numbers_of(a[6], batch) || !numbers_of(a[10], table) ||
       (a[11] != Py_None && !tensor_of(a[11], &given)))
     KQ_NONE;
   const int64_t tokens = static_cast<int64_t>(batch[5]), kv_heads = PyLong_AsLongLong(a[2]), dim = PyLong_AsLongLong(a[3]);
   const int64_t budget = PyLong_AsLongLong(a[7]), first = PyLong_AsLongLong(a[8]), last = PyLong_AsLongLong(a[9]);
-  const int type = dtype_code(*q);
+  const int64_t device = PyLong_AsLongLong(a[12]);
   if (PyErr_Occurred()) {
     PyErr_Clear();
     KQ_NONE;
   }
+  const int type = q->get_device() == device ? dtype_code(*q) : -1;
   if (type < 0 || q->dim() != 3 || q->numel() == 0 || !rows_of(*q, tokens, q->size(1), dim, &q_stride) || budget <= 0 || budget > (1 << 20) || first < 0 ||
       first > budget || last < 0 || last > budget)
     KQ_NONE;
@@ -455,10 +460,10 @@ PyObject* cache_select(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 }
 
 // ---- books of pages: (table, sequences, width, lengths, refs, pages, page_tokens, report) -----------------
-// An i32 array with a number for each sequence.
-bool each_sequence(PyObject* o, const uint64_t (&book)[8], uint64_t* address) {
+// An i32 array with a number for each sequence, on the context's device.
+bool each_sequence(PyObject* o, const uint64_t (&book)[8], int64_t device, uint64_t* address) {
   const at::Tensor* t;
-  if (!tensor_of(o, &t) || t->scalar_type() != at::kInt || !plain(*t) || static_cast<uint64_t>(t->numel()) != book[1]) return false;
+  if (!tensor_of(o, &t) || t->scalar_type() != at::kInt || !plain(*t) || t->get_device() != device || static_cast<uint64_t>(t->numel()) != book[1]) return false;
   *address = ptr(*t);
   return true;
 }
@@ -467,10 +472,10 @@ at::Tensor pairs_for(uint64_t count, int64_t device) {
   return at::detail::empty_cuda(shape, at::kInt, at::Device(at::kCUDA, static_cast<at::DeviceIndex>(device)), c10::nullopt);
 }
 
-// pages_grow(ctx, book args, news): 0, or the status
+// pages_grow(ctx, book args, news, device index): 0, or the status
 PyObject* pages_grow(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   uint64_t k[8], news;
-  if (nargs != 3 || a[0] == Py_None || !numbers_of(a[1], k) || !each_sequence(a[2], k, &news)) KQ_NONE;
+  if (nargs != 4 || a[0] == Py_None || !numbers_of(a[1], k) || !each_sequence(a[2], k, PyLong_AsLongLong(a[3]), &news)) KQ_NONE;
   void* ctx = PyLong_AsVoidPtr(a[0]);
   return status_of(without_gil([&] { return g_grow(ctx, k[0], u32(k[1]), u32(k[2]), k[3], k[4], u32(k[5]), u32(k[6]), k[7], news); }));
 }
@@ -478,8 +483,10 @@ PyObject* pages_grow(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 // pages_fork(ctx, book args, parents, keep, device index) -> pairs
 PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   uint64_t k[8], parents, keep = 0;
-  if (nargs != 5 || a[0] == Py_None || !numbers_of(a[1], k) || !each_sequence(a[2], k, &parents) || (a[3] != Py_None && !each_sequence(a[3], k, &keep))) KQ_NONE;
-  at::Tensor pairs = pairs_for(k[1], PyLong_AsLongLong(a[4]));
+  if (nargs != 5 || a[0] == Py_None || !numbers_of(a[1], k)) KQ_NONE;
+  const int64_t device = PyLong_AsLongLong(a[4]);
+  if (!each_sequence(a[2], k, device, &parents) || (a[3] != Py_None && !each_sequence(a[3], k, device, &keep))) KQ_NONE;
+  at::Tensor pairs = pairs_for(k[1], device);
   void* ctx = PyLong_AsVoidPtr(a[0]);
   const uint64_t to = ptr(pairs);
   const int rc = without_gil([&] { return g_fork(ctx, k[0], u32(k[1]), u32(k[2]), k[3], k[4], u32(k[5]), u32(k[6]), k[7], parents, keep, to); });
@@ -497,23 +504,24 @@ PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return rc != 0 ? status_of(rc) : THPVariable_Wrap(std::move(pairs));
 }
 
-// pages_copy(ctx, book args, pairs, pools): tensors, or caches' page_args (pages, bytes of one, address); 0, or the status
+// pages_copy(ctx, book args, pairs, pools, device index): tensors, or caches' page_args (pages, bytes of one, address, device); 0, or the status
 PyObject* pages_copy(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   uint64_t k[8];
   const at::Tensor *pairs, *t;
-  if (nargs != 4 || a[0] == Py_None || !numbers_of(a[1], k) || !tensor_of(a[2], &pairs) || !PyList_CheckExact(a[3])) KQ_NONE;
-  if (pairs->scalar_type() != at::kInt || !plain(*pairs) || pairs->dim() != 2 || pairs->size(1) != 2 || pairs->size(0) >= (1 << 30)) KQ_NONE;
+  if (nargs != 5 || a[0] == Py_None || !numbers_of(a[1], k) || !tensor_of(a[2], &pairs) || !PyList_CheckExact(a[3])) KQ_NONE;
+  const int64_t device = PyLong_AsLongLong(a[4]);
+  if (pairs->get_device() != device || pairs->scalar_type() != at::kInt || !plain(*pairs) || pairs->dim() != 2 || pairs->size(1) != 2 || pairs->size(0) >= (1 << 30)) KQ_NONE;
   const Py_ssize_t count = PyList_GET_SIZE(a[3]);
   c10::SmallVector<uint64_t, 128> pools(count), bytes(count);
   for (Py_ssize_t i = 0; i < count; ++i) {
     PyObject* o = PyList_GET_ITEM(a[3], i);
-    uint64_t of[3];
+    uint64_t of[4];
     if (tensor_of(o, &t)) {
-      if (!plain(*t) || t->dim() == 0 || static_cast<uint64_t>(t->size(0)) < k[5]) KQ_NONE;
+      if (t->get_device() != device || !plain(*t) || t->dim() == 0 || static_cast<uint64_t>(t->size(0)) < k[5]) KQ_NONE;
       bytes[i] = static_cast<uint64_t>(t->numel() / t->size(0)) * t->element_size();
       pools[i] = ptr(*t);
     } else {
-      if (!PyTuple_CheckExact(o) || !numbers_of(o, of) || of[0] < k[5]) KQ_NONE;
+      if (!PyTuple_CheckExact(o) || !numbers_of(o, of) || of[0] < k[5] || static_cast<int64_t>(of[3]) != device) KQ_NONE;
       bytes[i] = of[1];
       pools[i] = of[2];
     }

@@ -151,7 +151,7 @@ class KvCache:
     head_dim: int
 
     def __post_init__(self):
-        self.page_args = (self.pages, self.kv_heads * self.page_tokens * (self.head_dim + 8), self.pool.data_ptr())
+        self.page_args = (self.pages, self.kv_heads * self.page_tokens * (self.head_dim + 8), self.pool.data_ptr(), self.pool.get_device())
 
     def free(self) -> None:
         if self.handle:
@@ -172,9 +172,10 @@ class SharedPrefixes:
         self.groups = int(tokens.numel())
         if first.numel() != self.groups + 1:
             raise KqError(2, f"{self.groups} groups have {self.groups + 1} boundaries, not {first.numel()}")
+        _on_device(first.device.index, tokens=tokens)
         if least is not None and not 0 <= least < KQ_SHARED_AUTO:
             raise KqError(2, f"least {least}: a number of bytes")
-        self.first, self.tokens = first, tokens
+        self.first, self.tokens, self.index = first, tokens, first.get_device()
         self.args = (self.groups, first.data_ptr(), tokens.data_ptr(), KQ_SHARED_AUTO if least is None else int(least))
 
 
@@ -187,12 +188,15 @@ class CacheSummaries:
         if codes.dtype != torch.int8 or scales.dtype != torch.float32 or not (codes.is_cuda and scales.is_cuda) or codes.dim() != 4 or scales.dim() != 3 or \
                 tuple(scales.shape) != tuple(codes.shape[:3]) or codes.shape[2] != 2 or not (codes.is_contiguous() and scales.is_contiguous()):
             raise KqError(2, "summaries are contiguous CUDA tensors: codes int8 [pages, kv_heads, 2, head_dim], scales f32 [pages, kv_heads, 2]")
-        self.codes, self.scales = codes, scales
+        _on_device(codes.device.index, scales=scales)
+        self.codes, self.scales, self.index = codes, scales, codes.get_device()
         self.args = (codes.data_ptr(), scales.data_ptr())
 
         self.shape = tuple(int(n) for n in codes.shape)
 
-    def check(self, cache: "KvCache") -> None:
+    def check(self, cache: "KvCache", index: int) -> None:
+        if self.index != index:
+            _on_device(index, codes=self.codes)
         pages, heads, _, dim = self.shape
         if pages < cache.pages or heads != cache.kv_heads or dim != cache.head_dim:
             raise KqError(2, f"summaries {list(self.shape)} are not those of {cache.pages} pages of {cache.kv_heads} heads of {cache.head_dim}")
@@ -214,9 +218,16 @@ class CachePages:
         self.sequences, self.width = (int(n) for n in table.shape)
         if lengths.numel() != self.sequences or report.numel() != 4:
             raise KqError(2, f"{self.sequences} sequences need as many lengths, a report four numbers")
-        self.table, self.lengths, self.refs, self.report = table, lengths, refs, report
+        _on_device(table.device.index, lengths=lengths, refs=refs, report=report)
+        self.table, self.lengths, self.refs, self.report, self.index = table, lengths, refs, report, table.get_device()
         self.pages, self.page_tokens = int(refs.numel()), int(page_tokens)
         self.args = (table.data_ptr(), self.sequences, self.width, lengths.data_ptr(), refs.data_ptr(), self.pages, self.page_tokens, report.data_ptr())
+
+
+def _on_device(index: int, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.device.index != index:
+            raise KqError(2, f"{name} is on {t.device}, the context's device is cuda:{index}")
 
 
 def _per_sequence(t, book: CachePages, name: str) -> int:
@@ -567,13 +578,18 @@ class Gpu:
         if shared is None and selected is None:
             done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window, angles, out)
         elif selected is None:
-            done = _fast.cache_attention_shared(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, shared.args, scale, window, angles, out)
+            done = _fast.cache_attention_shared(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, shared.args, scale, window, angles, out, self.index) \
+                if shared.index == self.index else None
         elif window or shared is not None:
             raise KqError(2, "selected pages are all that a row sees: no window, no shared prefixes")
         else:
-            done = _fast.cache_attention_selected(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, q, batch.args, selected, scale, angles, out)
+            done = _fast.cache_attention_selected(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, q, batch.args, selected, scale, angles, out, self.index)
         if done is not None:
             return self._done(done)
+        if shared is not None:
+            _on_device(self.index, q=q, first=shared.first)
+        if selected is not None:
+            _on_device(self.index, q=q, selected=selected)
         torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
@@ -608,7 +624,7 @@ class Gpu:
 
     def cache_summarize(self, cache: KvCache, summaries: CacheSummaries, batch: CacheBatch) -> None:
         """Brings the summaries of the pages that the batch's new tokens are in up to date (behind cache_append)."""
-        summaries.check(cache)
+        summaries.check(cache, self.index)
         done = _fast.cache_summarize(self._ctx_addr, cache.handle, summaries.args, batch.args)
         if done is not None:
             return self._check(done)
@@ -618,11 +634,12 @@ class Gpu:
                      rope: "Rope | None" = None, out=None):
         """Up to `budget` pages for every row of q [tokens, heads, head_dim] and kv head, int32 [tokens, kv_heads, budget]: ascending indices into
         the sequence's pages, -1 behind them; always the first `first` and the last `last` ones, then those whose summaries promise most."""
-        summaries.check(cache)
+        summaries.check(cache, self.index)
         done = _fast.cache_select(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, summaries.args, q, batch.args, budget, first, last,
-                                  rope.args if rope is not None else None, out)
+                                  rope.args if rope is not None else None, out, self.index)
         if done is not None:
             return self._done(done)
+        _on_device(self.index, q=q)
         torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
@@ -651,17 +668,19 @@ class Gpu:
 
     def pages_grow(self, book: CachePages, news) -> None:
         """Sequence b gets the pages of its next news[b] tokens (CUDA int32) and is that much longer."""
-        done = _fast.pages_grow(self._ctx_addr, book.args, news)
+        done = _fast.pages_grow(self._ctx_addr, book.args, news, self.index) if book.index == self.index else None
         if done is not None:
             return self._check(done)
+        _on_device(self.index, table=book.table, news=news)
         self._check(L.kq_pages_grow(self._ctx, *book.args, _per_sequence(news, book, "news")))
 
     def pages_fork(self, book: CachePages, parents, keep=None):
         """Every sequence b becomes the first min(keep[b], length) tokens of parents[b] (CUDA int32; negative: it ends), all at once.
         Returns the pairs [sequences, 2] of pages to copy, for pages_copy."""
-        done = _fast.pages_fork(self._ctx_addr, book.args, parents, keep, self.index)
+        done = _fast.pages_fork(self._ctx_addr, book.args, parents, keep, self.index) if book.index == self.index else None
         if done is not None:
             return self._done(done)
+        _on_device(self.index, table=book.table, parents=parents, keep=parents if keep is None else keep)
         torch = _torch()
         pairs = torch.empty((book.sequences, 2), dtype=torch.int32, device=self.device)
         self._check(L.kq_pages_fork(self._ctx, *book.args, _per_sequence(parents, book, "parents"),
@@ -670,9 +689,10 @@ class Gpu:
 
     def pages_compact(self, book: CachePages):
         """Moves the pages in use to the lowest numbers; returns the pairs [pages, 2] (from, to), for pages_copy."""
-        done = _fast.pages_compact(self._ctx_addr, book.args, self.index)
+        done = _fast.pages_compact(self._ctx_addr, book.args, self.index) if book.index == self.index else None
         if done is not None:
             return self._done(done)
+        _on_device(self.index, table=book.table)
         torch = _torch()
         pairs = torch.empty((book.pages, 2), dtype=torch.int32, device=self.device)
         self._check(L.kq_pages_compact(self._ctx, *book.args, pairs.data_ptr()))
@@ -680,17 +700,20 @@ class Gpu:
 
     def pages_copy(self, book: CachePages, pairs, pools) -> None:
         """Copies the pages of the book's last fork or compact in every pool: KvCaches, or CUDA tensors whose first axis is the pages."""
-        pools = [pool.page_args if isinstance(pool, KvCache) else pool for pool in pools]
-        done = _fast.pages_copy(self._ctx_addr, book.args, pairs, pools)
+        given, pools = pools, [pool.page_args if isinstance(pool, KvCache) else pool for pool in pools]
+        done = _fast.pages_copy(self._ctx_addr, book.args, pairs, pools, self.index) if book.index == self.index else None
         if done is not None:
             return self._check(done)
+        _on_device(self.index, table=book.table, pairs=pairs)
+        for pool in given:
+            _on_device(self.index, pool=pool.pool if isinstance(pool, KvCache) else pool)
         torch = _torch()
         if pairs.dtype != torch.int32 or not pairs.is_cuda or not pairs.is_contiguous() or pairs.dim() != 2 or pairs.shape[1] != 2:
             raise KqError(2, "pairs must be a contiguous CUDA int32 tensor [pairs, 2]")
         addresses, sizes = [], []
         for pool in pools:
             if isinstance(pool, tuple):
-                pages, each, address = pool
+                pages, each, address, _ = pool
             elif not pool.is_cuda or not pool.is_contiguous() or pool.dim() == 0:
                 raise KqError(2, "a pool is a KvCache or a contiguous CUDA tensor [pages, ...]")
             else:

@@ -320,3 +320,54 @@ def test_refusals(gpu):  # noqa: F811
         with pytest.raises(kb.KqError):
             kb.SharedPrefixes(good.first, good.tokens, least=least)
     g.free()
+
+
+def test_calls_on_other_streams(gpu):  # noqa: F811
+    """The whole chain on the library's own stream beside torch's default one, on a side stream, and on two contexts at once: the same results."""
+    import karume_b200 as kb
+    g = Groups(gpu, [(300, [5, 30, 1, 9])], 16, 2, 64, seed=10)
+    table, length, pool, pages = g.table.clone(), g.length.clone(), g.cache.pool.clone(), g.cache.pages
+    q0, prefixes = torch.randn(4, 8, 64, device="cuda"), g.prefixes()
+    refs = g.book.refs.clone()
+    torch.cuda.synchronize()
+
+    def chain(on):
+        """Everything that a step of branching sequences does, from fresh copies; torch and the library in turn."""
+        book = kb.CachePages(table.clone(), length.clone(), refs.clone(), 16)
+        mine = pool.clone()
+        cache = on.kv_cache(pages, 16, 2, 64, pool=mine)
+        pairs = on.pages_fork(book, i32([0, 1, 1, 3]), i32([301, 320, 307, 306]))
+        on.pages_copy(book, pairs, [cache])
+        on.pages_grow(book, i32([1, 1, 1, 1]))
+        batch = kb.CacheBatch(book.table, book.lengths)
+        k = q0[:, :2].contiguous() * 2
+        on.cache_append(cache, k, k, batch)
+        made = on.cache_summaries(cache)
+        on.cache_summarize(cache, made, kb.CacheBatch(book.table, book.lengths, i32([0, 302, 623, 931, 1238]), tokens=1238))
+        taken = on.cache_select(cache, made, q0, batch, 6)
+        out = [on.cache_attention(cache, q0, batch, shared=prefixes), on.cache_attention(cache, q0.bfloat16(), batch, selected=taken), taken, book.table, book.refs, mine, pairs]
+        return [t + 0 for t in out]
+
+    want = chain(gpu)
+    gpu.sync()
+    before = torch.cuda.current_stream()
+    side = torch.cuda.Stream()
+    contexts = []
+    for stream in (torch.cuda.default_stream(), side):
+        torch.cuda.set_stream(stream)
+        on = kb.Gpu(0)
+        contexts.append((on, stream))
+        got = chain(on)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), stream
+    both = []
+    for _ in range(20):  # enqueued on both, neither waits for the other
+        for on, stream in contexts:
+            torch.cuda.set_stream(stream)
+            both.append(chain(on))
+    torch.cuda.synchronize()
+    torch.cuda.set_stream(before)
+    assert all(torch.equal(a, b) for got in both for a, b in zip(got, want))
+    for on, _ in contexts:
+        on.destroy()
+    g.free()
