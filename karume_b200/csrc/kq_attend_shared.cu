@@ -13,58 +13,65 @@ bool attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, const 
 cudaError_t attend_shared_rest_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 
 // Bytes that are read once instead of often, from which on that is faster: without it they come from L2 mostly, with it there is a launch more
-// and every row's sums are joined.  bfloat16, 32 heads over 8, this way / the other: 64 sequences behind 2048 common tokens (140 MB saved) 52 / 48 us,
-// behind 4096 (281 MB) 55 / 75, behind 32768 (2.2 GB) 103 / 449; f32, 12 over 2: 16 behind 4096 (17 MB) 46 / 26, behind 32768 (134 MB) 64 / 69.
-constexpr uint64_t kWorth = 150ull << 20;
+// and every row's sums are joined.  This way / the other, 32 heads over 8: bfloat16, 64 sequences behind 2048 common tokens (140 MB saved) 52 / 48 us,
+// behind 4096 (281 MB) 55 / 75, behind 32768 (2.2 GB) 104 / 450; 16 behind 8192 (134 MB) 47 / 41; f32 51 / 45. 8 heads over 4 of 64, 64 behind
+// 8192 (149 MB) 37 / 46.
+constexpr uint64_t kWorth = 128ull << 20;
 // Sequences of so many query rows a kv head fill the tensor cores' blocks of rows by themselves: 16 of up to 300 new tokens behind 16384, 4 heads a
 // kv head, bfloat16 1511 / 1045 us; 8 of up to 100 behind 32768, 497 / 648.
 constexpr uint64_t kAlone = 512;
+constexpr uint32_t kGroupsAtOnce = 128;
 
 cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, SharedArgs sh, int* launches) {
-  // The end of the scratch: a place for each row, and its sums where they are in one part; in front of it the parts of the sums over common
-  // keys, a third of the rest.  Where the rows would take more than half of it, every sequence walks over all of its keys.
-  const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, each = 16 + 4ull * (a.cache.head_dim + 2);
   // What a call can save at most; then what it does save, as the lengths say on the device.
   const double most = static_cast<double>(a.batch.sequences) * a.batch.width * static_cast<double>(cache_block_bytes(a.cache.page_tokens, a.cache.head_dim)) *
                       a.cache.kv_heads;
   const uint64_t group = a.heads / a.cache.kv_heads;
   if (sh.least == KQ_SHARED_AUTO) sh.least = static_cast<uint64_t>(a.batch.tokens) * group / a.batch.sequences > kAlone ? ~0ull : kWorth;
-  if (most < static_cast<double>(sh.least)) return launch_attend(env, a, launches);
+  // The end of the scratch: a place for each row, and its sums where they are in one part; in front of it the parts of the sums over common
+  // keys, a third of the rest.  Where the rows would take more than half of it, every sequence walks over all of its keys.
+  // (Places count in pairs of floats, so no more than 32 GB of the scratch is used.)
+  const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, each = 16 + 4ull * (a.cache.head_dim + 2);
+  const uint64_t scratch = std::min<uint64_t>(env.workspace_bytes, 32ull << 30);
+  const bool once = most >= static_cast<double>(sh.least) && env.workspace && rows * each + 64 <= scratch / 2;
+  const uint64_t mine = static_cast<uint64_t>(a.batch.most) * group;
+  const bool many = mine > kFewRows && attend_many_supports(a);
+  if (!once && many) return launch_attend(env, a, launches);
   sh.all_first = sh.first;
   sh.all_tokens = sh.tokens;
   sh.all_groups = sh.groups;
-  // (Places count in pairs of floats, so no more than 32 GB of the scratch is used.)
-  const uint64_t scratch = std::min<uint64_t>(env.workspace_bytes, 32ull << 30);
-  if (!env.workspace || rows * each + 64 > scratch / 2) return launch_attend(env, a, launches);
-  uint8_t* const base = static_cast<uint8_t*>(env.workspace);
-  const uint64_t left = (scratch - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
-  sh.scratch = static_cast<float*>(env.workspace);
-  sh.places = reinterpret_cast<uint4*>(base + left);
-  sh.sums = (left + rows * 16) / 4;
-  LaunchEnv in = env, parts = env;
-  in.workspace_bytes = own;
-  parts.workspace = base + own;
-  parts.workspace_bytes = left - own;
   *launches = 0;
-  LaunchEnv alone = parts;  // groups that come in turns: none may leave its parts where the next one's go
-  if (sh.groups > 128) alone.workspace = nullptr;
+  LaunchEnv in = env;
   cudaError_t e = cudaSuccess;
-  for (uint32_t g = 0; g < sh.groups && e == cudaSuccess; g += 128) {
-    SharedArgs some = sh;
-    some.first += g;
-    some.tokens += g;
-    some.groups = std::min(sh.groups - g, 128u);
-    if (!attend_shared_prefix_many(alone, a, some, &e)) {
-      FewParams p = few_params(parts, a, 0xFFFFFFFFu);
-      p.prefix = true;
-      p.sh = some;
-      e = launch_few<kShared>(parts, p, (a.batch.tokens + sh.groups - 1) / sh.groups * group);
+  if (once) {
+    uint8_t* const base = static_cast<uint8_t*>(env.workspace);
+    const uint64_t left = (scratch - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
+    sh.scratch = static_cast<float*>(env.workspace);
+    sh.places = reinterpret_cast<uint4*>(base + left);
+    sh.sums = (left + rows * 16) / 4;
+    LaunchEnv parts = env;
+    in.workspace_bytes = own;
+    parts.workspace = base + own;
+    parts.workspace_bytes = left - own;
+    LaunchEnv alone = parts;  // groups that come in turns: none may leave its parts where the next one's go
+    if (sh.groups > kGroupsAtOnce) alone.workspace = nullptr;
+    for (uint32_t g = 0; g < sh.groups && e == cudaSuccess; g += kGroupsAtOnce) {
+      SharedArgs some = sh;
+      some.first += g;
+      some.tokens += g;
+      some.groups = std::min(sh.groups - g, kGroupsAtOnce);
+      if (!attend_shared_prefix_many(alone, a, some, &e)) {
+        FewParams p = few_params(parts, a, 0xFFFFFFFFu);
+        p.prefix = true;
+        p.sh = some;
+        e = launch_few<kShared>(parts, p, (a.batch.tokens + sh.groups - 1) / sh.groups * group);
+      }
+      *launches += 1;
     }
-    *launches += 1;
+    if (e != cudaSuccess) return e;
+  } else {
+    sh.least = ~0ull;  // nothing is common
   }
-  if (e != cudaSuccess) return e;
-  const uint64_t mine = static_cast<uint64_t>(a.batch.most) * group;
-  const bool many = mine > kFewRows && attend_many_supports(a);
   FewParams p = few_params(in, a, many ? kFewRows : 0xFFFFFFFFu);
   p.sh = sh;
   e = launch_few<kShared>(in, p, many ? kFewRows : mine);

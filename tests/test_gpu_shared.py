@@ -238,7 +238,8 @@ def test_little_scratch(gpu):  # noqa: F811
 
 
 def test_what_reading_once_has_to_save(gpu):  # noqa: F811
-    """Less saved than asked for: every sequence reads its own, as without groups; by what the device arrays say, in a recorded call too."""
+    """Less saved than asked for: every sequence reads its own; by what the device arrays say, in a recorded call too.  (Where the work is cut
+    differs from a call without groups: sums of f32, each relative to 2^-24 of some hundreds.)"""
     import karume_b200 as kb
     g = Groups(gpu, [(300, [5, 30, 1, 9]), (64, [70, 3])], 16, 2, 64, seed=9)
     saved = (3 * 300 + 64) * 2 * 72
@@ -247,10 +248,12 @@ def test_what_reading_once_has_to_save(gpu):  # noqa: F811
         alone, once = (gpu.cache_attention(g.cache, q, batch, shared=s) for s in (None, g.prefixes()))
         gpu.sync()
         assert not torch.equal(alone, once)
-        for least, want in ((None, alone), (saved, once), (1, once), (1 << 40, alone)):
-            got = gpu.cache_attention(g.cache, q, batch, shared=kb.SharedPrefixes(g.prefixes().first, g.prefixes().tokens, least=least))
-            gpu.sync()
-            assert torch.equal(got, want), least
+        far = {}
+        for least in (None, saved, 1, 1 << 40):
+            far[least] = gpu.cache_attention(g.cache, q, batch, shared=kb.SharedPrefixes(g.prefixes().first, g.prefixes().tokens, least=least))
+        gpu.sync()
+        assert torch.equal(far[saved], once) and torch.equal(far[1], once) and torch.equal(far[None], far[1 << 40]) and not torch.equal(far[None], once)
+        assert float((far[None] - alone).norm() / alone.norm()) < 1e-6
         prefixes, out = kb.SharedPrefixes(g.prefixes().first, g.prefixes().tokens, least=saved), torch.zeros_like(q)
         gpu.sync()
         gpu.graph_begin()
