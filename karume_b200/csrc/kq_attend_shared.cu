@@ -9,7 +9,7 @@
 
 namespace kq {
 
-bool attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, const SharedArgs& sh, cudaError_t* e);
+cudaError_t attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 cudaError_t attend_shared_rest_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 
 // Bytes that are read once instead of often, from which on that is faster: without it they come from L2 mostly, with it there is a launch more
@@ -55,18 +55,26 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
     parts.workspace_bytes = left - own;
     LaunchEnv alone = parts;  // groups that come in turns: none may leave its parts where the next one's go
     if (sh.groups > kGroupsAtOnce) alone.workspace = nullptr;
+    // Each group is the work of one kernel, by its own rows; where they are many on the average, all are the tensor cores'.  (The few rows' kernel
+    // first: what it leaves in the parts' place it has joined itself.)
+    const uint64_t all = static_cast<uint64_t>(a.batch.tokens) * group;
+    const bool tensor = all > kFewRows && attend_many_supports(a), both = tensor && all / sh.groups <= kFewRows;
     for (uint32_t g = 0; g < sh.groups && e == cudaSuccess; g += kGroupsAtOnce) {
       SharedArgs some = sh;
       some.first += g;
       some.tokens += g;
       some.groups = std::min(sh.groups - g, kGroupsAtOnce);
-      if (!attend_shared_prefix_many(alone, a, some, &e)) {
-        FewParams p = few_params(parts, a, 0xFFFFFFFFu);
+      if (!tensor || both) {
+        FewParams p = few_params(parts, a, both ? kFewRows : 0xFFFFFFFFu);
         p.prefix = true;
         p.sh = some;
-        e = launch_few<kShared>(parts, p, (a.batch.tokens + sh.groups - 1) / sh.groups * group);
+        e = launch_few<kShared>(parts, p, both ? kFewRows : (a.batch.tokens + sh.groups - 1) / sh.groups * group);
+        *launches += 1;
       }
-      *launches += 1;
+      if (e == cudaSuccess && tensor) {
+        e = attend_shared_prefix_many(alone, a, both ? kFewRows : 0, some);
+        *launches += 1;
+      }
     }
     if (e != cudaSuccess) return e;
   } else {

@@ -160,6 +160,20 @@ def test_so_many_groups_that_they_come_in_turns(gpu, kind):  # noqa: F811
 
 
 @KINDS
+def test_large_and_small_groups_in_one_call(gpu, kind):  # noqa: F811
+    """Few rows a group on the average, so that each group goes to the kernel for its rows; and boundaries for more groups than there are."""
+    g = Groups(gpu, [(700, [3] * 30), (90, [5]), (-1, [40]), (400, [2, 90]), (33, [1]), (64, [7]), (640, [9] * 12), (20, [1]), (21, [2]), (22, [3]), (23, [4]),
+                     (24, [5]), (25, [6])], 16, 2, 64, seed=11)
+    n = len(g.lengths)
+    g.check(kind, [1] * n, 8, rotary=64)
+    g.check(kind, [1] * n, 8, window=300)
+    g.check(kind, [min(2, m + 1) for m in range(n)], 12, padding=2)
+    more = g.prefixes(first=g.first + [n] * (n - len(g.common)), common=g.common + [0] * (n - len(g.common)))
+    g.check(kind, [1] * n, 8, rotary=64, prefixes=more)
+    g.free()
+
+
+@KINDS
 @pytest.mark.parametrize("rows", ["few", "many"])
 def test_beginnings_that_reach_into_the_new_tokens(gpu, kind, rows):  # noqa: F811
     """More tokens said to be common than are in front of a sequence's new ones: those count as its own."""
