@@ -397,3 +397,54 @@ def test_refusals(gpu):  # noqa: F811
         with pytest.raises(kb.KqError):
             gpu.plan_end()
     f.free()
+
+
+def test_pages_beyond_4_gib(gpu):  # noqa: F811
+    """Pages, and their summaries, more than 4 GiB into the pool: selected, shared and summarised as those in front."""
+    import karume_b200 as kb
+    page, dim, heads = 256, 128, 2
+    block = page * (dim + 8)
+    count = (5 << 30) // (block * heads)
+    cache = gpu.kv_cache(count, page, heads, dim, pool=torch.zeros(count, heads, block, dtype=torch.uint8, device="cuda"))
+    near = gpu.kv_cache(8, page, heads, dim)
+    far_rows, near_rows = i32([[count - 1, count - 3, count - 2], [count - 1, count - 4, count - 5]]), i32([[7, 5, 6], [7, 4, 3]])
+    k, v = (torch.randn(1300, heads, dim, device="cuda") for _ in range(2))
+    lengths, q = i32([700, 600]), torch.randn(2, 8, dim, device="cuda")
+    out = []
+    for c, rows in ((cache, far_rows), (near, near_rows)):
+        both, one = kb.CacheBatch(rows, lengths, i32([0, 700, 1300]), tokens=1300), kb.CacheBatch(rows, lengths)
+        gpu.cache_append(c, k, v, both)
+        gpu.cache_append(c, k[:700], v[:700], kb.CacheBatch(rows[:1], lengths[:1], i32([0, 700]), tokens=700))  # the first page is the first one's
+        made = gpu.cache_summaries(c)
+        gpu.cache_summarize(c, made, both)
+        taken = gpu.cache_select(c, made, q, one, 2, first=0, last=1)
+        out.append([taken, made.codes[rows.long()], made.scales[rows.long()], gpu.cache_attention(c, q, one, selected=taken),
+                    gpu.cache_attention(c, q.half(), one, shared=kb.SharedPrefixes(i32([0, 2]), i32([256]), least=0))])
+        gpu.sync()
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    cache.free()
+    near.free()
+
+
+def test_summaries_beyond_4_gib(gpu):  # noqa: F811
+    """Selecting reads nothing of the pool, so that it may be a small one: 9000 pages of 1024 heads of 256."""
+    import ctypes
+    import karume_b200 as kb
+    pages, heads, dim, page = 9000, 1024, 256, 16
+    handle, small = ctypes.c_uint64(0), torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    assert kb.lib.kq_cache_create(gpu._ctx, small.data_ptr(), pages, page, heads, dim, ctypes.byref(handle)) == 0
+    cache = kb.KvCache(gpu, handle.value, small, pages, page, heads, dim)
+    codes, scales = torch.zeros(pages, heads, 2, dim, dtype=torch.int8, device="cuda"), torch.zeros(pages, heads, 2, device="cuda")
+    table = torch.arange(pages - 60, pages, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    of = table[0].long()
+    codes[of] = torch.randint(-127, 128, (60, heads, 2, dim), generator=gen, device="cuda").to(torch.int8)
+    codes[of, :, 1] = codes[of, :, 1].abs()
+    scales[of] = torch.rand(60, heads, 2, generator=gen, device="cuda")
+    q = torch.randn(1, heads, dim, generator=gen, device="cuda")
+    got = gpu.cache_select(cache, kb.CacheSummaries(codes, scales), q, kb.CacheBatch(table, i32([60 * page - 3])), 7, first=1, last=2)
+    gpu.sync()
+    for h in (0, 1, 511, 1022, 1023):
+        score = sel.scores(as_numpy(q)[0, h:h + 1], as_numpy(codes[of, h]), as_numpy(scales[of, h]))
+        assert got[0, h].tolist() == sel.select(score, 7, 1, 2), h
+    cache.free()
