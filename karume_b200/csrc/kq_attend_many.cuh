@@ -16,11 +16,12 @@
 // O is one tile's, added in registers, so that a long row does not drift.
 // Few blocks of rows: the tiles of keys of each are shared by several CTAs, and the last one joins their sums in order.
 //
-// Measured: 4096 new tokens behind 904, 32 heads over 8, bfloat16: 305 us (650 TFLOP/s; tensor pipe 33 %, issue slots 52 %).  Of it a tile
+// Measured: 4096 new tokens behind 904, 32 heads over 8, bfloat16: 291 us (682 TFLOP/s; with a lane's rows of queries one after the other instead of
+// step by step 299; tensor pipe 33 %, issue slots 52 %).  At 305 us of it a tile
 // of 256 rows is 2.6 us of a CTA (the MMAs 1.1): the turn from scores to weights and back, neither the unpacking (left out: 292 of 305 us)
 // nor the exponentials (left out: 307) alone; a CTA's beginning and end were 21 us (rows found 1.8, queries 7.2, the first
 // tile's way 4, output 5.9 (2.4 since it leaves in whole rows: 305 -> 293 us), the next CTA's start 1.8), three to four times an SM; the last CTAs end 27 us after the mean one.
-// Three f32 prompts of up to 777 tokens behind 724, 12 heads over 2: 66 us, two products for one (queries and weights have two parts).
+// Three f32 prompts of up to 777 tokens behind 724, 12 heads over 2: 65 us, two products for one (queries and weights have two parts).
 //
 //   16-bit queries  keys and values are unpacked to what they stand for, rounded to binary16 once (2^-11, as the weights); rows beyond
 //                   binary16's range to a sixteenth of it, which scores and weights make up for.

@@ -311,15 +311,16 @@ __global__ void __launch_bounds__(kScoreWarps * 32, D == 256 ? 4 : 6) score_kern
   int base = first + static_cast<int>(warp) * 16;
   look(base);
   load();  // while the queries are worked on
-  look(base + kScorePages);
+  if (p.turns > 1) look(base + kScorePages);
   const int position = place_of_row(p.a.batch, row).x;
   const uint32_t blocks = (p.group + kHeads - 1) / kHeads;
   float best[2];
   bool unknown[2];
-  for (uint32_t turn = 0; turn < p.turns; ++turn, base += kScorePages) {
+  const uint32_t turns = min(p.turns, static_cast<uint32_t>(pages - first + kScorePages - 1) / kScorePages);  // that have pages
+  for (uint32_t turn = 0; turn < turns; ++turn, base += kScorePages) {
     if (turn) {
       load();
-      look(base + kScorePages);
+      if (turn + 1 < turns) look(base + kScorePages);
     }
     best[0] = best[1] = -INFINITY;
     unknown[0] = unknown[1] = false;
@@ -476,6 +477,7 @@ cudaError_t launch_select(const LaunchEnv& env, const AttendArgs& a, const Summa
   const uint64_t blocks = static_cast<uint64_t>(a.batch.tokens) * a.cache.kv_heads, most = (a.batch.width + kScorePages - 1) / kScorePages;
   p.turns = static_cast<uint32_t>(std::min<uint64_t>({std::max<uint64_t>((blocks * most + 6ull * env.sm_count - 1) / (6ull * env.sm_count), 1), most, 32}));
   p.chunks = static_cast<uint32_t>((most + p.turns - 1) / p.turns);
+  p.turns = static_cast<uint32_t>((most + p.chunks - 1) / p.chunks);  // even shares
   *launches = 0;
   // as many rows at a time as have room in the scratch and in a grid
   const bool fused = a.batch.width <= kFusedPages;
