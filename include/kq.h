@@ -407,7 +407,7 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
                               uint32_t rope_flags, uint64_t out_dptr, uint64_t out_stride);
 
 /* kq_cache_attention_shared: kq_cache_attention for sequences that begin alike, the keys that they have in common read once.  Group g is the
- * sequences first[g] .. first[g + 1] - 1 (i32 [groups + 1], ascending); their first shared[g] tokens (i32 [groups]) are the same: their
+ * sequences first[g] .. first[g + 1] - 1 (i32 [groups + 1], ascending; groups <= sequences); their first shared[g] tokens (i32 [groups]) are the same: their
  * tables name the same pages for them, or (a last page that is not full) copies.  What is shared beyond a sequence's new tokens' beginning counts as
  * its own; sequences outside the groups, and a group of one, are as in kq_cache_attention.  The same results but for roundings.  Reading
  * once takes a launch more and joins every row's sums, reading often hits L2: `least` is how many bytes (tokens in common x members but one
@@ -427,7 +427,9 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
  * Scratch: 4 * kv_heads * table_width bytes at least (KQ_ERR_UNSUPPORTED).
  * kq_cache_attention_selected: attention of every new token over the tokens of its selected pages up to its position; `selected` as kq_cache_select
  * gives it: min(budget, pages up to the position) indices are read, the last of which is the position's own page.  An index outside the table reads
- * as NaN.  For few rows a sequence: each reads its own pages. */
+ * as NaN.  For few rows a sequence: each reads its own pages.
+ *
+ * None of these can be part of a fused plan, as above. */
 #define KQ_SHARED_AUTO 0xFFFFFFFFFFFFFFFFull
 KQ_API int kq_cache_attention_shared(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint64_t q_stride, int q_dtype, uint32_t heads,
                                      uint32_t sequences, uint64_t page_table_dptr, uint32_t table_width, uint64_t lengths_dptr,
@@ -470,7 +472,9 @@ KQ_API int kq_cache_attention_selected(kq_ctx* ctx, kq_cache cache, uint64_t q_d
  *   `pairs` (from, to), i32 [pages, 2], (-1, -1) behind report[2] of them; table and refs have the new numbers.
  * kq_pages_copy: copies page from to page to for the pairs of such a call, in `count` pools (host arrays of addresses and of the bytes of a
  *   page, multiples of 16: the pool of a kq_cache has kq_cache_bytes(1, ..) a page): the report's number of them, or (report_dptr == 0) all `most`.
- *   Pairs with a number outside the pool are passed over; one page may be the target of one pair, and not the source of another. */
+ *   Pairs with a number outside the pool are passed over; one page may be the target of one pair, and not the source of another.
+ *
+ * None of these can be part of a fused plan, as above. */
 KQ_API int kq_pages_grow(kq_ctx* ctx, uint64_t table_dptr, uint32_t sequences, uint32_t width, uint64_t lengths_dptr, uint64_t refs_dptr,
                          uint32_t pages, uint32_t page_tokens, uint64_t report_dptr, uint64_t news_dptr);
 KQ_API int kq_pages_fork(kq_ctx* ctx, uint64_t table_dptr, uint32_t sequences, uint32_t width, uint64_t lengths_dptr, uint64_t refs_dptr,

@@ -1079,6 +1079,15 @@ cudaError_t launch_few(const LaunchEnv& env, const FewParams& p, uint64_t rows) 
   return few_in<__nv_bfloat16, kMode>(env, p, rows);
 }
 
+// Over common keys (prefix) or behind them.
+template <typename T>
+cudaError_t few_shared(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, bool prefix, const SharedArgs& sh, uint64_t rows) {
+  FewParams p = few_params(env, a, beyond);
+  p.prefix = prefix;
+  p.sh = sh;
+  return few_in<T, kShared>(env, p, rows);
+}
+
 // Query rows (of a sequence and kv head) up to which this kernel is faster than 128-row MMAs.  16 sequences of 4096 tokens, 8 kv heads,
 // this one / the other: bfloat16 16 rows 43 / 95 us, 32 rows 88 / 96, 48 rows 141 / 97; f32 32 rows 104 / 148, 48 rows 147 / 148.
 constexpr uint32_t kFewRows = 32;

@@ -9,6 +9,9 @@
 
 namespace kq {
 
+// The walk for few rows with f32 and float16 queries, each in a source of its own: they take the compiler longest.
+cudaError_t attend_shared_few_f32(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, bool prefix, const SharedArgs& sh, uint64_t rows);
+cudaError_t attend_shared_few_f16(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, bool prefix, const SharedArgs& sh, uint64_t rows);
 cudaError_t attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 cudaError_t attend_shared_rest_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 
@@ -21,6 +24,16 @@ constexpr uint64_t kWorth = 128ull << 20;
 // kv head, bfloat16 1511 / 1045 us; 8 of up to 100 behind 32768, 497 / 648.
 constexpr uint64_t kAlone = 512;
 constexpr uint32_t kGroupsAtOnce = 128;
+
+namespace {
+
+cudaError_t attend_shared_few(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, bool prefix, const SharedArgs& sh, uint64_t rows) {
+  if (a.dtype == KQ_F32) return attend_shared_few_f32(env, a, beyond, prefix, sh, rows);
+  if (a.dtype == KQ_F16) return attend_shared_few_f16(env, a, beyond, prefix, sh, rows);
+  return few_shared<__nv_bfloat16>(env, a, beyond, prefix, sh, rows);
+}
+
+}  // namespace
 
 cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, SharedArgs sh, int* launches) {
   // What a call can save at most; then what it does save, as the lengths say on the device.
@@ -65,10 +78,8 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
       some.tokens += g;
       some.groups = std::min(sh.groups - g, kGroupsAtOnce);
       if (!tensor || both) {
-        FewParams p = few_params(parts, a, both ? kFewRows : 0xFFFFFFFFu);
-        p.prefix = true;
-        p.sh = some;
-        e = launch_few<kShared>(parts, p, both ? kFewRows : (a.batch.tokens + sh.groups - 1) / sh.groups * group);
+        e = attend_shared_few(parts, a, both ? kFewRows : 0xFFFFFFFFu, true, some,
+                              both ? kFewRows : (a.batch.tokens + sh.groups - 1) / sh.groups * group);
         *launches += 1;
       }
       if (e == cudaSuccess && tensor) {
@@ -80,9 +91,7 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
   } else {
     sh.least = ~0ull;  // nothing is common
   }
-  FewParams p = few_params(in, a, many ? kFewRows : 0xFFFFFFFFu);
-  p.sh = sh;
-  e = launch_few<kShared>(in, p, many ? kFewRows : mine);
+  e = attend_shared_few(in, a, many ? kFewRows : 0xFFFFFFFFu, false, sh, many ? kFewRows : mine);
   if (e == cudaSuccess && many) e = attend_shared_rest_many(in, a, kFewRows, sh);
   *launches += many ? 2 : 1;
   return e;
