@@ -471,7 +471,8 @@ KQ_API int kq_cache_attention_selected(kq_ctx* ctx, kq_cache cache, uint64_t q_d
  * kq_pages_compact: the pages in use move to the lowest numbers: of those beyond as many as are in use the r-th to the r-th free one below, as
  *   `pairs` (from, to), i32 [pages, 2], (-1, -1) behind report[2] of them; table and refs have the new numbers.
  * kq_pages_copy: copies page from to page to for the pairs of such a call, in `count` pools (host arrays of addresses and of the bytes of a
- *   page, multiples of 16: the pool of a kq_cache has kq_cache_bytes(1, ..) a page): the report's number of them, or (report_dptr == 0) all `most`.
+ *   page, multiples of 4, and of 16 for bulk copies: the pool of a kq_cache has kq_cache_bytes(1, ..) a page, summaries kv_heads * 2 * head_dim and
+ *   kv_heads * 8): the report's number of them, or (report_dptr == 0) all `most`.
  *   Pairs with a number outside the pool are passed over; one page may be the target of one pair, and not the source of another.
  *
  * None of these can be part of a fused plan, as above. */

@@ -1115,9 +1115,9 @@ int kq_pages_copy(kq_ctx* ctx, uint32_t count, const uint64_t* pools, const uint
   if (pages > (1u << 30) || most > (1u << 30)) return fail(ctx, KQ_ERR_SHAPE, "kq_pages_copy: %u pages, %u pairs: up to 2^30", pages, most);
   if (!pairs || ((pairs | report) & 3u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: pairs [most, 2] and report [4] are i32 device arrays");
   for (uint32_t i = 0; i < count; ++i) {
-    if (!pools[i] || (pools[i] & 15u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: pool %u must be a 16-byte aligned device pointer", i);
-    if (!page_bytes[i] || page_bytes[i] % 16 || page_bytes[i] > (1ull << 32))
-      return fail(ctx, KQ_ERR_SHAPE, "kq_pages_copy: pages of pool %u have %llu bytes: a multiple of 16, up to 2^32", i, (unsigned long long)page_bytes[i]);
+    if (!pools[i] || (pools[i] & 3u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: pool %u must be a 4-byte aligned device pointer", i);
+    if (!page_bytes[i] || page_bytes[i] % 4 || page_bytes[i] > (1ull << 32))
+      return fail(ctx, KQ_ERR_SHAPE, "kq_pages_copy: pages of pool %u have %llu bytes: a multiple of 4, up to 2^32", i, (unsigned long long)page_bytes[i]);
   }
   if (!pages || !most) return KQ_OK;
   DeviceGuard guard(ctx->device);

@@ -134,7 +134,7 @@ def test_what_sequences_hold_behind_forks_and_moves(gpu):  # noqa: F811
         c.free()
 
 
-@pytest.mark.parametrize("page_bytes", [16, 272, 4096, 16384, 16400, 69632, 70000])
+@pytest.mark.parametrize("page_bytes", [4, 8, 16, 44, 272, 4096, 16384, 16388, 16400, 50004, 69632, 70000])
 @pytest.mark.parametrize("pools", [1, 3, 130])
 def test_copies(gpu, page_bytes, pools):  # noqa: F811
     rng = np.random.default_rng(page_bytes)
@@ -165,6 +165,40 @@ def test_copies_without_a_report_and_of_nothing(gpu):  # noqa: F811
     assert kb.lib.kq_pages_copy(gpu._ctx, 0, None, None, 8, pairs.data_ptr(), 2, 0) == 0
     gpu.sync()
     assert t[:, 0].tolist() == [0, 4, 8, 12, 16, 8, 24, 0]
+
+
+def test_copies_of_pools_that_begin_between_sixteen_bytes(gpu):  # noqa: F811
+    rng = np.random.default_rng(3)
+    for first, wide in ((1, 4), (3, 1000), (2, 9001)):
+        whole = torch.from_numpy(rng.integers(0, 1 << 30, first + 9 * wide + 5, dtype=np.int32)).cuda()
+        want, book = whole.clone(), gpu.cache_pages(1, 16, 9, 16)
+        want[first:first + 9 * wide].view(9, wide)[[8, 0]] = want[first:first + 9 * wide].view(9, wide)[[1, 5]]
+        book.report.copy_(i32([0, 0, 2, 0]))
+        gpu.pages_copy(book, i32([[1, 8], [5, 0]]), [whole[first:first + 9 * wide].view(9, wide)])
+        gpu.sync()
+        assert torch.equal(whole, want), (first, wide)
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3])
+def test_summaries_move_with_their_pages(gpu, heads):  # noqa: F811
+    import karume_b200 as kb
+    page, dim = 16, 64
+    book, cache = gpu.cache_pages(3, 6 * page, 20, page), gpu.kv_cache(20, page, heads, dim)
+    made = gpu.cache_summaries(cache)
+    gpu.pages_grow(book, i32([70, 40, 33]))
+    gen = torch.Generator(device="cuda").manual_seed(heads)
+    k, v = (torch.randn(143, heads, dim, generator=gen, device="cuda") for _ in range(2))
+    batch = kb.CacheBatch(book.table, book.lengths, i32([0, 70, 110, 143]), tokens=143)
+    gpu.cache_append(cache, k, v, batch)
+    gpu.cache_summarize(cache, made, batch)
+    gpu.pages_fork(book, i32([-1, 1, 2]))
+    gpu.pages_copy(book, gpu.pages_compact(book), [cache, made])
+    assert book.report.tolist()[2] == 5  # two sequences' pages 5 .. 10 are 0 .. 5 now, of which one was free to stay
+    again = gpu.cache_summaries(cache)
+    gpu.cache_summarize(cache, again, kb.CacheBatch(book.table, book.lengths, i32([0, 0, 40, 73]), tokens=73))
+    gpu.sync()
+    assert torch.equal(made.codes[:6], again.codes[:6]) and torch.equal(made.scales[:6], again.scales[:6]) and bool((again.scales[:6] > 0).all())
+    cache.free()
 
 
 def test_copies_of_pages_beyond_4_gib(gpu):  # noqa: F811
@@ -231,7 +265,7 @@ def test_refusals(gpu):  # noqa: F811
     for call in (lambda: gpu.pages_grow(book, good.long()), lambda: gpu.pages_grow(book, good[:2]), lambda: gpu.pages_grow(book, good.cpu()),
                  lambda: gpu.pages_fork(book, i32([0] * 6)[::2]), lambda: gpu.pages_fork(book, good, good[:1]),
                  lambda: gpu.pages_copy(book, good, []), lambda: gpu.pages_copy(book, i32([[0, 1]]), [torch.zeros(7, 16, device="cuda")]),
-                 lambda: gpu.pages_copy(book, i32([[0, 1]]), [torch.zeros(8, 3, device="cuda")]),
+                 lambda: gpu.pages_copy(book, i32([[0, 1]]), [torch.zeros(8, 6, dtype=torch.uint8, device="cuda")]),
                  lambda: gpu.pages_copy(book, i32([[0, 1]]), [torch.zeros(8, 32, device="cuda")[:, :16]]),
                  lambda: kb.CachePages(book.table.long(), book.lengths, book.refs, 16), lambda: kb.CachePages(book.table, good[:2], book.refs, 16),
                  lambda: gpu.pages_grow(kb.CachePages(book.table, book.lengths, book.refs, 24), good),
