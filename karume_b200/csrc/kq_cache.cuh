@@ -85,7 +85,10 @@ __device__ __forceinline__ int common_keys(const CacheBatch& batch, const Shared
     if (__ldg(sh.first + mid) <= static_cast<int>(b)) lo = mid;
     else hi = mid;
   }
-  if (__ldg(sh.first + lo) > static_cast<int>(b) || __ldg(sh.first + lo + 1) <= static_cast<int>(b)) return 0;
+  const int b0 = __ldg(sh.first + lo), b1 = __ldg(sh.first + lo + 1);
+  if (b0 > static_cast<int>(b) || b1 <= static_cast<int>(b)) return 0;
+  // Rows that are not among the group's (starts that do not ascend) have no sums over common keys.
+  if (batch.starts && (batch.starts[max(b0, 0)] > span.first || batch.starts[min(b1, static_cast<int>(batch.sequences))] < span.first + span.count)) return 0;
   return min(max(__ldg(sh.tokens + lo), 0), max(span.length - span.count, 0));
 }
 // By a warp: the new rows of group g's sequences (first, number), the keys that any of them has in common, the first of these that a row

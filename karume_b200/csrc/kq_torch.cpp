@@ -344,6 +344,7 @@ struct Rows {
     if (type < 0 || q->dim() != 3 || q->numel() == 0) return false;
     heads = q->size(1);
     if (!rows_of(*q, tokens, heads, dim, &q_stride) || (device >= 0 && q->get_device() != device)) return false;
+    if (given != nullptr && device >= 0 && given->get_device() != device) return false;
     if (given == nullptr) made = at::detail::empty_cuda(q->sizes(), q->scalar_type(), q->device(), c10::nullopt);
     const at::Tensor& o = given != nullptr ? *given : made;
     if (o.scalar_type() != q->scalar_type() || !rows_of(o, tokens, heads, dim, &out_stride)) return false;
@@ -443,7 +444,7 @@ PyObject* cache_select(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       first > budget || last < 0 || last > budget)
     KQ_NONE;
   const int64_t shape[3] = {tokens, kv_heads, budget};
-  if (given != nullptr && (given->scalar_type() != at::kInt || !plain(*given) || given->sizes() != at::IntArrayRef(shape))) KQ_NONE;
+  if (given != nullptr && (given->scalar_type() != at::kInt || !plain(*given) || given->get_device() != device || given->sizes() != at::IntArrayRef(shape))) KQ_NONE;
   at::Tensor made;
   if (given == nullptr) made = at::detail::empty_cuda(shape, at::kInt, q->device(), c10::nullopt);
   void* ctx = PyLong_AsVoidPtr(a[0]);

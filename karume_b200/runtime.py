@@ -111,6 +111,7 @@ class Rope:
         if t.dtype != _torch().float32 or not t.is_cuda or t.dim() != 3 or t.shape[2] != 2 or not t.is_contiguous():
             raise KqError(2, "the rotation table is a contiguous CUDA f32 tensor [positions, rotary / 2, 2]")
         self.positions, self.rotary = int(t.shape[0]), 2 * int(t.shape[1])
+        self.index = t.get_device()
         self.args = (t.data_ptr(), self.positions, self.rotary, 1 if self.interleaved else 0)
 
 
@@ -133,6 +134,9 @@ class CacheBatch:
         if most < 0:
             raise KqError(2, f"most {most}: a bound of a sequence's new tokens, 0 if not known")
         self.pages, self.lengths, self.starts = pages, lengths, starts
+        self.index = pages.get_device()  # -1: the tensors are on several devices
+        if any(t is not None and t.get_device() != self.index for t in (lengths, starts)):
+            self.index = -1
         self.tokens = int(tokens) if starts is not None else self.sequences
         self.most = min(int(most), self.tokens) if starts is not None else 1
         self.args = (self.sequences, pages.data_ptr(), self.width, lengths.data_ptr(), starts.data_ptr() if starts is not None else 0,
@@ -228,6 +232,14 @@ def _on_device(index: int, **tensors) -> None:
     for name, t in tensors.items():
         if t.device.index != index:
             raise KqError(2, f"{name} is on {t.device}, the context's device is cuda:{index}")
+
+
+def _batch_here(index: int, batch: "CacheBatch", rope: "Rope | None" = None) -> None:
+    """Raises where a batch's tensors or the angles are not on the context's device."""
+    if batch.index != index:
+        raise KqError(2, f"the batch is on {'several devices' if batch.index < 0 else f'cuda:{batch.index}'}, the context's device is cuda:{index}")
+    if rope is not None and rope.index != index:
+        _on_device(index, table=rope.table)
 
 
 def _per_sequence(t, book: CachePages, name: str) -> int:
@@ -575,6 +587,8 @@ class Gpu:
             raise KqError(2, f"window {window}: a number of keys, 0 for all")
         window = min(int(window), 0xFFFFFFFF)  # the ABI's number has 32 bits; no sequence is longer
         angles = rope.args if rope is not None else None
+        if shared is not None or selected is not None:
+            _batch_here(self.index, batch, rope)
         if shared is None and selected is None:
             done = _fast.cache_attention(self._ctx_addr, cache.handle, cache.head_dim, q, batch.args, batch.most, scale, window, angles, out)
         elif selected is None:
@@ -587,9 +601,9 @@ class Gpu:
         if done is not None:
             return self._done(done)
         if shared is not None:
-            _on_device(self.index, q=q, first=shared.first)
+            _on_device(self.index, q=q, first=shared.first, out=q if out is None else out)
         if selected is not None:
-            _on_device(self.index, q=q, selected=selected)
+            _on_device(self.index, q=q, selected=selected, out=q if out is None else out)
         torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
@@ -625,6 +639,7 @@ class Gpu:
     def cache_summarize(self, cache: KvCache, summaries: CacheSummaries, batch: CacheBatch) -> None:
         """Brings the summaries of the pages that the batch's new tokens are in up to date (behind cache_append)."""
         summaries.check(cache, self.index)
+        _batch_here(self.index, batch)
         done = _fast.cache_summarize(self._ctx_addr, cache.handle, summaries.args, batch.args)
         if done is not None:
             return self._check(done)
@@ -635,11 +650,12 @@ class Gpu:
         """Up to `budget` pages for every row of q [tokens, heads, head_dim] and kv head, int32 [tokens, kv_heads, budget]: ascending indices into
         the sequence's pages, -1 behind them; always the first `first` and the last `last` ones, then those whose summaries promise most."""
         summaries.check(cache, self.index)
+        _batch_here(self.index, batch, rope)
         done = _fast.cache_select(self._ctx_addr, cache.handle, cache.kv_heads, cache.head_dim, summaries.args, q, batch.args, budget, first, last,
                                   rope.args if rope is not None else None, out, self.index)
         if done is not None:
             return self._done(done)
-        _on_device(self.index, q=q)
+        _on_device(self.index, q=q, out=q if out is None else out)
         torch = _torch()
         heads, dim = int(q.shape[1]), cache.head_dim
         if q.shape[0] != batch.tokens:
@@ -699,14 +715,21 @@ class Gpu:
         return pairs
 
     def pages_copy(self, book: CachePages, pairs, pools) -> None:
-        """Copies the pages of the book's last fork or compact in every pool: KvCaches, or CUDA tensors whose first axis is the pages."""
-        given, pools = pools, [pool.page_args if isinstance(pool, KvCache) else pool for pool in pools]
+        """Copies the pages of the book's last fork or compact in every pool: KvCaches, CacheSummaries, or CUDA tensors whose first axis is the pages."""
+        given, pools = pools, []
+        for pool in given:
+            if isinstance(pool, KvCache):
+                pools.append(pool.page_args)
+            elif isinstance(pool, CacheSummaries):
+                pools += pool.codes, pool.scales
+            else:
+                pools.append(pool)
         done = _fast.pages_copy(self._ctx_addr, book.args, pairs, pools, self.index) if book.index == self.index else None
         if done is not None:
             return self._check(done)
         _on_device(self.index, table=book.table, pairs=pairs)
         for pool in given:
-            _on_device(self.index, pool=pool.pool if isinstance(pool, KvCache) else pool)
+            _on_device(self.index, pool=pool.pool if isinstance(pool, KvCache) else pool.codes if isinstance(pool, CacheSummaries) else pool)
         torch = _torch()
         if pairs.dtype != torch.int32 or not pairs.is_cuda or not pairs.is_contiguous() or pairs.dim() != 2 or pairs.shape[1] != 2:
             raise KqError(2, "pairs must be a contiguous CUDA int32 tensor [pairs, 2]")

@@ -17,6 +17,7 @@ with FakeTensorMode():
     q = torch.empty(3, 4, 64, device="cuda")
     taken = torch.empty(3, 2, 5, device="cuda", dtype=torch.int32)
     each = torch.empty(3, device="cuda", dtype=torch.int32)
+    out, places = torch.empty(3, 4, 64, device="cuda:1"), torch.empty(3, 2, 5, device="cuda:1", dtype=torch.int32)
     fewer, one_head, two, long = torch.empty(2, 4, 64, device="cuda"), taken[:, :1], each[:2], torch.empty(3, device="cuda", dtype=torch.int64)
 batch, book = (3, 4096, 8, 8192, 0, 3), (4096, 3, 8, 8192, 12288, 40, 16, 16384)
 raises = {
@@ -49,6 +50,10 @@ assert native.pages_grow(8, book, each, 1) is None and native.pages_fork(8, book
 assert native.cache_attention_shared(8, 1, 64, q, batch, 1, (1, 64, 128, 0), 1.0, 0, None, None, 1) is None
 assert native.cache_attention_selected(8, 1, 2, 64, q, batch, taken, 1.0, None, None, 1) is None
 assert native.cache_select(8, 1, 2, 64, (16, 32), q, batch, 5, 1, 1, None, None, 1) is None
+# ... for the output alone
+assert native.cache_attention_shared(8, 1, 64, q, batch, 1, (1, 64, 128, 0), 1.0, 0, None, out, 0) is None
+assert native.cache_attention_selected(8, 1, 2, 64, q, batch, taken, 1.0, None, out, 0) is None
+assert native.cache_select(8, 1, 2, 64, (16, 32), q, batch, 5, 1, 1, None, places, 0) is None
 """
 
 
@@ -74,3 +79,22 @@ def test_tensors_of_another_device_are_refused():
     with pytest.raises(KqError) as e:
         _on_device(0, a=OnDevice(0), b=OnDevice(1))
     assert e.value.status == "KQ_ERR_SHAPE" and "b is on cuda:1" in str(e.value)
+
+
+def test_batches_and_angles_of_another_device_are_refused():
+    from types import SimpleNamespace as Like
+    from karume_b200.runtime import CacheSummaries, Gpu, KqError, SharedPrefixes
+    gpu, here = object.__new__(Gpu), Like(index=0)
+    gpu.index = 0
+    cache, summaries, shared = Like(head_dim=64, kv_heads=2, handle=1), object.__new__(CacheSummaries), object.__new__(SharedPrefixes)
+    summaries.check = lambda cache, index: None
+    elsewhere, mixed, angles = Like(index=1), Like(index=-1), Like(index=1, table=OnDevice(1), args=None)
+    for batch, rope, says in ((elsewhere, None, "cuda:1"), (mixed, None, "several devices"), (here, angles, "table is on cuda:1")):
+        calls = [lambda: gpu.cache_attention(cache, None, batch, rope=rope, shared=shared), lambda: gpu.cache_attention(cache, None, batch, rope=rope, selected=0),
+                 lambda: gpu.cache_select(cache, summaries, None, batch, 4, rope=rope)]
+        if rope is None:
+            calls.append(lambda: gpu.cache_summarize(cache, summaries, batch))
+        for call in calls:
+            with pytest.raises(KqError) as e:
+                call()
+            assert e.value.status == "KQ_ERR_SHAPE" and says in str(e.value)
