@@ -1371,9 +1371,7 @@ cudaError_t many_as(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, 
   p.status = env.status;
   p.prefix = prefix;
   p.sh = sh;
-  // at most so many blocks of rows: full ones, and one begun for each sequence
-  const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * p.group;
-  const uint64_t blocks = rows / F::kBlock + std::min<uint64_t>(prefix ? sh.groups : a.batch.sequences, rows / (beyond + 1));
+  const uint64_t blocks = groups::most_blocks(static_cast<uint64_t>(a.batch.tokens) * p.group, F::kBlock, prefix ? sh.groups : a.batch.sequences, beyond);
   cudaLaunchConfig_t cfg = {};
   const uint64_t units = blocks * a.cache.kv_heads;
   // Few units: their keys are shared, so that every SM has its part (a part more for each unit's odd end).

@@ -60,6 +60,7 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
     uint8_t* const base = static_cast<uint8_t*>(env.workspace);
     const uint64_t left = (scratch - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
     sh.scratch = static_cast<float*>(env.workspace);
+    sh.floats = scratch / 4;
     sh.places = reinterpret_cast<uint4*>(base + left);
     sh.sums = (left + rows * 16) / 4;
     LaunchEnv parts = env;

@@ -8,6 +8,7 @@
 #pragma once
 
 #include "kq_common.cuh"
+#include "kq_groups.h"
 #include "kq_internal.h"
 
 namespace kq {
@@ -61,7 +62,9 @@ __device__ __forceinline__ int2 place_of_row(const CacheBatch& batch, uint32_t r
 }
 
 // ---- sequences that begin alike ---------------------------------------------------------------
-// By a warp: whether reading what the groups have in common once saves enough (the other way re-reads it, mostly from L2).
+// By a warp: whether reading what the groups have in common once saves enough (the other way re-reads it, mostly from L2).  Not where their
+// boundaries are out of order: groups with rows in common would ask for more blocks than there are.  (That is looked at last: `starts` are a trip to memory
+// behind the boundaries, 1.4 us of a call that saves nothing.)
 __device__ __forceinline__ bool worth_sharing(const AttendArgs& a, const SharedArgs& sh) {
   unsigned long long keys = 0;
   for (uint32_t g = threadIdx.x % 32; g < sh.all_groups; g += 32) {
@@ -72,7 +75,12 @@ __device__ __forceinline__ bool worth_sharing(const AttendArgs& a, const SharedA
   }
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) keys += __shfl_xor_sync(0xffffffffu, keys, o);
-  return keys * (a.cache.kv_heads * (a.cache.head_dim + 8u)) >= sh.least;
+  if (keys * (a.cache.kv_heads * (a.cache.head_dim + 8u)) < sh.least) return false;
+  bool ordered = true;
+  for (uint32_t g = threadIdx.x % 32; g < sh.all_groups; g += 32)
+    ordered &= groups::in_order(__ldg(sh.all_first + g), __ldg(sh.all_first + g + 1), a.batch.starts, static_cast<int>(a.batch.sequences),
+                                static_cast<int>(a.batch.tokens));
+  return __all_sync(0xffffffffu, ordered);
 }
 __device__ __forceinline__ uint32_t first_of_group(const CacheBatch& batch, const SharedArgs& sh, uint32_t g) {
   return min(static_cast<uint32_t>(max(__ldg(sh.first + g), 0)), batch.sequences - 1);
@@ -94,11 +102,10 @@ __device__ __forceinline__ int common_keys(const CacheBatch& batch, const Shared
 // By a warp: the new rows of group g's sequences (first, number), the keys that any of them has in common, the first of these that a row
 // sees; every: first and last of the keys that all the rows see.
 __device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const SharedArgs& sh, uint32_t g, int window, int2& every) {
-  const int sequences = static_cast<int>(batch.sequences), tokens = static_cast<int>(batch.tokens);
-  const int b0 = min(max(__ldg(sh.first + g), 0), sequences), b1 = min(max(__ldg(sh.first + g + 1), b0), sequences);
-  const int row0 = min(batch.starts ? max(batch.starts[b0], 0) : b0, tokens), row1 = min(max(batch.starts ? batch.starts[b1] : b1, row0), tokens);
+  const groups::Range members = groups::sequences_of(__ldg(sh.first + g), __ldg(sh.first + g + 1), static_cast<int>(batch.sequences));
+  const groups::Range rows = groups::rows_of(members, batch.starts, static_cast<int>(batch.tokens));
   int least = 0x7fffffff, far = 0, last = -1;
-  for (int b = b0 + static_cast<int>(threadIdx.x % 32); b < b1; b += 32) {
+  for (int b = members.begin + static_cast<int>(threadIdx.x % 32); b < members.end; b += 32) {
     const Span s = span_of(batch, static_cast<uint32_t>(b));
     if (s.count == 0) continue;
     least = min(least, s.length - s.count);
@@ -112,17 +119,24 @@ __device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const Sha
   // (a window may hide all of them: one is walked over all the same, so that the rows' sums are written)
   const int from = window && least >= window ? min(least - window + 1, max(keys - 1, 0)) : 0;
   every = make_int2(window && last >= window ? last - window + 1 : 0, min(keys, max(least, 0)) - 1);
-  return make_int4(row0, row1 - row0, keys, from);
+  return make_int4(rows.begin, rows.end - rows.begin, keys, from);
 }
 
+__device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7FC00000); }
 __device__ __forceinline__ float power_of_two(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 // Four of the sums of a row, not divided yet, relative to 2^m, and the sum of its weights: joined with what the row sees of the common keys,
-// which is at the row's place `at`.
+// which is at the row's place `at`.  A place that is none (a launch in front gave up waiting, and left the row's out) gives NaN.
+constexpr uint32_t kMostParts = 1024;  // CTAs that share a row's common keys: no more than there are SMs
 __device__ __forceinline__ void join_common(const SharedArgs& sh, const uint4& at, int quad, float& m, float& total, float (&v)[4]) {
+  const uint64_t last = static_cast<uint64_t>(at.w - 1) * at.z, end_sums = (static_cast<uint64_t>(at.x) + quad) * 4 + last + 4, end_stats = static_cast<uint64_t>(at.y) * 2 + last + 2;
+  if (at.w - 1 >= kMostParts || max(end_sums, end_stats) > sh.floats) {
+    total = quiet_nan();
+    return;
+  }
   const float4* const sums = reinterpret_cast<const float4*>(sh.scratch) + at.x + quad;
   const float2* const stats = reinterpret_cast<const float2*>(sh.scratch) + at.y;
   constexpr uint32_t kBatch = 12;
@@ -183,7 +197,6 @@ __device__ __forceinline__ uint32_t selected_page(const AttendArgs& a, const Sel
 __device__ __forceinline__ float2 rotate_pair(float x0, float x1, float2 cs) {
   return make_float2(__fsub_rn(__fmul_rn(x0, cs.x), __fmul_rn(x1, cs.y)), __fadd_rn(__fmul_rn(x1, cs.x), __fmul_rn(x0, cs.y)));
 }
-__device__ __forceinline__ float quiet_nan() { return __int_as_float(0x7FC00000); }
 
 // Eight consecutive values as f32, 16-byte aligned.
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {

@@ -244,6 +244,7 @@ struct SharedArgs {
   uint32_t all_groups;
   uint64_t least;     // bytes that reading common keys once has to save, else nothing is common
   float* scratch;
+  uint64_t floats;    // in it
   uint4* places;      // [tokens of the call][heads]: first part's sums in `scratch` (of four floats), its (exponent of two that the weights are
                       // relative to, their sum) (of two), floats between parts, parts
   uint64_t sums;      // where in `scratch` a kernel that has no parts leaves a row's sums [tokens][heads][head_dim], and behind them the pairs
