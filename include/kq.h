@@ -409,10 +409,11 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
 /* kq_cache_attention_shared: kq_cache_attention for sequences that begin alike, the keys that they have in common read once.  Group g is the
  * sequences first[g] .. first[g + 1] - 1 (i32 [groups + 1], ascending; groups <= sequences); their first shared[g] tokens (i32 [groups]) are the same: their
  * tables name the same pages for them, or (a last page that is not full) copies.  What is shared beyond a sequence's new tokens' beginning counts as
- * its own; sequences outside the groups, and a group of one, are as in kq_cache_attention.  The same results but for roundings.  Reading
+ * its own.  A sequence that ended or was cut back has fewer: the common keys are read through the first of a group's first 32 sequences that has
+ * shared[g] tokens, else the first of them that has any, as far as it has them.  Boundaries that do not ascend: nothing is read once.  Sequences outside the groups, and a group of one, are as in kq_cache_attention.  The same results but for roundings.  Reading
  * once takes a launch more and joins every row's sums, reading often hits L2: `least` is how many bytes (tokens in common x members but one
  * x kv_heads (head_dim + 8), as the device arrays say) have to be saved for it, 0 for always, KQ_SHARED_AUTO for what measured faster.  The sums
- * over the common keys take 4 (head_dim + 6) bytes a row and query head of the context's scratch; where that is more than half of it, nothing is
+ * over the common keys take 4 (head_dim + 6) bytes a row and query head, and 4 a group, of the context's scratch; where that is more than half of it, nothing is
  * read once.
  *
  * kq_cache_summarize: for the pages that new tokens of the batch are in (behind their kq_cache_append), what kq_cache_select goes by: codes i8 [pages,

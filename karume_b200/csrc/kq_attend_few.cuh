@@ -50,7 +50,7 @@ constexpr int kFewTimeout = 40;      // status word: a copy of the cache did not
 
 // What a run of the list is.
 //   kWhole     a sequence's new rows and all keys they see
-//   kShared    prefix: the new rows of a group of sequences and the keys that the group has in common, read through its first sequence's
+//   kShared    prefix: the new rows of a group of sequences and the keys that the group has in common, read through one member's
 //              pages; the sums go to `sh`.  Rest: a sequence's new rows and the keys behind those, joined with the sums
 //   kSelected  one new row and the tokens of the pages selected for it (and a kv head), in the order of the list, as if they were a sequence
 enum FewMode { kWhole, kShared, kSelected };
@@ -94,7 +94,8 @@ struct Few {
   static constexpr int kScan = kWarpStat + (kWarps * kRows * 12 + 15) / 16 * 16;  // sums of the warps, what the scan found
   static constexpr int kSpan = kScan + kWarps * 8 + 32 + kWarps * 8;
   static constexpr int kAll = kSpan + kSpans * 16;     // kShared: keys that every row of a group sees
-  static constexpr int kBars = kAll + (kMode == kShared ? kSpans * 8 : 0);
+  static constexpr int kLead = kAll + (kMode == kShared ? kSpans * 8 : 0);  // ... and through whose pages they are read
+  static constexpr int kBars = kLead + (kMode == kShared ? kSpans * 4 : 0);
   static constexpr int kMisc = kBars + kWarps * kStages * 8;
   static constexpr int kSmem = kMisc + 16;
   // CTAs of an SM: what waits in one is hidden by the others; as many as registers and shared memory allow
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
   unsigned long long* found = scan + kWarps;  // sequence and tiles in front of it, of both cuts; runs of each warp's sequences
   int4* spans = reinterpret_cast<int4*>(smem + F::kSpan);
   int2* all = reinterpret_cast<int2*>(smem + F::kAll);
+  int* leads = reinterpret_cast<int*>(smem + F::kLead);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F::kMisc);
   volatile unsigned int* arrived = reinterpret_cast<volatile unsigned int*>(smem + F::kMisc + 4);
   const uint32_t bars = smem_u32(smem + F::kBars) + warp * kStages * 8;
@@ -289,11 +291,13 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
   if constexpr (kMode == kShared) {
     if (prefix) {  // (no more groups than are kept)
       for (uint32_t g_at = warp; g_at < items; g_at += kWarps) {
-        int2 every;
-        const int4 item = group_of_rows(p.a.batch, p.sh, g_at, static_cast<int>(min(p.a.window, 0x7fffffffu)), every);
+        int2 every, lead;
+        const int4 item = group_of_rows(p.a.batch, p.sh, g_at, static_cast<int>(min(p.a.window, 0x7fffffffu)), every, lead);
         if (lane == 0) {
           spans[g_at] = item;
           all[g_at] = every;
+          leads[g_at] = lead.x;
+          if (blockIdx.x == 0) p.sh.keys[g_at] = lead.y;
         }
       }
       __syncthreads();
@@ -433,7 +437,7 @@ __global__ void __launch_bounds__(Few<T, D, NT, kPair, kMode>::kThreads, Few<T, 
       if constexpr (kMode == kSelected) {
         if (wanted) page = selected_page(p.a, p.sel, ahead.b, ahead.head, ahead.runs.sequence, index);
       } else {
-        const uint32_t of = prefix ? first_of_group(p.a.batch, p.sh, ahead.b) : ahead.b;
+        const uint32_t of = prefix ? static_cast<uint32_t>(leads[ahead.b]) : ahead.b;
         if (wanted && index < p.a.batch.width) page = static_cast<uint32_t>(__ldg(p.a.batch.pages + static_cast<size_t>(of) * p.a.batch.width + index));
       }
       waiting = true;

@@ -92,7 +92,7 @@ struct ManyParams {
   SharedArgs sh;
 };
 
-// kGroups: prefix: a "sequence" is a group of them, its rows all their new ones, its keys those in common, read through the first one's
+// kGroups: prefix: a "sequence" is a group of them, its rows all their new ones, its keys those in common, read through one member's
 // pages; the sums go to `sh`.  Rest: the keys behind those, joined with the sums.
 constexpr uint32_t kGroupsAtOnce = 128;
 
@@ -351,12 +351,17 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   if (prefix && !sharing) return;
   const uint32_t sequences = prefix ? p.sh.groups : p.a.batch.sequences, each = (sequences + F::kThreads - 1) / F::kThreads, heads = p.a.cache.kv_heads;
   int4* const groups = reinterpret_cast<int4*>(smem + F::kRaw);  // until the codes come
-  static_assert(kGroupsAtOnce * 16 <= F::kRawBytes, "the groups' place");
+  int* const leads = reinterpret_cast<int*>(groups + kGroupsAtOnce);
+  static_assert(kGroupsAtOnce * 20 <= F::kRawBytes, "the groups' place");
   if (prefix) {
     for (uint32_t g = warp; g < sequences; g += F::kThreads / 32) {
-      int2 every;
-      const int4 of = group_of_rows(p.a.batch, p.sh, g, static_cast<int>(min(p.a.window, 0x7fffffffu)), every);
-      if (lane == 0) groups[g] = of;
+      int2 every, lead;
+      const int4 of = group_of_rows(p.a.batch, p.sh, g, static_cast<int>(min(p.a.window, 0x7fffffffu)), every, lead);
+      if (lane == 0) {
+        groups[g] = of;
+        leads[g] = lead.x;
+        if (blockIdx.x == 0) p.sh.keys[g] = lead.y;
+      }
     }
     __syncthreads();
   }
@@ -461,6 +466,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   const uint32_t seq = found[0];
   if (seq == 0xFFFFFFFFu) return;
   const Span span = rows_of(seq);
+  const uint32_t read_through = prefix ? static_cast<uint32_t>(leads[seq]) : seq;  // whose row of the page table
   const int common = kGroups && !prefix && sharing ? common_keys(p.a.batch, p.sh, seq, span) : 0;
   const uint32_t blocks = blocks_of(seq), head = found[1] % heads, block = blocks - 1 - found[1] / heads;  // the longest first
   const uint32_t all_parts = found[3], my_part = all_parts > 1 ? found[2] : 0;
@@ -1292,7 +1298,7 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
     } else if (warp == F::kCopyWarp) {
       // ---- copies --------------------------------------------------------------------------------------
       const uint32_t P = p.a.cache.page_tokens, block_bytes = static_cast<uint32_t>(cache_block_bytes(P, D));
-      const int* const pages = p.a.batch.pages + static_cast<size_t>(prefix ? first_of_group(p.a.batch, p.sh, seq) : seq) * p.a.batch.width;
+      const int* const pages = p.a.batch.pages + static_cast<size_t>(read_through) * p.a.batch.width;
       const auto page_of = [&](int key) -> uint32_t {
         const uint32_t index = static_cast<uint32_t>(key) >> p.page_shift;
         return key <= key_last && index < p.a.batch.width ? static_cast<uint32_t>(__ldg(pages + index)) : 0xFFFFFFFFu;

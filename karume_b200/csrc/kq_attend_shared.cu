@@ -46,7 +46,8 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
   // (Places count in pairs of floats, so no more than 32 GB of the scratch is used.)
   const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.heads, each = 16 + 4ull * (a.cache.head_dim + 2);
   const uint64_t scratch = std::min<uint64_t>(env.workspace_bytes, 32ull << 30);
-  const bool once = most >= static_cast<double>(sh.least) && env.workspace && rows * each + 64 <= scratch / 2;
+  const uint64_t kept = rows * each + 4ull * sh.groups;
+  const bool once = most >= static_cast<double>(sh.least) && env.workspace && kept + 64 <= scratch / 2;
   const uint64_t mine = static_cast<uint64_t>(a.batch.most) * group;
   const bool many = mine > kFewRows && attend_many_supports(a);
   if (!once && many) return launch_attend(env, a, launches);
@@ -58,11 +59,12 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
   cudaError_t e = cudaSuccess;
   if (once) {
     uint8_t* const base = static_cast<uint8_t*>(env.workspace);
-    const uint64_t left = (scratch - rows * each) / 16 * 16, own = left / 3 * 2 / 16 * 16;
+    const uint64_t left = (scratch - kept) / 16 * 16, own = left / 3 * 2 / 16 * 16;
     sh.scratch = static_cast<float*>(env.workspace);
-    sh.floats = scratch / 4;
+    sh.quads = static_cast<uint32_t>(scratch / 16);
     sh.places = reinterpret_cast<uint4*>(base + left);
     sh.sums = (left + rows * 16) / 4;
+    sh.keys = reinterpret_cast<int*>(base + left + rows * each);
     LaunchEnv parts = env;
     in.workspace_bytes = own;
     parts.workspace = base + own;
@@ -77,6 +79,7 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
       SharedArgs some = sh;
       some.first += g;
       some.tokens += g;
+      some.keys += g;
       some.groups = std::min(sh.groups - g, kGroupsAtOnce);
       if (!tensor || both) {
         e = attend_shared_few(parts, a, both ? kFewRows : 0xFFFFFFFFu, true, some,

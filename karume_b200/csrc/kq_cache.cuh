@@ -63,27 +63,27 @@ __device__ __forceinline__ int2 place_of_row(const CacheBatch& batch, uint32_t r
 
 // ---- sequences that begin alike ---------------------------------------------------------------
 // By a warp: whether reading what the groups have in common once saves enough (the other way re-reads it, mostly from L2).  Not where their
-// boundaries are out of order: groups with rows in common would ask for more blocks than there are.  (That is looked at last: `starts` are a trip to memory
+// boundaries are out of order: groups with rows in common would ask for more blocks than there are.  (`starts` are looked at last: a trip to memory
 // behind the boundaries, 1.4 us of a call that saves nothing.)
 __device__ __forceinline__ bool worth_sharing(const AttendArgs& a, const SharedArgs& sh) {
   unsigned long long keys = 0;
+  bool ordered = true;
   for (uint32_t g = threadIdx.x % 32; g < sh.all_groups; g += 32) {
-    const long long members = static_cast<long long>(__ldg(sh.all_first + g + 1)) - __ldg(sh.all_first + g);
+    const int first = __ldg(sh.all_first + g), next = __ldg(sh.all_first + g + 1);
+    ordered &= first <= next;
+    const long long members = static_cast<long long>(next) - first;
     unsigned tokens = static_cast<unsigned>(max(__ldg(sh.all_tokens + g), 0));
     if (a.window) tokens = min(tokens, a.window);
     if (members > 1) keys += static_cast<unsigned long long>(members - 1) * tokens;
   }
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) keys += __shfl_xor_sync(0xffffffffu, keys, o);
-  if (keys * (a.cache.kv_heads * (a.cache.head_dim + 8u)) < sh.least) return false;
-  bool ordered = true;
+  if (!__all_sync(0xffffffffu, ordered) || keys * (a.cache.kv_heads * (a.cache.head_dim + 8u)) < sh.least) return false;
+  if (!a.batch.starts) return true;
   for (uint32_t g = threadIdx.x % 32; g < sh.all_groups; g += 32)
     ordered &= groups::in_order(__ldg(sh.all_first + g), __ldg(sh.all_first + g + 1), a.batch.starts, static_cast<int>(a.batch.sequences),
                                 static_cast<int>(a.batch.tokens));
   return __all_sync(0xffffffffu, ordered);
-}
-__device__ __forceinline__ uint32_t first_of_group(const CacheBatch& batch, const SharedArgs& sh, uint32_t g) {
-  return min(static_cast<uint32_t>(max(__ldg(sh.first + g), 0)), batch.sequences - 1);
 }
 // How many keys sequence b has in common with its group, all of them in front of its new tokens; 0 where it is in none.
 __device__ __forceinline__ int common_keys(const CacheBatch& batch, const SharedArgs& sh, uint32_t b, const Span& span) {
@@ -97,11 +97,13 @@ __device__ __forceinline__ int common_keys(const CacheBatch& batch, const Shared
   if (b0 > static_cast<int>(b) || b1 <= static_cast<int>(b)) return 0;
   // Rows that are not among the group's (starts that do not ascend) have no sums over common keys.
   if (batch.starts && (batch.starts[max(b0, 0)] > span.first || batch.starts[min(b1, static_cast<int>(batch.sequences))] < span.first + span.count)) return 0;
-  return min(max(__ldg(sh.tokens + lo), 0), max(span.length - span.count, 0));
+  return min(max(__ldcg(sh.keys + lo), 0), max(span.length - span.count, 0));
 }
 // By a warp: the new rows of group g's sequences (first, number), the keys that any of them has in common, the first of these that a row
-// sees; every: first and last of the keys that all the rows see.
-__device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const SharedArgs& sh, uint32_t g, int window, int2& every) {
+// sees; every: first and last of the keys that all the rows see; lead: the member through whose row of the page table they are read, and how many
+// keys the group has at most.  Members that ended or were cut back have fewer tokens than the others, so this is the first of 32 that has all
+// that are said to be common, else the first that has any; what it has not is each other one's own.
+__device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const SharedArgs& sh, uint32_t g, int window, int2& every, int2& lead) {
   const groups::Range members = groups::sequences_of(__ldg(sh.first + g), __ldg(sh.first + g + 1), static_cast<int>(batch.sequences));
   const groups::Range rows = groups::rows_of(members, batch.starts, static_cast<int>(batch.tokens));
   int least = 0x7fffffff, far = 0, last = -1;
@@ -115,7 +117,12 @@ __device__ __forceinline__ int4 group_of_rows(const CacheBatch& batch, const Sha
   least = __reduce_min_sync(0xffffffffu, least);
   far = __reduce_max_sync(0xffffffffu, far);
   last = __reduce_max_sync(0xffffffffu, last);
-  const int keys = min(max(__ldg(sh.tokens + g), 0), far);
+  const int common = __ldg(sh.tokens + g), looked_at = members.begin + static_cast<int>(threadIdx.x % 32);
+  const int tokens = looked_at < members.end ? max(batch.lengths[looked_at], 0) : 0;
+  const uint32_t any = __ballot_sync(0xffffffffu, tokens > 0), all = __ballot_sync(0xffffffffu, tokens > 0 && tokens >= common);
+  const int at = max(__ffs(static_cast<int>(all ? all : any)) - 1, 0);
+  lead = make_int2(members.begin + at, min(max(common, 0), __shfl_sync(0xffffffffu, tokens, at)));
+  const int keys = min(lead.y, far);
   // (a window may hide all of them: one is walked over all the same, so that the rows' sums are written)
   const int from = window && least >= window ? min(least - window + 1, max(keys - 1, 0)) : 0;
   every = make_int2(window && last >= window ? last - window + 1 : 0, min(keys, max(least, 0)) - 1);
@@ -132,8 +139,9 @@ __device__ __forceinline__ float power_of_two(float x) {
 // which is at the row's place `at`.  A place that is none (a launch in front gave up waiting, and left the row's out) gives NaN.
 constexpr uint32_t kMostParts = 1024;  // CTAs that share a row's common keys: no more than there are SMs
 __device__ __forceinline__ void join_common(const SharedArgs& sh, const uint4& at, int quad, float& m, float& total, float (&v)[4]) {
-  const uint64_t last = static_cast<uint64_t>(at.w - 1) * at.z, end_sums = (static_cast<uint64_t>(at.x) + quad) * 4 + last + 4, end_stats = static_cast<uint64_t>(at.y) * 2 + last + 2;
-  if (at.w - 1 >= kMostParts || max(end_sums, end_stats) > sh.floats) {
+  // (in units of four floats, of which the scratch has 2^31 at most)
+  const uint32_t last = (at.w - 1) * (at.z / 4), end = max(at.x + quad, at.y / 2) + last;
+  if (at.w - 1 >= kMostParts || at.z > (1u << 20) || at.x >= sh.quads || end >= sh.quads) {
     total = quiet_nan();
     return;
   }

@@ -243,8 +243,9 @@ struct SharedArgs {
   const int* all_tokens;
   uint32_t all_groups;
   uint64_t least;     // bytes that reading common keys once has to save, else nothing is common
+  int* keys;          // [groups] in the scratch: how many keys each has in common, as the launch that reads them found
   float* scratch;
-  uint64_t floats;    // in it
+  uint32_t quads;     // of floats in it
   uint4* places;      // [tokens of the call][heads]: first part's sums in `scratch` (of four floats), its (exponent of two that the weights are
                       // relative to, their sum) (of two), floats between parts, parts
   uint64_t sums;      // where in `scratch` a kernel that has no parts leaves a row's sums [tokens][heads][head_dim], and behind them the pairs
