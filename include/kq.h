@@ -473,10 +473,12 @@ KQ_API int kq_cache_attention_selected(kq_ctx* ctx, kq_cache cache, uint64_t q_d
  *   `pairs` (from, to), i32 [pages, 2], (-1, -1) behind report[2] of them; table and refs have the new numbers.
  * kq_pages_copy: copies page from to page to for the pairs of such a call, in `count` pools (host arrays of addresses and of the bytes of a
  *   page, multiples of 4, and of 16 for bulk copies: the pool of a kq_cache has kq_cache_bytes(1, ..) a page, summaries kv_heads * 2 * head_dim and
- *   kv_heads * 8): the report's number of them, or (report_dptr == 0) all `most`.
+ *   kv_heads * 8).  How many of the pairs: report_dptr == KQ_PAIRS_END: those in front of the first negative one, which is what kq_pages_fork and
+ *   kq_pages_compact leave, whatever was called since; a report: as many as it says (every call on the book writes it, kq_pages_grow a 0); 0: all `most`.
  *   Pairs with a number outside the pool are passed over; one page may be the target of one pair, and not the source of another.
  *
  * None of these can be part of a fused plan, as above. */
+#define KQ_PAIRS_END 0xFFFFFFFFFFFFFFFFull
 KQ_API int kq_pages_grow(kq_ctx* ctx, uint64_t table_dptr, uint32_t sequences, uint32_t width, uint64_t lengths_dptr, uint64_t refs_dptr,
                          uint32_t pages, uint32_t page_tokens, uint64_t report_dptr, uint64_t news_dptr);
 KQ_API int kq_pages_fork(kq_ctx* ctx, uint64_t table_dptr, uint32_t sequences, uint32_t width, uint64_t lengths_dptr, uint64_t refs_dptr,

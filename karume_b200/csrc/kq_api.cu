@@ -1113,6 +1113,8 @@ int kq_pages_copy(kq_ctx* ctx, uint32_t count, const uint64_t* pools, const uint
   if (ctx->recording) return fail(ctx, KQ_ERR_STATE, "kq_pages_copy cannot be recorded into a fused plan (record a graph)");
   if (count && (!pools || !page_bytes)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: null argument");
   if (pages > (1u << 30) || most > (1u << 30)) return fail(ctx, KQ_ERR_SHAPE, "kq_pages_copy: %u pages, %u pairs: up to 2^30", pages, most);
+  const bool until_end = report == KQ_PAIRS_END;
+  if (until_end) report = 0;
   if (!pairs || ((pairs | report) & 3u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: pairs [most, 2] and report [4] are i32 device arrays");
   for (uint32_t i = 0; i < count; ++i) {
     if (!pools[i] || (pools[i] & 3u)) return fail(ctx, KQ_ERR_BAD_ARG, "kq_pages_copy: pool %u must be a 4-byte aligned device pointer", i);
@@ -1123,7 +1125,7 @@ int kq_pages_copy(kq_ctx* ctx, uint32_t count, const uint64_t* pools, const uint
   DeviceGuard guard(ctx->device);
   for (uint32_t i = 0; i < count; i += kq::kPoolsAtOnce) {
     cudaError_t e = kq::launch_pages_copy(env_of(ctx), std::min(kq::kPoolsAtOnce, count - i), pools + i, page_bytes + i, pages,
-                                          reinterpret_cast<const int*>(pairs), most, reinterpret_cast<const int*>(report));
+                                          reinterpret_cast<const int*>(pairs), most, reinterpret_cast<const int*>(report), until_end);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "pages_copy launch");
     ctx->launches += 1;
   }

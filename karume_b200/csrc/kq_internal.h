@@ -294,5 +294,5 @@ cudaError_t launch_pages_grow(const LaunchEnv& env, const PageBook& book, const 
 cudaError_t launch_pages_fork(const LaunchEnv& env, const PageBook& book, const int* parents, const int* keep, int* pairs);
 cudaError_t launch_pages_compact(const LaunchEnv& env, const PageBook& book, int* pairs);
 cudaError_t launch_pages_copy(const LaunchEnv& env, uint32_t count, const uint64_t* pools, const uint64_t* page_bytes, uint32_t pages, const int* pairs,
-                              uint32_t most, const int* report);
+                              uint32_t most, const int* report, bool until_end);
 }  // namespace kq

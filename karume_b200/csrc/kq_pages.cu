@@ -461,10 +461,25 @@ struct CopyParams {
   uint8_t* pool[kPoolsAtOnce];
   uint64_t bytes[kPoolsAtOnce];  // of a page
   const int* pairs;
-  const int* report;  // null: all `most` pairs
+  const int* report;  // null: all `most` pairs,
+  bool until_end;     // or those in front of the first negative one
   int* status;
   uint32_t pools, pages, most, parts;  // parts that a page is copied in, kPiece or less each
 };
+
+// How many pairs are in front of the first negative one, or `most`; by a warp, 32 places at a time: as many trips to memory as a report up to 32 pairs, one
+// more for every factor of 32 (7696 pairs: 3, of a copy of 290 us).
+__device__ __forceinline__ uint32_t pairs_until_end(const int* pairs, uint32_t most) {
+  uint32_t lo = 0, hi = most;  // pairs in front of lo, none at hi
+  while (lo < hi) {
+    const uint32_t at = lo + static_cast<uint32_t>(static_cast<uint64_t>(hi - lo) * (threadIdx.x % 32) / 32);
+    const uint32_t none = __ballot_sync(0xffffffffu, __ldcg(pairs + 2 * static_cast<size_t>(at)) < 0);
+    const int first = none ? __ffs(static_cast<int>(none)) - 1 : 32;  // the lane whose place is the first without a pair
+    if (first < 32) hi = __shfl_sync(0xffffffffu, at, first);
+    if (first > 0) lo = __shfl_sync(0xffffffffu, at, first - 1) + 1;
+  }
+  return hi;
+}
 
 // kWords: some pages are not whole sixteen bytes (without it: 307 us instead of 309 for the 1660 pages and the compaction in front of them).
 template <bool kWords>
@@ -479,7 +494,7 @@ __global__ void __launch_bounds__(32) pages_copy_kernel(const __grid_constant__ 
   __syncwarp();
   pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const uint32_t count = p.report ? min(static_cast<uint32_t>(max(p.report[2], 0)), p.most) : p.most;
+  const uint32_t count = p.until_end ? pairs_until_end(p.pairs, p.most) : p.report ? min(static_cast<uint32_t>(max(p.report[2], 0)), p.most) : p.most;
   const uint64_t all = static_cast<uint64_t>(count) * p.pools * p.parts;
   uint32_t n = 0;     // pieces asked for
   uint32_t done = 0;  // pieces handed on
@@ -632,7 +647,7 @@ cudaError_t launch_pages_compact(const LaunchEnv& env, const PageBook& book, int
 }
 
 cudaError_t launch_pages_copy(const LaunchEnv& env, uint32_t count, const uint64_t* pools, const uint64_t* page_bytes, uint32_t pages, const int* pairs,
-                              uint32_t most, const int* report) {
+                              uint32_t most, const int* report, bool until_end) {
   static OncePerDevice once;
   cudaError_t e = once.run([] {
     const cudaError_t e = cudaFuncSetAttribute(pages_copy_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCopySmem);
@@ -650,6 +665,7 @@ cudaError_t launch_pages_copy(const LaunchEnv& env, uint32_t count, const uint64
   }
   p.pairs = pairs;
   p.report = report;
+  p.until_end = until_end;
   p.status = env.status;
   p.pools = count;
   p.pages = pages;

@@ -38,6 +38,7 @@ class KqError(RuntimeError):
 
 
 KQ_SHARED_AUTO = (1 << 64) - 1
+KQ_PAIRS_END = (1 << 64) - 1
 
 _NP_DTYPES = {np.dtype(np.float32): KQ_F32, np.dtype(np.float16): KQ_F16}
 
@@ -226,6 +227,8 @@ class CachePages:
         self.table, self.lengths, self.refs, self.report, self.index = table, lengths, refs, report, table.get_device()
         self.pages, self.page_tokens = int(refs.numel()), int(page_tokens)
         self.args = (table.data_ptr(), self.sequences, self.width, lengths.data_ptr(), refs.data_ptr(), self.pages, self.page_tokens, report.data_ptr())
+        self.args_for_pairs = (*self.args[:-1], KQ_PAIRS_END)  # of a call, which end by themselves
+        self.counted = True  # the report may say how many pairs there are: no grow has written it since
 
 
 def _on_device(index: int, **tensors) -> None:
@@ -684,6 +687,7 @@ class Gpu:
 
     def pages_grow(self, book: CachePages, news) -> None:
         """Sequence b gets the pages of its next news[b] tokens (CUDA int32) and is that much longer."""
+        book.counted = False
         done = _fast.pages_grow(self._ctx_addr, book.args, news, self.index) if book.index == self.index else None
         if done is not None:
             return self._check(done)
@@ -695,27 +699,38 @@ class Gpu:
         Returns the pairs [sequences, 2] of pages to copy, for pages_copy."""
         done = _fast.pages_fork(self._ctx_addr, book.args, parents, keep, self.index) if book.index == self.index else None
         if done is not None:
-            return self._done(done)
+            return self._pairs(book, self._done(done))
         _on_device(self.index, table=book.table, parents=parents, keep=parents if keep is None else keep)
         torch = _torch()
         pairs = torch.empty((book.sequences, 2), dtype=torch.int32, device=self.device)
         self._check(L.kq_pages_fork(self._ctx, *book.args, _per_sequence(parents, book, "parents"),
                                     _per_sequence(keep, book, "keep") if keep is not None else 0, pairs.data_ptr()))
+        return self._pairs(book, pairs)
+
+    @staticmethod
+    def _pairs(book: CachePages, pairs):
+        """Pairs that a call made: pages_copy needs no report for them."""
+        pairs.end_by_themselves, book.counted = True, True
         return pairs
 
     def pages_compact(self, book: CachePages):
         """Moves the pages in use to the lowest numbers; returns the pairs [pages, 2] (from, to), for pages_copy."""
         done = _fast.pages_compact(self._ctx_addr, book.args, self.index) if book.index == self.index else None
         if done is not None:
-            return self._done(done)
+            return self._pairs(book, self._done(done))
         _on_device(self.index, table=book.table)
         torch = _torch()
         pairs = torch.empty((book.pages, 2), dtype=torch.int32, device=self.device)
         self._check(L.kq_pages_compact(self._ctx, *book.args, pairs.data_ptr()))
-        return pairs
+        return self._pairs(book, pairs)
 
     def pages_copy(self, book: CachePages, pairs, pools) -> None:
-        """Copies the pages of the book's last fork or compact in every pool: KvCaches, CacheSummaries, or CUDA tensors whose first axis is the pages."""
+        """Copies the pages of a fork or compact in every pool: KvCaches, CacheSummaries, or CUDA tensors whose first axis is the pages.  pairs: what the
+        call returned, whatever was called since; of other tensors as many as the book's report says, which a pages_grow has overwritten (refused)."""
+        of_a_call = getattr(pairs, "end_by_themselves", False)
+        if not of_a_call and not book.counted:
+            raise KqError(2, "pages_grow has overwritten the number of pairs in the report: give the tensor that pages_fork or pages_compact returned")
+        args = book.args_for_pairs if of_a_call else book.args
         given, pools = pools, []
         for pool in given:
             if isinstance(pool, KvCache):
@@ -724,7 +739,7 @@ class Gpu:
                 pools += pool.codes, pool.scales
             else:
                 pools.append(pool)
-        done = _fast.pages_copy(self._ctx_addr, book.args, pairs, pools, self.index) if book.index == self.index else None
+        done = _fast.pages_copy(self._ctx_addr, args, pairs, pools, self.index) if book.index == self.index else None
         if done is not None:
             return self._check(done)
         _on_device(self.index, table=book.table, pairs=pairs)
@@ -748,7 +763,7 @@ class Gpu:
             sizes.append(each)
         n = len(addresses)
         self._check(L.kq_pages_copy(self._ctx, n, (ctypes.c_uint64 * n)(*addresses), (ctypes.c_uint64 * n)(*sizes), book.pages, pairs.data_ptr(),
-                                    pairs.shape[0], book.report.data_ptr()))
+                                    pairs.shape[0], args[-1]))
 
     # -- replayable plans -------------------------------------------------------
     def graph_begin(self) -> None:
