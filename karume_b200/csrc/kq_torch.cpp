@@ -518,7 +518,8 @@ PyObject* pages_copy(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     PyObject* o = PyList_GET_ITEM(a[3], i);
     uint64_t of[4];
     if (tensor_of(o, &t)) {
-      if (t->get_device() != device || !plain(*t) || t->dim() == 0 || static_cast<uint64_t>(t->size(0)) < k[5]) KQ_NONE;
+      // (a pool without pages has no page's bytes: dividing by none would end the process)
+      if (t->get_device() != device || !plain(*t) || t->dim() == 0 || t->size(0) == 0 || static_cast<uint64_t>(t->size(0)) < k[5]) KQ_NONE;
       bytes[i] = static_cast<uint64_t>(t->numel() / t->size(0)) * t->element_size();
       pools[i] = ptr(*t);
     } else {

@@ -131,3 +131,15 @@ def test_a_number_that_a_grow_has_overwritten_is_refused(gpu):  # noqa: F811
         gpu.pages_copy(book, pairs[:1], [pool])
     gpu.sync()
     assert torch.equal(pool, kept)
+
+
+def test_an_empty_book_and_pools_without_pages_are_refused(gpu):  # noqa: F811
+    import karume_b200 as kb
+    book = kb.CachePages(torch.full((2, 4), -1, dtype=torch.int32, device="cuda"), i32([0, 0]), i32([]), 16)
+    for pool in (torch.empty(0, 4, device="cuda"), torch.empty(0, device="cuda"), torch.empty(3, 0, device="cuda")):
+        with pytest.raises(kb.KqError):
+            gpu.pages_copy(book, i32([[0, 1]]), [pool])
+    for call in (lambda: gpu.pages_grow(book, i32([1, 0])), lambda: gpu.pages_fork(book, i32([0, 0])), lambda: gpu.pages_compact(book)):
+        with pytest.raises(kb.KqError):
+            call()
+    assert book.table.tolist() == [[-1] * 4] * 2 and book.lengths.tolist() == [0, 0]
