@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "kq_cache.cuh"
+#include "kq_select_geometry.h"
 
 namespace kq {
 namespace {
@@ -423,6 +424,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
 
 template <typename Kernel, typename Params>
 cudaError_t launch_after(const LaunchEnv& env, Kernel kernel, uint64_t grid, int threads, const Params& p) {
+  if (grid > select::kMostBlocks) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(threads);
@@ -449,9 +451,8 @@ cudaError_t score_as(const LaunchEnv& env, const SelectParams& p) {
 }  // namespace
 
 cudaError_t launch_summarize(const LaunchEnv& env, const Cache& cache, const CacheBatch& batch, const Summaries& to) {
-  // one token each: every one has a page; else one of sixteen, or less
-  const SummaryParams p = {cache, batch, to, batch.starts ? 4u : 1u};
-  const uint64_t grid = (static_cast<uint64_t>(batch.tokens) + p.each - 1) / p.each * cache.kv_heads;
+  const SummaryParams p = {cache, batch, to, select::summary_rows(batch.tokens, cache.kv_heads, !batch.starts)};
+  const uint64_t grid = select::summary_blocks(batch.tokens, cache.kv_heads, p.each);
   switch (cache.head_dim) {
     case 64: return launch_after(env, summarize_kernel<64>, grid, kSummaryThreads, p);
     case 128: return launch_after(env, summarize_kernel<128>, grid, kSummaryThreads, p);
