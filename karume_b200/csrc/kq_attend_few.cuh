@@ -85,6 +85,7 @@ struct Few {
   // Whole sequences are cut by tiles, and selections, which are alike.
   static constexpr int kHead = kMode == kShared ? 640 / kTile : 0;
   static constexpr int kSpans = 128;                   // sequences whose lengths are kept in shared memory
+  static_assert(kMode != kShared || kSpans >= static_cast<int>(groups::kAtOnce), "a place for every group of a launch");
 
   static constexpr int kRing = 0;
   static constexpr int kMerge = kRing + kWarps * kStages * kTileBytes;

@@ -92,10 +92,6 @@ struct ManyParams {
   SharedArgs sh;
 };
 
-// kGroups: prefix: a "sequence" is a group of them, its rows all their new ones, its keys those in common, read through one member's
-// pages; the sums go to `sh`.  Rest: the keys behind those, joined with the sums.
-constexpr uint32_t kGroupsAtOnce = 128;
-
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -291,6 +287,8 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const fl
   *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// kGroups: prefix: a "sequence" is a group of them, its rows all their new ones, its keys those in common, read through one member's
+// pages; the sums go to `sh`.  Rest: the keys behind those, joined with the sums.
 template <typename T, int D, bool kGroups>
 __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(const __grid_constant__ ManyParams p) {
   using F = Many<T, D>;
@@ -351,8 +349,8 @@ __global__ void __launch_bounds__(Many<T, D>::kThreads, 1) attend_many_kernel(co
   if (prefix && !sharing) return;
   const uint32_t sequences = prefix ? p.sh.groups : p.a.batch.sequences, each = (sequences + F::kThreads - 1) / F::kThreads, heads = p.a.cache.kv_heads;
   int4* const groups = reinterpret_cast<int4*>(smem + F::kRaw);  // until the codes come
-  int* const leads = reinterpret_cast<int*>(groups + kGroupsAtOnce);
-  static_assert(kGroupsAtOnce * 20 <= F::kRawBytes, "the groups' place");
+  int* const leads = reinterpret_cast<int*>(groups + groups::kAtOnce);
+  static_assert(groups::kAtOnce * 20 <= F::kRawBytes, "the groups' place");
   if (prefix) {
     for (uint32_t g = warp; g < sequences; g += F::kThreads / 32) {
       int2 every, lead;

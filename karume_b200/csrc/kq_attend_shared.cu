@@ -23,7 +23,6 @@ constexpr uint64_t kWorth = 128ull << 20;
 // Sequences of so many query rows a kv head fill the tensor cores' blocks of rows by themselves: 16 of up to 300 new tokens behind 16384, 4 heads a
 // kv head, bfloat16 1511 / 1045 us; 8 of up to 100 behind 32768, 497 / 648.
 constexpr uint64_t kAlone = 512;
-constexpr uint32_t kGroupsAtOnce = 128;
 
 namespace {
 
@@ -70,17 +69,17 @@ cudaError_t launch_attend_shared(const LaunchEnv& env, const AttendArgs& a, Shar
     parts.workspace = base + own;
     parts.workspace_bytes = left - own;
     LaunchEnv alone = parts;  // groups that come in turns: none may leave its parts where the next one's go
-    if (sh.groups > kGroupsAtOnce) alone.workspace = nullptr;
+    if (sh.groups > groups::kAtOnce) alone.workspace = nullptr;
     // Each group is the work of one kernel, by its own rows; where they are many on the average, all are the tensor cores'.  (The few rows' kernel
     // first: what it leaves in the parts' place it has joined itself.)
     const uint64_t all = static_cast<uint64_t>(a.batch.tokens) * group;
     const bool tensor = all > kFewRows && attend_many_supports(a), both = tensor && all / sh.groups <= kFewRows;
-    for (uint32_t g = 0; g < sh.groups && e == cudaSuccess; g += kGroupsAtOnce) {
+    for (uint32_t g = 0; g < sh.groups && e == cudaSuccess; g += groups::kAtOnce) {
       SharedArgs some = sh;
       some.first += g;
       some.tokens += g;
       some.keys += g;
-      some.groups = std::min(sh.groups - g, kGroupsAtOnce);
+      some.groups = std::min(sh.groups - g, groups::kAtOnce);
       if (!tensor || both) {
         e = attend_shared_few(parts, a, both ? kFewRows : 0xFFFFFFFFu, true, some,
                               both ? kFewRows : (a.batch.tokens + sh.groups - 1) / sh.groups * group);

@@ -17,6 +17,9 @@
 namespace kq {
 namespace groups {
 
+// Groups of a launch: a kernel keeps what it found of each in shared memory; more come in turns.
+constexpr uint32_t kAtOnce = 128;
+
 struct Range {
   int begin, end;
 };
