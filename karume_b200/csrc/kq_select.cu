@@ -2,8 +2,9 @@
 //
 //   summary  of a page and kv head, over the page's tokens, for each channel: c = (max + min) / 2, r = (max - min) / 2 of what the keys
 //            stand for; both rows as 8-bit codes with a scale, by kq_quantize_rows' rule
-//   score    a query held likewise (codes a, scale s): s ((a . c) s_c + (|a| . r) s_r), which bounds s a . k over the page's keys;
-//            the largest of the query heads that share the kv head
+//   score    a query held likewise (codes a, scale s): s ((a . c) s_c + (|a| . r) s_r), about the most that s a . k can be for the page's
+//            keys; the largest of the query heads that share the kv head.  An estimate: codes are rounded to the nearest, so c may be off
+//            by s_c / 2 and r short by s_r / 2 in each channel, and a key be above the score by up to s (sum |a|) (s_c + s_r) / 2
 //   select   the first and last pages and, up to the budget, those with the largest scores, ties to the lower page
 //
 // What bounds them: at few rows the trips to memory one behind the other (lengths, page numbers, summaries or keys, and the queries beside them): a
