@@ -410,11 +410,12 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
  * sequences first[g] .. first[g + 1] - 1 (i32 [groups + 1], ascending; groups <= sequences); their first shared[g] tokens (i32 [groups]) are the same: their
  * tables name the same pages for them, or (a last page that is not full) copies.  What is shared beyond a sequence's new tokens' beginning counts as
  * its own.  A sequence that ended or was cut back has fewer: the common keys are read through the first of a group's first 32 sequences that has
- * shared[g] tokens, else the first of them that has any, as far as it has them.  Boundaries that do not ascend: nothing is read once.  Sequences outside the groups, and a group of one, are as in kq_cache_attention.  The same results but for roundings.  Reading
- * once takes a launch more and joins every row's sums, reading often hits L2: `least` is how many bytes (tokens in common x members but one
- * x kv_heads (head_dim + 8), as the device arrays say) have to be saved for it, 0 for always, KQ_SHARED_AUTO for what measured faster.  The sums
- * over the common keys take 4 (head_dim + 6) bytes a row and query head, and 4 a group, of the context's scratch; where that is more than half of it, nothing is
- * read once.
+ * shared[g] tokens, else the first of them that has any, as far as it has them.  Where boundaries do not ascend nothing is read once.  Sequences outside
+ * the groups, and a group of one, are as in kq_cache_attention.  The same results but for the order of f32 sums and, with 16-bit queries, one rounding to
+ * binary16 each of rotated queries and weights (and of keys and values, of groups with many rows).  Reading once takes a launch more and joins every
+ * row's sums, reading often hits L2: `least` is how many bytes (tokens in common x members but one x kv_heads (head_dim + 8), as the device arrays say)
+ * have to be saved for it, 0 for always, KQ_SHARED_AUTO for what measured faster.  The sums over the common keys take 4 (head_dim + 6) bytes a row and
+ * query head, and 4 a group, of the context's scratch; where that is more than half of it, nothing is read once.
  *
  * kq_cache_summarize: for the pages that new tokens of the batch are in (behind their kq_cache_append), what kq_cache_select goes by: codes i8 [pages,
  * kv_heads, 2, head_dim] and scales f32 [pages, kv_heads, 2], the host's, 16- and 8-byte aligned.  Over the page's tokens up to the sequence's
@@ -428,7 +429,7 @@ KQ_API int kq_cache_attention(kq_ctx* ctx, kq_cache cache, uint64_t q_dptr, uint
  * Scratch: 4 * kv_heads * table_width bytes at least (KQ_ERR_UNSUPPORTED).
  * kq_cache_attention_selected: attention of every new token over the tokens of its selected pages up to its position; `selected` as kq_cache_select
  * gives it: min(budget, pages up to the position) indices are read, the last of which is the position's own page.  An index outside the table reads
- * as NaN.  For few rows a sequence: each reads its own pages.
+ * as NaN.  For few rows a sequence: each reads its own pages.  16-bit queries: rotated ones and weights are rounded to binary16 once.
  *
  * None of these can be part of a fused plan, as above. */
 #define KQ_SHARED_AUTO 0xFFFFFFFFFFFFFFFFull

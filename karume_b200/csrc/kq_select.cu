@@ -8,8 +8,8 @@
 //   select   the first and last pages and, up to the budget, those with the largest scores, ties to the lower page
 //
 // What bounds them: at few rows the trips to memory one behind the other (lengths, page numbers, summaries or keys, and the queries beside them): a
-// summary 6 us, scores and selection of 128 pages 8, of 3126 18. Of 64 rows, 8 kv heads and 320 pages: summaries 10 us, scores and selection 22 (43 MB
-// of summaries, 2 TB/s).
+// summary 5 us, scores and selection of 128 pages 8.5, of 3126 16. Of 64 rows, 8 kv heads and 320 pages: summaries 8 us, scores and selection 23 (43 MB
+// of summaries, 1.9 TB/s).
 //
 // The dot products are of whole numbers, up to 127 * 127 * 256, which f32 holds exactly, and each of the few roundings behind them is
 // part of the definition: which pages are selected does not depend on the order of any sum.
