@@ -21,10 +21,10 @@ cudaError_t attend_shared_few_f16(const LaunchEnv& env, const AttendArgs& a, uin
 cudaError_t attend_shared_prefix_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 cudaError_t attend_shared_rest_many(const LaunchEnv& env, const AttendArgs& a, uint32_t beyond, const SharedArgs& sh);
 
-// Bytes that are read once instead of often, from which on that is faster: without it they come from L2 mostly, with it there is a launch more
-// and every row's sums are joined.  This way / the other, 32 heads over 8: bfloat16, 64 sequences behind 2048 common tokens (140 MB saved) 52 / 48 us,
-// behind 4096 (281 MB) 55 / 75, behind 32768 (2.2 GB) 104 / 450; 16 behind 8192 (134 MB) 47 / 41; f32 51 / 45. 8 heads over 4 of 64, 64 behind
-// 8192 (149 MB) 37 / 46.
+// Bytes that are read once instead of often, from about which on that is faster: without it they come from L2 mostly, with it there is a launch more
+// and every row's sums are joined.  This way / the other, 32 heads over 8: bfloat16, 16 sequences behind 8192 common tokens (134 MB saved, just under the line)
+// 47 / 41 us, f32 51 / 45; bfloat16, 64 behind 2048 (140 MB, which the rule has on the slower side) 52 / 48, behind 4096 (281 MB) 55 / 75, behind 32768
+// (2.2 GB) 104 / 450. 8 heads over 4 of 64, 64 behind 8192 (149 MB) 37 / 46.
 constexpr uint64_t kWorth = 128ull << 20;
 // Sequences of so many query rows a kv head fill the tensor cores' blocks of rows by themselves: 16 of up to 300 new tokens behind 16384, 4 heads a
 // kv head, bfloat16 1511 / 1045 us; 8 of up to 100 behind 32768, 497 / 648.
